@@ -28,6 +28,7 @@ LEVELS = 8
 SLICES = 16      # 8-dim slices of the vec8 decode table (two per level)
 SLICE_DIMS = 8
 PAGE_SIZE = 16
+Q8_MIN_EXP, Q8_MAX_EXP = -110, 119  # exponents of the 8-bit cache
 LAYOUT_HALF_SPLIT = 0
 LAYOUT_SORTED_PAIR = 1
 PREFILL_BLOCK_M = 32
@@ -47,6 +48,11 @@ SIGNATURES = {
     "atf_last_error": (ctypes.c_char_p, []),
     "atf_kv_write_bf16": (_i, [_p, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                _i, _i, _p, _p, _i, _p, _i, _i, _p]),
+    "atf_kv_write_packed_bf16": (_i, [_p, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _i, _p, _i, _i, _p, _p, _i,
+                                      _p, _i, _i, _p]),
+    "atf_kv_write_q8": (_i, [_p, _p, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _p, _i, _p, _p, _i,
+                             _p, _i, _i, _p]),
+    "atf_kv_expand_q8": (_i, [_p, _p, _p, _p, _i, _i, _p, _i, _i, _i, _p]),
     "atf_prefill_bf16": (_i, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i, _p, _i,
                               _i, _i, _i, _i, _i, _i, _p, _f, _p, _i, _i, _p]),
     "atf_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
@@ -57,6 +63,9 @@ SIGNATURES = {
                                           _i, _i, _i, _i, _p, _f, _p, _i, _i, _p, _sz, _p]),
     "atf_decode_paged_bf16_noalloc": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i, _p, _i, _p,
                                            _i, _i, _i, _i, _p, _f, _p, _i, _i, _p]),
+    "atf_decode_q8_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "atf_decode_paged_q8": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i, _p, _i, _p,
+                                 _i, _i, _i, _i, _p, _i, _f, _p, _i, _i, _p, _sz, _p]),
     "atf_decode_rows_bf16": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                   _i, _i, _i, _i, _p, _i, _f, _p, _i, _i, _p, _sz, _p]),
     "atf_prefill_mfma_probe": (_i, [_p, _i, _i, _p]),
@@ -139,6 +148,16 @@ def ptr(t):
     """Device address of a tensor as an int (None for an absent tensor): the
     bound argument types convert it, which costs less than a c_void_p object."""
     return t.data_ptr() if t is not None else None
+
+
+def launch(device, entry, *args):
+    """entry(*args, stream): a library call on the current stream of `device`, made
+    with that device current (a kernel is launched on the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(entry(*args, stream_of(device)))
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, stream_of(device)))
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -10,6 +10,16 @@ and r+P; a 16-dim level l is slices 2l and 2l+1), so the window's surviving
 prefix of a page is one contiguous run and out-of-window slices are never
 fetched; with V first in the block, a page's windowed read is one run (V, then
 that prefix).  `k_half` and `v_half` give the two halves as strided views.
+
+With kv_dtype=torch.float8_e4m3fn the cache holds 8-bit floats, half the bytes:
+
+    kv    float8_e4m3fn [num_pages, num_kv_heads, 2, 2048]: one 4 KB block per (page, kv head)
+        kv[:, :, 0]  V half: [2 j, 4 g, 16 r, 4 d, 4 t] = dim 8r + 4j + d of token 4g + t
+        kv[:, :, 1]  K half: [8 levels, 16 tokens, slices 2l and 2l + 1 of 8 dims]
+    exps  int8 [num_pages, num_kv_heads, 2]: the exponents of the V and the K half; a
+          code c stands for c * 2 ** exponent
+
+`dequantize` gives the values that the codes of some pages stand for.
 Pages are zero-initialised.  Sequences own lists of page ids; page_table()
 packs them into the int32 [batch, max_pages] table the kernels take.
 """
@@ -26,6 +36,27 @@ def new_kv_cache(num_pages: int, num_kv_heads: int, device="cuda") -> torch.Tens
                        device=device)
 
 
+def new_kv_cache_q8(num_pages: int, num_kv_heads: int, device="cuda"):
+    """An empty 8-bit cache: (codes float8_e4m3fn [num_pages, num_kv_heads, 2, 2048],
+    exponents int8 [num_pages, num_kv_heads, 2])."""
+    shape = (int(num_pages), int(num_kv_heads))
+    codes = torch.zeros((*shape, *_lib.KV_BLOCK_SHAPE), dtype=torch.uint8, device=device)
+    return codes.view(torch.float8_e4m3fn), torch.full((*shape, 2), _lib.Q8_MIN_EXP, dtype=torch.int8, device=device)
+
+
+def dequantize(kv: torch.Tensor, exps: torch.Tensor, pages) -> tuple:
+    """fp32 (k, v) [n, 16 tokens, num_kv_heads, 128] of the pages with these ids of an
+    8-bit cache, k by slices in wavelength order as the cache holds it (half-split
+    dims: slice s is rotary pairs 60 - 4s .. 63 - 4s, first halves and then second)."""
+    ids = torch.as_tensor(pages, dtype=torch.long, device=kv.device)
+    x = kv.view(torch.uint8)[ids].view(kv.dtype).float() * torch.exp2(exps[ids].float())[..., None]
+    n, h = x.shape[:2]
+    k = x[:, :, _lib.K_HALF].reshape(n, h, _lib.LEVELS, PAGE, 2 * _lib.SLICE_DIMS)
+    v = x[:, :, _lib.V_HALF].reshape(n, h, 2, 4, 16, 4, 4)
+    return (k.permute(0, 3, 1, 2, 4).reshape(n, PAGE, h, _lib.HEAD_DIM),
+            v.permute(0, 3, 6, 1, 4, 2, 5).reshape(n, PAGE, h, _lib.HEAD_DIM))
+
+
 def k_half(kv: torch.Tensor) -> torch.Tensor:
     """The K halves of a cache as a view [num_pages, num_kv_heads, 16, 16, 8]."""
     return kv[:, :, _lib.K_HALF].unflatten(-1, _lib.K_BLOCK_SHAPE)
@@ -37,15 +68,26 @@ def v_half(kv: torch.Tensor) -> torch.Tensor:
 
 
 class PagedKVCache:
-    def __init__(self, num_pages: int, num_kv_heads: int, device="cuda", head_dim: int = 128):
+    """One layer's pool of pages and the sequences that own them.  kv_dtype:
+    torch.bfloat16, or torch.float8_e4m3fn for the cache of 8-bit floats (`exps` then
+    holds its exponents, None otherwise)."""
+
+    def __init__(self, num_pages: int, num_kv_heads: int, device="cuda", head_dim: int = 128,
+                 kv_dtype: torch.dtype = torch.bfloat16):
         if head_dim != _lib.HEAD_DIM:
             raise ValueError(f"head_dim {head_dim} unsupported (this build supports {_lib.HEAD_DIM})")
         self.num_pages = int(num_pages)
         self.num_kv_heads = int(num_kv_heads)
         self.device = torch.device(device)
-        self.kv = new_kv_cache(num_pages, num_kv_heads, self.device)
-        self.k = k_half(self.kv)  # views of the two halves
-        self.v = v_half(self.kv)
+        self.exps = None
+        if kv_dtype == torch.float8_e4m3fn:
+            self.kv, self.exps = new_kv_cache_q8(num_pages, num_kv_heads, self.device)
+        elif kv_dtype == torch.bfloat16:
+            self.kv = new_kv_cache(num_pages, num_kv_heads, self.device)
+            self.k = k_half(self.kv)  # views of the two halves
+            self.v = v_half(self.kv)
+        else:
+            raise ValueError(f"kv_dtype must be bfloat16 or float8_e4m3fn, got {kv_dtype}")
         self._free = list(range(num_pages - 1, -1, -1))
         self.pages = {}    # seq id -> list of page ids
         self.lengths = {}  # seq id -> tokens written

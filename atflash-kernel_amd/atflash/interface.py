@@ -125,16 +125,32 @@ def decode_contiguous(q, k, v, zhi, scale, rope, layout):
 
 
 def prefill_paged(q, cache, page_table, nk, q_offset, zhi=None, sm_scale=None, rope=None, layout="half_split"):
+    """Windowed causal prefill against a PagedKVCache (either kv_dtype)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
+    if getattr(cache, "exps", None) is not None:
+        return ops.prefill_q8(q, cache.kv, cache.exps, page_table, int(nk), int(q_offset), _zhi_list(zhi), scale, rope,
+                              _layout_id(layout))
     return ops.prefill(q, cache.kv, page_table, int(nk), int(q_offset), _zhi_list(zhi), scale, rope,
                        _layout_id(layout))
 
 
 def decode_paged(q, cache, page_table, seq_lens, max_seq_len, zhi=None, sm_scale=None, rope=None,
                  layout="half_split"):
+    """One decode step over a PagedKVCache (either kv_dtype)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
+    if getattr(cache, "exps", None) is not None:
+        return ops.decode_paged_q8(q, cache.kv, cache.exps, page_table, seq_lens, int(max_seq_len),
+                                   _zhi_list(zhi, _DECODE_TABLES), scale, rope, _layout_id(layout))
     return ops.decode_paged(q, cache.kv, page_table, seq_lens, int(max_seq_len),
                             _zhi_list(zhi, _DECODE_TABLES), scale, rope, _layout_id(layout))
+
+
+def kv_write_packed(cache, k, v, cu_seqlens, max_tokens, start_pos, page_table, rope=None, layout="half_split"):
+    """New tokens of several sequences, rows packed one after the other (k, v
+    [T, Hkv, 128], sequence b's rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 from
+    position start_pos[b] on), into a PagedKVCache (either kv_dtype)."""
+    ops.kv_write_packed(cache.kv, cache.exps, k, v, cu_seqlens, int(max_tokens), start_pos, page_table, rope,
+                        _layout_id(layout))
 
 
 def decode_plan(cache, page_table, seq_lens, max_seq_len, num_q_heads, zhi=None, sm_scale=None, rope=None,
@@ -144,4 +160,4 @@ def decode_plan(cache, page_table, seq_lens, max_seq_len, num_q_heads, zhi=None,
     window table, scale, RoPE table); plan.run(q) per step."""
     scale = 1.0 / math.sqrt(_lib.HEAD_DIM) if sm_scale is None else float(sm_scale)
     return ops.DecodePlan(cache.kv, page_table, seq_lens, int(max_seq_len), _zhi_list(zhi, _DECODE_TABLES), scale,
-                          rope, _layout_id(layout), num_q_heads, q_strides)
+                          rope, _layout_id(layout), num_q_heads, q_strides, getattr(cache, "exps", None))

@@ -7,7 +7,21 @@
                                    sm_scale, rope_cs, layout) -> out
 
 kv_cache is the paged cache, bf16 [num_pages, num_kv_heads, 2, 2048]
-(atflash.cache: V half, then K half, per page and kv head).
+(atflash.cache: V half, then K half, per page and kv head).  The cache of 8-bit
+floats is float8_e4m3fn of the same shape with int8 exponents kv_exps
+[num_pages, num_kv_heads, 2]:
+
+    torch.ops.atflash.kv_write_q8(kv_cache, kv_exps, k, v, start_pos, page_table, rope_cs, layout)
+    torch.ops.atflash.decode_paged_q8(q, kv_cache, kv_exps, page_table, seq_lens, max_seq_len, zhi,
+                                      sm_scale, rope_cs, layout) -> out
+    torch.ops.atflash.prefill_q8(q, kv_cache, kv_exps, page_table, nk, q_offset, zhi, sm_scale,
+                                 rope_cs, layout) -> (out, lse)
+
+Rows of several sequences packed one after the other (either cache; kv_exps None:
+the bf16 cache):
+
+    torch.ops.atflash.kv_write_packed(kv_cache, kv_exps, k, v, cu_seqlens, max_tokens, start_pos,
+                                      page_table, rope_cs, layout)
 
 Each op checks shapes and dtypes, then calls the HIP library on the current
 stream of the tensors' device.  There is no CPU or PyTorch fallback: a CPU
@@ -103,6 +117,136 @@ def _(kv_cache, k, v, start_pos, page_table, rope_cs, layout):
     return None
 
 
+# ---- the cache of 8-bit floats, packed rows ----
+
+_F8 = torch.float8_e4m3fn
+
+
+def _one_device(first, *ts):
+    """The GPU that all of these tensors are on (None: an absent one)."""
+    dev = first.device
+    for t in (first, *ts):
+        if t is not None and t.device != dev:
+            raise ValueError(f"the tensors of a call must be on one device (got {dev} and {t.device})")
+    if dev.type != "cuda":
+        raise ValueError("atflash ops run on the GPU only (got a tensor on %s)" % dev)
+    return dev
+
+
+def _check_cache_q8(kv_cache, kv_exps):
+    s = kv_cache.shape
+    _need(kv_cache.dtype == _F8, "the 8-bit kv_cache must be float8_e4m3fn")
+    _need(len(s) == 4 and tuple(s[2:]) == _lib.KV_BLOCK_SHAPE, "kv_cache must be [num_pages, num_kv_heads, 2, 2048]")
+    _need(kv_cache.is_contiguous(), "kv_cache must be contiguous")
+    _need(kv_exps.dtype == torch.int8 and kv_exps.shape == (s[0], s[1], 2) and kv_exps.is_contiguous(),
+          "kv_exps must be contiguous int8 [num_pages, num_kv_heads, 2]")
+
+
+def _check_rows(k, v, dims, hkv):
+    names = {3: "[T, Hkv, 128]", 4: "[B, T, Hkv, 128]"}
+    _need(k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16, "k and v must be bf16")
+    _need(k.dim() == dims and v.shape == k.shape and k.shape[-1] == _lib.HEAD_DIM,
+          f"k and v must be {names[dims]} of equal shape")
+    _need(k.shape[-2] == hkv, "k heads must equal the cache's kv heads")
+    _need(k.stride(-1) == 1 and v.stride(-1) == 1, "last dim of k and v must be contiguous")
+
+
+def _check_table(page_table, B):
+    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
+          and page_table.is_contiguous(), "page_table must be contiguous int32 [B, max_pages]")
+
+
+def _check_ints(t, n, name):
+    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(),
+          f"{name} must be contiguous int32 [{n}]")
+
+
+def kv_write_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                start_pos: torch.Tensor, page_table: torch.Tensor, rope_cs: Optional[torch.Tensor],
+                layout: int) -> None:
+    """kv_write into the cache of 8-bit floats: k/v [B, T, Hkv, 128] bf16, K rotated
+    with rope_cs.  Sequences are appended to: the slots behind a call's last
+    token in its last page become zero (atf_kv_write_q8 in include/atflash.h)."""
+    dev = _one_device(kv_cache, kv_exps, k, v, start_pos, page_table, rope_cs)
+    _check_cache_q8(kv_cache, kv_exps)
+    pool = kv_cache.shape
+    _check_rows(k, v, 4, pool[1])
+    B, T = k.shape[:2]
+    _check_ints(start_pos, B, "start_pos")
+    _check_table(page_table, B)
+    rope_cs, max_pos = _rope(rope_cs)
+    _lib.launch(dev, _lib.lib().atf_kv_write_q8,
+                kv_cache.data_ptr(), kv_exps.data_ptr(), pool[0], pool[1], k.data_ptr(), *k.stride()[:3],
+                v.data_ptr(), *v.stride()[:3], B, T, None, 0, start_pos.data_ptr(), page_table.data_ptr(),
+                page_table.shape[1], _lib.ptr(rope_cs), max_pos, _layout(layout))
+
+
+_kv_write_q8_op = torch.library.custom_op("atflash::kv_write_q8", kv_write_q8, mutates_args=("kv_cache", "kv_exps"))
+
+
+@_kv_write_q8_op.register_fake
+def _(kv_cache, kv_exps, k, v, start_pos, page_table, rope_cs, layout):
+    return None
+
+
+def kv_write_packed(kv_cache: torch.Tensor, kv_exps: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                    cu_seqlens: torch.Tensor, max_tokens: int, start_pos: torch.Tensor, page_table: torch.Tensor,
+                    rope_cs: Optional[torch.Tensor], layout: int) -> None:
+    """Packed rows into the paged cache, bf16 (kv_exps None) or of 8-bit floats:
+    sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of k and v
+    [T, Hkv, 128], the first at position start_pos[b].  max_tokens: the most of
+    a sequence; rows past it are not written."""
+    dev = _one_device(kv_cache, kv_exps, k, v, cu_seqlens, start_pos, page_table, rope_cs)
+    if kv_exps is None:
+        _check_cache(kv_cache)
+    else:
+        _check_cache_q8(kv_cache, kv_exps)
+    pool = kv_cache.shape
+    _check_rows(k, v, 3, pool[1])
+    B, T = page_table.shape[0], k.shape[0]
+    _check_table(page_table, B)
+    _check_ints(cu_seqlens, B + 1, "cu_seqlens")
+    _check_ints(start_pos, B, "start_pos")
+    max_tokens = min(int(max_tokens), T)
+    rope_cs, max_pos = _rope(rope_cs)
+    L = _lib.lib()
+    tail = (start_pos.data_ptr(), page_table.data_ptr(), page_table.shape[1], _lib.ptr(rope_cs), max_pos,
+            _layout(layout))
+    ks_t, ks_h, _ = k.stride()
+    vs_t, vs_h, _ = v.stride()
+    if kv_exps is None:
+        _lib.launch(dev, L.atf_kv_write_packed_bf16, kv_cache.data_ptr(), pool[0], pool[1], k.data_ptr(), ks_t, ks_h,
+                    v.data_ptr(), vs_t, vs_h, B, cu_seqlens.data_ptr(), T, max_tokens, *tail)
+    else:
+        _lib.launch(dev, L.atf_kv_write_q8, kv_cache.data_ptr(), kv_exps.data_ptr(), pool[0], pool[1],
+                    k.data_ptr(), 0, ks_t, ks_h, v.data_ptr(), 0, vs_t, vs_h, B, max_tokens, cu_seqlens.data_ptr(), T,
+                    *tail)
+
+
+_kv_write_packed_op = torch.library.custom_op("atflash::kv_write_packed", kv_write_packed,
+                                              mutates_args=("kv_cache", "kv_exps"))
+
+
+@_kv_write_packed_op.register_fake
+def _(kv_cache, kv_exps, k, v, cu_seqlens, max_tokens, start_pos, page_table, rope_cs, layout):
+    return None
+
+
+def kv_expand_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torch.Tensor, n_pages: int):
+    """The first n_pages pages of each sequence of an 8-bit cache as bf16 pages,
+    exactly: (bf16 cache [B * n_pages, Hkv, 2, 2048], its page table [B, n_pages])."""
+    dev = _one_device(kv_cache, kv_exps, page_table)
+    _check_cache_q8(kv_cache, kv_exps)
+    B = page_table.shape[0]
+    _check_table(page_table, B)
+    pool = kv_cache.shape
+    out = torch.empty((B * int(n_pages), pool[1], *_lib.KV_BLOCK_SHAPE), dtype=torch.bfloat16, device=dev)
+    table = torch.empty((B, int(n_pages)), dtype=torch.int32, device=dev)
+    _lib.launch(dev, _lib.lib().atf_kv_expand_q8, out.data_ptr(), table.data_ptr(), kv_cache.data_ptr(),
+                kv_exps.data_ptr(), pool[0], pool[1], page_table.data_ptr(), B, page_table.shape[1], int(n_pages))
+    return out, table
+
+
 def prefill(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor,
             nk: int, q_offset: int, zhi: Optional[List[int]], sm_scale: float,
             rope_cs: Optional[torch.Tensor], layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -139,6 +283,28 @@ _prefill_op = torch.library.custom_op("atflash::prefill", prefill, mutates_args=
 
 @_prefill_op.register_fake
 def _(q, kv_cache, page_table, nk, q_offset, zhi, sm_scale, rope_cs, layout):
+    B, Nq, Hq, D = q.shape
+    return q.new_empty((B, Nq, Hq, D)), q.new_empty((B, Hq, Nq), dtype=torch.float32)
+
+
+def prefill_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torch.Tensor,
+               nk: int, q_offset: int, zhi: Optional[List[int]], sm_scale: float,
+               rope_cs: Optional[torch.Tensor], layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """prefill over the cache of 8-bit floats.  The keys' pages are expanded into
+    temporary bf16 pages first (exact; 12 bytes moved an element pair of K and V
+    against the attention's work on it, which grows with the queries), then read by
+    prefill's kernels: their results on the values that the codes stand for."""
+    _need(int(nk) >= 0 and -(-int(nk) // _lib.PAGE_SIZE) <= page_table.shape[-1],
+          f"page table too small for nk={nk}")
+    kv, table = kv_expand_q8(kv_cache, kv_exps, page_table, -(-int(nk) // _lib.PAGE_SIZE))
+    return prefill(q, kv, table, nk, q_offset, zhi, sm_scale, rope_cs, layout)
+
+
+_prefill_q8_op = torch.library.custom_op("atflash::prefill_q8", prefill_q8, mutates_args=())
+
+
+@_prefill_q8_op.register_fake
+def _(q, kv_cache, kv_exps, page_table, nk, q_offset, zhi, sm_scale, rope_cs, layout):
     B, Nq, Hq, D = q.shape
     return q.new_empty((B, Nq, Hq, D)), q.new_empty((B, Hq, Nq), dtype=torch.float32)
 
@@ -230,6 +396,42 @@ def decode_paged(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tens
     return out
 
 
+def decode_paged_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torch.Tensor,
+                    seq_lens: torch.Tensor, max_seq_len: int, zhi: Optional[List[int]], sm_scale: float,
+                    rope_cs: Optional[torch.Tensor], layout: int) -> torch.Tensor:
+    """decode_paged over the cache of 8-bit floats: q [B, Hq, 128] bf16, zhi the
+    level table (8 entries) or the per-slice table (16), out bf16 [B, Hq, 128]."""
+    dev = _one_device(q, kv_cache, kv_exps, page_table, seq_lens, rope_cs)
+    _check_cache_q8(kv_cache, kv_exps)
+    qs = q.shape
+    _need(q.dtype == torch.bfloat16 and len(qs) == 3 and qs[2] == _lib.HEAD_DIM, "q must be bf16 [B, Hq, 128]")
+    q_sb, q_sh, q_sd = q.stride()
+    _need(q_sd == 1, "last dim of q must be contiguous")
+    B, Hq, D = qs
+    _check_ints(seq_lens, B, "seq_lens")
+    _check_table(page_table, B)
+    pool = kv_cache.shape
+    rope_cs, max_pos = _rope(rope_cs)
+    L = _lib.lib()
+    n = 0 if zhi is None else len(zhi)
+    table = None if zhi is None else _table(zhi, _lib.SLICES if n == _lib.SLICES else _lib.LEVELS)
+    ws = _decode_workspace(dev, _lib.stream_of(dev), B, Hq, pool[1], int(max_seq_len), L)
+    out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
+    _lib.launch(dev, L.atf_decode_paged_q8, out.data_ptr(), Hq * D, D, q.data_ptr(), q_sb, q_sh, kv_cache.data_ptr(),
+                kv_exps.data_ptr(), pool[0], page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), B, Hq,
+                pool[1], int(max_seq_len), table, n, float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout),
+                ws[0], ws[1])
+    return out
+
+
+_decode_paged_q8_op = torch.library.custom_op("atflash::decode_paged_q8", decode_paged_q8, mutates_args=())
+
+
+@_decode_paged_q8_op.register_fake
+def _(q, kv_cache, kv_exps, page_table, seq_lens, max_seq_len, zhi, sm_scale, rope_cs, layout):
+    return q.new_empty(q.shape)
+
+
 # Longest token stride (elements) of the K and V rows atf_decode_rows_bf16 reads.
 _ROWS_MAX_STRIDE = 1 << 26
 
@@ -287,9 +489,14 @@ class DecodePlan:
     """
 
     def __init__(self, kv_cache, page_table, seq_lens, max_seq_len, zhi, sm_scale, rope_cs, layout,
-                 num_q_heads, q_strides=None):
+                 num_q_heads, q_strides=None, kv_exps=None):
+        """kv_exps: the exponents of a cache of 8-bit floats (None: a bf16 cache)."""
         _need_gpu(kv_cache, page_table, seq_lens, rope_cs)
-        _check_cache(kv_cache)
+        if kv_exps is None:
+            _check_cache(kv_cache)
+        else:
+            _one_device(kv_cache, kv_exps, page_table, seq_lens, rope_cs)
+            _check_cache_q8(kv_cache, kv_exps)
         B = page_table.shape[0] if page_table.dim() == 2 else -1
         _need(seq_lens.dtype == torch.int32 and seq_lens.numel() == B and seq_lens.is_contiguous(),
               "seq_lens must be contiguous int32 [B]")
@@ -304,14 +511,19 @@ class DecodePlan:
         self.device = kv_cache.device
         self.shape = (B, Hq, D)
         self.q_strides = (q_sb, q_sh, 1)
-        nbytes = int(L.atf_decode_workspace_bytes_even(B, Hq, kv_cache.shape[1], int(max_seq_len)))
+        size = L.atf_decode_workspace_bytes_even if kv_exps is None else L.atf_decode_q8_workspace_bytes
+        nbytes = int(size(B, Hq, kv_cache.shape[1], int(max_seq_len)))
         self._ws = torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=self.device)
-        self._keep = (kv_cache, page_table, seq_lens, rope_cs)  # the tensors the addresses point into
+        self._keep = (kv_cache, kv_exps, page_table, seq_lens, rope_cs)  # the tensors the addresses point into
         self._table = _lib.zhi_array(None if zhi is None else tuple(zhi), _lib.SLICES if slices else _lib.LEVELS)
         self._entry = L.atf_decode_paged_slices_bf16 if slices else L.atf_decode_paged_bf16
-        self._mid = (kv_cache.data_ptr(), kv_cache.shape[0], page_table.data_ptr(), page_table.shape[1],
-                     seq_lens.data_ptr(), B, Hq, kv_cache.shape[1], int(max_seq_len), self._table, float(sm_scale),
-                     _lib.ptr(rope_cs), max_pos, _layout(layout), self._ws.data_ptr(), self._ws.numel() * 4)
+        cache, entries = (kv_cache.data_ptr(),), ()
+        if kv_exps is not None:
+            self._entry = L.atf_decode_paged_q8
+            cache, entries = (*cache, kv_exps.data_ptr()), (0 if zhi is None else len(zhi),)
+        self._mid = (*cache, kv_cache.shape[0], page_table.data_ptr(), page_table.shape[1],
+                     seq_lens.data_ptr(), B, Hq, kv_cache.shape[1], int(max_seq_len), self._table, *entries,
+                     float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout), self._ws.data_ptr(), self._ws.numel() * 4)
 
     def run(self, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Decode for q [B, Hq, 128] bf16 (the plan's shape and strides);

@@ -37,6 +37,7 @@ COMMON = [
 # lane; its MFMAs keep their results in ordinary registers (left to itself the
 # compiler puts them in accumulation registers there and copies every score out).
 EXTRA = {"atf_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
+         "atf_decode_q8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
          "atf_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

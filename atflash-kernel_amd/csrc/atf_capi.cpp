@@ -159,6 +159,48 @@ bool spread_batch(int batch, int hkv, int n_splits, int waves, int group, int ma
   return spread_bytes(batch, hkv, n_splits, group) * 32 <= static_cast<size_t>(pages) * (atf::kKvBlockElems * 2);
 }
 
+// Validation and argument packing shared by the cache writers (everything except
+// packed rows and the 8-bit cache's exponents).
+int kv_write_prepare(void* kv_cache, int num_pages, int num_kv_heads, const void* k_src, int64_t ks_b, int64_t ks_t,
+                     int64_t ks_h, const void* v_src, int64_t vs_b, int64_t vs_t, int64_t vs_h, int batch, int n_tokens,
+                     const int32_t* start_pos, const int32_t* page_table, int max_pages, const float* rope_cs,
+                     int rope_max_pos, int layout, atf::KvWriteArgs* a) {
+  if (batch < 0 || n_tokens < 0) return fail(ATF_ERR_INVALID, "batch and n_tokens must be >= 0");
+  if (batch == 0 || n_tokens == 0) return ATF_OK;
+  if (!kv_cache || !k_src || !v_src || !start_pos || !page_table)
+    return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (num_pages <= 0 || num_kv_heads <= 0 || max_pages <= 0)
+    return fail(ATF_ERR_INVALID, "num_pages, num_kv_heads and max_pages must be positive");
+  if (int r = check_layout(layout, rope_cs, rope_max_pos)) return r;
+  if (!aligned(k_src, 16) || !aligned(v_src, 16) || !aligned(kv_cache, 16))
+    return fail(ATF_ERR_INVALID, "k/v sources and kv_cache must be 16-byte aligned");
+  for (int64_t s : {ks_b, ks_t, ks_h, vs_b, vs_t, vs_h})
+    if (s % 8 != 0) return fail(ATF_ERR_INVALID, "source strides must be multiples of 8 elements");
+  a->kv_cache = static_cast<uint16_t*>(kv_cache);
+  a->num_pages = num_pages;
+  a->hkv = num_kv_heads;
+  a->k_src = static_cast<const uint16_t*>(k_src);
+  a->v_src = static_cast<const uint16_t*>(v_src);
+  a->ks_b = ks_b; a->ks_t = ks_t; a->ks_h = ks_h;
+  a->vs_b = vs_b; a->vs_t = vs_t; a->vs_h = vs_h;
+  a->batch = batch;
+  a->n_tokens = n_tokens;
+  a->start_pos = start_pos;
+  a->page_table = page_table;
+  a->max_pages = max_pages;
+  a->rope_cs = rope_cs;
+  a->rope_max_pos = rope_max_pos;
+  a->layout = layout;
+  return ATF_OK;
+}
+
+// Packed rows: first rows of the sequences [batch + 1] in device memory, total_tokens rows.
+int check_packed(int batch, const int32_t* cu_tokens, int total_tokens) {
+  if (batch > 0 && !cu_tokens) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (total_tokens < 0) return fail(ATF_ERR_INVALID, "total_tokens must be >= 0");
+  return ATF_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -171,36 +213,77 @@ int atf_kv_write_bf16(void* kv_cache, int num_pages, int num_kv_heads, const voi
                       int64_t ks_b, int64_t ks_t, int64_t ks_h, const void* v_src, int64_t vs_b, int64_t vs_t,
                       int64_t vs_h, int batch, int n_tokens, const int32_t* start_pos, const int32_t* page_table,
                       int max_pages, const float* rope_cs, int rope_max_pos, int layout, void* stream) {
-  if (batch < 0 || n_tokens < 0) return fail(ATF_ERR_INVALID, "batch and n_tokens must be >= 0");
-  if (batch == 0 || n_tokens == 0) return ok();
-  if (!kv_cache || !k_src || !v_src || !start_pos || !page_table)
-    return fail(ATF_ERR_INVALID, "null pointer argument");
-  if (num_pages <= 0 || num_kv_heads <= 0 || max_pages <= 0)
-    return fail(ATF_ERR_INVALID, "num_pages, num_kv_heads and max_pages must be positive");
-  if (int r = check_layout(layout, rope_cs, rope_max_pos)) return r;
-  if (!aligned(k_src, 16) || !aligned(v_src, 16) || !aligned(kv_cache, 16))
-    return fail(ATF_ERR_INVALID, "k/v sources and kv_cache must be 16-byte aligned");
-  const int64_t strides[6] = {ks_b, ks_t, ks_h, vs_b, vs_t, vs_h};
-  for (int64_t s : strides)
-    if (s % 8 != 0) return fail(ATF_ERR_INVALID, "source strides must be multiples of 8 elements");
   atf::KvWriteArgs a{};
-  a.kv_cache = static_cast<uint16_t*>(kv_cache);
-  a.num_pages = num_pages;
-  a.hkv = num_kv_heads;
-  a.k_src = static_cast<const uint16_t*>(k_src);
-  a.v_src = static_cast<const uint16_t*>(v_src);
-  a.ks_b = ks_b; a.ks_t = ks_t; a.ks_h = ks_h;
-  a.vs_b = vs_b; a.vs_t = vs_t; a.vs_h = vs_h;
-  a.batch = batch;
-  a.n_tokens = n_tokens;
-  a.start_pos = start_pos;
-  a.page_table = page_table;
-  a.max_pages = max_pages;
-  a.rope_cs = rope_cs;
-  a.rope_max_pos = rope_max_pos;
-  a.layout = layout;
+  if (int r = kv_write_prepare(kv_cache, num_pages, num_kv_heads, k_src, ks_b, ks_t, ks_h, v_src, vs_b, vs_t, vs_h,
+                               batch, n_tokens, start_pos, page_table, max_pages, rope_cs, rope_max_pos, layout, &a))
+    return r;
+  if (batch == 0 || n_tokens == 0) return ok();
   hipError_t e = atf::launch_kv_write(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "kv_write launch");
+  return ok();
+}
+
+int atf_kv_write_packed_bf16(void* kv_cache, int num_pages, int num_kv_heads, const void* k_src, int64_t ks_t,
+                             int64_t ks_h, const void* v_src, int64_t vs_t, int64_t vs_h, int batch,
+                             const int32_t* cu_tokens, int total_tokens, int max_tokens, const int32_t* start_pos,
+                             const int32_t* page_table, int max_pages, const float* rope_cs, int rope_max_pos,
+                             int layout, void* stream) {
+  atf::KvWriteArgs a{};
+  if (int r = kv_write_prepare(kv_cache, num_pages, num_kv_heads, k_src, 0, ks_t, ks_h, v_src, 0, vs_t, vs_h, batch,
+                               max_tokens, start_pos, page_table, max_pages, rope_cs, rope_max_pos, layout, &a))
+    return r;
+  if (int r = check_packed(batch, cu_tokens, total_tokens)) return r;
+  if (batch == 0 || max_tokens == 0 || total_tokens == 0) return ok();
+  a.cu_tokens = cu_tokens;
+  a.total_tokens = total_tokens;
+  hipError_t e = atf::launch_kv_write(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "packed kv_write launch");
+  return ok();
+}
+
+int atf_kv_write_q8(void* kv_cache, int8_t* kv_exps, int num_pages, int num_kv_heads, const void* k_src, int64_t ks_b,
+                    int64_t ks_t, int64_t ks_h, const void* v_src, int64_t vs_b, int64_t vs_t, int64_t vs_h, int batch,
+                    int n_tokens, const int32_t* cu_tokens, int total_tokens, const int32_t* start_pos,
+                    const int32_t* page_table, int max_pages, const float* rope_cs, int rope_max_pos, int layout,
+                    void* stream) {
+  atf::KvWriteArgs a{};
+  if (int r = kv_write_prepare(kv_cache, num_pages, num_kv_heads, k_src, ks_b, ks_t, ks_h, v_src, vs_b, vs_t, vs_h,
+                               batch, n_tokens, start_pos, page_table, max_pages, rope_cs, rope_max_pos, layout, &a))
+    return r;
+  if (cu_tokens) {
+    if (int r = check_packed(batch, cu_tokens, total_tokens)) return r;
+    if (ks_b != 0 || vs_b != 0) return fail(ATF_ERR_INVALID, "packed rows have no batch stride (got %lld and %lld)",
+                                            static_cast<long long>(ks_b), static_cast<long long>(vs_b));
+    if (total_tokens == 0) return ok();
+  }
+  if (batch == 0 || n_tokens == 0) return ok();
+  if (!kv_exps) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (batch > 65535 || num_kv_heads > 65535)
+    return fail(ATF_ERR_UNSUPPORTED, "at most 65535 sequences and kv heads, got %d and %d", batch, num_kv_heads);
+  a.kv_exps = kv_exps;
+  a.cu_tokens = cu_tokens;
+  a.total_tokens = total_tokens;
+  hipError_t e = atf::launch_kv_write_q8(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "8-bit kv_write launch");
+  return ok();
+}
+
+int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const int8_t* kv_exps, int num_pages,
+                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages, void* stream) {
+  if (batch < 0 || n_pages < 0) return fail(ATF_ERR_INVALID, "batch and n_pages must be >= 0");
+  if (batch == 0 || n_pages == 0) return ok();
+  if (!out || !out_table || !kv_cache || !kv_exps || !page_table) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (num_pages <= 0 || num_kv_heads <= 0 || max_pages < n_pages)
+    return fail(ATF_ERR_INVALID, "num_pages and num_kv_heads must be positive, max_pages (%d) at least n_pages (%d)",
+                max_pages, n_pages);
+  if (!aligned(out, 16) || !aligned(kv_cache, 16)) return fail(ATF_ERR_INVALID, "the caches must be 16-byte aligned");
+  if (batch > 65535 || num_kv_heads > 65535 || static_cast<int64_t>(batch) * n_pages > INT32_MAX)
+    return fail(ATF_ERR_UNSUPPORTED, "at most 65535 sequences and kv heads and 2^31 - 1 pages, got %d, %d and %lld", batch,
+                num_kv_heads, static_cast<long long>(batch) * n_pages);
+  const atf::KvExpandArgs a{static_cast<const uint8_t*>(kv_cache), kv_exps, num_pages, num_kv_heads, page_table, batch,
+                            max_pages, n_pages, static_cast<uint16_t*>(out), out_table};
+  hipError_t e = atf::launch_kv_expand_q8(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "8-bit expand launch");
   return ok();
 }
 
@@ -417,6 +500,36 @@ int atf_decode_paged_slices_bf16(void* out, int64_t o_sb, int64_t o_sh, const vo
   return decode_with_workspace(out, o_sb, o_sh, q, q_sb, q_sh, kv_cache, num_pages, page_table, max_pages,
                                seq_lens, batch, num_q_heads, num_kv_heads, max_seq_len, zhi_slice, true, sm_scale,
                                rope_cs, rope_max_pos, layout, workspace, workspace_bytes, stream);
+}
+
+size_t atf_decode_q8_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_seq_len) {
+  return atf_decode_workspace_bytes_even(batch, num_q_heads, num_kv_heads, max_seq_len);
+}
+
+int atf_decode_paged_q8(void* out, int64_t o_sb, int64_t o_sh, const void* q, int64_t q_sb, int64_t q_sh,
+                        const void* kv_cache, const int8_t* kv_exps, int num_pages, const int32_t* page_table,
+                        int max_pages, const int32_t* seq_lens, int batch, int num_q_heads, int num_kv_heads,
+                        int max_seq_len, const int32_t* zhi, int zhi_entries, float sm_scale, const float* rope_cs,
+                        int rope_max_pos, int layout, void* workspace, size_t workspace_bytes, void* stream) {
+  if (batch < 0) return fail(ATF_ERR_INVALID, "batch must be >= 0");
+  if (batch == 0) return ok();
+  if (!kv_exps) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (zhi && zhi_entries != ATF_LEVELS && zhi_entries != ATF_SLICES)
+    return fail(ATF_ERR_INVALID, "window table must have %d or %d entries, got %d", ATF_LEVELS, ATF_SLICES, zhi_entries);
+  if (batch > 65535 || num_kv_heads > 65535 / atf::kDecWaves)
+    return fail(ATF_ERR_UNSUPPORTED, "at most 65535 sequences and %d kv heads, got %d and %d", 65535 / atf::kDecWaves,
+                batch, num_kv_heads);
+  atf::DecodeArgs a{};
+  if (int r = decode_prepare(out, o_sb, o_sh, q, q_sb, q_sh, kv_cache, num_pages, page_table, max_pages, seq_lens, batch,
+                             num_q_heads, num_kv_heads, max_seq_len, zhi, zhi_entries == ATF_SLICES, sm_scale, rope_cs,
+                             rope_max_pos, layout, &a))
+    return r;
+  a.kv_exps = kv_exps;
+  if (!set_spread_workspace(workspace, workspace_bytes, &a))
+    if (int r = set_workspace(workspace, workspace_bytes, &a)) return r;
+  hipError_t e = atf::launch_decode_q8(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "8-bit decode launch");
+  return ok();
 }
 
 int atf_decode_rows_bf16(void* out, int64_t o_sb, int64_t o_sh, const void* q, int64_t q_sb, int64_t q_sh,

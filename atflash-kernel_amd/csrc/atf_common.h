@@ -49,6 +49,21 @@ constexpr int kPage = 16;
 constexpr int kBlockElems = kSlices * kPage * kSliceDims;  // one half: 2048 bf16 = 4096 B
 constexpr int kKvBlockElems = 2 * kBlockElems;            // a (page, kv head) block: 8192 B
 constexpr int kKHalfElems = kBlockElems;                  // offset of the K half in a block
+// The cache of 8-bit floats: one 4 KB block of e4m3 codes per (page, kv head), V half
+// first, and two signed exponents (V's, K's) beside it; a code c of a half with
+// exponent e stands for c 2^e.
+//   V half  [2][4][16][4 dims][4 tokens]: element (j, g, r, d, t) is dim 8r + 4j + d of
+//           token 4g + t;
+//   K half  [8 levels][16 tokens][slices 2l, 2l + 1 of the token, 8 dims each].
+// Either half is two rows of 1 KB of which lane 16g + r (K: 16g + t) of a wave takes 16
+// bytes: MFMA operands without a shuffle.  The exponent is the smallest with the
+// half's largest magnitude at most 448 2^e (448: the largest e4m3 number); with powers
+// of two, code 2^e is a bf16 number exactly and codes move to a larger exponent by a
+// shift (exactly, save those that become subnormal).
+constexpr int kQ8HalfBytes = kBlockElems;
+constexpr int kQ8BlockBytes = 2 * kQ8HalfBytes;
+constexpr int kQ8MinExp = -110;  // 2^-9 2^e, the smallest code, is a normal bf16 number
+constexpr int kQ8MaxExp = 119;   // 448 2^e is finite in bf16
 constexpr int kLayoutHalfSplit = 0;
 constexpr int kLayoutSortedPair = 1;
 

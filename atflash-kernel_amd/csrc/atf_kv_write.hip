@@ -40,7 +40,8 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
   const int h_end = min(a.hkv, h0 + per);
   const int tid = threadIdx.x;
   const int start = a.start_pos[b];
-  const int64_t end64 = static_cast<int64_t>(start) + a.n_tokens;  // exclusive
+  const KvRows rows = kv_rows(a, b);
+  const int64_t end64 = static_cast<int64_t>(start) + rows.count;  // exclusive
   const int first = max(start, 0) >> 4;
   const int pidx = first + static_cast<int>(kHeadsFirst ? blockIdx.y : blockIdx.x);
   const int64_t p0 = static_cast<int64_t>(pidx) * kPage;
@@ -54,7 +55,7 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
   const int pg = a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx];
   if (pg < 0 || pg >= a.num_pages) return;
   const size_t blk0 = static_cast<size_t>(pg) * a.hkv * kKvBlockElems;  // the page's block of head 0
-  const int t0 = static_cast<int>(p0 - start);  // source token of slot 0
+  const int64_t t0 = rows.first + (p0 - start);  // source row of slot 0
 
   // K lane roles and the (cos, sin) of the lane's position and level, loaded once
   const int l = tid >> 4, slot = tid & 15;
@@ -66,7 +67,7 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
 
   // ---- K: the heads' rows loaded first, then rotated and written ----
   if (k_on) {
-    const uint16_t* krow = a.k_src + static_cast<int64_t>(b) * a.ks_b + static_cast<int64_t>(t0 + slot) * a.ks_t;
+    const uint16_t* krow = a.k_src + static_cast<int64_t>(b) * a.ks_b + (t0 + slot) * a.ks_t;
     u32x4 x1[kHeads], x2[kHeads];
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
       const int tok = idx >> 4, ch = idx & 15;
       if (h0 + j < h_end && tok >= s0 && tok < s1) {
         const uint16_t* vrow = a.v_src + static_cast<int64_t>(b) * a.vs_b +
-                               static_cast<int64_t>(t0 + tok) * a.vs_t + static_cast<int64_t>(h0 + j) * a.vs_h;
+                               (t0 + tok) * a.vs_t + static_cast<int64_t>(h0 + j) * a.vs_h;
         *reinterpret_cast<u32x4*>(&sv[j][tok][8 * ch]) = ldg16(vrow + 8 * ch);
       }
     }
@@ -157,9 +158,11 @@ constexpr int kKvAppendTokens = 4;
 __global__ __launch_bounds__(128) void kv_append_kernel(KvWriteArgs a) {
   const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x;
-  const uint16_t* krow = a.k_src + static_cast<int64_t>(b) * a.ks_b + static_cast<int64_t>(t) * a.ks_t +
+  const KvRows rows = kv_rows(a, b);
+  if (t >= rows.count) return;
+  const uint16_t* krow = a.k_src + static_cast<int64_t>(b) * a.ks_b + (rows.first + t) * a.ks_t +
                          static_cast<int64_t>(h) * a.ks_h;
-  const uint16_t* vrow = a.v_src + static_cast<int64_t>(b) * a.vs_b + static_cast<int64_t>(t) * a.vs_t +
+  const uint16_t* vrow = a.v_src + static_cast<int64_t>(b) * a.vs_b + (rows.first + t) * a.vs_t +
                          static_cast<int64_t>(h) * a.vs_h;
   const int l = tid & (kLevels - 1);
   const int c0 = level_chunk0(a.layout, l);

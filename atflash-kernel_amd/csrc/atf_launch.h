@@ -38,7 +38,25 @@ struct KvWriteArgs {
   const float* rope_cs;
   int rope_max_pos;
   int layout;
+  // Packed rows: sequence b's tokens are rows cu_tokens[b] .. cu_tokens[b + 1] - 1 of
+  // k_src and v_src (total_tokens rows), at most n_tokens of them; null: row t of
+  // sequence b lies at b ks_b + t ks_t.
+  const int32_t* cu_tokens;
+  int total_tokens;
+  int8_t* kv_exps;  // the 8-bit cache's exponents [num_pages][hkv][2] (kv_cache: its codes)
 };
+
+// The rows of sequence b in a call: the first, relative to k_src's and v_src's row 0
+// of the sequence (strides ks_b, vs_b), and how many.
+struct KvRows {
+  int64_t first;
+  int count;
+};
+__device__ __forceinline__ KvRows kv_rows(const KvWriteArgs& a, int b) {
+  if (a.cu_tokens == nullptr) return KvRows{0, a.n_tokens};
+  const int lo = max(a.cu_tokens[b], 0), hi = min(a.cu_tokens[b + 1], a.total_tokens);
+  return KvRows{lo, max(0, min(hi - lo, a.n_tokens))};
+}
 
 struct PrefillArgs {
   const uint16_t* q;
@@ -64,7 +82,8 @@ struct DecodeArgs {
   int64_t q_sb, q_sh;
   uint16_t* out;  // [B][Hq][128] (strided)
   int64_t o_sb, o_sh;
-  const uint16_t* kv_cache;  // [num_pages][hkv][V half | K half]
+  const uint16_t* kv_cache;  // [num_pages][hkv][V half | K half]; the 8-bit decode's codes
+  const int8_t* kv_exps;     // 8-bit decode: [num_pages][hkv][2], V's and K's exponent
   int num_pages;
   const int32_t* page_table;
   int max_pages;
@@ -98,6 +117,21 @@ struct DecodeRows {
 };
 
 hipError_t launch_kv_write(const KvWriteArgs& a, hipStream_t s);
+// The writer of the 8-bit cache.
+hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s);
+// Blocks of the 8-bit cache -> blocks of a bf16 cache: entry (b, p), p < n_pages, of the
+// page table to block b n_pages + p of `out`, that number (or -1 for an entry outside
+// the pool, whose block is left as it is) to out_table[b][p].
+struct KvExpandArgs {
+  const uint8_t* codes;
+  const int8_t* exps;
+  int num_pages, hkv;
+  const int32_t* page_table;
+  int batch, max_pages, n_pages;
+  uint16_t* out;
+  int32_t* out_table;
+};
+hipError_t launch_kv_expand_q8(const KvExpandArgs& a, hipStream_t s);
 hipError_t launch_prefill(const PrefillArgs& a, hipStream_t s);
 // The MFMA-ceiling probe of the prefill (measurement only): sink holds
 // ceil(ceil(nq / 256) / 8) * 8 * hq * 512 floats.
@@ -105,6 +139,10 @@ hipError_t launch_prefill_mfma_probe(float* sink, int nq, int hq, hipStream_t s)
 hipError_t launch_prefill_tile_levels(int32_t* out, int n_row_tiles, int n_kblocks, int q_offset,
                                       const LevelTable& lt, hipStream_t s);
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t s);
+// The decode over the 8-bit cache (a.kv_exps).
+hipError_t launch_decode_q8(const DecodeArgs& a, hipStream_t s);
+// The merge of a call's split partials (nothing to do with one split in one workgroup).
+hipError_t launch_decode_merge(const DecodeArgs& a, hipStream_t s);
 // The decode over contiguous rows; every sequence has a.max_seq_len tokens.
 hipError_t launch_decode_rows(const DecodeArgs& a, const DecodeRows& r, hipStream_t s);
 // launch_decode with the workspace pointers taken from the device's fixed

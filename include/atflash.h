@@ -33,6 +33,15 @@
  * may hold any finite value.  A windowed read of a page is one contiguous run:
  * the V half and the in-window prefix of the K half.
  *
+ * Paged cache of 8-bit floats (one layer), the same pages with half the bytes:
+ *   kv_cache  e4m3 codes [num_pages][num_kv_heads][2][2048]: one 4 KB block per
+ *             (page, kv head), 16-byte aligned,
+ *     [0]  V half: [2 j][4 g][16 r][4 d][4 t] = dim 8r + 4j + d of token 4g + t
+ *     [1]  K half: [8 levels][16 tokens][slices 2l, 2l + 1][8 dims]
+ *   kv_exps   int8 [num_pages][num_kv_heads][2]: V's and K's exponent, between
+ *             ATF_Q8_MIN_EXP and ATF_Q8_MAX_EXP; a code c stands for c 2^exponent
+ * written by atf_kv_write_q8.
+ *
  * RoPE.  rope_cs, when not NULL, is fp32 [rope_max_pos][64][2] holding
  * (cos, sin) of position * inv_freq[r] (HF rotate-half convention); NULL means
  * the inputs are already rotated.  Layout ATF_LAYOUT_SORTED_PAIR (the
@@ -60,6 +69,8 @@ extern "C" {
 #define ATF_PREFILL_BLOCK_N 32
 #define ATF_DECODE_BLOCK_N 16
 #define ATF_MAX_GQA_GROUP 16
+#define ATF_Q8_MIN_EXP (-110)
+#define ATF_Q8_MAX_EXP 119
 
 enum {
   ATF_OK = 0,
@@ -96,6 +107,53 @@ int atf_kv_write_bf16(void* kv_cache, int num_pages, int num_kv_heads,
                       int batch, int n_tokens, const int32_t* start_pos,
                       const int32_t* page_table, int max_pages,
                       const float* rope_cs, int rope_max_pos, int layout, void* stream);
+
+/*
+ * atf_kv_write_bf16 for packed rows: sequence b's tokens are rows cu_tokens[b]
+ * to cu_tokens[b + 1] - 1 (device int32 [batch + 1]) of k_src and v_src, which have
+ * total_tokens rows; at most max_tokens of a sequence are written.  Rows outside
+ * [0, total_tokens) are not read.  It has no counterpart in the reference.
+ */
+int atf_kv_write_packed_bf16(void* kv_cache, int num_pages, int num_kv_heads,
+                             const void* k_src, int64_t ks_t, int64_t ks_h,
+                             const void* v_src, int64_t vs_t, int64_t vs_h,
+                             int batch, const int32_t* cu_tokens, int total_tokens, int max_tokens,
+                             const int32_t* start_pos, const int32_t* page_table, int max_pages,
+                             const float* rope_cs, int rope_max_pos, int layout, void* stream);
+
+/*
+ * The writer of the cache of 8-bit floats: rows, positions, RoPE and skips as
+ * atf_kv_write_bf16's (cu_tokens NULL) or atf_kv_write_packed_bf16's (cu_tokens given,
+ * n_tokens the most of a sequence, batch strides 0).  Per page, kv head and half the
+ * exponent is the smallest e with every magnitude at most 448 2^e (between the
+ * limits above), and the codes are the values times 2^-e, rotated in fp32 and
+ * rounded once, to nearest even.
+ *   A call that writes a page's first slot begins the page anew: its exponent is
+ * that of the written tokens.  One that starts inside a page keeps the tokens
+ * before its first: the exponent is at least the page's, and where it grows the
+ * kept codes move to it (exact, save those that become subnormal).  The slots
+ * behind the call's last token in its last page become zero: sequences are
+ * appended to, and what lay behind is forgotten.  Infinities and NaN become the
+ * NaN code and count for no exponent.  Two sequences of a call must not write the
+ * same page.  batch and num_kv_heads are at most 65535.
+ */
+int atf_kv_write_q8(void* kv_cache, int8_t* kv_exps, int num_pages, int num_kv_heads,
+                    const void* k_src, int64_t ks_b, int64_t ks_t, int64_t ks_h,
+                    const void* v_src, int64_t vs_b, int64_t vs_t, int64_t vs_h,
+                    int batch, int n_tokens, const int32_t* cu_tokens, int total_tokens,
+                    const int32_t* start_pos, const int32_t* page_table, int max_pages,
+                    const float* rope_cs, int rope_max_pos, int layout, void* stream);
+
+/*
+ * Pages of the 8-bit cache as bf16 pages, exactly (a code times a power of two is
+ * a bf16 number): entry (b, p), p < n_pages, of the page table (rows of max_pages) to
+ * block b * n_pages + p of out (bf16 [batch * n_pages][num_kv_heads][2][2048]), and
+ * that number to out_table (int32 [batch][n_pages]).  An entry outside
+ * [0, num_pages) gets -1 there and leaves its block as it is.  With out and
+ * out_table atf_prefill_bf16 attends to an 8-bit cache.
+ */
+int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const int8_t* kv_exps, int num_pages,
+                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages, void* stream);
 
 /*
  * Windowed causal GQA prefill: out[b, i, h, :] = attention of query row i
@@ -182,6 +240,22 @@ int atf_decode_paged_slices_bf16(void* out, int64_t o_sb, int64_t o_sh,
                                  const int32_t* zhi_slice, float sm_scale, const float* rope_cs,
                                  int rope_max_pos, int layout, void* workspace, size_t workspace_bytes,
                                  void* stream);
+
+/*
+ * The decode over the cache of 8-bit floats: arguments and window rules as
+ * atf_decode_paged_bf16 (zhi_entries = ATF_LEVELS) or atf_decode_paged_slices_bf16
+ * (ATF_SLICES; ignored where zhi is NULL), the workspace of
+ * atf_decode_q8_workspace_bytes (atf_decode_workspace_bytes is enough, slower for
+ * ragged batches).  Keys and values are the codes times their powers of two,
+ * exactly; Q, P and the sums have atf_decode_paged_bf16's precision.
+ */
+size_t atf_decode_q8_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_seq_len);
+int atf_decode_paged_q8(void* out, int64_t o_sb, int64_t o_sh, const void* q, int64_t q_sb, int64_t q_sh,
+                        const void* kv_cache, const int8_t* kv_exps, int num_pages,
+                        const int32_t* page_table, int max_pages, const int32_t* seq_lens,
+                        int batch, int num_q_heads, int num_kv_heads, int max_seq_len,
+                        const int32_t* zhi, int zhi_entries, float sm_scale, const float* rope_cs, int rope_max_pos,
+                        int layout, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The same decode over contiguous K and V, read in place: k and v are bf16
