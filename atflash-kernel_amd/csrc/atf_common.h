@@ -189,6 +189,17 @@ __device__ __forceinline__ u32x4 pack8(const float* f) {
   return r;
 }
 
+// x1 c - x2 s and x2 c + x1 s of a rotated pair.  Which of the two products is
+// rounded before the sum is written out here: left to the compiler it may differ from
+// one place of inlining to the next, and with it a rounding to bf16 (the 128-row and
+// the 256-row prefill kernel so rotated a query element differently now and then).
+__device__ __forceinline__ float rope_first(float x1, float x2, float c, float s) {
+  return __builtin_fmaf(x1, c, -(x2 * s));
+}
+__device__ __forceinline__ float rope_second(float x1, float x2, float c, float s) {
+  return __builtin_fmaf(x2, c, x1 * s);
+}
+
 // Rotate-half RoPE on one 8-pair chunk: lane keeps the first half
 // (x1 c - x2 s) or the second half (x2 c + x1 s), times `scale`.  cs holds
 // (cos, sin) per pair.
@@ -200,7 +211,7 @@ __device__ __forceinline__ u32x4 rope_half(const u32x4& x1v, const u32x4& x2v, c
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float c = cs[2 * i], s = cs[2 * i + 1];
-    y[i] = scale * (second ? (x2[i] * c + x1[i] * s) : (x1[i] * c - x2[i] * s));
+    y[i] = scale * (second ? rope_second(x1[i], x2[i], c, s) : rope_first(x1[i], x2[i], c, s));
   }
   return pack8(y);
 }
@@ -214,8 +225,8 @@ __device__ __forceinline__ u32x4 rope_slice(const u32x4& x, const float* cs, flo
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float c = cs[2 * i], s = cs[2 * i + 1];
-    y[i] = scale * (v[i] * c - v[4 + i] * s);
-    y[4 + i] = scale * (v[4 + i] * c + v[i] * s);
+    y[i] = scale * rope_first(v[i], v[4 + i], c, s);
+    y[4 + i] = scale * rope_second(v[i], v[4 + i], c, s);
   }
   return pack8(y);
 }
