@@ -55,6 +55,12 @@ SIGNATURES = {
     "atf_kv_expand_q8": (_i, [_p, _p, _p, _p, _i, _i, _p, _i, _i, _i, _p]),
     "atf_prefill_bf16": (_i, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i, _p, _i,
                               _i, _i, _i, _i, _i, _i, _p, _f, _p, _i, _i, _p]),
+    "atf_prefill_plan_bytes": (_sz, [_i, _i, _i]),
+    "atf_prefill_plan": (_i, [_p, _sz, _p, _p, _i, _i, _i, _i, _p, _i, _p, _p]),
+    "atf_prefill_packed_bf16": (_i, [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i,
+                                     _p, _f, _p, _i, _i, _p, _sz, _p]),
+    "atf_extend_tables": (_i, [_p, _i, _p, _p, _p, _i, _p, _i, _i, _i, _p, _p, _p, _p, _p, _p]),
+    "atf_release_tables": (_i, [_p, _i, _p, _p, _i, _p, _p, _i, _i, _i, _p]),
     "atf_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "atf_decode_workspace_bytes_even": (_sz, [_i, _i, _i, _i]),
     "atf_decode_paged_bf16": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i, _p, _i, _p,

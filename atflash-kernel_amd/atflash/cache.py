@@ -67,6 +67,48 @@ def v_half(kv: torch.Tensor) -> torch.Tensor:
     return kv[:, :, _lib.V_HALF].unflatten(-1, _lib.V_BLOCK_SHAPE)
 
 
+class PageTables:
+    """Page tables of up to `batch` sequences over a pool, kept and changed on the GPU:
+    what PagedKVCache's lists are for a host that knows every length.  All layers of a
+    model that grow together share one.
+
+        page_table int32 [batch, max_pages]   -1 where a row has no page
+        seq_lens   int32 [batch]              tokens of each sequence
+        free_pages int32 [num_pages], free_count int32 [1]
+
+    The tensors keep their addresses, so that captured steps and prepared decode plans
+    go on reading them."""
+
+    def __init__(self, num_pages: int, batch: int, max_pages: int, device="cuda"):
+        self.num_pages = int(num_pages)
+        self.device = torch.device(device)
+        i32 = dict(dtype=torch.int32, device=self.device)
+        self.page_table = torch.full((int(batch), int(max_pages)), -1, **i32)
+        self.seq_lens = torch.zeros(int(batch), **i32)
+        self.free_pages = torch.arange(self.num_pages - 1, -1, -1, **i32)  # page 0 is taken first
+        self.free_count = torch.full((1,), self.num_pages, **i32)
+
+    def extend(self, new_lens: torch.Tensor, total_tokens: int):
+        """Room for new_lens[b] (int32 [batch] on the GPU) more tokens of each sequence,
+        total_tokens in all.  Returns (start_pos [batch], cu_seqlens [batch + 1], positions
+        [total_tokens], slots [total_tokens]): what the cache writer and the packed
+        prefill take.  Where the pool is short of pages, free_count becomes negative and
+        the entries, and the slots of the tokens without a page, are -1 (writers skip
+        those)."""
+        from . import ops
+        lens, left, cu, pos, slots = ops.extend_tables(self.page_table, self.seq_lens, new_lens, self.free_pages,
+                                                       self.free_count, total_tokens, self.num_pages)
+        start = self.seq_lens.clone()
+        self.seq_lens.copy_(lens)
+        self.free_count.copy_(left)
+        return start, cu, pos, slots
+
+    def release(self, rows: torch.Tensor):
+        """Give back the pages of the finished sequences `rows` (int32 on the GPU)."""
+        from . import ops
+        ops.release_tables(self.page_table, self.seq_lens, self.free_pages, self.free_count, rows, self.num_pages)
+
+
 class PagedKVCache:
     """One layer's pool of pages and the sequences that own them.  kv_dtype:
     torch.bfloat16, or torch.float8_e4m3fn for the cache of 8-bit floats (`exps` then

@@ -97,6 +97,17 @@ def _flash_attn_fwd(q, k, v, causal=True, pack_gqa=None, atflash_window_zhi=None
                        _layout_id(layout))
 
 
+def flash_attn_packed(q, k, v, cu_seqlens, max_seqlen, zhi=None, softmax_scale=None, rope=None, layout="half_split"):
+    """Causal attention of whole prompts packed one after the other: q [T, Hq, 128], k, v
+    [T, Hkv, 128], sequence b's rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 on the
+    GPU), at most max_seqlen of each.  Returns (out [T, Hq, 128] bf16, lse [Hq, T] fp32),
+    each sequence's the bits of a `_flash_attn_fwd` call of its own."""
+    if q.dim() != 3 or k.dim() != 3 or q.shape[1] % k.shape[1] != 0:
+        raise ValueError("q, k, v must be [T, heads, 128], num q heads a multiple of num kv heads")
+    scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
+    return ops.flash_attn_packed(q, k, v, cu_seqlens, int(max_seqlen), _zhi_list(zhi), scale, rope, _layout_id(layout))
+
+
 def single_decode_with_kv_cache(q, k, v, maybe_zhi=None, sm_scale=None, kv_layout="NHD", rope=None,
                                 layout="half_split"):
     """One query token per q head against a contiguous KV, read in place.
@@ -132,6 +143,27 @@ def prefill_paged(q, cache, page_table, nk, q_offset, zhi=None, sm_scale=None, r
                               _layout_id(layout))
     return ops.prefill(q, cache.kv, page_table, int(nk), int(q_offset), _zhi_list(zhi), scale, rope,
                        _layout_id(layout))
+
+
+def prefill_packed(q, cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi=None, sm_scale=None, rope=None,
+                   layout="half_split", plan=None, out=None, lse=None):
+    """Windowed causal prefill of packed rows against a PagedKVCache (ops.prefill_packed;
+    `plan`: packed_plan of these lengths, shared by the layers of a step).  A cache of
+    8-bit floats is expanded into temporary bf16 pages first, as by prefill_paged."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
+    kv = cache.kv
+    if getattr(cache, "exps", None) is not None:
+        pages = -(-int(max_seq_len) // PAGE)
+        if page_table.dim() != 2 or page_table.shape[1] < pages:
+            raise ValueError(f"page table too small for max_seq_len={max_seq_len}")
+        kv, page_table = ops.kv_expand_q8(kv, cache.exps, page_table, pages)
+    return ops.prefill_packed(q, kv, page_table, cu_seqlens, seq_lens, int(max_seq_len), _zhi_list(zhi), scale, rope,
+                              _layout_id(layout), plan, out, lse)
+
+
+def packed_plan(cu_seqlens, seq_lens, total_q, max_seq_len, num_q_heads):
+    """ops.PackedPlan: the query tiles of packed rows, listed once for all layers of a step."""
+    return ops.PackedPlan(cu_seqlens, seq_lens, total_q, max_seq_len, num_q_heads)
 
 
 def decode_paged(q, cache, page_table, seq_lens, max_seq_len, zhi=None, sm_scale=None, rope=None,

@@ -22,6 +22,14 @@ the bf16 cache):
 
     torch.ops.atflash.kv_write_packed(kv_cache, kv_exps, k, v, cu_seqlens, max_tokens, start_pos,
                                       page_table, rope_cs, layout)
+    torch.ops.atflash.prefill_packed(q, kv_cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi,
+                                     sm_scale, rope_cs, layout) -> (out, lse)
+
+and the tables of such a step, from lengths that the GPU holds:
+
+    torch.ops.atflash.extend_tables(page_table, seq_lens, new_lens, free_pages, free_count, total_tokens,
+                                    num_pages) -> (seq_lens, free_left, cu_seqlens, positions, slots)
+    torch.ops.atflash.release_tables(page_table, seq_lens, free_pages, free_count, rows, num_pages)
 
 Each op checks shapes and dtypes, then calls the HIP library on the current
 stream of the tensors' device.  There is no CPU or PyTorch fallback: a CPU
@@ -307,6 +315,194 @@ _prefill_q8_op = torch.library.custom_op("atflash::prefill_q8", prefill_q8, muta
 def _(q, kv_cache, kv_exps, page_table, nk, q_offset, zhi, sm_scale, rope_cs, layout):
     B, Nq, Hq, D = q.shape
     return q.new_empty((B, Nq, Hq, D)), q.new_empty((B, Hq, Nq), dtype=torch.float32)
+
+
+# ---- packed queries ----
+
+class PackedPlan:
+    """The query tiles of packed rows, listed once on the GPU for a step's lengths and
+    used by every layer's prefill_packed.  cu_seqlens [B + 1] and seq_lens [B] (None: as
+    many keys as queries) are device tensors; total_q the rows of q; max_seq_len the
+    most keys of a sequence.  The list is made by the constructor and by refresh(),
+    which takes the lengths as they are then (in a captured graph: call refresh inside)."""
+
+    def __init__(self, cu_seqlens, seq_lens, total_q, max_seq_len, num_q_heads, listed=True):
+        self.device = _one_device(cu_seqlens, seq_lens)
+        self.batch = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
+        _need(self.batch >= 0, "cu_seqlens must be contiguous int32 [B + 1]")
+        _check_ints(cu_seqlens, self.batch + 1, "cu_seqlens")
+        if seq_lens is not None:
+            _check_ints(seq_lens, self.batch, "seq_lens")
+        self.cu_seqlens, self.seq_lens = cu_seqlens, seq_lens
+        self.total_q, self.max_seq_len, self.num_q_heads = int(total_q), int(max_seq_len), int(num_q_heads)
+        nbytes = int(_lib.lib().atf_prefill_plan_bytes(self.batch, self.total_q, self.num_q_heads))
+        self.tiles = torch.empty(max(nbytes, 8) // 4, dtype=torch.int32, device=self.device)
+        if listed:
+            self.refresh()
+
+    def refresh(self, page_table=None, start_pos=None):
+        """List the tiles; with page_table [B, max_pages] and start_pos [B] (int32), also
+        lay out pages for rows that are to be written (page p of sequence b is
+        cu_seqlens[b] / 16 + b + p) and starts of 0."""
+        width = 0 if page_table is None else page_table.shape[1]
+        _lib.launch(self.device, _lib.lib().atf_prefill_plan, self.tiles.data_ptr(), self.tiles.numel() * 4,
+                    self.cu_seqlens.data_ptr(), _lib.ptr(self.seq_lens), self.batch, self.total_q, self.max_seq_len,
+                    self.num_q_heads, _lib.ptr(page_table), width, _lib.ptr(start_pos))
+
+
+def _prefill_packed(q, kv_cache, page_table, plan, zhi, sm_scale, rope_cs, layout, out, lse):
+    """prefill_packed's launch with its plan made and its arguments other than q, out and lse checked."""
+    _need(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[2] == _lib.HEAD_DIM, "q must be bf16 [T, Hq, 128]")
+    _need(q.stride(2) == 1, "last dim of q must be contiguous")
+    T, Hq, D = q.shape
+    _need(plan.total_q == T and plan.num_q_heads == Hq and plan.device == q.device,
+          f"the plan is for {plan.total_q} rows of {plan.num_q_heads} heads on {plan.device}")
+    dev = _one_device(q, kv_cache, page_table, rope_cs, out, lse)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+    if lse is None:
+        lse = torch.empty((Hq, T), dtype=torch.float32, device=dev)
+    _need(out.dtype == torch.bfloat16 and out.shape == q.shape and out.stride(2) == 1, "out must be bf16 [T, Hq, 128]")
+    _need(lse.dtype == torch.float32 and lse.shape == (Hq, T) and lse.is_contiguous(), "lse must be contiguous fp32 [Hq, T]")
+    rope_cs, max_pos = _rope(rope_cs)
+    pool = kv_cache.shape
+    _lib.launch(dev, _lib.lib().atf_prefill_packed_bf16, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+                q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), pool[0], page_table.data_ptr(),
+                page_table.shape[1], plan.cu_seqlens.data_ptr(), _lib.ptr(plan.seq_lens), plan.batch, T,
+                plan.max_seq_len, Hq, pool[1], _lib.zhi_array(zhi), float(sm_scale), _lib.ptr(rope_cs), max_pos,
+                _layout(layout), plan.tiles.data_ptr(), plan.tiles.numel() * 4)
+    return out, lse
+
+
+def prefill_packed(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                   seq_lens: Optional[torch.Tensor], max_seq_len: int, zhi: Optional[List[int]], sm_scale: float,
+                   rope_cs: Optional[torch.Tensor], layout: int, plan: Optional[PackedPlan] = None,
+                   out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Windowed causal GQA prefill of packed rows q [T, Hq, 128]: sequence b's queries
+    are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1, the last of its seq_lens[b] cached
+    keys (None: as many as queries), at most max_seq_len.  Returns (out bf16 [T, Hq,
+    128], lse fp32 [Hq, T]); rows outside every sequence are not written.  plan: a
+    PackedPlan of these lengths."""
+    _one_device(q, kv_cache, page_table, cu_seqlens, seq_lens, rope_cs)
+    _check_cache(kv_cache)
+    if plan is None:
+        _need(q.dim() == 3, "q must be bf16 [T, Hq, 128]")
+        plan = PackedPlan(cu_seqlens, seq_lens, q.shape[0], max_seq_len, q.shape[1])
+    else:
+        same = (plan.cu_seqlens.data_ptr() == cu_seqlens.data_ptr() and plan.max_seq_len == int(max_seq_len)
+                and _lib.ptr(plan.seq_lens) == _lib.ptr(seq_lens) and plan.batch == cu_seqlens.shape[0] - 1)
+        _need(same, "the plan was made for other lengths")
+    _check_table(page_table, plan.batch)
+    return _prefill_packed(q, kv_cache, page_table, plan, zhi, sm_scale, rope_cs, layout, out, lse)
+
+
+def _prefill_packed_schema(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor,
+                           cu_seqlens: torch.Tensor, seq_lens: Optional[torch.Tensor], max_seq_len: int,
+                           zhi: Optional[List[int]], sm_scale: float, rope_cs: Optional[torch.Tensor],
+                           layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return prefill_packed(q, kv_cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi, sm_scale, rope_cs, layout)
+
+
+_prefill_packed_op = torch.library.custom_op("atflash::prefill_packed", _prefill_packed_schema, mutates_args=())
+
+
+@_prefill_packed_op.register_fake
+def _(q, kv_cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi, sm_scale, rope_cs, layout):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+
+
+def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int,
+                      zhi, sm_scale: float, rope_cs: Optional[torch.Tensor],
+                      layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """prefill_packed of whole prompts whose keys and values are packed rows too
+    (k, v [T, Hkv, 128]): they are written to temporary pages first."""
+    dev = _one_device(q, k, v, cu_seqlens, rope_cs)
+    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0], "q, k and v must have the same rows [T, heads, 128]")
+    _check_rows(k, v, 3, k.shape[1])
+    T, hkv, _ = k.shape
+    plan = PackedPlan(cu_seqlens, None, T, max_seqlen, q.shape[1], listed=False)  # (with the page table, below)
+    B = plan.batch
+    width = -(-int(max_seqlen) // _lib.PAGE_SIZE)
+    ints = torch.empty((B, width + 1), dtype=torch.int32, device=dev).view(-1)
+    table, start = ints[:B * width].view(B, width), ints[B * width:]
+    kv = torch.empty((T // _lib.PAGE_SIZE + B, hkv, *_lib.KV_BLOCK_SHAPE), dtype=torch.bfloat16, device=dev)
+    plan.refresh(table, start)
+    kv_write_packed(kv, None, k, v, cu_seqlens, max_seqlen, start, table, rope_cs, layout)
+    return _prefill_packed(q, kv, table, plan, zhi, sm_scale, rope_cs, layout, None, None)
+
+
+# ---- tables on the GPU ----
+
+def extend_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, total_tokens: int, num_pages: int
+                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages for new_lens[b] more tokens of each sequence, taken from the end of
+    free_pages[:free_count] and entered into page_table [B, max_pages] in place.
+    Returns (lengths afterwards [B], free pages left [1], cu_seqlens [B + 1], positions
+    int32 [total_tokens], slots int64 [total_tokens]); see atf_extend_tables in
+    include/atflash.h.  The lengths and the free count are only read."""
+    dev = _one_device(page_table, seq_lens, new_lens, free_pages, free_count)
+    B = page_table.shape[0] if page_table.dim() == 2 else -1
+    _check_table(page_table, B)
+    _check_ints(seq_lens, B, "seq_lens")
+    _check_ints(new_lens, B, "new_lens")
+    _check_ints(free_count, 1, "free_count")
+    _check_ints(free_pages, free_pages.numel(), "free_pages")
+    T = int(total_tokens)
+    _need(T >= 0, "total_tokens must be >= 0")
+    # one allocation: slots first (8-byte aligned)
+    buf = torch.empty(3 * T + 2 * B + 2, dtype=torch.int32, device=dev)
+    slots, pos = buf[:2 * T].view(torch.int64), buf[2 * T:3 * T]
+    lens, left, cu = buf[3 * T:3 * T + B], buf[3 * T + B:3 * T + B + 1], buf[3 * T + B + 1:]
+    _lib.launch(dev, _lib.lib().atf_extend_tables, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),
+                new_lens.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), B, T,
+                int(num_pages), lens.data_ptr(), left.data_ptr(), cu.data_ptr(), pos.data_ptr(), slots.data_ptr())
+    return lens, left, cu, pos, slots
+
+
+def _extend_tables_schema(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
+                          free_pages: torch.Tensor, free_count: torch.Tensor, total_tokens: int, num_pages: int
+                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    # (an operator's outputs may not share storage)
+    return tuple(x.clone() for x in extend_tables(page_table, seq_lens, new_lens, free_pages, free_count, total_tokens,
+                                                  num_pages))
+
+
+_extend_tables_op = torch.library.custom_op("atflash::extend_tables", _extend_tables_schema,
+                                            mutates_args=("page_table",))
+
+
+@_extend_tables_op.register_fake
+def _(page_table, seq_lens, new_lens, free_pages, free_count, total_tokens, num_pages):
+    B = page_table.shape[0]
+    return (seq_lens.new_empty(B), seq_lens.new_empty(1), seq_lens.new_empty(B + 1), seq_lens.new_empty(total_tokens),
+            seq_lens.new_empty(total_tokens, dtype=torch.int64))
+
+
+def release_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
+                   free_count: torch.Tensor, rows: torch.Tensor, num_pages: int) -> None:
+    """The pages of the sequences `rows` (int32) back to the end of the free pages, in
+    place: their table rows become -1, their lengths 0, free_count grows."""
+    dev = _one_device(page_table, seq_lens, free_pages, free_count, rows)
+    B = page_table.shape[0] if page_table.dim() == 2 else -1
+    _check_table(page_table, B)
+    _check_ints(seq_lens, B, "seq_lens")
+    _check_ints(free_count, 1, "free_count")
+    _check_ints(free_pages, free_pages.numel(), "free_pages")
+    _check_ints(rows, rows.numel(), "rows")
+    _lib.launch(dev, _lib.lib().atf_release_tables, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),
+                free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), rows.data_ptr(), rows.shape[0], B,
+                int(num_pages))
+
+
+_release_tables_op = torch.library.custom_op("atflash::release_tables", release_tables,
+                                             mutates_args=("page_table", "seq_lens", "free_pages", "free_count"))
+
+
+@_release_tables_op.register_fake
+def _(page_table, seq_lens, free_pages, free_count, rows, num_pages):
+    return None
 
 
 # Decode workspaces, one per (device, stream), grown on demand.  A workspace

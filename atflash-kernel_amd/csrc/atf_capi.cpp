@@ -194,6 +194,63 @@ int kv_write_prepare(void* kv_cache, int num_pages, int num_kv_heads, const void
   return ATF_OK;
 }
 
+// Validation and argument packing shared by the prefill entry points: nk keys of a
+// sequence at most, queries at positions below `positions`.
+int prefill_prepare(void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float* lse, const void* q, int64_t q_sb,
+                    int64_t q_st, int64_t q_sh, const void* kv_cache, int num_pages, const int32_t* page_table,
+                    int max_pages, int batch, int nk, int positions, int num_q_heads, int num_kv_heads,
+                    const int32_t* zhi, float sm_scale, const float* rope_cs, int rope_max_pos, int layout,
+                    atf::PrefillArgs* a) {
+  if (!out || !q || !kv_cache || !page_table) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0)
+    return fail(ATF_ERR_INVALID, "num_q_heads (%d) must be a positive multiple of num_kv_heads (%d)", num_q_heads,
+                num_kv_heads);
+  if (nk >= (1 << 24)) return fail(ATF_ERR_UNSUPPORTED, "nk must be < 2^24");
+  if (num_pages <= 0 || max_pages <= 0 || static_cast<int64_t>(max_pages) * atf::kPage < nk)
+    return fail(ATF_ERR_INVALID, "page table too small for nk=%d (max_pages=%d)", nk, max_pages);
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return fail(ATF_ERR_INVALID, "sm_scale must be positive");
+  if (int r = check_layout(layout, rope_cs, rope_max_pos)) return r;
+  if (rope_cs && positions > rope_max_pos)
+    return fail(ATF_ERR_INVALID, "rope table has %d positions, need %d", rope_max_pos, positions);
+  if (!aligned(q, 16) || !aligned(out, 8) || !aligned(kv_cache, 16))
+    return fail(ATF_ERR_INVALID, "q and kv_cache must be 16-byte and out 8-byte aligned");
+  if (q_sb % 8 || q_st % 8 || q_sh % 8) return fail(ATF_ERR_INVALID, "q strides must be multiples of 8 elements");
+  if (o_sb % 4 || o_st % 4 || o_sh % 4) return fail(ATF_ERR_INVALID, "out strides must be multiples of 4 elements");
+  if (int r = make_table(zhi, &a->lt, static_cast<int64_t>(nk) - 1)) return r;
+  a->q = static_cast<const uint16_t*>(q);
+  a->q_sb = q_sb; a->q_st = q_st; a->q_sh = q_sh;
+  a->out = static_cast<uint16_t*>(out);
+  a->o_sb = o_sb; a->o_st = o_st; a->o_sh = o_sh;
+  a->lse = lse;
+  a->kv_cache = static_cast<const uint16_t*>(kv_cache);
+  a->num_pages = num_pages;
+  a->page_table = page_table;
+  a->max_pages = max_pages;
+  a->batch = batch;
+  a->nk = nk;
+  a->hq = num_q_heads;
+  a->hkv = num_kv_heads;
+  a->group = num_q_heads / num_kv_heads;
+  a->sm_scale = sm_scale;
+  a->scale_log2 = sm_scale * 1.4426950408889634f;
+  a->rope_cs = rope_cs;
+  a->layout = layout;
+  return ATF_OK;
+}
+
+// The tile list of packed queries.
+int check_plan(const void* plan, size_t plan_bytes, const int32_t* cu_seqlens, int batch, int total_q, int max_seq_len,
+               int num_q_heads) {
+  if (!cu_seqlens) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (num_q_heads <= 0 || max_seq_len <= 0)
+    return fail(ATF_ERR_INVALID, "num_q_heads and max_seq_len must be positive");
+  if (max_seq_len >= (1 << 24)) return fail(ATF_ERR_UNSUPPORTED, "max_seq_len must be < 2^24");
+  const size_t need = atf::prefill_plan_bytes(batch, total_q, num_q_heads);
+  if (!plan || plan_bytes < need || !aligned(plan, 8))
+    return fail(ATF_ERR_WORKSPACE, "plan of %zu bytes (8-byte aligned) required, got %zu", need, plan ? plan_bytes : 0);
+  return ATF_OK;
+}
+
 // Packed rows: first rows of the sequences [batch + 1] in device memory, total_tokens rows.
 int check_packed(int batch, const int32_t* cu_tokens, int total_tokens) {
   if (batch > 0 && !cu_tokens) return fail(ATF_ERR_INVALID, "null pointer argument");
@@ -294,48 +351,99 @@ int atf_prefill_bf16(void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float*
                      const float* rope_cs, int rope_max_pos, int layout, void* stream) {
   if (batch < 0 || nq < 0) return fail(ATF_ERR_INVALID, "batch and nq must be >= 0");
   if (batch == 0 || nq == 0) return ok();
-  if (!out || !q || !kv_cache || !page_table) return fail(ATF_ERR_INVALID, "null pointer argument");
-  if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0)
-    return fail(ATF_ERR_INVALID, "num_q_heads (%d) must be a positive multiple of num_kv_heads (%d)", num_q_heads,
-                num_kv_heads);
   if (q_offset < 0 || nk < q_offset + nq)
     return fail(ATF_ERR_INVALID, "need 0 <= q_offset and q_offset + nq <= nk (q_offset=%d nq=%d nk=%d)", q_offset,
                 nq, nk);
-  if (nk >= (1 << 24)) return fail(ATF_ERR_UNSUPPORTED, "nk must be < 2^24");
-  if (num_pages <= 0 || max_pages <= 0 || static_cast<int64_t>(max_pages) * atf::kPage < nk)
-    return fail(ATF_ERR_INVALID, "page table too small for nk=%d (max_pages=%d)", nk, max_pages);
-  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return fail(ATF_ERR_INVALID, "sm_scale must be positive");
-  if (int r = check_layout(layout, rope_cs, rope_max_pos)) return r;
-  if (rope_cs && q_offset + nq > rope_max_pos)
-    return fail(ATF_ERR_INVALID, "rope table has %d positions, need %d", rope_max_pos, q_offset + nq);
-  if (!aligned(q, 16) || !aligned(out, 8) || !aligned(kv_cache, 16))
-    return fail(ATF_ERR_INVALID, "q and kv_cache must be 16-byte and out 8-byte aligned");
-  if (q_sb % 8 || q_st % 8 || q_sh % 8) return fail(ATF_ERR_INVALID, "q strides must be multiples of 8 elements");
-  if (o_sb % 4 || o_st % 4 || o_sh % 4) return fail(ATF_ERR_INVALID, "out strides must be multiples of 4 elements");
   atf::PrefillArgs a{};
-  if (int r = make_table(zhi, &a.lt, static_cast<int64_t>(nk) - 1)) return r;
-  a.q = static_cast<const uint16_t*>(q);
-  a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
-  a.out = static_cast<uint16_t*>(out);
-  a.o_sb = o_sb; a.o_st = o_st; a.o_sh = o_sh;
-  a.lse = lse;
-  a.kv_cache = static_cast<const uint16_t*>(kv_cache);
-  a.num_pages = num_pages;
-  a.page_table = page_table;
-  a.max_pages = max_pages;
-  a.batch = batch;
+  if (int r = prefill_prepare(out, o_sb, o_st, o_sh, lse, q, q_sb, q_st, q_sh, kv_cache, num_pages, page_table, max_pages,
+                              batch, nk, q_offset + nq, num_q_heads, num_kv_heads, zhi, sm_scale, rope_cs, rope_max_pos,
+                              layout, &a))
+    return r;
   a.nq = nq;
-  a.nk = nk;
   a.q_offset = q_offset;
-  a.hq = num_q_heads;
-  a.hkv = num_kv_heads;
-  a.group = num_q_heads / num_kv_heads;
-  a.sm_scale = sm_scale;
-  a.scale_log2 = sm_scale * 1.4426950408889634f;
-  a.rope_cs = rope_cs;
-  a.layout = layout;
   hipError_t e = atf::launch_prefill(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "prefill launch");
+  return ok();
+}
+
+size_t atf_prefill_plan_bytes(int batch, int total_q, int num_q_heads) {
+  if (batch <= 0 || total_q <= 0 || num_q_heads <= 0) return 0;
+  return atf::prefill_plan_bytes(batch, total_q, num_q_heads);
+}
+
+int atf_prefill_plan(void* plan, size_t plan_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens, int batch,
+                     int total_q, int max_seq_len, int num_q_heads, int32_t* page_table, int max_pages,
+                     int32_t* start_pos, void* stream) {
+  if (batch < 0 || total_q < 0) return fail(ATF_ERR_INVALID, "batch and total_q must be >= 0");
+  if (batch == 0 || total_q == 0) return ok();
+  if (int r = check_plan(plan, plan_bytes, cu_seqlens, batch, total_q, max_seq_len, num_q_heads)) return r;
+  if ((page_table == nullptr) != (start_pos == nullptr))
+    return fail(ATF_ERR_INVALID, "page_table and start_pos are laid out together");
+  if (page_table && static_cast<int64_t>(max_pages) * atf::kPage < max_seq_len)
+    return fail(ATF_ERR_INVALID, "page table too small for max_seq_len=%d (max_pages=%d)", max_seq_len, max_pages);
+  atf::PrefillArgs a{};
+  a.batch = batch;
+  a.hq = num_q_heads;
+  a.max_pages = max_pages;
+  a.pk.cu = cu_seqlens;
+  a.pk.seq_lens = seq_lens;
+  a.pk.total_q = total_q;
+  a.pk.max_k = max_seq_len;
+  hipError_t e = atf::launch_prefill_plan(a, static_cast<int32_t*>(plan), page_table, start_pos,
+                                          static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "prefill plan launch");
+  return ok();
+}
+
+int atf_prefill_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse, const void* q, int64_t q_st,
+                            int64_t q_sh, const void* kv_cache, int num_pages, const int32_t* page_table, int max_pages,
+                            const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int total_q, int max_seq_len,
+                            int num_q_heads, int num_kv_heads, const int32_t* zhi, float sm_scale, const float* rope_cs,
+                            int rope_max_pos, int layout, const void* plan, size_t plan_bytes, void* stream) {
+  if (batch < 0 || total_q < 0) return fail(ATF_ERR_INVALID, "batch and total_q must be >= 0");
+  if (batch == 0 || total_q == 0) return ok();
+  if (int r = check_plan(plan, plan_bytes, cu_seqlens, batch, total_q, max_seq_len, num_q_heads)) return r;
+  atf::PrefillArgs a{};
+  if (int r = prefill_prepare(out, 0, o_st, o_sh, lse, q, 0, q_st, q_sh, kv_cache, num_pages, page_table, max_pages, batch,
+                              max_seq_len, max_seq_len, num_q_heads, num_kv_heads, zhi, sm_scale, rope_cs, rope_max_pos,
+                              layout, &a))
+    return r;
+  a.pk = atf::PackedRows{cu_seqlens, seq_lens, total_q, max_seq_len, static_cast<const int32_t*>(plan)};
+  hipError_t e = atf::launch_prefill_packed(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "packed prefill launch");
+  return ok();
+}
+
+int atf_extend_tables(int32_t* page_table, int max_pages, const int32_t* seq_lens, const int32_t* new_lens,
+                      const int32_t* free_pages, int num_free, const int32_t* free_count, int batch, int total_tokens,
+                      int num_pages, int32_t* seq_lens_out, int32_t* free_left, int32_t* cu_seqlens, int32_t* positions,
+                      int64_t* slots, void* stream) {
+  if (batch <= 0 || total_tokens < 0 || max_pages <= 0 || num_free < 0 || num_pages <= 0)
+    return fail(ATF_ERR_INVALID, "batch, max_pages and num_pages must be positive, total_tokens and num_free >= 0");
+  if (!page_table || !seq_lens || !new_lens || (num_free > 0 && !free_pages) || !free_count || !seq_lens_out ||
+      !free_left || !cu_seqlens || (total_tokens > 0 && (!positions || !slots)))
+    return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (!aligned(slots, 8)) return fail(ATF_ERR_INVALID, "slots must be 8-byte aligned");
+  if (batch > atf::kTabMaxBatch)
+    return fail(ATF_ERR_UNSUPPORTED, "at most %d sequences, got %d", atf::kTabMaxBatch, batch);
+  const atf::ExtendTablesArgs a{page_table, max_pages, seq_lens,  new_lens,  free_pages, num_free,  free_count, batch,
+                                total_tokens, num_pages, seq_lens_out, free_left, cu_seqlens, positions, slots};
+  hipError_t e = atf::launch_extend_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "table extension launch");
+  return ok();
+}
+
+int atf_release_tables(int32_t* page_table, int max_pages, int32_t* seq_lens, int32_t* free_pages, int num_free,
+                       int32_t* free_count, const int32_t* rows, int n_rows, int batch, int num_pages, void* stream) {
+  if (batch <= 0 || n_rows < 0 || max_pages <= 0 || num_free < 0 || num_pages <= 0)
+    return fail(ATF_ERR_INVALID, "batch, max_pages and num_pages must be positive, n_rows and num_free >= 0");
+  if (n_rows == 0) return ok();
+  if (!page_table || !seq_lens || (num_free > 0 && !free_pages) || !free_count || !rows)
+    return fail(ATF_ERR_INVALID, "null pointer argument");
+  const atf::ReleaseTablesArgs a{page_table, max_pages, seq_lens, free_pages, num_free, free_count, rows, n_rows, batch,
+                                 num_pages};
+  hipError_t e = atf::launch_release_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "table release launch");
   return ok();
 }
 

@@ -58,6 +58,15 @@ __device__ __forceinline__ KvRows kv_rows(const KvWriteArgs& a, int b) {
   return KvRows{lo, max(0, min(hi - lo, a.n_tokens))};
 }
 
+// Queries of several sequences packed one after the other.
+struct PackedRows {
+  const int32_t* cu;        // [batch + 1] first rows
+  const int32_t* seq_lens;  // [batch] keys, the sequence's queries the last of them; null: as many as queries
+  int total_q;              // rows of q, out and lse
+  int max_k;                // keys of a sequence at most
+  const int32_t* tiles;     // launch_prefill_plan's list
+};
+
 struct PrefillArgs {
   const uint16_t* q;
   int64_t q_sb, q_st, q_sh;
@@ -75,6 +84,7 @@ struct PrefillArgs {
   const float* rope_cs;
   int layout;
   LevelTable lt;
+  PackedRows pk;  // prefill_packed kernels (nq, nk, q_offset, q_sb and o_sb unused there)
 };
 
 struct DecodeArgs {
@@ -116,6 +126,36 @@ struct DecodeRows {
   int64_t ks_b, ks_t, ks_h, vs_b, vs_t, vs_h;
 };
 
+// Block tables and slot maps of a step's new tokens (atf_extend_tables).
+constexpr int kTabMaxBatch = 8191;  // sequences: two prefix sums in 64 KB of LDS
+struct ExtendTablesArgs {
+  int32_t* page_table;
+  int max_pages;
+  const int32_t* seq_lens;
+  const int32_t* new_lens;
+  const int32_t* free_pages;
+  int num_free;
+  const int32_t* free_count;
+  int batch, total, num_pages;
+  int32_t* lens_out;
+  int32_t* free_left;
+  int32_t* cu_out;
+  int32_t* positions;
+  int64_t* slots;
+};
+hipError_t launch_extend_tables(const ExtendTablesArgs& a, hipStream_t s);
+struct ReleaseTablesArgs {
+  int32_t* page_table;
+  int max_pages;
+  int32_t* seq_lens;
+  int32_t* free_pages;
+  int num_free;
+  int32_t* free_count;
+  const int32_t* rows;
+  int n_rows, batch, num_pages;
+};
+hipError_t launch_release_tables(const ReleaseTablesArgs& a, hipStream_t s);
+
 hipError_t launch_kv_write(const KvWriteArgs& a, hipStream_t s);
 // The writer of the 8-bit cache.
 hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s);
@@ -133,6 +173,13 @@ struct KvExpandArgs {
 };
 hipError_t launch_kv_expand_q8(const KvExpandArgs& a, hipStream_t s);
 hipError_t launch_prefill(const PrefillArgs& a, hipStream_t s);
+// Packed rows: the list of query tiles (prefill_plan_bytes; a.pk, batch, heads and with
+// `table` max_pages are read), then the attention over it.  table, start: a page table
+// [batch][max_pages] with a page of its own for each 16 rows of each sequence and
+// starts of 0, for rows that are to be written into pages; or null.
+size_t prefill_plan_bytes(int batch, int total_q, int hq);
+hipError_t launch_prefill_plan(const PrefillArgs& a, int32_t* tiles, int32_t* table, int32_t* start, hipStream_t s);
+hipError_t launch_prefill_packed(const PrefillArgs& a, hipStream_t s);
 // The MFMA-ceiling probe of the prefill (measurement only): sink holds
 // ceil(ceil(nq / 256) / 8) * 8 * hq * 512 floats.
 hipError_t launch_prefill_mfma_probe(float* sink, int nq, int hq, hipStream_t s);

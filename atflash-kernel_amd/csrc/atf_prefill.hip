@@ -100,18 +100,64 @@ __device__ __forceinline__ bf16x8 lds_frag(const lds_u8* p) {
   return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(p);
 }
 
-// Raw page-table entry of page `pidx` of sequence b (-1 past the keys), in a
+// What a workgroup works on.  One sequence of a batch of equal lengths: the call's own
+// arguments.
+struct BatchSeq {
+  const PrefillArgs& a;
+  int b;
+  __device__ __forceinline__ int nq() const { return a.nq; }
+  __device__ __forceinline__ int nk() const { return a.nk; }
+  __device__ __forceinline__ int q_offset() const { return a.q_offset; }
+  __device__ __forceinline__ const int32_t* pages() const { return a.page_table + static_cast<int64_t>(b) * a.max_pages; }
+  __device__ __forceinline__ const uint16_t* q(int h) const {
+    return a.q + static_cast<int64_t>(b) * a.q_sb + static_cast<int64_t>(h) * a.q_sh;
+  }
+  __device__ __forceinline__ uint16_t* out(int h) const {
+    return a.out + static_cast<int64_t>(b) * a.o_sb + static_cast<int64_t>(h) * a.o_sh;
+  }
+  __device__ __forceinline__ float* lse(int h) const { return a.lse + (static_cast<int64_t>(b) * a.hq + h) * a.nq; }
+};
+
+// One sequence of packed rows: first row, lengths and offset from device memory.
+struct PackedSeq {
+  const PrefillArgs& a;
+  int b, row0, n_q, n_k;
+  __device__ __forceinline__ int nq() const { return n_q; }
+  __device__ __forceinline__ int nk() const { return n_k; }
+  __device__ __forceinline__ int q_offset() const { return n_k - n_q; }
+  __device__ __forceinline__ const int32_t* pages() const { return a.page_table + static_cast<int64_t>(b) * a.max_pages; }
+  __device__ __forceinline__ const uint16_t* q(int h) const {
+    return a.q + static_cast<int64_t>(row0) * a.q_st + static_cast<int64_t>(h) * a.q_sh;
+  }
+  __device__ __forceinline__ uint16_t* out(int h) const {
+    return a.out + static_cast<int64_t>(row0) * a.o_st + static_cast<int64_t>(h) * a.o_sh;
+  }
+  __device__ __forceinline__ float* lse(int h) const { return a.lse + static_cast<int64_t>(h) * a.pk.total_q + row0; }
+};
+
+// Rows and keys of sequence b of packed rows; no rows where its lengths do not fit the
+// call (more rows than keys, more keys than the call's bound or the page table).
+__device__ __forceinline__ PackedSeq packed_seq(const PrefillArgs& a, int b) {
+  const int lo = max(a.pk.cu[b], 0), hi = min(a.pk.cu[b + 1], a.pk.total_q);
+  int n = max(hi - lo, 0);
+  const int keys = a.pk.seq_lens != nullptr ? a.pk.seq_lens[b] : n;
+  if (keys < n || keys > a.pk.max_k) n = 0;
+  return PackedSeq{a, b, lo, n, keys};
+}
+
+// Raw page-table entry of page `pidx` of the sequence (-1 past the keys), in a
 // vector register (every lane holds the same value).  Each wave fetches the
 // entry of its next page one tile ahead, so the table read is never waited for
 // at the start of a phase.  The load is kept a vector load on purpose: a scalar
 // load inside the tile loop shares the LDS wait counter and, since scalar loads
 // return out of order, would force every LDS wait behind it to drain fully.
-__device__ __forceinline__ int fetch_page(const PrefillArgs& a, int b, int pidx) {
+template <class Seq>
+__device__ __forceinline__ int fetch_page(const Seq& sq, int pidx) {
   int lane_zero;
   asm volatile("v_mov_b32 %0, 0" : "=v"(lane_zero));  // a value the compiler cannot prove uniform
-  const int n_pages_k = (a.nk + kPage - 1) / kPage;
+  const int n_pages_k = (sq.nk() + kPage - 1) / kPage;
   int pg = -1;
-  if (pidx < n_pages_k) pg = a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx + lane_zero];
+  if (pidx < n_pages_k) pg = sq.pages()[pidx + lane_zero];
   return pg;
 }
 
@@ -449,21 +495,23 @@ struct QRows {
 };
 
 // Rows past nq read row nq - 1, in bounds.
-__device__ __forceinline__ void q_request(const PrefillArgs& a, int b, int h, int lr0, int lane, QRows& q) {
+template <class Seq>
+__device__ __forceinline__ void q_request(const Seq& sq, int h, int lr0, int lane, QRows& q) {
+  const PrefillArgs& a = sq.a;
   const int j = lane & 7;
   const bool half = a.layout == kLayoutHalfSplit;
   const int c0 = half ? 8 * j : 8 * (14 - 2 * j), c1 = half ? kP + 8 * j : 8 * (15 - 2 * j);
-  const uint16_t* qh = a.q + static_cast<int64_t>(b) * a.q_sb + static_cast<int64_t>(h) * a.q_sh;
+  const uint16_t* qh = sq.q(h);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint16_t* qrow = qh + static_cast<int64_t>(min(lr0 + 8 * i + (lane >> 3), a.nq - 1)) * a.q_st;
+    const uint16_t* qrow = qh + static_cast<int64_t>(min(lr0 + 8 * i + (lane >> 3), sq.nq() - 1)) * a.q_st;
     q.x[i][0] = ldg16(qrow + c0);
     q.x[i][1] = ldg16(qrow + c1);
   }
   if (a.rope_cs != nullptr) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      load_cs8(a.rope_cs, a.q_offset + min(lr0 + 8 * i + (lane >> 3), a.nq - 1), 8 * j, q.cs[i]);
+      load_cs8(a.rope_cs, sq.q_offset() + min(lr0 + 8 * i + (lane >> 3), sq.nq() - 1), 8 * j, q.cs[i]);
   }
 }
 
@@ -472,8 +520,10 @@ __device__ __forceinline__ void q_request(const PrefillArgs& a, int b, int h, in
 // level l is slice 2l + h, as in the cache's K pages.  Slice s of row r lies at
 // 512 s + 16 (r ^ 8 (s/2 % 4)): the 8 rows x 8 slices of a write, and the 32 rows
 // of a read, spread over all banks.
-__device__ __forceinline__ void q_fragments(const PrefillArgs& a, const QRows& q, lds_u8* st, int lr0, int lane,
+template <class Seq>
+__device__ __forceinline__ void q_fragments(const Seq& sq, const QRows& q, lds_u8* st, int lr0, int lane,
                                             u32x4 (&Qf)[kLevels]) {
+  const PrefillArgs& a = sq.a;
   const int j = lane & 7;
   const bool half = a.layout == kLayoutHalfSplit;
   auto at = [&](int s, int r) {
@@ -496,14 +546,15 @@ __device__ __forceinline__ void q_fragments(const PrefillArgs& a, const QRows& q
 #pragma unroll
   for (int l = 0; l < kLevels; ++l) {
     const u32x4 v = *at(2 * l + (lane >> 5), lane & 31);
-    Qf[l] = (lr0 + (lane & 31) < a.nq) ? v : u32x4{0u, 0u, 0u, 0u};
+    Qf[l] = (lr0 + (lane & 31) < sq.nq()) ? v : u32x4{0u, 0u, 0u, 0u};
   }
 }
 
 // O / l of the wave's 32 rows to memory.  In LDS row r is 256 bytes, its 16-byte
 // chunk c at c ^ (r % 16).
-__device__ __forceinline__ void store_rows(const PrefillArgs& a, int b, int h, int lr0, int lane, const f32x16 (&O)[4],
-                                           float inv, lds_u8* st) {
+template <class Seq>
+__device__ __forceinline__ void store_rows(const Seq& sq, int h, int lr0, int lane, const f32x16 (&O)[4], float inv,
+                                           lds_u8* st) {
   const int r = lane & 31;
 #pragma unroll
   for (int db = 0; db < 4; ++db)
@@ -516,12 +567,12 @@ __device__ __forceinline__ void store_rows(const PrefillArgs& a, int b, int h, i
                                                                   8 * (lane >> 5)) = w;
     }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  uint16_t* oh = a.out + static_cast<int64_t>(b) * a.o_sb + static_cast<int64_t>(h) * a.o_sh + 8 * (lane & 15);
+  uint16_t* oh = sq.out(h) + 8 * (lane & 15);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int rr = 4 * i + (lane >> 4);
     const u32x4 w = *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(st + 256 * rr + 16 * ((lane ^ rr) & 15));
-    if (lr0 + rr < a.nq) *reinterpret_cast<u32x4_a8*>(oh + static_cast<int64_t>(lr0 + rr) * a.o_st) = w;
+    if (lr0 + rr < sq.nq()) *reinterpret_cast<u32x4_a8*>(oh + static_cast<int64_t>(lr0 + rr) * sq.a.o_st) = w;
   }
 }
 
@@ -562,28 +613,26 @@ __device__ __forceinline__ bool prefill_block(const PrefillArgs& a, int bid, int
 //         fp32 scores in the softmax (one multiply per score).  Scaling an
 //         already-rounded bf16 Q and rounding it again would add a second
 //         rounding error to every score, which grows with the score magnitude.
-template <bool kRaw>
-__global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a) {
+template <bool kRaw, class Seq>
+__device__ __forceinline__ void prefill_rows(const Seq& sq, int h, int qt) {
+  const PrefillArgs& a = sq.a;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_raw[];
   lds_u8* smem = (lds_u8*)(smem_raw);
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-
-  int b, h, qt;
-  if (!prefill_block(a, blockIdx.x, b, h, qt)) return;
   const int kvh = h / a.group;
 
   const int lr0_wg = qt * kPfRowsWg;
   const int lr0 = lr0_wg + wave * kPfRowsWave;
-  const int pos0_wg = a.q_offset + lr0_wg;
-  const int pos0 = a.q_offset + lr0;
-  const int n_ktiles = (a.nk + kPfTileN - 1) / kPfTileN;
-  const int last_wg = a.q_offset + min(a.nq, lr0_wg + kPfRowsWg) - 1;
+  const int pos0_wg = sq.q_offset() + lr0_wg;
+  const int pos0 = sq.q_offset() + lr0;
+  const int n_ktiles = (sq.nk() + kPfTileN - 1) / kPfTileN;
+  const int last_wg = sq.q_offset() + min(sq.nq(), lr0_wg + kPfRowsWg) - 1;
   const int T = min(n_ktiles, last_wg / kPfTileN + 1);  // tiles of the workgroup
   const int T2 = (T + 1) & ~1;                          // rounded up to whole pairs
   const int t_end =
-      (lr0 < a.nq) ? min(n_ktiles, (a.q_offset + min(a.nq, lr0 + kPfRowsWave) - 1) / kPfTileN + 1) : 0;
+      (lr0 < sq.nq()) ? min(n_ktiles, (sq.q_offset() + min(sq.nq(), lr0 + kPfRowsWave) - 1) / kPfTileN + 1) : 0;
 
   f32x16 O[4];
 #pragma unroll
@@ -624,15 +673,15 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a
   // phase ahead.
   int e[4], pg_a = 0, pg_b = 0;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) e[t] = fetch_page(a, b, 4 * t + rank);
+  for (int t = 0; t < 4; ++t) e[t] = fetch_page(sq, 4 * t + rank);
   if (!copies_v) {
-    pg_a = fetch_page(a, b, 16 + rank);
-    pg_b = fetch_page(a, b, 20 + rank);
+    pg_a = fetch_page(sq, 16 + rank);
+    pg_b = fetch_page(sq, 20 + rank);
   }
   u32x4 Qf[kLevels];
   const int row = lr0 + (lane & 31);
   QRows q;
-  q_request(a, b, h, lr0, lane, q);
+  q_request(sq, h, lr0, lane, q);
   if (!copies_v) {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -643,7 +692,7 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a
 #pragma unroll
     for (int s = 0; s < 2; ++s) zero_page(smem + kPfVRegion + kPfPairBytes + s * kPfSlotBytes + rank * 4096, lane);
   }
-  q_fragments(a, q, smem + (copies_v ? kPfVRegion : 2 * kPfPairBytes) + rank * kRowStage, lr0, lane, Qf);
+  q_fragments(sq, q, smem + (copies_v ? kPfVRegion : 2 * kPfPairBytes) + rank * kRowStage, lr0, lane, Qf);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (copies_v) {
@@ -711,7 +760,7 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a
     // this wave's copies requested in its previous phase land before the
     // barrier after which they are first read
     __builtin_amdgcn_s_waitcnt(kWaitVm);
-    if (copies_v && 2 * u < T2 && (2 * u + 2) * kPfTileN > a.nk) {
+    if (copies_v && 2 * u < T2 && (2 * u + 2) * kPfTileN > sq.nk()) {
       // the V of tiles 2u, 2u+1 (pair u % 2) has landed: zero the slots of keys
       // past nk in this wave's pages (0 * V must stay 0); first read next phase
 #pragma unroll
@@ -722,7 +771,7 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a
         for (int rr = 0; rr < 2; ++rr)
 #pragma unroll
           for (int tk = 0; tk < kPage; ++tk)
-            if (n0 + tk >= a.nk)
+            if (n0 + tk >= sq.nk())
               *reinterpret_cast<__attribute__((address_space(3))) uint16_t*>(vpage + v_lds_elem(lane * 2 + rr, v_slot(tk))) =
                   0;
       }
@@ -756,10 +805,10 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[2 * hh + kb][r] = NEG_INF;
-        } else if ((n0 + kPfTileN - 1 > pos0) || (n0 + kPfTileN > a.nk)) {
+        } else if ((n0 + kPfTileN - 1 > pos0) || (n0 + kPfTileN > sq.nk())) {
           // element (kb, r) holds key n0 + 4*(lane/32) + c with c = 32kb + 8(r/4) + r%4;
           // masked when key > min(row position, nk - 1).  Selects, no branches.
-          const int thr = min(pos0 + (lane & 31), a.nk - 1) - n0 - 4 * (lane >> 5);
+          const int thr = min(pos0 + (lane & 31), sq.nk() - 1) - n0 - 4 * (lane >> 5);
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -816,8 +865,8 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a
 #pragma unroll
       for (int i = 0; i < 8; ++i) Pf[i] = bf16x8{};
     }
-    pg_a = fetch_page(a, b, 4 * (ct + 2) + rank);
-    pg_b = fetch_page(a, b, 4 * (ct + 3) + rank);
+    pg_a = fetch_page(sq, 4 * (ct + 2) + rank);
+    pg_b = fetch_page(sq, 4 * (ct + 3) + rank);
     L0 = w_far.advance(a.lt, 2 * u + 2);
     L1 = w_near.advance(a.lt, 2 * u + 2);
     L2 = w_far.advance(a.lt, 2 * u + 3);
@@ -830,9 +879,9 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a
   const float l = pair_sum(l_run);
   const float inv = l > 0.f ? 1.f / l : 0.f;
   // (no wave reads a K pair past the last barrier, and every copy has landed)
-  store_rows(a, b, h, lr0, lane, O, inv, smem + wave * kRowStage);
-  if (a.lse != nullptr && lane < 32 && row < a.nq)
-    a.lse[(static_cast<int64_t>(b) * a.hq + h) * a.nq + row] = (l > 0.f) ? m_ref * kLn2 + __logf(l) : NEG_INF;
+  store_rows(sq, h, lr0, lane, O, inv, smem + wave * kRowStage);
+  if (a.lse != nullptr && lane < 32 && row < sq.nq())
+    sq.lse(h)[row] = (l > 0.f) ? m_ref * kLn2 + __logf(l) : NEG_INF;
 }
 
 // ---- one wave per SIMD: launches that leave CUs idle ----
@@ -957,32 +1006,30 @@ __device__ __forceinline__ void qk_blocks(uint64_t lm, const lds_u8* kb, const u
 // 32 rows of a SIMD where prefill_kernel takes 5000 to 5700 for 64.
 constexpr int kSoloWaves = 4;
 constexpr int kSoloRowsWg = kSoloWaves * kPfRowsWave;
-template <bool kRaw>
-__global__ __launch_bounds__(kSoloWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void prefill_solo_kernel(PrefillArgs a) {
+template <bool kRaw, class Seq>
+__device__ __forceinline__ void prefill_solo_rows(const Seq& sq, int h, int qt) {
+  const PrefillArgs& a = sq.a;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_raw[];
   lds_u8* smem = (lds_u8*)(smem_raw);
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int b, h, qt;
-  if (!prefill_block(a, blockIdx.x, b, h, qt)) return;
   const int kvh = h / a.group;
 
   const int lr0_wg = qt * kSoloRowsWg;
   const int lr0 = lr0_wg + wave * kPfRowsWave;
-  const int pos0_wg = a.q_offset + lr0_wg;
-  const int pos0 = a.q_offset + lr0;
-  const int n_ktiles = (a.nk + kPfTileN - 1) / kPfTileN;
-  const int last_wg = a.q_offset + min(a.nq, lr0_wg + kSoloRowsWg) - 1;
+  const int pos0_wg = sq.q_offset() + lr0_wg;
+  const int pos0 = sq.q_offset() + lr0;
+  const int n_ktiles = (sq.nk() + kPfTileN - 1) / kPfTileN;
+  const int last_wg = sq.q_offset() + min(sq.nq(), lr0_wg + kSoloRowsWg) - 1;
   const int T = min(n_ktiles, last_wg / kPfTileN + 1);
   const int U = (T + 1) >> 1;
   const int t_end =
-      (lr0 < a.nq) ? min(n_ktiles, (a.q_offset + min(a.nq, lr0 + kPfRowsWave) - 1) / kPfTileN + 1) : 0;
+      (lr0 < sq.nq()) ? min(n_ktiles, (sq.q_offset() + min(sq.nq(), lr0 + kPfRowsWave) - 1) / kPfTileN + 1) : 0;
 
   // page-table entries of 64 pages (8 tile pairs) at a time, one per lane
-  const int n_pages_k = (a.nk + kPage - 1) / kPage;
-  const int32_t* prow = a.page_table + static_cast<int64_t>(b) * a.max_pages;
+  const int n_pages_k = (sq.nk() + kPage - 1) / kPage;
+  const int32_t* prow = sq.pages();
   auto fetch64 = [&](int chunk) {
     const int p = chunk * 64 + lane;
     int v = prow[min(p, n_pages_k - 1)];
@@ -997,7 +1044,7 @@ void prefill_solo_kernel(PrefillArgs a) {
   u32x4 Qf[kLevels];
   const int row = lr0 + (lane & 31);
   QRows q;
-  q_request(a, b, h, lr0, lane, q);
+  q_request(sq, h, lr0, lane, q);
 
   f32x16 O[4];
 #pragma unroll
@@ -1059,7 +1106,7 @@ void prefill_solo_kernel(PrefillArgs a) {
     for (int r = 0; r < 8; ++r) copy_row_n(r < 4 ? c0 : c1, k_off, r & 3);
   }
   // staged in V pair 0, which is copied to after the barrier
-  q_fragments(a, q, smem + kPfVRegion + wave * kRowStage, lr0, lane, Qf);
+  q_fragments(sq, q, smem + kPfVRegion + wave * kRowStage, lr0, lane, Qf);
   // V pair 1: read by the first PV with P = 0
   zero_page(smem + kPfVRegion + kPfPairBytes + wave * 4096, lane);
   zero_page(smem + kPfVRegion + kPfPairBytes + kPfSlotBytes + wave * 4096, lane);
@@ -1100,13 +1147,13 @@ void prefill_solo_kernel(PrefillArgs a) {
     };
     const lds_u8* kb = smem + ((u + 1) % kPfKPairs) * kPfPairBytes + k_lane;
     const lds_u8* vb = smem + kPfVRegion + ((u + 1) & 1) * kPfPairBytes + v_lane;
-    if (__builtin_expect((2 * u + 2) * kPfTileN - 1 > pos0 || (2 * u + 2) * kPfTileN > a.nk, 0)) {
+    if (__builtin_expect((2 * u + 2) * kPfTileN - 1 > pos0 || (2 * u + 2) * kPfTileN > sq.nk(), 0)) {
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         const int n0 = (2 * u + hh) * kPfTileN;
         // element (kb, r) holds key n0 + 4*(lane/32) + 32kb + 8(r/4) + r%4; masked
         // when key > min(row position, nk - 1), every key of a tile past t_end
-        const int thr = 2 * u + hh >= t_end ? -1 : min(pos0 + (lane & 31), a.nk - 1) - n0 - 4 * (lane >> 5);
+        const int thr = 2 * u + hh >= t_end ? -1 : min(pos0 + (lane & 31), sq.nk() - 1) - n0 - 4 * (lane >> 5);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -1167,7 +1214,7 @@ void prefill_solo_kernel(PrefillArgs a) {
     // V of pair u and K of pair u + 2 have landed (K of u + 3, this wave's last 8
     // loads, may still be in flight)
     __builtin_amdgcn_s_waitcnt(kWaitVm | 8);
-    if ((2 * u + 2) * kPfTileN > a.nk) {
+    if ((2 * u + 2) * kPfTileN > sq.nk()) {
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         const int n0 = (2 * u + hh) * kPfTileN + wave * kPage;
@@ -1176,7 +1223,7 @@ void prefill_solo_kernel(PrefillArgs a) {
         for (int rr = 0; rr < 2; ++rr)
 #pragma unroll
           for (int tk = 0; tk < kPage; ++tk)
-            if (n0 + tk >= a.nk)
+            if (n0 + tk >= sq.nk())
               *reinterpret_cast<__attribute__((address_space(3))) uint16_t*>(vpage + v_lds_elem(lane * 2 + rr, v_slot(tk))) =
                   0;
       }
@@ -1201,9 +1248,130 @@ void prefill_solo_kernel(PrefillArgs a) {
   const float inv = l > 0.f ? 1.f / l : 0.f;
   // The V pair that the last barrier freed (the other one is read above; zeros past
   // the end may still land in a K pair).
-  store_rows(a, b, h, lr0, lane, O, inv, smem + kPfVRegion + (U & 1) * kPfPairBytes + wave * kRowStage);
-  if (a.lse != nullptr && lane < 32 && row < a.nq)
-    a.lse[(static_cast<int64_t>(b) * a.hq + h) * a.nq + row] = (l > 0.f) ? m_ref * kLn2 + __logf(l) : NEG_INF;
+  store_rows(sq, h, lr0, lane, O, inv, smem + kPfVRegion + (U & 1) * kPfPairBytes + wave * kRowStage);
+  if (a.lse != nullptr && lane < 32 && row < sq.nq())
+    sq.lse(h)[row] = (l > 0.f) ? m_ref * kLn2 + __logf(l) : NEG_INF;
+}
+
+template <bool kRaw>
+__global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a) {
+  int b, h, qt;
+  if (prefill_block(a, blockIdx.x, b, h, qt)) prefill_rows<kRaw>(BatchSeq{a, b}, h, qt);
+}
+
+template <bool kRaw>
+__global__ __launch_bounds__(kSoloWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void prefill_solo_kernel(PrefillArgs a) {
+  int b, h, qt;
+  if (prefill_block(a, blockIdx.x, b, h, qt)) prefill_solo_rows<kRaw>(BatchSeq{a, b}, h, qt);
+}
+
+// ---- packed rows of sequences of different lengths ----
+// The same two kernels where sequence b's queries are rows cu[b] .. cu[b + 1] - 1 of q
+// and out, the last of its seq_lens[b] keys.  The lengths are known to the GPU alone:
+// prefill_plan_kernel lists the query tiles, the one with the most keys first, and a
+// workgroup takes its tile, and q head, from the list as prefill_block deals out
+// units.  The grid covers as many tiles as total_q rows of `batch` sequences can have
+// (total_q / rows + batch); workgroups past the list end at once.  A sequence's results
+// are those of a prefill call of its own to the bit (the same tiles of 32 rows, the
+// same order of keys).
+
+// The tile of block `bid`: false past the list.
+__device__ __forceinline__ bool packed_block(const PrefillArgs& a, int bid, int rows, int& b, int& h, int& qt) {
+  const int xcd = bid & 7;
+  const int j = bid >> 3;
+  const int rnd = j / a.group;
+  const int unit = rnd * 8 + ((rnd & 1) ? 7 - xcd : xcd);
+  const int rank = unit / a.hkv;
+  h = (unit - rank * a.hkv) * a.group + (j - rnd * a.group);
+  if (rank >= min(a.pk.tiles[0], a.n_qtiles)) return false;
+  b = a.pk.tiles[2 + 2 * rank];
+  qt = a.pk.tiles[3 + 2 * rank];
+  return b >= 0 && b < a.batch && qt >= 0 && qt <= INT32_MAX / rows - 1;  // (a list of another call: in bounds all the same)
+}
+
+template <bool kRaw>
+__global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_packed_kernel(PrefillArgs a) {
+  int b, h, qt;
+  if (!packed_block(a, blockIdx.x, kPfRowsWg, b, h, qt)) return;
+  const PackedSeq sq = packed_seq(a, b);
+  if (qt * kPfRowsWg < sq.n_q) prefill_rows<kRaw>(sq, h, qt);
+}
+
+template <bool kRaw>
+__global__ __launch_bounds__(kSoloWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void prefill_packed_solo_kernel(PrefillArgs a) {
+  int b, h, qt;
+  if (!packed_block(a, blockIdx.x, kSoloRowsWg, b, h, qt)) return;
+  const PackedSeq sq = packed_seq(a, b);
+  if (qt * kSoloRowsWg < sq.n_q) prefill_solo_rows<kRaw>(sq, h, qt);
+}
+
+// The tile list: [0] the number of tiles, then (sequence, tile) pairs from [2] on, most
+// keys first (ties: by sequence).  A wave per tile place: sequence b's places start at
+// cu[b] / rows + b, which leaves room for ceil(n / rows) tiles of each, so that no sums
+// over sequences have to be formed first; the wave finds its sequence by counting the
+// starts up to its place, 64 sequences at a time, and its rank by counting the tiles of
+// every sequence that have more keys, a closed form each.
+//   Latency bound: the lengths are read twice.  With `table`, workgroups also lay out a
+// page table for rows that are to be written page by page: page p of sequence b is
+// cu[b] / 16 + b + p, start 0.
+constexpr int kPlanWaves = 4;
+__global__ __launch_bounds__(kPlanWaves * 64) void prefill_plan_kernel(PrefillArgs a, int rows, int places, int32_t* tiles,
+                                                                       int32_t* table, int32_t* start) {
+  const int lane = threadIdx.x & 63;
+  const int place = blockIdx.x * kPlanWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (table != nullptr) {
+    const int64_t n = static_cast<int64_t>(a.batch) * a.max_pages, step = static_cast<int64_t>(gridDim.x) * kPlanWaves * 64;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPlanWaves * 64 + threadIdx.x; i < n; i += step) {
+      const int b = static_cast<int>(i / a.max_pages), p = static_cast<int>(i - static_cast<int64_t>(b) * a.max_pages);
+      const int lo = min(max(a.pk.cu[b], 0), a.pk.total_q);
+      table[i] = lo / kPage + b + p;
+      if (p == 0) start[b] = 0;
+    }
+  }
+  if (place >= places) return;
+  // the sequence of this place, and the number of tiles of all
+  int before = 0, total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    bool reached = false;
+    int n = 0;
+    if (b < a.batch) {
+      const PackedSeq sq = packed_seq(a, b);
+      reached = min(sq.row0, a.pk.total_q) / rows + b <= place;
+      n = (sq.n_q + rows - 1) / rows;
+    }
+    before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(reached));
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) n += __shfl_xor(n, m);
+    total += n;
+  }
+  if (place == 0 && lane == 0) tiles[0] = total;
+  if (before == 0) return;
+  const int mine = before - 1;
+  const PackedSeq me = packed_seq(a, mine);
+  const int i = place - (min(me.row0, a.pk.total_q) / rows + mine);
+  if (i < 0 || i * rows >= me.n_q) return;  // (i < 0: first rows that decrease)
+  const int keys = me.q_offset() + min(me.n_q, (i + 1) * rows);
+  int rank = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    if (b >= a.batch) continue;
+    const PackedSeq sq = packed_seq(a, b);
+    const int n = (sq.n_q + rows - 1) / rows;
+    if (n == 0) continue;
+    const int over = keys - sq.q_offset();  // tile j has more keys where min(n_q, (j + 1) rows) > over
+    if (sq.n_q > over) rank += n - min(max(over, 0) / rows, n - 1);
+    // a tile with as many keys, of an earlier sequence (tiles of one differ)
+    if (b < mine && over > 0 && over <= sq.n_q && (over == sq.n_q || over % rows == 0)) ++rank;
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) rank += __shfl_xor(rank, m);
+  if (lane == 0 && rank < places) {
+    tiles[2 + 2 * rank] = mine;
+    tiles[3 + 2 * rank] = i;
+  }
 }
 
 // ---- measurement probe: the MFMA ceiling of this kernel's structure ----
@@ -1344,6 +1512,10 @@ hipError_t ensure_lds_attribute() {
                         reinterpret_cast<const void*>(prefill_kernel<true>),
                         reinterpret_cast<const void*>(prefill_solo_kernel<false>),
                         reinterpret_cast<const void*>(prefill_solo_kernel<true>),
+                        reinterpret_cast<const void*>(prefill_packed_kernel<false>),
+                        reinterpret_cast<const void*>(prefill_packed_kernel<true>),
+                        reinterpret_cast<const void*>(prefill_packed_solo_kernel<false>),
+                        reinterpret_cast<const void*>(prefill_packed_solo_kernel<true>),
                         reinterpret_cast<const void*>(prefill_mfma_probe_kernel)}) {
     e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kPfLdsTotal);
     if (e != hipSuccess) return e;
@@ -1381,6 +1553,47 @@ hipError_t launch_prefill(const PrefillArgs& a, hipStream_t s) {
   } else {
     if (a.rope_cs != nullptr) ATF_PF_LAUNCH(prefill_kernel<false>, kPfWaves);
     else ATF_PF_LAUNCH(prefill_kernel<true>, kPfWaves);
+  }
+#undef ATF_PF_LAUNCH
+  return hipGetLastError();
+}
+
+// Tiles of packed rows at most, and whether the 128-row kernel takes them: where every
+// workgroup of the expected tiles (half a tile lost a sequence) gets a CU of its own.
+static int packed_tiles(int batch, int total_q, int rows) { return total_q / rows + batch; }
+static bool packed_solo(int batch, int total_q, int hq) {
+  return (static_cast<int64_t>(total_q) / kSoloRowsWg + (batch + 1) / 2) * hq <= 256;
+}
+
+size_t prefill_plan_bytes(int batch, int total_q, int hq) {
+  const int rows = packed_solo(batch, total_q, hq) ? kSoloRowsWg : kPfRowsWg;
+  return (2 + 2 * static_cast<size_t>(packed_tiles(batch, total_q, rows))) * sizeof(int32_t);
+}
+
+hipError_t launch_prefill_plan(const PrefillArgs& a, int32_t* tiles, int32_t* table, int32_t* start, hipStream_t s) {
+  if (a.batch <= 0 || a.pk.total_q <= 0) return hipSuccess;
+  const int rows = packed_solo(a.batch, a.pk.total_q, a.hq) ? kSoloRowsWg : kPfRowsWg;
+  const int places = packed_tiles(a.batch, a.pk.total_q, rows);
+  hipLaunchKernelGGL(prefill_plan_kernel, dim3((places + kPlanWaves - 1) / kPlanWaves), dim3(kPlanWaves * 64), 0, s, a,
+                     rows, places, tiles, table, start);
+  return hipGetLastError();
+}
+
+hipError_t launch_prefill_packed(const PrefillArgs& a, hipStream_t s) {
+  if (a.batch <= 0 || a.pk.total_q <= 0) return hipSuccess;
+  if (hipError_t e = ensure_lds_attribute(); e != hipSuccess) return e;
+  PrefillArgs k = a;
+  const bool solo = packed_solo(a.batch, a.pk.total_q, a.hq);
+  k.n_qtiles = packed_tiles(a.batch, a.pk.total_q, solo ? kSoloRowsWg : kPfRowsWg);
+  const int64_t blocks = (static_cast<int64_t>(k.n_qtiles) * a.hkv + 7) / 8 * 8 * a.group;
+  if (blocks > INT32_MAX) return hipErrorInvalidConfiguration;
+#define ATF_PF_LAUNCH(K, W) hipLaunchKernelGGL(K, dim3(blocks), dim3((W) * 64), kPfLdsTotal, s, k)
+  if (solo) {
+    if (a.rope_cs != nullptr) ATF_PF_LAUNCH(prefill_packed_solo_kernel<false>, kSoloWaves);
+    else ATF_PF_LAUNCH(prefill_packed_solo_kernel<true>, kSoloWaves);
+  } else {
+    if (a.rope_cs != nullptr) ATF_PF_LAUNCH(prefill_packed_kernel<false>, kPfWaves);
+    else ATF_PF_LAUNCH(prefill_packed_kernel<true>, kPfWaves);
   }
 #undef ATF_PF_LAUNCH
   return hipGetLastError();

@@ -177,6 +177,69 @@ int atf_prefill_bf16(void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float*
                      int layout, void* stream);
 
 /*
+ * The prefill of packed rows: sequences of different lengths in one call, their
+ * lengths in device memory.  Sequence b's queries are rows cu_seqlens[b] to
+ * cu_seqlens[b + 1] - 1 (device int32 [batch + 1], not decreasing) of q and out
+ * (bf16 [total_q][num_q_heads][128], strides as atf_prefill_bf16's), the last of
+ * its seq_lens[b] keys (device int32 [batch]; NULL: as many keys as queries, whole
+ * prompts) in the paged cache.  lse (nullable): fp32 [num_q_heads][total_q].  A
+ * sequence's rows get the bits of an atf_prefill_bf16 call of its own.  Rows outside
+ * every sequence are left as they are, and so are those of a sequence with more
+ * queries than keys or more than max_seq_len keys.
+ *   atf_prefill_plan first lists the query tiles in `plan` (device memory of
+ * atf_prefill_plan_bytes, no initialisation needed), heaviest first; one plan serves
+ * every layer of a step.  With page_table (int32 [batch][max_pages]) and start_pos
+ * (int32 [batch]) it also lays out a page table for rows that are to be written to
+ * pages of their own (page p of sequence b: cu_seqlens[b] / 16 + b + p, a pool of
+ * total_q / 16 + batch pages) and starts of 0.  A plan made for other lengths gives
+ * rows that are not computed, never an access out of bounds.
+ */
+size_t atf_prefill_plan_bytes(int batch, int total_q, int num_q_heads);
+int atf_prefill_plan(void* plan, size_t plan_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens, int batch,
+                     int total_q, int max_seq_len, int num_q_heads, int32_t* page_table, int max_pages,
+                     int32_t* start_pos, void* stream);
+int atf_prefill_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
+                            const void* q, int64_t q_st, int64_t q_sh, const void* kv_cache, int num_pages,
+                            const int32_t* page_table, int max_pages,
+                            const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int total_q,
+                            int max_seq_len, int num_q_heads, int num_kv_heads,
+                            const int32_t* zhi, float sm_scale, const float* rope_cs, int rope_max_pos, int layout,
+                            const void* plan, size_t plan_bytes, void* stream);
+
+/*
+ * Block tables and slot maps of a step from request lengths, on the GPU.  Sequence b
+ * has seq_lens[b] tokens and gets new_lens[b] more (negative: none).  The pages it
+ * needs beyond those of its tokens are taken from the end of the free pages
+ * (free_pages[0 .. *free_count - 1], an array of num_free entries), sequence by
+ * sequence, and entered into its row of page_table ([batch][max_pages], in place;
+ * pages past max_pages are not taken).  Written:
+ *   seq_lens_out [batch]    lengths afterwards
+ *   free_left    [1]        *free_count less the pages taken; negative: so many were
+ *                           missing, their entries are -1
+ *   cu_seqlens   [batch+1]  first new token of each sequence in the packed order
+ *   positions    [total_tokens], slots [total_tokens] (int64): position of each new
+ *                           token in its sequence, and page * 16 + position % 16; slot -1
+ *                           where it has no page of the pool (num_pages); both -1 past
+ *                           the last new token.  New tokens past total_tokens are not
+ *                           listed.
+ * seq_lens and free_count are read only, so that a call can be repeated.  batch is at
+ * most 8191; the new tokens of a call and their positions are below 2^31.
+ */
+int atf_extend_tables(int32_t* page_table, int max_pages, const int32_t* seq_lens, const int32_t* new_lens,
+                      const int32_t* free_pages, int num_free, const int32_t* free_count, int batch, int total_tokens,
+                      int num_pages, int32_t* seq_lens_out, int32_t* free_left, int32_t* cu_seqlens, int32_t* positions,
+                      int64_t* slots, void* stream);
+
+/*
+ * The pages of the sequences rows[0 .. n_rows - 1] (device int32) go back to the end
+ * of the free pages, sequence by sequence; their page-table rows become -1 and their
+ * lengths 0, *free_count grows (to num_free at most).  Rows outside [0, batch) and
+ * repeated rows give nothing.
+ */
+int atf_release_tables(int32_t* page_table, int max_pages, int32_t* seq_lens, int32_t* free_pages, int num_free,
+                       int32_t* free_count, const int32_t* rows, int n_rows, int batch, int num_pages, void* stream);
+
+/*
  * Bytes of device workspace atf_decode_paged_bf16 needs for these sizes: the
  * fp32 split partials (m, l, o) of every (sequence, kv head, split), 0 when the
  * call runs one split per (sequence, kv head).  The workspace needs no

@@ -124,3 +124,80 @@ def test_the_restated_cache_keeps_and_forgets():
     c.write(1000 * x[:1], x[:1], 5, [1, 0], None)
     assert (c.k[1, :5] == 1).all() and (c.k[1, 5] == 1024).all() and (c.k[1, 6:] == 0).all()
     assert int(c.e[1, 0, 1]) == exponent(1000.0) and int(c.e[1, 0, 0]) == exponent(2.0)
+
+
+PLAN = dict(plan=1 << 20, plan_bytes=1 << 20, cu=1 << 20, lens=None, batch=2, total=100, most=60, hq=4, table=None,
+            max_pages=0, start=None, stream=None)
+PREFILL = dict(out=1 << 20, o_st=512, o_sh=128, lse=None, q=1 << 20, q_st=512, q_sh=128, kv=1 << 20, pages=9, table=1 << 20,
+               max_pages=4, cu=1 << 20, lens=None, batch=2, total=100, most=60, hq=4, hkv=2, zhi=None, scale=0.1, rope=None,
+               rope_pos=0, layout=0, plan=1 << 20, plan_bytes=1 << 20, stream=None)
+EXTEND = dict(table=1 << 20, max_pages=4, lens=1 << 20, new=1 << 20, free=1 << 20, num_free=4, count=1 << 20, batch=2,
+              total=9, pages=9, lens_out=1 << 20, left=1 << 20, cu=1 << 20, pos=1 << 20, slots=1 << 20, stream=None)
+RELEASE = dict(table=1 << 20, max_pages=4, lens=1 << 20, free=1 << 20, num_free=4, count=1 << 20, rows=1 << 20, n=1, batch=2,
+               pages=9, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(batch=-1), 1), (dict(total=-1), 1), (dict(cu=None), 1), (dict(most=0), 1), (dict(hq=0), 1), (dict(most=1 << 24), 2),
+    (dict(plan=None), 4), (dict(plan_bytes=8), 4), (dict(plan=(1 << 20) + 4), 4), (dict(table=1 << 20), 1),
+    (dict(start=1 << 20), 1), (dict(table=1 << 20, start=1 << 20, max_pages=3), 1), (dict(batch=0), 0), (dict(total=0), 0)])
+def test_plan_validation(no_gpu, change, code):
+    assert call(no_gpu.atf_prefill_plan, PLAN, **change) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(batch=-1), 1), (dict(total=-1), 1), (dict(cu=None), 1), (dict(out=None), 1), (dict(q=None), 1), (dict(kv=None), 1),
+    (dict(hkv=3), 1), (dict(max_pages=3), 1), (dict(most=1 << 24), 2), (dict(scale=-1.0), 1), (dict(rope=1 << 20, rope_pos=59), 1),
+    (dict(layout=1, rope=1 << 20, rope_pos=99), 1), (dict(q=(1 << 20) + 8), 1), (dict(out=(1 << 20) + 4), 1), (dict(q_st=4), 1),
+    (dict(o_st=2), 1), (dict(plan=None), 4), (dict(plan_bytes=9), 4), (dict(batch=0), 0), (dict(total=0), 0)])
+def test_packed_prefill_validation(no_gpu, change, code):
+    assert call(no_gpu.atf_prefill_packed_bf16, PREFILL, **change) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(batch=0), 1), (dict(batch=-2), 1), (dict(total=-1), 1), (dict(max_pages=0), 1), (dict(pages=0), 1),
+    (dict(num_free=-1), 1), (dict(table=None), 1), (dict(lens=None), 1), (dict(new=None), 1), (dict(free=None), 1),
+    (dict(count=None), 1), (dict(pos=None), 1), (dict(slots=None), 1), (dict(slots=(1 << 20) + 4), 1), (dict(cu=None), 1),
+    (dict(batch=8192), 2)])
+def test_extend_validation(no_gpu, change, code):
+    assert call(no_gpu.atf_extend_tables, EXTEND, **change) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(batch=0), 1), (dict(n=-1), 1), (dict(rows=None), 1), (dict(table=None), 1), (dict(free=None), 1), (dict(pages=0), 1),
+    (dict(n=0, rows=None), 0)])
+def test_release_validation(no_gpu, change, code):
+    assert call(no_gpu.atf_release_tables, RELEASE, **change) == code
+
+
+def test_plan_size_covers_every_split_of_the_rows(no_gpu):
+    # tiles of `batch` sequences with total rows: at most one started tile more for each
+    for batch, total, hq in ((1, 1, 4), (3, 1000, 28), (300, 20000, 8), (2, 100, 64), (8, 60, 2)):
+        places = (no_gpu.atf_prefill_plan_bytes(batch, total, hq) // 4 - 2) // 2
+        assert any(places == total // r + batch for r in (128, 256))
+    assert no_gpu.atf_prefill_plan_bytes(0, 5, 4) == no_gpu.atf_prefill_plan_bytes(1, 0, 4) == 0
+
+
+def test_tables_and_packed_operators_refuse():
+    from atflash import interface, ops
+    from atflash.cache import PagedKVCache, PageTables
+    i32 = torch.int32
+    tabs = PageTables(8, 2, 4, "cpu")
+    assert tabs.free_pages.tolist() == [7, 6, 5, 4, 3, 2, 1, 0] and int(tabs.free_count) == 8
+    with pytest.raises(ValueError, match="GPU only"):
+        tabs.extend(torch.ones(2, dtype=i32), 2)
+    with pytest.raises(ValueError, match="GPU only"):
+        tabs.release(torch.zeros(1, dtype=i32))
+    q, k = torch.zeros((4, 6, 128), dtype=torch.bfloat16), torch.zeros((4, 4, 128), dtype=torch.bfloat16)
+    cu = torch.tensor([0, 4], dtype=i32)
+    with pytest.raises(ValueError, match="multiple"):
+        interface.flash_attn_packed(q, k, k, cu, 4)
+    with pytest.raises(ValueError, match="GPU only"):
+        interface.flash_attn_packed(q, k[:, :2], k[:, :2], cu, 4)
+    cache = PagedKVCache(2, 2, "cpu")
+    with pytest.raises(ValueError, match="GPU only"):
+        interface.prefill_packed(q, cache, torch.zeros((1, 1), dtype=i32), cu, None, 4)
+    with pytest.raises(ValueError, match="too small"):
+        interface.prefill_packed(q, PagedKVCache(2, 2, "cpu", kv_dtype=F8), torch.zeros((1, 1), dtype=i32), cu, None, 40)
+    with pytest.raises(ValueError, match="GPU only"):
+        ops.PackedPlan(cu, None, 4, 4, 6)
