@@ -509,18 +509,19 @@ def _(page_table, seq_lens, free_pages, free_count, rows, num_pages):
 # needs no initialisation (each call writes the split partials it reads), and
 # calls on one stream are ordered, so they can share it.
 _DECODE_WS = {}
-_WS_BYTES = {}  # (batch, hq, hkv, max_seq_len) -> workspace bytes the split rule needs
+_WS_BYTES = {}  # (batch, hq, hkv, max_seq_len, 8-bit cache) -> workspace bytes the split rule needs
 
 
-def _decode_workspace(device, handle, B, hq, hkv, max_seq_len, L):
+def _decode_workspace(device, handle, B, hq, hkv, max_seq_len, L, q8=False):
     """(address, bytes) of the workspace of (device, stream), grown to what a
     call of this shape needs."""
-    shape = (B, hq, hkv, max_seq_len)
+    shape = (B, hq, hkv, max_seq_len, q8)
     nbytes = _WS_BYTES.get(shape)
     if nbytes is None:
         if len(_WS_BYTES) >= 4096:
             _WS_BYTES.clear()
-        nbytes = _WS_BYTES[shape] = int(L.atf_decode_workspace_bytes_even(B, hq, hkv, max_seq_len))
+        size = L.atf_decode_q8_workspace_bytes if q8 else L.atf_decode_workspace_bytes_even
+        nbytes = _WS_BYTES[shape] = int(size(B, hq, hkv, max_seq_len))
     key = (device.index, handle)
     ws = _DECODE_WS.get(key)
     if ws is None or ws[1] < nbytes:
@@ -611,7 +612,7 @@ def decode_paged_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tens
     L = _lib.lib()
     n = 0 if zhi is None else len(zhi)
     table = None if zhi is None else _table(zhi, _lib.SLICES if n == _lib.SLICES else _lib.LEVELS)
-    ws = _decode_workspace(dev, _lib.stream_of(dev), B, Hq, pool[1], int(max_seq_len), L)
+    ws = _decode_workspace(dev, _lib.stream_of(dev), B, Hq, pool[1], int(max_seq_len), L, True)
     out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
     _lib.launch(dev, L.atf_decode_paged_q8, out.data_ptr(), Hq * D, D, q.data_ptr(), q_sb, q_sh, kv_cache.data_ptr(),
                 kv_exps.data_ptr(), pool[0], page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), B, Hq,

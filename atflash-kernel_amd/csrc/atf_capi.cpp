@@ -123,6 +123,44 @@ void decode_split(int batch, int hkv, int max_seq_len, int* n_splits, int* pages
   *n_splits = (pages + pps - 1) / pps;
 }
 
+// The 8-bit decode: pages of a split and splits of the longest sequence.  A workgroup
+// streams a page in about 0.16 us when one runs on each of 256 CUs (two thirds of that
+// when few do), and costs as much as 16 pages to start and end; merging costs 25 (4 us).
+// With n splits a (sequence, kv head) pair there are `rounds` workgroups a CU:
+//   us = 0.16 (rounds (pages / n + 16) u + 25), u = 0.65 + 0.35 min(1, workgroups / 256).
+// Measured (us a call) at 1, 2, 3 and 5 rounds: 1 x 131072 OFF (28 / 4 heads) 30.2, 34.2,
+// 37.8, 46.3; 4 x 16384 (24 / 8) 28.1, 26.9, 33.9, 37.5; 40 x 8192 (28 / 4) 66, 60.3, 64.9,
+// 65.7; with fewer than 256 workgroups: 1 x 8192 (24 / 8), 256, 128 and 64 of them, 11.7, 12.8,
+// 15.3; 1 x 1003 with 32 and 8 10.6, 12.2.  The lengths of a batch are not known here, and
+// a ragged one is the better for smaller splits: of the choices within 6% of the best a
+// batch takes the finest (12 sequences of 1084 to 32768 tokens, 24 / 8 heads: 2, 5, 8
+// and 16 splits 109, 67, 45 and 37 us).  Not with more than 8 heads a kv head, whose
+// workgroups have a CU each (4 x 65536 at 32 / 2: 1 round 32.3, 2 rounds 41.1).
+void decode_q8_split(int batch, int hkv, int group, int max_seq_len, int* n_splits, int* pages_per_split) {
+  const int64_t pages = max_seq_len > 0 ? (max_seq_len + atf::kPage - 1) / atf::kPage : 1;
+  const int64_t pairs = static_cast<int64_t>(batch) * hkv;
+  const int64_t most = (pages + 15) / 16;  // a workgroup's waves take 16 pages at a time
+  auto cost = [&](int64_t n) {
+    const int64_t wgs = pairs * n, rounds = (wgs + 255) / 256, each = (pages + n - 1) / n;
+    const double u = 0.65 + 0.35 * static_cast<double>(std::min<int64_t>(wgs, 256)) / 256.0;
+    return static_cast<double>(rounds) * static_cast<double>(each + 16) * u + (n > 1 ? 25.0 : 0.0);
+  };
+  int64_t best = 1;
+  double low = cost(1);
+  constexpr int kRounds = 6;
+  for (int r = 1; r <= kRounds; ++r) {
+    const int64_t n = std::min(256 * r / pairs, most);
+    if (n > 1 && cost(n) < low) low = cost(best = n);
+  }
+  for (int r = 1; batch > 1 && group <= 8 && r <= kRounds; ++r) {
+    const int64_t n = std::min(256 * r / pairs, most);
+    if (n > best && cost(n) <= 1.06 * low) best = n;
+  }
+  const int64_t pps = (pages + best - 1) / best;
+  *pages_per_split = static_cast<int>(pps);
+  *n_splits = static_cast<int>((pages + pps - 1) / pps);
+}
+
 // Bytes of split partials ([ws_ml][ws_o], fp32): none with one split.
 size_t partial_bytes(int batch, int hkv, int ns) {
   if (ns <= 1) return 0;
@@ -611,7 +649,10 @@ int atf_decode_paged_slices_bf16(void* out, int64_t o_sb, int64_t o_sh, const vo
 }
 
 size_t atf_decode_q8_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_seq_len) {
-  return atf_decode_workspace_bytes_even(batch, num_q_heads, num_kv_heads, max_seq_len);
+  if (batch <= 0 || num_kv_heads <= 0 || max_seq_len <= 0) return 0;
+  int ns = 1, pps = 1;
+  decode_q8_split(batch, num_kv_heads, num_q_heads / num_kv_heads, max_seq_len, &ns, &pps);
+  return partial_bytes(batch, num_kv_heads, ns);
 }
 
 int atf_decode_paged_q8(void* out, int64_t o_sb, int64_t o_sh, const void* q, int64_t q_sb, int64_t q_sh,
@@ -632,9 +673,11 @@ int atf_decode_paged_q8(void* out, int64_t o_sb, int64_t o_sh, const void* q, in
                              num_q_heads, num_kv_heads, max_seq_len, zhi, zhi_entries == ATF_SLICES, sm_scale, rope_cs,
                              rope_max_pos, layout, &a))
     return r;
+  if (static_cast<int64_t>(num_pages) * num_kv_heads >= (int64_t(1) << 30))
+    return fail(ATF_ERR_UNSUPPORTED, "at most 2^30 - 1 blocks (pages x kv heads), got %d x %d", num_pages, num_kv_heads);
   a.kv_exps = kv_exps;
-  if (!set_spread_workspace(workspace, workspace_bytes, &a))
-    if (int r = set_workspace(workspace, workspace_bytes, &a)) return r;
+  decode_q8_split(batch, num_kv_heads, a.group, max_seq_len, &a.n_splits, &a.pages_per_split);
+  if (int r = set_workspace(workspace, workspace_bytes, &a)) return r;
   hipError_t e = atf::launch_decode_q8(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "8-bit decode launch");
   return ok();

@@ -2,12 +2,18 @@
 // attention with half its bytes.
 //
 // Mathematics.  A page's keys are K = code 2^eK and its values V = code 2^eV (e4m3
-// codes, one exponent per page, kv head and half), so S = scale q K^T and O =
-// softmax(S) V are formed as in decode_kernel once the codes have become bf16: e4m3
-// has 4 significant bits and the scales are powers of two, so code 2^e is a bf16
-// number exactly and nothing is rounded on the way (v_cvt_scalef32_pk_bf16_fp8: two
-// codes times the scale an instruction).  Q keeps its bf16 precision, which a product
-// on 8-bit operands would not leave it; the running maximum, the sum and O are fp32.
+// codes, one exponent per page, kv head and half).  S = scale q K^T, O = softmax(S) V on
+// bf16 matrix instructions: e4m3 has 4 significant bits and the scales are powers of
+// two, so code 2^e is a bf16 number exactly (v_cvt_scalef32_pk_bf16_fp8: two codes times
+// the scale an instruction).  Q (rotated in fp32) and P would lose bits as bf16, and so
+// are split in two: x = hi + lo, hi = bf16(x), lo = bf16(x - hi), 2^-17 of x left.  With
+// up to 8 query heads a kv head (kWide false) this costs no matrix instruction: columns
+// 0-7 of an MFMA hold the hi parts of the heads and columns 8-15 their lo parts, of Q
+// and of P alike, and the two halves of the result are added (S: a row rotation of the
+// lanes; O: once, at the end).  Larger groups take every MFMA twice.  The running
+// maximum, the sum and O are fp32; the output is rounded once.
+//   Error against 64 bits (2-norm): 1.7e-3, bf16's own; with Q and P rounded to bf16
+// it was 2.8e-3 to 4.3e-3.
 //
 // Layout (atf_common.h): a page's block is 4 KB, V and then K, in the order in which
 // the lanes of a wave take them: four loads of 16 bytes a lane, each 1 KB of
@@ -15,65 +21,48 @@
 //   K: load j, lane (token t = lane % 16, g = lane / 16): the two slices of level
 //      4j + g.  Slice i of it is the lane's share of MFMA 2j + i, whose 32 dims are
 //      slice i of levels 4j .. 4j + 3.
-//   V: load j, lane (row r, g): dims 8r + 4j .. + 3 of tokens 4g .. 4g + 3; dim d of them
-//      is the lane's share of MFMA 4j + d, whose row r is dim 8r + 4j + d.
+//   V: load j, lane (row r, g): dims 8r + 4j .. + 3 of tokens 4g .. 4g + 3; dim d of them,
+//      of two pages, is the lane's share of MFMA 4j + d, whose row r is dim 8r + 4j + d.
 // The window shortens the K read to whole levels (256 bytes); a last odd slice is
 // zeroed in registers with the per-key rule's.
+//
+// Work.  A sequence of P pages is cut into ceil(P / C) splits (C: a.pages_per_split, from
+// the call's sizes), page s, s + n, s + 2n, ... to split s of n; a workgroup of 8 waves
+// takes a split of a kv head, each wave two pages at a time.  So the splits of a ragged
+// batch are all about C pages, long sequences have more of them, and a sequence's results
+// do not depend on the lengths of others.  The registers of a wave stay below 128, so
+// that four share a SIMD and hide each other's chain of conversions, MFMAs and
+// exponentials, which is what bounds a wave; one pair of pages a wave in flight is
+// enough for the memory then.
 #include "atf_decode_common.h"
 
 namespace atf {
 
-// Pages in flight per wave: their registers are half of a bf16 page's.  The order of
-// a wave's pages is decode_kernel's, groups of kDecUnroll.
-constexpr int kQ8Unroll = 8;
-static_assert(kQ8Unroll % kDecUnroll == 0, "whole groups");
+constexpr int kQ8Waves = 8;
 
+// A page's block as a range-checked buffer: V, then the first ns slices of K (whole levels);
+// empty for a page past the sequence or an entry outside the pool.  What lies past the
+// range is zero without a memory request.
 struct Q8Page {
-  u32x4 k[2];
-  u32x4 v[2];
-  uint32_t e;  // eV | eK << 8
-  int n0;
-  bool mask;  // slices to zero by key
+  __amdgpu_buffer_rsrc_t block;
+  uint32_t exps;  // byte offset of the page's two exponents (past the buffer: none, read as 0)
 };
-
-// Local page of the split that is the wave's i-th.
-template <int kWaves>
-__device__ __forceinline__ int q8_local(int wave, int i) {
-  return kDecUnroll * (wave + kWaves * (i / kDecUnroll)) + i % kDecUnroll;
-}
-
-struct Q8Ref {
-  size_t blk;  // index of the (page, kv head) block
-  bool ok;
-};
-__device__ __forceinline__ Q8Ref q8_ref(const DecHot& hot, int h, int raw, bool in_split) {
+__device__ __forceinline__ Q8Page q8_page(const DecHot& hot, int h, int raw, bool in_seq, int ns) {
   const int pg = __builtin_amdgcn_readfirstlane(raw);
-  const bool ok = in_split && pg >= 0 && pg < hot.num_pages;
-  return Q8Ref{static_cast<size_t>(ok ? pg : 0) * hot.hkv + h, ok};
+  const bool ok = in_seq && static_cast<uint32_t>(pg) < static_cast<uint32_t>(hot.num_pages);
+  const uint32_t blk = ok ? static_cast<uint32_t>(pg) * hot.hkv + h : 0u;  // (below 2^31)
+  const uint8_t* base = reinterpret_cast<const uint8_t*>(hot.kv_cache) + static_cast<uint64_t>(blk) * kQ8BlockBytes;
+  const int range = __builtin_amdgcn_readfirstlane(ok ? kQ8HalfBytes + (ns + 1) / 2 * (kPage * 2 * kSliceDims) : 0);
+  return Q8Page{__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, range, kBufferWord3), ok ? 2 * blk : ~0u};
 }
-// The first ns slices of K (whole levels) and the exponents; ranges as in decode_kernel:
-// what lies past them is zero without a memory request.
-__device__ __forceinline__ void q8_load_k(const DecHot& hot, const DecodeArgs& a, const Q8Ref& ref, int ns, int lane,
-                                          Q8Page& p) {
-  const uint8_t* base = reinterpret_cast<const uint8_t*>(hot.kv_cache) + ref.blk * kQ8BlockBytes + kQ8HalfBytes;
-  const int range = __builtin_amdgcn_readfirstlane(ref.ok ? (ns + 1) / 2 * (kPage * 2 * kSliceDims) : 0);
-  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, range, kBufferWord3);
+__device__ __forceinline__ void q8_load(const __amdgpu_buffer_rsrc_t& block, int lane, int at, u32x4 (&x)[2]) {
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    p.k[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, (static_cast<uint32_t>(lane) << 4) + j * 1024u,
-                                                                             0, kLoadStream));
-  const __amdgpu_buffer_rsrc_t re =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.kv_exps) + 2 * ref.blk, 0, ref.ok ? 2 : 0, kBufferWord3);
-  p.e = static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(re, 0, 0, 0));
+    x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                         block, (static_cast<uint32_t>(lane) << 4) + at + j * 1024u, 0, kLoadStream));
 }
-__device__ __forceinline__ void q8_load_v(const DecHot& hot, const Q8Ref& ref, int lane, Q8Page& p) {
-  const uint8_t* base = reinterpret_cast<const uint8_t*>(hot.kv_cache) + ref.blk * kQ8BlockBytes;
-  const __amdgpu_buffer_rsrc_t rv =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, ref.ok ? kQ8HalfBytes : 0, kBufferWord3);
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    p.v[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (static_cast<uint32_t>(lane) << 4) + j * 1024u,
-                                                                             0, kLoadStream));
+__device__ __forceinline__ uint32_t q8_exps(const __amdgpu_buffer_rsrc_t& all, const Q8Page& p) {
+  return static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(all, p.exps, 0, 0));  // eV | eK << 8
 }
 
 // 2^e as a float, e the signed byte at bit kAt of w (the cache's exponents are normal floats).
@@ -87,67 +76,141 @@ __device__ __forceinline__ u32x2 q8_bf16(uint32_t codes, float scale) {
   return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))};
 }
-
-// The slices a page reads (page_slices), and whether some are to be zeroed by key: a
-// boundary inside the page, or a last level of which only the first slice is read.
-template <bool kPerKey>
-__device__ __forceinline__ void q8_slices(const DecodeArgs& a, int zc, int p, int N, int& ns, bool& mask) {
-  page_slices<kPerKey>(a, zc, p, N, ns, mask);
-  if (kPerKey) mask = mask || (ns & 1) != 0;
+__device__ __forceinline__ bf16x8 join(const u32x2& lo, const u32x2& hi) {
+  return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
 }
 
-// Decode of one split (pages `ord`) of sequence b: this wave's pages (kWaves waves
-// take the split), its partial (m, l, o) to row `out` of sh_o, sh_m and sh_l.
-template <bool kPerKey, int kWaves>
-__device__ __forceinline__ void decode_pages_q8(const DecHot& hot, const DecodeArgs& a, int h, int b, int N,
-                                                const int32_t* row, const PageOrder& ord, int wave, int out,
-                                                int (&ent)[kQ8Unroll], float* sh_o, float* sh_m, float* sh_l) {
-  const int count = ord.count, po = ord.po, pm = ord.pm;
+// Two values less `m` times their bf16 parts (m = 0: as they are), as bf16.
+__device__ __forceinline__ uint32_t pack_part(float x, float y, float m) {
+  const uint32_t w = pack_bf16x2(x, y);
+  return pack_bf16x2(__builtin_fmaf(-m, __uint_as_float(w << 16), x), __builtin_fmaf(-m, __uint_as_float(w & 0xffff0000u), y));
+}
+
+// The slices a page reads, counted by lane (zc: page_slices; the level rule's table holds
+// each level's entry for its two slices, and level 0 has no limit), and whether some of
+// them are to be zeroed by key: a boundary inside the page, or a last level of which
+// only the first slice is read.
+template <bool kPerKey>
+__device__ __forceinline__ void q8_slices(int zc, int p, int N, int& ns, bool& mask) {
+  const int z_young = (N - 1) - (p * kPage + kPage - 1);
+  if constexpr (kPerKey) {
+    const int cy = __builtin_popcountll(__builtin_amdgcn_ballot_w64(zc >= z_young));
+    const int co = __builtin_popcountll(__builtin_amdgcn_ballot_w64(zc >= z_young + kPage - 1));
+    ns = cy;
+    mask = co != cy || (cy & 1) != 0;
+  } else {
+    ns = __builtin_popcountll(__builtin_amdgcn_ballot_w64(zc >= max(z_young, 0)));
+    mask = false;
+  }
+}
+
+// Splits of a sequence of `pages` pages.
+__device__ __forceinline__ int q8_splits(int pages, int pages_per_split, int n_splits) {
+  return n_splits == 1 ? 1 : max(1, (pages + pages_per_split - 1) / pages_per_split);
+}
+
+template <bool kPerKey, bool kWide>
+__global__ __launch_bounds__(kQ8Waves * 64) __attribute__((amdgpu_waves_per_eu(kWide ? 2 : 4)))
+void decode_q8_kernel(const int32_t* page_table, const int32_t* seq_lens, const uint16_t* kv_cache, int max_pages,
+                      int pages_per_split, int max_seq_len, int hkv, int num_pages, int n_splits, DecodeArgs a) {
+  const DecHot hot{page_table, seq_lens, kv_cache, max_pages, pages_per_split, max_seq_len, hkv, num_pages, n_splits};
+  // wave partials
+  __shared__ __attribute__((aligned(16))) float sh_o[kQ8Waves * kDecMaxGroup * kD];
+  __shared__ float sh_m[kQ8Waves * kDecMaxGroup], sh_l[kQ8Waves * kDecMaxGroup];
+  // The splits are turned by head and sequence: workgroups go to the XCDs in turn, and
+  // without this the sequences that have few splits would all lie on the first ones (12
+  // sequences of 1084 to 32768 tokens, 24 / 8 heads, vec8 k = 2: 66.5 us a call).
+  const int h = blockIdx.y, b = blockIdx.z, s = (blockIdx.x + h + b) % n_splits;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
   const float NEG_INF = -__builtin_huge_valf();
   const float c = a.scale_log2;
-
-  Q8Page pr[kQ8Unroll];
-  int zc = INT32_MIN;  // lane s < 16: zhi8[s] (page_slices)
+  // Pair i of this wave is pages p and p + n, p = s + 2 n (wave + 8 i).  The entries of the
+  // first two pairs are fetched together with the length, as if the sequence had the
+  // call's longest length (a round trip less where it has as many splits).
+  const int32_t* row = page_table + static_cast<int64_t>(b) * max_pages;
+  int ent[2], ent_next[2];
 #pragma unroll
-  for (int s = 0; s < kSlices && kPerKey; ++s)
-    if (lane == s) zc = a.st.zhi[s];
-#pragma unroll
-  for (int u = 0; u < kQ8Unroll; ++u) {
-    const int j = q8_local<kWaves>(wave, u), p = po + pm * j;
-    int ns;
-    q8_slices<kPerKey>(a, zc, p, N, ns, pr[u].mask);
-    pr[u].n0 = p * kPage;
-    const Q8Ref ref = q8_ref(hot, h, ent[u], j < count);
-    q8_load_k(hot, a, ref, ns, lane, pr[u]);
-    q8_load_v(hot, ref, lane, pr[u]);
+  for (int u = 0; u < 2; ++u) {
+    ent[u] = row[min(s + n_splits * (2 * wave + u), max_pages - 1)];
+    ent_next[u] = row[min(s + n_splits * (2 * (wave + kQ8Waves) + u), max_pages - 1)];
   }
+  const int N = max(0, min(seq_lens[b], max_seq_len));
+  const int n_pages = (N + kPage - 1) / kPage;
+  const int n = q8_splits(n_pages, pages_per_split, n_splits);
+  if (s >= n) return;
+  const int step = 2 * kQ8Waves * n;
+  int p = s + 2 * n * wave;
+  auto fetch = [&](int page) { return row[max(min(page, n_pages - 1), 0)]; };
+  if (n != n_splits) {
 #pragma unroll
-  for (int u = 0; u < kQ8Unroll; ++u) ent[u] = dec_fetch_entry(row, ord, q8_local<kWaves>(wave, kQ8Unroll + u));
+    for (int u = 0; u < 2; ++u) {
+      ent[u] = fetch(p + u * n);
+      ent_next[u] = fetch(p + step + u * n);
+    }
+  }
+  int zc = INT32_MIN;  // lane s < 16: zhi8[s], the others a limit that no age meets
+#pragma unroll
+  for (int i = 0; i < kSlices; ++i)
+    if (lane == i) zc = !kPerKey && i < 2 ? INT32_MAX : a.st.zhi[i];
+  const __amdgpu_buffer_rsrc_t all_exps =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.kv_exps), 0, 2 * num_pages * hkv, kBufferWord3);
 
-  // Q^T fragments: lane holds query head t; fragment m is slice 2g + m % 2 + 8 (m / 2)
-  u32x4 Qf[4];
+  // Entries of the next pair lie in `ent` when a pair is worked on; those of the one
+  // behind it are requested before the next pair's loads.
+  u32x4 K[2][2], V[2][2];
+  uint32_t e[2];
+  bool mask[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    int ns;
+    q8_slices<kPerKey>(zc, p + u * n, N, ns, mask[u]);
+    const Q8Page page = q8_page(hot, h, ent[u], p + u * n < n_pages, ns);
+    e[u] = q8_exps(all_exps, page);
+    q8_load(page.block, lane, kQ8HalfBytes, K[u]);
+    q8_load(page.block, lane, 0, V[u]);
+    ent[u] = ent_next[u];
+  }
+
+  // Q^T fragments: fragment m is slice 2g + m % 2 + 8 (m / 2) of a head.  Lane t holds head
+  // t % 8, its hi part for t < 8, its lo part above; kWide: head t, both parts.
+  u32x4 Qf[4], Ql[kWide ? 4 : 1];
   {
-    const int qh = h * a.group + min(t, a.group - 1);
-    const bool valid = t < a.group && N > 0;
+    const int head = kWide ? t : t & 7;
+    const int qh = h * a.group + min(head, a.group - 1);
+    const bool valid = head < a.group && N > 0;
+    const float part = !kWide && t >= 8 ? 1.f : 0.f;
     const uint16_t* qrow = a.q + static_cast<int64_t>(b) * a.q_sb + static_cast<int64_t>(qh) * a.q_sh;
+    u32x4 x[4];
     if (a.layout == kLayoutHalfSplit) {
 #pragma unroll
-      for (int m = 0; m < 4; ++m) Qf[m] = load_slice(qrow, kLayoutHalfSplit, 2 * g + (m & 1) + 8 * (m >> 1));
+      for (int m = 0; m < 4; ++m) x[m] = load_slice(qrow, kLayoutHalfSplit, 2 * g + (m & 1) + 8 * (m >> 1));
     } else {
 #pragma unroll
-      for (int m = 0; m < 4; ++m) Qf[m] = load_slice(qrow, kLayoutSortedPair, 2 * g + (m & 1) + 8 * (m >> 1));
-    }
-    if (a.rope_cs != nullptr) {
-      float cs[4][8];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) load_cs4(a.rope_cs, max(N - 1, 0), slice_pair0(2 * g + (m & 1) + 8 * (m >> 1)), cs[m]);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) Qf[m] = rope_slice(Qf[m], cs[m]);
+      for (int m = 0; m < 4; ++m) x[m] = load_slice(qrow, kLayoutSortedPair, 2 * g + (m & 1) + 8 * (m >> 1));
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
-      if (!valid) Qf[m] = u32x4{0u, 0u, 0u, 0u};
+    for (int m = 0; m < 4; ++m) {
+      float v[8], y[8];
+      unpack8(x[m], v);
+      if (a.rope_cs != nullptr) {
+        float cs[8];
+        load_cs4(a.rope_cs, max(N - 1, 0), slice_pair0(2 * g + (m & 1) + 8 * (m >> 1)), cs);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[i] = rope_first(v[i], v[4 + i], cs[2 * i], cs[2 * i + 1]);
+          y[4 + i] = rope_second(v[i], v[4 + i], cs[2 * i], cs[2 * i + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = v[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        Qf[m][i] = valid ? pack_part(y[2 * i], y[2 * i + 1], part) : 0u;
+        if constexpr (kWide) Ql[m][i] = valid ? pack_part(y[2 * i], y[2 * i + 1], 1.f) : 0u;
+      }
+    }
   }
   // per-key rule: the distance limits of the lane's slices
   int zl[4] = {0, 0, 0, 0};
@@ -156,177 +219,179 @@ __device__ __forceinline__ void decode_pages_q8(const DecHot& hot, const DecodeA
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (g == i) zl[m] = a.st.zhi[2 * i + (m & 1) + 8 * (m >> 1)];
+  const float p_part = !kWide && t >= 8 ? 1.f : 0.f;
 
   f32x4 O[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) O[e] = f32x4{};
   float m_run = NEG_INF, l_run = 0.f;
 
-  for (int i0 = 0; q8_local<kWaves>(wave, i0) < count; i0 += kQ8Unroll) {
+  float msc = 0.f;   // m_run in log2 units
+  bool first = true;
+  for (; p < n_pages; p += step) {
 #pragma unroll
-    for (int u = 0; u < kQ8Unroll; ++u) {
-      if (q8_local<kWaves>(wave, i0 + u) >= count) break;
-      Q8Page& r = pr[u];
-      if (kPerKey && r.mask) {
-        const int age = (N - 1) - (r.n0 + t);
+    for (int u = 0; u < 2; ++u) ent_next[u] = fetch(p + 2 * step + u * n);
+    f32x4 S[2];
+    float sv[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (kPerKey && mask[u]) {
+        const int age = (N - 1) - ((p + u * n) * kPage + t);
 #pragma unroll
         for (int m = 0; m < 4; ++m)
           if (age > zl[m]) {
-            r.k[m >> 1][2 * (m & 1)] = 0u;
-            r.k[m >> 1][2 * (m & 1) + 1] = 0u;
+            K[u][m >> 1][2 * (m & 1)] = 0u;
+            K[u][m >> 1][2 * (m & 1) + 1] = 0u;
           }
       }
-      const float sk = q8_scale<8>(r.e), sv = q8_scale<0>(r.e);
-      f32x4 S = f32x4{};
+      const float sk = q8_scale<8>(e[u]);
+      sv[u] = q8_scale<0>(e[u]);
+      S[u] = f32x4{};
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        const u32x2 lo = q8_bf16(r.k[m >> 1][2 * (m & 1)], sk), hi = q8_bf16(r.k[m >> 1][2 * (m & 1) + 1], sk);
-        S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}),
-                                                    __builtin_bit_cast(bf16x8, Qf[m]), S, 0, 0, 0);
+        const bf16x8 A = join(q8_bf16(K[u][m >> 1][2 * (m & 1)], sk), q8_bf16(K[u][m >> 1][2 * (m & 1) + 1], sk));
+        S[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, __builtin_bit_cast(bf16x8, Qf[m]), S[u], 0, 0, 0);
+        if constexpr (kWide) S[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, __builtin_bit_cast(bf16x8, Ql[m]), S[u], 0, 0, 0);
       }
-      // S lane layout: query head t, tokens 4g + i
-      const int tok0 = r.n0 + 4 * g;
-      const bool tail = r.n0 + kPage > N;
-      const int jn = q8_local<kWaves>(wave, i0 + kQ8Unroll + u);
-      const bool reload = jn < count;
-      bool mask_n = false;
-      Q8Ref ref_n{0, false};
-      if (reload) {
-        int ns;
-        q8_slices<kPerKey>(a, zc, po + pm * jn, N, ns, mask_n);
-        ref_n = q8_ref(hot, h, ent[u], true);
-        q8_load_k(hot, a, ref_n, ns, lane, r);
-      }
-      float mx = NEG_INF;
+    }
+    // K of the next pair (past the sequence: nothing)
+    Q8Page next[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (tail && tok0 + i >= N) S[i] = NEG_INF;
-        mx = fmaxf(mx, S[i]);
-      }
-      if (tail) {  // V codes of tokens past N to zero, so that 0 * V stays 0
-        const int live = max(0, min(N - tok0, 4));
-        const uint32_t keep = live == 4 ? 0xffffffffu : (1u << (8 * live)) - 1u;
+    for (int u = 0; u < 2; ++u) {
+      const int q = p + step + u * n;
+      int ns;
+      q8_slices<kPerKey>(zc, q, N, ns, mask[u]);
+      next[u] = q8_page(hot, h, ent[u], q < n_pages, ns);
+      e[u] = q8_exps(all_exps, next[u]);
+      q8_load(next[u].block, lane, kQ8HalfBytes, K[u]);
+    }
+    // S lane layout: query head t (hi part; lo part in t + 8), tokens 4g + i
+    if constexpr (!kWide) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[u][i] += row_ror<8>(S[u][i]);
+    }
+    if ((p + n + 1) * kPage > N) {  // the sequence ends in this pair, or between its pages
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int left = N - (p + u * n) * kPage - 4 * g;  // of the lane's four tokens
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i >= left) S[u][i] = NEG_INF;
+        // V codes past the sequence to zero, so that 0 * V stays 0
+        const uint32_t keep = left >= 4 ? 0xffffffffu : (1u << (8 * max(left, 0))) - 1u;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int d = 0; d < 4; ++d) r.v[j][d] &= keep;
+          for (int w = 0; w < 4; ++w) V[u][j][w] &= keep;
       }
+    }
+    // P against the reference maximum so far.  It moves only where a lane's P add up to
+    // more than 256 (a score above it by 5 or more), and with the first pair.
+    float P[2][4];
+    auto exps = [&] {
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          P[u][i] = fast_exp2(__builtin_fmaf(S[u][i], c, -msc));
+          sum += P[u][i];
+        }
+      return sum;
+    };
+    float sum = exps();
+    if (__builtin_amdgcn_ballot_w64(first || !(sum <= 256.f)) != 0) {
+      float mx = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
+                       fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
       mx = quad_max(mx);
-      const bool grow = (mx - m_run) * c > 8.f;  // the lazy reference max of decode_kernel
-      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-        const float alpha = !grow ? 1.f : (m_run == NEG_INF ? 0.f : fast_exp2((m_run - mx) * c));
+      if (mx > m_run) {
+        const float alpha = m_run == NEG_INF ? 0.f : fast_exp2((m_run - mx) * c);
         l_run *= alpha;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) O[e] *= alpha;
-        m_run = grow ? mx : m_run;
+        for (int d = 0; d < 8; ++d) O[d] *= alpha;
+        m_run = mx;
+        msc = mx * c;
       }
-      const float msc = (m_run == NEG_INF) ? 0.f : m_run * c;
-      float pv[4];
-      float ls = 0.f;
+      first = false;
+      sum = exps();
+    }
+    l_run += sum;
+    u32x2 Ph[2], Pl[kWide ? 2 : 1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pv[i] = fast_exp2(__builtin_fmaf(S[i], c, -msc));
-        ls += pv[i];
-      }
-      l_run += ls;
-      const s16x4 pb = __builtin_bit_cast(s16x4, u32x2{pack_bf16x2(pv[0], pv[1]), pack_bf16x2(pv[2], pv[3])});
+    for (int u = 0; u < 2; ++u) {
+      Ph[u] = u32x2{pack_part(P[u][0], P[u][1], p_part), pack_part(P[u][2], P[u][3], p_part)};
+      if constexpr (kWide) Pl[u] = u32x2{pack_part(P[u][0], P[u][1], 1.f), pack_part(P[u][2], P[u][3], 1.f)};
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        O[e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, q8_bf16(r.v[e >> 2][e & 3], sv)), pb,
-                                                         O[e], 0, 0, 0);
-      if (reload) {
-        q8_load_v(hot, ref_n, lane, r);
-        r.n0 = (po + pm * jn) * kPage;
-        r.mask = mask_n;
-        ent[u] = dec_fetch_entry(row, ord, q8_local<kWaves>(wave, i0 + 2 * kQ8Unroll + u));
-      }
+    for (int d = 0; d < 8; ++d) {
+      const bf16x8 A = join(q8_bf16(V[0][d >> 2][d & 3], sv[0]), q8_bf16(V[1][d >> 2][d & 3], sv[1]));
+      O[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, join(Ph[0], Ph[1]), O[d], 0, 0, 0);
+      if constexpr (kWide) O[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, join(Pl[0], Pl[1]), O[d], 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      q8_load(next[u].block, lane, 0, V[u]);
+      ent[u] = ent_next[u];
     }
   }
 
+  // ---- the split's partial: combine the wave partials in LDS ----
   const float l_tot = quad_sum(l_run);
+  if constexpr (!kWide) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) O[e][i] += row_ror<8>(O[e][i]);
+  }
   if (t < a.group) {
     // O[e][i]: dim 8 (4g + i) + e
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float* o = &sh_o[(out * kDecMaxGroup + t) * kD + 8 * (4 * g + i)];
+      float* o = &sh_o[(wave * kDecMaxGroup + t) * kD + 8 * (4 * g + i)];
       *reinterpret_cast<f32x4*>(o) = f32x4{O[0][i], O[1][i], O[2][i], O[3][i]};
       *reinterpret_cast<f32x4*>(o + 4) = f32x4{O[4][i], O[5][i], O[6][i], O[7][i]};
     }
     if (lane < 16) {
-      sh_m[out * kDecMaxGroup + t] = m_run;
-      sh_l[out * kDecMaxGroup + t] = l_tot;
+      sh_m[wave * kDecMaxGroup + t] = m_run;
+      sh_l[wave * kDecMaxGroup + t] = l_tot;
     }
   }
-}
-
-template <int kWaves>
-__device__ __forceinline__ void q8_first_entries(const int32_t* row, const PageOrder& ord, int wave, int max_pages,
-                                                 int (&ent)[kQ8Unroll]) {
-#pragma unroll
-  for (int u = 0; u < kQ8Unroll; ++u) ent[u] = row[min(ord.po + ord.pm * q8_local<kWaves>(wave, u), max_pages - 1)];
-}
-
-template <bool kPerKey, int kWaves>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
-void decode_q8_kernel(const int32_t* page_table, const int32_t* seq_lens, const uint16_t* kv_cache, int max_pages,
-                      int pages_per_split, int max_seq_len, int hkv, int num_pages, int n_splits, DecodeArgs a) {
-  const DecHot hot{page_table, seq_lens, kv_cache, max_pages, pages_per_split, max_seq_len, hkv, num_pages, n_splits};
-  __shared__ __attribute__((aligned(16))) float sh_o[kWaves * kDecMaxGroup * kD];
-  __shared__ float sh_m[kWaves * kDecMaxGroup], sh_l[kWaves * kDecMaxGroup];
-  const int s = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  PageOrder ord = page_order(s, n_splits, pages_per_split);
-  int ent[kQ8Unroll];
-  const int32_t* row = page_table + static_cast<int64_t>(b) * max_pages;
-  q8_first_entries<kWaves>(row, ord, wave, max_pages, ent);
-  const int N = max(0, min(seq_lens[b], max_seq_len));
-  set_page_count(ord, s, n_splits, pages_per_split, (N + kPage - 1) / kPage);
-  decode_pages_q8<kPerKey, kWaves>(hot, a, h, b, N, row, ord, wave, wave, ent, sh_o, sh_m, sh_l);
   __syncthreads();
-  store_split<kWaves>(a, (static_cast<int64_t>(b) * hkv + h) * a.n_splits + s, h, b, sh_o, sh_m, sh_l);
+  store_split<kQ8Waves>(a, (static_cast<int64_t>(b) * hkv + h) * n_splits + s, n == 1, h, b, sh_o, sh_m, sh_l);
 }
 
-// A workgroup per wave of a split, as decode_wave_kernel.
-template <bool kPerKey>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
-void decode_q8_wave_kernel(const int32_t* page_table, const int32_t* seq_lens, const uint16_t* kv_cache, int max_pages,
-                           int pages_per_split, int max_seq_len, int hkv, int num_pages, int n_splits, DecodeArgs a) {
-  const DecHot hot{page_table, seq_lens, kv_cache, max_pages, pages_per_split, max_seq_len, hkv, num_pages, n_splits};
-  const int s = blockIdx.x, h = blockIdx.y % hkv, wave = blockIdx.y / hkv;
-  int b = blockIdx.z;
-  if (a.by_length) b = a.batch <= 64 ? nth_longest<1>(seq_lens, a.batch, max_seq_len, b)
-                                     : nth_longest<kDecSpreadBatch / 64>(seq_lens, a.batch, max_seq_len, b);
-  PageOrder ord = page_order(s, n_splits, pages_per_split);
-  int ent[kQ8Unroll];
-  const int32_t* row = page_table + static_cast<int64_t>(b) * max_pages;
-  q8_first_entries<kDecWaves>(row, ord, wave, max_pages, ent);
-  const int N = max(0, min(seq_lens[b], max_seq_len));
-  set_page_count(ord, s, n_splits, pages_per_split, (N + kPage - 1) / kPage);
-  const int64_t unit = ((static_cast<int64_t>(b) * hkv + h) * n_splits + s) * kDecWaves + wave;
-  float* ml = a.ws_ml + unit * 2 * a.group;
-  decode_pages_q8<kPerKey, kDecWaves>(hot, a, h, b, N, row, ord, wave, 0, ent, a.ws_o + unit * a.group * kD, ml,
-                                      ml + a.group);
+// The merge of the splits that each sequence has (those with one have written their output).
+__global__ __launch_bounds__(512) void decode_q8_merge_kernel(const int32_t* seq_lens, int pages_per_split, int max_seq_len,
+                                                              const float* ws_ml, const float* ws_o, int n_splits, int group,
+                                                              int hkv, float scale_log2, uint16_t* out, int64_t o_sb,
+                                                              int64_t o_sh) {
+  const int N = max(0, min(seq_lens[blockIdx.z], max_seq_len));
+  const int n = q8_splits((N + kPage - 1) / kPage, pages_per_split, n_splits);
+  if (n > 1) merge_splits<false>(MergeArgs{ws_ml, ws_o, out, o_sb, o_sh, n_splits, group, hkv, scale_log2}, n);
 }
 
 hipError_t launch_decode_q8(const DecodeArgs& a, hipStream_t s) {
   if (a.batch <= 0) return hipSuccess;
-#define ATF_Q8_LAUNCH(K, GRID, THREADS)                                                                              \
-  hipLaunchKernelGGL(K, GRID, dim3(THREADS), 0, s, a.page_table, a.seq_lens, a.kv_cache, a.max_pages,                \
-                     a.pages_per_split, a.max_seq_len, a.hkv, a.num_pages, a.n_splits, a)
-  const dim3 grid(a.n_splits, a.hkv, a.batch), wgrid(a.n_splits, a.hkv * kDecWaves, a.batch);
-  if (a.spread) {
-    if (a.per_key) ATF_Q8_LAUNCH(decode_q8_wave_kernel<true>, wgrid, 64);
-    else ATF_Q8_LAUNCH(decode_q8_wave_kernel<false>, wgrid, 64);
-  } else if (a.waves == kDecWaves) {
-    if (a.per_key) ATF_Q8_LAUNCH((decode_q8_kernel<true, kDecWaves>), grid, kDecWaves * 64);
-    else ATF_Q8_LAUNCH((decode_q8_kernel<false, kDecWaves>), grid, kDecWaves * 64);
+  const dim3 grid(a.n_splits, a.hkv, a.batch);
+#define ATF_Q8_LAUNCH(PK, WIDE)                                                                                         \
+  hipLaunchKernelGGL((decode_q8_kernel<PK, WIDE>), grid, dim3(kQ8Waves * 64), 0, s, a.page_table, a.seq_lens, a.kv_cache, \
+                     a.max_pages, a.pages_per_split, a.max_seq_len, a.hkv, a.num_pages, a.n_splits, a)
+  if (a.group > 8) {
+    if (a.per_key) ATF_Q8_LAUNCH(true, true); else ATF_Q8_LAUNCH(false, true);
   } else {
-    if (a.per_key) ATF_Q8_LAUNCH((decode_q8_kernel<true, kDecWavesShort>), grid, kDecWavesShort * 64);
-    else ATF_Q8_LAUNCH((decode_q8_kernel<false, kDecWavesShort>), grid, kDecWavesShort * 64);
+    if (a.per_key) ATF_Q8_LAUNCH(true, false); else ATF_Q8_LAUNCH(false, false);
   }
 #undef ATF_Q8_LAUNCH
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  return launch_decode_merge(a, s);
+  if (a.n_splits > 1) {
+    hipLaunchKernelGGL(decode_q8_merge_kernel, dim3(kMergeChunks, a.hkv, a.batch), dim3(512), 0, s, a.seq_lens,
+                       a.pages_per_split, a.max_seq_len, a.ws_ml, a.ws_o, a.n_splits, a.group, a.hkv, a.scale_log2, a.out,
+                       a.o_sb, a.o_sh);
+    return hipGetLastError();
+  }
+  return hipSuccess;
 }
 
 }  // namespace atf

@@ -201,3 +201,13 @@ def test_tables_and_packed_operators_refuse():
         interface.prefill_packed(q, PagedKVCache(2, 2, "cpu", kv_dtype=F8), torch.zeros((1, 1), dtype=i32), cu, None, 40)
     with pytest.raises(ValueError, match="GPU only"):
         ops.PackedPlan(cu, None, 4, 4, 6)
+
+
+def test_decode_workspace_holds_every_split(no_gpu):
+    # partials of (batch, kv head, split): 16 rows of 130 floats; none where a sequence is one split
+    for shape in ((1, 28, 4, 131072), (12, 24, 8, 32768), (40, 28, 4, 8192), (1, 24, 8, 1003), (64, 32, 8, 4096), (1, 4, 4, 16),
+                  (300, 8, 8, 5000), (4, 32, 2, 65536), (1, 28, 4, 1 << 20)):
+        size = no_gpu.atf_decode_q8_workspace_bytes(*shape)
+        unit = shape[0] * shape[2] * 16 * 130 * 4
+        assert size % unit == 0 and size // unit <= max(1, -(-shape[3] // 16)) and size <= 64 << 20
+    assert no_gpu.atf_decode_q8_workspace_bytes(1, 4, 4, 16) == 0 == no_gpu.atf_decode_q8_workspace_bytes(0, 4, 4, 16)
