@@ -56,7 +56,10 @@ SIGNATURES = {
     "atf_prefill_bf16": (_i, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i, _p, _i,
                               _i, _i, _i, _i, _i, _i, _p, _f, _p, _i, _i, _p]),
     "atf_prefill_plan_bytes": (_sz, [_i, _i, _i]),
-    "atf_prefill_plan": (_i, [_p, _sz, _p, _p, _i, _i, _i, _i, _p, _i, _p, _p]),
+    "atf_prefill_plan": (_i, [_p, _sz, _p, _p, _i, _i, _i, _i, _p]),
+    "atf_flash_packed_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "atf_flash_packed_bf16": (_i, [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i, _i, _i, _i,
+                                   _i, _p, _f, _p, _i, _i, _p, _sz, _p]),
     "atf_prefill_packed_bf16": (_i, [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i,
                                      _p, _f, _p, _i, _i, _p, _sz, _p]),
     "atf_extend_tables": (_i, [_p, _i, _p, _p, _p, _i, _p, _i, _i, _i, _p, _p, _p, _p, _p, _p]),
@@ -156,16 +159,6 @@ def ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def launch(device, entry, *args):
-    """entry(*args, stream): a library call on the current stream of `device`, made
-    with that device current (a kernel is launched on the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(entry(*args, stream_of(device)))
-    else:
-        with torch.cuda.device(device):
-            check(entry(*args, stream_of(device)))
-
-
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -174,3 +167,22 @@ def stream_of(device):
     if _RAW_STREAM is not None and device.index is not None:
         return _RAW_STREAM(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(index):
+    """The current HIP stream of the GPU `index`, as an int handle."""
+    if _RAW_STREAM is not None:
+        return _RAW_STREAM(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def launch(index, entry, *args):
+    """entry(*args, stream): a library call on the current stream of the GPU `index`,
+    made with that device current (a kernel is launched on the current device)."""
+    if index == torch._C._cuda_getDevice():
+        code = entry(*args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = entry(*args, raw_stream(index))
+    if code != ATF_OK:
+        check(code)

@@ -51,6 +51,8 @@ def _zhi_list(zhi, sizes=(_lib.LEVELS,)):
     decode also the per-slice vec8 table (SLICES entries)."""
     if zhi is None:
         return None
+    if type(zhi) is tuple and len(zhi) in sizes:
+        return zhi  # (cannot change: its array is found by identity, ops._table)
     vals = [int(x) for x in (zhi.tolist() if isinstance(zhi, torch.Tensor) else zhi)]
     if len(vals) not in sizes:
         raise ValueError(f"window table must have {' or '.join(map(str, sizes))} entries, got {len(vals)}")

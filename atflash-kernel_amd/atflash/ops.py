@@ -130,43 +130,62 @@ def _(kv_cache, k, v, start_pos, page_table, rope_cs, layout):
 _F8 = torch.float8_e4m3fn
 
 
+# The checks below run on every call: the passing case is one test each, what is wrong
+# is found out behind it.
+
 def _one_device(first, *ts):
-    """The GPU that all of these tensors are on (None: an absent one)."""
-    dev = first.device
-    for t in (first, *ts):
-        if t is not None and t.device != dev:
-            raise ValueError(f"the tensors of a call must be on one device (got {dev} and {t.device})")
-    if dev.type != "cuda":
-        raise ValueError("atflash ops run on the GPU only (got a tensor on %s)" % dev)
-    return dev
+    """The index of the GPU that all of these tensors are on (None: an absent one)."""
+    i = first.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != i:
+            raise ValueError(f"the tensors of a call must be on one device (got {first.device} and {t.device})")
+    if i < 0:
+        for t in ts:
+            if t is not None and t.device != first.device:
+                raise ValueError(f"the tensors of a call must be on one device (got {first.device} and {t.device})")
+        raise ValueError("atflash ops run on the GPU only (got a tensor on %s)" % first.device)
+    return i
+
+
+_Q8_BLOCK = _lib.KV_BLOCK_SHAPE
 
 
 def _check_cache_q8(kv_cache, kv_exps):
     s = kv_cache.shape
+    if (kv_cache.dtype == _F8 and len(s) == 4 and s[2:] == _Q8_BLOCK and kv_cache.is_contiguous()
+            and kv_exps.dtype == torch.int8 and kv_exps.shape == (s[0], s[1], 2) and kv_exps.is_contiguous()):
+        return s
     _need(kv_cache.dtype == _F8, "the 8-bit kv_cache must be float8_e4m3fn")
-    _need(len(s) == 4 and tuple(s[2:]) == _lib.KV_BLOCK_SHAPE, "kv_cache must be [num_pages, num_kv_heads, 2, 2048]")
+    _need(len(s) == 4 and s[2:] == _Q8_BLOCK, "kv_cache must be [num_pages, num_kv_heads, 2, 2048]")
     _need(kv_cache.is_contiguous(), "kv_cache must be contiguous")
-    _need(kv_exps.dtype == torch.int8 and kv_exps.shape == (s[0], s[1], 2) and kv_exps.is_contiguous(),
-          "kv_exps must be contiguous int8 [num_pages, num_kv_heads, 2]")
+    raise ValueError("kv_exps must be contiguous int8 [num_pages, num_kv_heads, 2]")
 
 
 def _check_rows(k, v, dims, hkv):
-    names = {3: "[T, Hkv, 128]", 4: "[B, T, Hkv, 128]"}
+    """The strides of k and v, rows [.., Hkv, 128] of bf16."""
+    s, ks, vs = k.shape, k.stride(), v.stride()
+    if (len(s) == dims and v.shape == s and s[-1] == _lib.HEAD_DIM and s[-2] == hkv and ks[-1] == 1 and vs[-1] == 1
+            and k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16):
+        return ks, vs
     _need(k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16, "k and v must be bf16")
-    _need(k.dim() == dims and v.shape == k.shape and k.shape[-1] == _lib.HEAD_DIM,
-          f"k and v must be {names[dims]} of equal shape")
-    _need(k.shape[-2] == hkv, "k heads must equal the cache's kv heads")
-    _need(k.stride(-1) == 1 and v.stride(-1) == 1, "last dim of k and v must be contiguous")
+    _need(len(s) == dims and v.shape == s and s[-1] == _lib.HEAD_DIM,
+          "k and v must be %s of equal shape" % {3: "[T, Hkv, 128]", 4: "[B, T, Hkv, 128]"}[dims])
+    _need(s[-2] == hkv, "k heads must equal the cache's kv heads")
+    raise ValueError("last dim of k and v must be contiguous")
 
 
-def _check_table(page_table, B):
-    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
-          and page_table.is_contiguous(), "page_table must be contiguous int32 [B, max_pages]")
+def _check_table(page_table, B=None):
+    """The shape (B, max_pages) of a page table."""
+    s = page_table.shape
+    if (len(s) != 2 or (B is not None and s[0] != B) or page_table.dtype != torch.int32
+            or not page_table.is_contiguous()):
+        raise ValueError("page_table must be contiguous int32 [B, max_pages]")
+    return s
 
 
 def _check_ints(t, n, name):
-    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(),
-          f"{name} must be contiguous int32 [{n}]")
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{n}]")
 
 
 def kv_write_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -176,17 +195,16 @@ def kv_write_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, k: torch.Tensor, 
     with rope_cs.  Sequences are appended to: the slots behind a call's last
     token in its last page become zero (atf_kv_write_q8 in include/atflash.h)."""
     dev = _one_device(kv_cache, kv_exps, k, v, start_pos, page_table, rope_cs)
-    _check_cache_q8(kv_cache, kv_exps)
-    pool = kv_cache.shape
-    _check_rows(k, v, 4, pool[1])
+    pool = _check_cache_q8(kv_cache, kv_exps)
+    ks, vs = _check_rows(k, v, 4, pool[1])
     B, T = k.shape[:2]
     _check_ints(start_pos, B, "start_pos")
-    _check_table(page_table, B)
+    width = _check_table(page_table, B)[1]
     rope_cs, max_pos = _rope(rope_cs)
     _lib.launch(dev, _lib.lib().atf_kv_write_q8,
-                kv_cache.data_ptr(), kv_exps.data_ptr(), pool[0], pool[1], k.data_ptr(), *k.stride()[:3],
-                v.data_ptr(), *v.stride()[:3], B, T, None, 0, start_pos.data_ptr(), page_table.data_ptr(),
-                page_table.shape[1], _lib.ptr(rope_cs), max_pos, _layout(layout))
+                kv_cache.data_ptr(), kv_exps.data_ptr(), pool[0], pool[1], k.data_ptr(), ks[0], ks[1], ks[2],
+                v.data_ptr(), vs[0], vs[1], vs[2], B, T, None, 0, start_pos.data_ptr(), page_table.data_ptr(), width,
+                _lib.ptr(rope_cs), max_pos, _layout(layout))
 
 
 _kv_write_q8_op = torch.library.custom_op("atflash::kv_write_q8", kv_write_q8, mutates_args=("kv_cache", "kv_exps"))
@@ -207,28 +225,25 @@ def kv_write_packed(kv_cache: torch.Tensor, kv_exps: Optional[torch.Tensor], k: 
     dev = _one_device(kv_cache, kv_exps, k, v, cu_seqlens, start_pos, page_table, rope_cs)
     if kv_exps is None:
         _check_cache(kv_cache)
+        pool = kv_cache.shape
     else:
-        _check_cache_q8(kv_cache, kv_exps)
-    pool = kv_cache.shape
-    _check_rows(k, v, 3, pool[1])
-    B, T = page_table.shape[0], k.shape[0]
-    _check_table(page_table, B)
+        pool = _check_cache_q8(kv_cache, kv_exps)
+    (ks_t, ks_h, _), (vs_t, vs_h, _) = _check_rows(k, v, 3, pool[1])
+    B, width = _check_table(page_table)
+    T = k.shape[0]
     _check_ints(cu_seqlens, B + 1, "cu_seqlens")
     _check_ints(start_pos, B, "start_pos")
     max_tokens = min(int(max_tokens), T)
     rope_cs, max_pos = _rope(rope_cs)
-    L = _lib.lib()
-    tail = (start_pos.data_ptr(), page_table.data_ptr(), page_table.shape[1], _lib.ptr(rope_cs), max_pos,
-            _layout(layout))
-    ks_t, ks_h, _ = k.stride()
-    vs_t, vs_h, _ = v.stride()
+    rope = _lib.ptr(rope_cs)
     if kv_exps is None:
-        _lib.launch(dev, L.atf_kv_write_packed_bf16, kv_cache.data_ptr(), pool[0], pool[1], k.data_ptr(), ks_t, ks_h,
-                    v.data_ptr(), vs_t, vs_h, B, cu_seqlens.data_ptr(), T, max_tokens, *tail)
+        _lib.launch(dev, _lib.lib().atf_kv_write_packed_bf16, kv_cache.data_ptr(), pool[0], pool[1], k.data_ptr(), ks_t,
+                    ks_h, v.data_ptr(), vs_t, vs_h, B, cu_seqlens.data_ptr(), T, max_tokens, start_pos.data_ptr(),
+                    page_table.data_ptr(), width, rope, max_pos, _layout(layout))
     else:
-        _lib.launch(dev, L.atf_kv_write_q8, kv_cache.data_ptr(), kv_exps.data_ptr(), pool[0], pool[1],
+        _lib.launch(dev, _lib.lib().atf_kv_write_q8, kv_cache.data_ptr(), kv_exps.data_ptr(), pool[0], pool[1],
                     k.data_ptr(), 0, ks_t, ks_h, v.data_ptr(), 0, vs_t, vs_h, B, max_tokens, cu_seqlens.data_ptr(), T,
-                    *tail)
+                    start_pos.data_ptr(), page_table.data_ptr(), width, rope, max_pos, _layout(layout))
 
 
 _kv_write_packed_op = torch.library.custom_op("atflash::kv_write_packed", kv_write_packed,
@@ -244,14 +259,14 @@ def kv_expand_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torc
     """The first n_pages pages of each sequence of an 8-bit cache as bf16 pages,
     exactly: (bf16 cache [B * n_pages, Hkv, 2, 2048], its page table [B, n_pages])."""
     dev = _one_device(kv_cache, kv_exps, page_table)
-    _check_cache_q8(kv_cache, kv_exps)
-    B = page_table.shape[0]
-    _check_table(page_table, B)
-    pool = kv_cache.shape
-    out = torch.empty((B * int(n_pages), pool[1], *_lib.KV_BLOCK_SHAPE), dtype=torch.bfloat16, device=dev)
-    table = torch.empty((B, int(n_pages)), dtype=torch.int32, device=dev)
+    pool = _check_cache_q8(kv_cache, kv_exps)
+    B, width = _check_table(page_table)
+    n = int(n_pages)
+    _need(n >= 0, "n_pages must be >= 0")
+    out = torch.empty((B * n, pool[1], *_lib.KV_BLOCK_SHAPE), dtype=torch.bfloat16, device=kv_cache.device)
+    table = page_table.new_empty((B, n))
     _lib.launch(dev, _lib.lib().atf_kv_expand_q8, out.data_ptr(), table.data_ptr(), kv_cache.data_ptr(),
-                kv_exps.data_ptr(), pool[0], pool[1], page_table.data_ptr(), B, page_table.shape[1], int(n_pages))
+                kv_exps.data_ptr(), pool[0], pool[1], page_table.data_ptr(), B, width, n)
     return out, table
 
 
@@ -326,8 +341,9 @@ class PackedPlan:
     most keys of a sequence.  The list is made by the constructor and by refresh(),
     which takes the lengths as they are then (in a captured graph: call refresh inside)."""
 
-    def __init__(self, cu_seqlens, seq_lens, total_q, max_seq_len, num_q_heads, listed=True):
-        self.device = _one_device(cu_seqlens, seq_lens)
+    def __init__(self, cu_seqlens, seq_lens, total_q, max_seq_len, num_q_heads):
+        self._dev = _one_device(cu_seqlens, seq_lens)
+        self.device = cu_seqlens.device
         self.batch = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
         _need(self.batch >= 0, "cu_seqlens must be contiguous int32 [B + 1]")
         _check_ints(cu_seqlens, self.batch + 1, "cu_seqlens")
@@ -337,41 +353,20 @@ class PackedPlan:
         self.total_q, self.max_seq_len, self.num_q_heads = int(total_q), int(max_seq_len), int(num_q_heads)
         nbytes = int(_lib.lib().atf_prefill_plan_bytes(self.batch, self.total_q, self.num_q_heads))
         self.tiles = torch.empty(max(nbytes, 8) // 4, dtype=torch.int32, device=self.device)
-        if listed:
-            self.refresh()
+        self.refresh()
 
-    def refresh(self, page_table=None, start_pos=None):
-        """List the tiles; with page_table [B, max_pages] and start_pos [B] (int32), also
-        lay out pages for rows that are to be written (page p of sequence b is
-        cu_seqlens[b] / 16 + b + p) and starts of 0."""
-        width = 0 if page_table is None else page_table.shape[1]
-        _lib.launch(self.device, _lib.lib().atf_prefill_plan, self.tiles.data_ptr(), self.tiles.numel() * 4,
+    def refresh(self):
+        """List the tiles of the lengths as they are now."""
+        _lib.launch(self._dev, _lib.lib().atf_prefill_plan, self.tiles.data_ptr(), self.tiles.numel() * 4,
                     self.cu_seqlens.data_ptr(), _lib.ptr(self.seq_lens), self.batch, self.total_q, self.max_seq_len,
-                    self.num_q_heads, _lib.ptr(page_table), width, _lib.ptr(start_pos))
+                    self.num_q_heads)
 
 
-def _prefill_packed(q, kv_cache, page_table, plan, zhi, sm_scale, rope_cs, layout, out, lse):
-    """prefill_packed's launch with its plan made and its arguments other than q, out and lse checked."""
-    _need(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[2] == _lib.HEAD_DIM, "q must be bf16 [T, Hq, 128]")
-    _need(q.stride(2) == 1, "last dim of q must be contiguous")
-    T, Hq, D = q.shape
-    _need(plan.total_q == T and plan.num_q_heads == Hq and plan.device == q.device,
-          f"the plan is for {plan.total_q} rows of {plan.num_q_heads} heads on {plan.device}")
-    dev = _one_device(q, kv_cache, page_table, rope_cs, out, lse)
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
-    if lse is None:
-        lse = torch.empty((Hq, T), dtype=torch.float32, device=dev)
-    _need(out.dtype == torch.bfloat16 and out.shape == q.shape and out.stride(2) == 1, "out must be bf16 [T, Hq, 128]")
-    _need(lse.dtype == torch.float32 and lse.shape == (Hq, T) and lse.is_contiguous(), "lse must be contiguous fp32 [Hq, T]")
-    rope_cs, max_pos = _rope(rope_cs)
-    pool = kv_cache.shape
-    _lib.launch(dev, _lib.lib().atf_prefill_packed_bf16, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
-                q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), pool[0], page_table.data_ptr(),
-                page_table.shape[1], plan.cu_seqlens.data_ptr(), _lib.ptr(plan.seq_lens), plan.batch, T,
-                plan.max_seq_len, Hq, pool[1], _lib.zhi_array(zhi), float(sm_scale), _lib.ptr(rope_cs), max_pos,
-                _layout(layout), plan.tiles.data_ptr(), plan.tiles.numel() * 4)
-    return out, lse
+def _check_packed_q(q):
+    s, st = q.shape, q.stride()
+    if q.dtype != torch.bfloat16 or len(s) != 3 or s[2] != _lib.HEAD_DIM or st[2] != 1:
+        raise ValueError("q must be bf16 [T, Hq, 128], its last dim contiguous")
+    return s, st
 
 
 def prefill_packed(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -384,17 +379,30 @@ def prefill_packed(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Te
     keys (None: as many as queries), at most max_seq_len.  Returns (out bf16 [T, Hq,
     128], lse fp32 [Hq, T]); rows outside every sequence are not written.  plan: a
     PackedPlan of these lengths."""
-    _one_device(q, kv_cache, page_table, cu_seqlens, seq_lens, rope_cs)
+    dev = _one_device(q, kv_cache, page_table, cu_seqlens, seq_lens, rope_cs, out, lse)
     _check_cache(kv_cache)
+    (T, Hq, D), qst = _check_packed_q(q)
     if plan is None:
-        _need(q.dim() == 3, "q must be bf16 [T, Hq, 128]")
-        plan = PackedPlan(cu_seqlens, seq_lens, q.shape[0], max_seq_len, q.shape[1])
+        plan = PackedPlan(cu_seqlens, seq_lens, T, max_seq_len, Hq)
     else:
-        same = (plan.cu_seqlens.data_ptr() == cu_seqlens.data_ptr() and plan.max_seq_len == int(max_seq_len)
-                and _lib.ptr(plan.seq_lens) == _lib.ptr(seq_lens) and plan.batch == cu_seqlens.shape[0] - 1)
-        _need(same, "the plan was made for other lengths")
-    _check_table(page_table, plan.batch)
-    return _prefill_packed(q, kv_cache, page_table, plan, zhi, sm_scale, rope_cs, layout, out, lse)
+        _need(plan.cu_seqlens.data_ptr() == cu_seqlens.data_ptr() and plan.max_seq_len == int(max_seq_len)
+              and _lib.ptr(plan.seq_lens) == _lib.ptr(seq_lens) and plan.batch == cu_seqlens.shape[0] - 1
+              and plan.total_q == T and plan.num_q_heads == Hq, "the plan was made for other rows or lengths")
+    width = _check_table(page_table, plan.batch)[1]
+    if out is None:
+        out = q.new_empty((T, Hq, D))
+    if lse is None:
+        lse = torch.empty((Hq, T), dtype=torch.float32, device=q.device)
+    _need(out.dtype == torch.bfloat16 and out.shape == q.shape and out.stride(2) == 1, "out must be bf16 [T, Hq, 128]")
+    _need(lse.dtype == torch.float32 and lse.shape == (Hq, T) and lse.is_contiguous(), "lse must be contiguous fp32 [Hq, T]")
+    rope_cs, max_pos = _rope(rope_cs)
+    pool = kv_cache.shape
+    _lib.launch(dev, _lib.lib().atf_prefill_packed_bf16, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+                q.data_ptr(), qst[0], qst[1], kv_cache.data_ptr(), pool[0], page_table.data_ptr(), width,
+                cu_seqlens.data_ptr(), _lib.ptr(seq_lens), plan.batch, T, plan.max_seq_len, Hq, pool[1],
+                _lib.zhi_array(zhi), float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout), plan.tiles.data_ptr(),
+                plan.tiles.numel() * 4)
+    return out, lse
 
 
 def _prefill_packed_schema(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor,
@@ -418,18 +426,25 @@ def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     """prefill_packed of whole prompts whose keys and values are packed rows too
     (k, v [T, Hkv, 128]): they are written to temporary pages first."""
     dev = _one_device(q, k, v, cu_seqlens, rope_cs)
-    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0], "q, k and v must have the same rows [T, heads, 128]")
-    _check_rows(k, v, 3, k.shape[1])
-    T, hkv, _ = k.shape
-    plan = PackedPlan(cu_seqlens, None, T, max_seqlen, q.shape[1], listed=False)  # (with the page table, below)
-    B = plan.batch
-    width = -(-int(max_seqlen) // _lib.PAGE_SIZE)
-    ints = torch.empty((B, width + 1), dtype=torch.int32, device=dev).view(-1)
-    table, start = ints[:B * width].view(B, width), ints[B * width:]
-    kv = torch.empty((T // _lib.PAGE_SIZE + B, hkv, *_lib.KV_BLOCK_SHAPE), dtype=torch.bfloat16, device=dev)
-    plan.refresh(table, start)
-    kv_write_packed(kv, None, k, v, cu_seqlens, max_seqlen, start, table, rope_cs, layout)
-    return _prefill_packed(q, kv, table, plan, zhi, sm_scale, rope_cs, layout, None, None)
+    (T, Hq, D), qst = _check_packed_q(q)
+    _need(k.dim() == 3 and k.shape[0] == T, "q, k and v must have the same rows [T, heads, 128]")
+    hkv = k.shape[1]
+    (ks_t, ks_h, _), (vs_t, vs_h, _) = _check_rows(k, v, 3, hkv)
+    B = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
+    _need(B >= 0, "cu_seqlens must be contiguous int32 [B + 1]")
+    _check_ints(cu_seqlens, B + 1, "cu_seqlens")
+    rope_cs, max_pos = _rope(rope_cs)
+    L = _lib.lib()
+    most = int(max_seqlen)
+    nbytes = int(L.atf_flash_packed_workspace_bytes(B, T, most, Hq, hkv))
+    ws = q.new_empty(max(nbytes, 16) // 2)
+    out = q.new_empty((T, Hq, D))
+    lse = torch.empty((Hq, T), dtype=torch.float32, device=q.device)
+    _lib.launch(dev, L.atf_flash_packed_bf16, out.data_ptr(), Hq * D, D, lse.data_ptr(), q.data_ptr(), qst[0], qst[1],
+                k.data_ptr(), ks_t, ks_h, v.data_ptr(), vs_t, vs_h, cu_seqlens.data_ptr(), B, T, most, Hq, hkv,
+                _lib.zhi_array(zhi) if type(zhi) is not tuple else _table(zhi, _lib.LEVELS), float(sm_scale),
+                _lib.ptr(rope_cs), max_pos, _layout(layout), ws.data_ptr(), nbytes)
+    return out, lse
 
 
 # ---- tables on the GPU ----
@@ -443,22 +458,22 @@ def extend_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: to
     int32 [total_tokens], slots int64 [total_tokens]); see atf_extend_tables in
     include/atflash.h.  The lengths and the free count are only read."""
     dev = _one_device(page_table, seq_lens, new_lens, free_pages, free_count)
-    B = page_table.shape[0] if page_table.dim() == 2 else -1
-    _check_table(page_table, B)
+    B, width = _check_table(page_table)
     _check_ints(seq_lens, B, "seq_lens")
     _check_ints(new_lens, B, "new_lens")
     _check_ints(free_count, 1, "free_count")
-    _check_ints(free_pages, free_pages.numel(), "free_pages")
+    F = free_pages.numel()
+    _check_ints(free_pages, F, "free_pages")
     T = int(total_tokens)
     _need(T >= 0, "total_tokens must be >= 0")
     # one allocation: slots first (8-byte aligned)
-    buf = torch.empty(3 * T + 2 * B + 2, dtype=torch.int32, device=dev)
-    slots, pos = buf[:2 * T].view(torch.int64), buf[2 * T:3 * T]
-    lens, left, cu = buf[3 * T:3 * T + B], buf[3 * T + B:3 * T + B + 1], buf[3 * T + B + 1:]
-    _lib.launch(dev, _lib.lib().atf_extend_tables, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),
-                new_lens.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), B, T,
-                int(num_pages), lens.data_ptr(), left.data_ptr(), cu.data_ptr(), pos.data_ptr(), slots.data_ptr())
-    return lens, left, cu, pos, slots
+    buf = seq_lens.new_empty(3 * T + 2 * B + 2)
+    slots, pos, lens, left, cu = buf.split_with_sizes((2 * T, T, B, 1, B + 1))
+    at = buf.data_ptr()
+    _lib.launch(dev, _lib.lib().atf_extend_tables, page_table.data_ptr(), width, seq_lens.data_ptr(),
+                new_lens.data_ptr(), free_pages.data_ptr(), F, free_count.data_ptr(), B, T, int(num_pages),
+                at + 12 * T, at + 12 * T + 4 * B, at + 12 * T + 4 * B + 4, at + 8 * T, at)
+    return lens, left, cu, pos, slots.view(torch.int64)
 
 
 def _extend_tables_schema(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
@@ -485,13 +500,12 @@ def release_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages:
     """The pages of the sequences `rows` (int32) back to the end of the free pages, in
     place: their table rows become -1, their lengths 0, free_count grows."""
     dev = _one_device(page_table, seq_lens, free_pages, free_count, rows)
-    B = page_table.shape[0] if page_table.dim() == 2 else -1
-    _check_table(page_table, B)
+    B, width = _check_table(page_table)
     _check_ints(seq_lens, B, "seq_lens")
     _check_ints(free_count, 1, "free_count")
     _check_ints(free_pages, free_pages.numel(), "free_pages")
     _check_ints(rows, rows.numel(), "rows")
-    _lib.launch(dev, _lib.lib().atf_release_tables, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),
+    _lib.launch(dev, _lib.lib().atf_release_tables, page_table.data_ptr(), width, seq_lens.data_ptr(),
                 free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), rows.data_ptr(), rows.shape[0], B,
                 int(num_pages))
 
@@ -599,25 +613,25 @@ def decode_paged_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tens
     """decode_paged over the cache of 8-bit floats: q [B, Hq, 128] bf16, zhi the
     level table (8 entries) or the per-slice table (16), out bf16 [B, Hq, 128]."""
     dev = _one_device(q, kv_cache, kv_exps, page_table, seq_lens, rope_cs)
-    _check_cache_q8(kv_cache, kv_exps)
-    qs = q.shape
-    _need(q.dtype == torch.bfloat16 and len(qs) == 3 and qs[2] == _lib.HEAD_DIM, "q must be bf16 [B, Hq, 128]")
-    q_sb, q_sh, q_sd = q.stride()
-    _need(q_sd == 1, "last dim of q must be contiguous")
+    num_pages, hkv = _check_cache_q8(kv_cache, kv_exps)[:2]
+    qs, qst = q.shape, q.stride()
+    if q.dtype != torch.bfloat16 or len(qs) != 3 or qs[2] != _lib.HEAD_DIM or qst[2] != 1:
+        raise ValueError("q must be bf16 [B, Hq, 128], its last dim contiguous")
     B, Hq, D = qs
     _check_ints(seq_lens, B, "seq_lens")
-    _check_table(page_table, B)
-    pool = kv_cache.shape
+    width = _check_table(page_table, B)[1]
     rope_cs, max_pos = _rope(rope_cs)
     L = _lib.lib()
-    n = 0 if zhi is None else len(zhi)
-    table = None if zhi is None else _table(zhi, _lib.SLICES if n == _lib.SLICES else _lib.LEVELS)
-    ws = _decode_workspace(dev, _lib.stream_of(dev), B, Hq, pool[1], int(max_seq_len), L, True)
-    out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
-    _lib.launch(dev, L.atf_decode_paged_q8, out.data_ptr(), Hq * D, D, q.data_ptr(), q_sb, q_sh, kv_cache.data_ptr(),
-                kv_exps.data_ptr(), pool[0], page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), B, Hq,
-                pool[1], int(max_seq_len), table, n, float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout),
-                ws[0], ws[1])
+    n, table = 0, None
+    if zhi is not None:
+        n = len(zhi)
+        table = _table(zhi, _lib.SLICES if n == _lib.SLICES else _lib.LEVELS)
+    most = int(max_seq_len)
+    ws = _decode_workspace(q.device, _lib.raw_stream(dev), B, Hq, hkv, most, L, True)
+    out = q.new_empty(qs)
+    _lib.launch(dev, L.atf_decode_paged_q8, out.data_ptr(), Hq * D, D, q.data_ptr(), qst[0], qst[1], kv_cache.data_ptr(),
+                kv_exps.data_ptr(), num_pages, page_table.data_ptr(), width, seq_lens.data_ptr(), B, Hq, hkv, most,
+                table, n, float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout), ws[0], ws[1])
     return out
 
 

@@ -289,6 +289,36 @@ int check_plan(const void* plan, size_t plan_bytes, const int32_t* cu_seqlens, i
   return ATF_OK;
 }
 
+atf::PrefillArgs plan_args(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int total_q, int max_seq_len,
+                           int num_q_heads) {
+  atf::PrefillArgs a{};
+  a.batch = batch;
+  a.hq = num_q_heads;
+  a.pk.cu = cu_seqlens;
+  a.pk.seq_lens = seq_lens;
+  a.pk.total_q = total_q;
+  a.pk.max_k = max_seq_len;
+  return a;
+}
+
+// Workspace of a call on packed rows of queries, keys and values: the pages (a page of
+// its own for each 16 rows of each sequence), the tile list, the page table, the starts.
+struct PackedLayout {
+  int pages, width;
+  size_t plan, table, start, bytes;
+};
+PackedLayout packed_layout(int batch, int total_q, int max_seqlen, int num_q_heads, int num_kv_heads) {
+  PackedLayout w{};
+  w.pages = total_q / atf::kPage + batch;
+  w.width = (max_seqlen + atf::kPage - 1) / atf::kPage;
+  w.plan = static_cast<size_t>(w.pages) * num_kv_heads * atf::kKvBlockElems * 2;
+  w.table = (w.plan + atf::prefill_plan_bytes(batch, total_q, num_q_heads) + 15) / 16 * 16;
+  w.start = w.table + static_cast<size_t>(batch) * w.width * sizeof(int32_t);
+  w.bytes = w.start + static_cast<size_t>(batch) * sizeof(int32_t);
+  w.bytes = (w.bytes + 15) / 16 * 16;
+  return w;
+}
+
 // Packed rows: first rows of the sequences [batch + 1] in device memory, total_tokens rows.
 int check_packed(int batch, const int32_t* cu_tokens, int total_tokens) {
   if (batch > 0 && !cu_tokens) return fail(ATF_ERR_INVALID, "null pointer argument");
@@ -410,26 +440,56 @@ size_t atf_prefill_plan_bytes(int batch, int total_q, int num_q_heads) {
 }
 
 int atf_prefill_plan(void* plan, size_t plan_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens, int batch,
-                     int total_q, int max_seq_len, int num_q_heads, int32_t* page_table, int max_pages,
-                     int32_t* start_pos, void* stream) {
+                     int total_q, int max_seq_len, int num_q_heads, void* stream) {
   if (batch < 0 || total_q < 0) return fail(ATF_ERR_INVALID, "batch and total_q must be >= 0");
   if (batch == 0 || total_q == 0) return ok();
   if (int r = check_plan(plan, plan_bytes, cu_seqlens, batch, total_q, max_seq_len, num_q_heads)) return r;
-  if ((page_table == nullptr) != (start_pos == nullptr))
-    return fail(ATF_ERR_INVALID, "page_table and start_pos are laid out together");
-  if (page_table && static_cast<int64_t>(max_pages) * atf::kPage < max_seq_len)
-    return fail(ATF_ERR_INVALID, "page table too small for max_seq_len=%d (max_pages=%d)", max_seq_len, max_pages);
-  atf::PrefillArgs a{};
-  a.batch = batch;
-  a.hq = num_q_heads;
-  a.max_pages = max_pages;
-  a.pk.cu = cu_seqlens;
-  a.pk.seq_lens = seq_lens;
-  a.pk.total_q = total_q;
-  a.pk.max_k = max_seq_len;
-  hipError_t e = atf::launch_prefill_plan(a, static_cast<int32_t*>(plan), page_table, start_pos,
-                                          static_cast<hipStream_t>(stream));
+  const atf::PrefillArgs a = plan_args(cu_seqlens, seq_lens, batch, total_q, max_seq_len, num_q_heads);
+  hipError_t e = atf::launch_prefill_plan(a, static_cast<int32_t*>(plan), nullptr, nullptr, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "prefill plan launch");
+  return ok();
+}
+
+size_t atf_flash_packed_workspace_bytes(int batch, int total_q, int max_seqlen, int num_q_heads, int num_kv_heads) {
+  if (batch <= 0 || total_q <= 0 || max_seqlen <= 0 || num_q_heads <= 0 || num_kv_heads <= 0) return 0;
+  return packed_layout(batch, total_q, max_seqlen, num_q_heads, num_kv_heads).bytes;
+}
+
+int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse, const void* q, int64_t q_st, int64_t q_sh,
+                          const void* k, int64_t ks_t, int64_t ks_h, const void* v, int64_t vs_t, int64_t vs_h,
+                          const int32_t* cu_seqlens, int batch, int total_q, int max_seqlen, int num_q_heads,
+                          int num_kv_heads, const int32_t* zhi, float sm_scale, const float* rope_cs, int rope_max_pos,
+                          int layout, void* workspace, size_t workspace_bytes, void* stream) {
+  if (batch < 0 || total_q < 0) return fail(ATF_ERR_INVALID, "batch and total_q must be >= 0");
+  if (batch == 0 || total_q == 0) return ok();
+  if (max_seqlen <= 0 || num_q_heads <= 0 || num_kv_heads <= 0)
+    return fail(ATF_ERR_INVALID, "max_seqlen, num_q_heads and num_kv_heads must be positive");
+  if (max_seqlen >= (1 << 24)) return fail(ATF_ERR_UNSUPPORTED, "max_seqlen must be < 2^24");
+  const PackedLayout w = packed_layout(batch, total_q, max_seqlen, num_q_heads, num_kv_heads);
+  if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 16))
+    return fail(ATF_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", w.bytes,
+                workspace ? workspace_bytes : 0);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int32_t* plan = reinterpret_cast<int32_t*>(ws + w.plan);
+  int32_t* table = reinterpret_cast<int32_t*>(ws + w.table);
+  int32_t* start = reinterpret_cast<int32_t*>(ws + w.start);
+  // every argument is checked before the first launch
+  atf::PrefillArgs a{};
+  if (int r = prefill_prepare(out, 0, o_st, o_sh, lse, q, 0, q_st, q_sh, ws, w.pages, table, w.width, batch, max_seqlen,
+                              max_seqlen, num_q_heads, num_kv_heads, zhi, sm_scale, rope_cs, rope_max_pos, layout, &a))
+    return r;
+  if (int r = check_plan(plan, w.table - w.plan, cu_seqlens, batch, total_q, max_seqlen, num_q_heads)) return r;
+  atf::KvWriteArgs k_args{};
+  if (int r = kv_write_prepare(ws, w.pages, num_kv_heads, k, 0, ks_t, ks_h, v, 0, vs_t, vs_h, batch,
+                               std::min(max_seqlen, total_q), start, table, w.width, rope_cs, rope_max_pos, layout, &k_args))
+    return r;
+  k_args.cu_tokens = cu_seqlens;
+  k_args.total_tokens = total_q;
+  a.pk = atf::PackedRows{cu_seqlens, nullptr, total_q, max_seqlen, plan};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (hipError_t e = atf::launch_prefill_plan(a, plan, table, start, s); e != hipSuccess) return hip_fail(e, "prefill plan launch");
+  if (hipError_t e = atf::launch_kv_write(k_args, s); e != hipSuccess) return hip_fail(e, "packed kv_write launch");
+  if (hipError_t e = atf::launch_prefill_packed(a, s); e != hipSuccess) return hip_fail(e, "packed prefill launch");
   return ok();
 }
 

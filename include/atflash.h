@@ -188,16 +188,12 @@ int atf_prefill_bf16(void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float*
  * queries than keys or more than max_seq_len keys.
  *   atf_prefill_plan first lists the query tiles in `plan` (device memory of
  * atf_prefill_plan_bytes, no initialisation needed), heaviest first; one plan serves
- * every layer of a step.  With page_table (int32 [batch][max_pages]) and start_pos
- * (int32 [batch]) it also lays out a page table for rows that are to be written to
- * pages of their own (page p of sequence b: cu_seqlens[b] / 16 + b + p, a pool of
- * total_q / 16 + batch pages) and starts of 0.  A plan made for other lengths gives
- * rows that are not computed, never an access out of bounds.
+ * every layer of a step.  A plan made for other lengths gives rows that are not
+ * computed, never an access out of bounds.
  */
 size_t atf_prefill_plan_bytes(int batch, int total_q, int num_q_heads);
 int atf_prefill_plan(void* plan, size_t plan_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens, int batch,
-                     int total_q, int max_seq_len, int num_q_heads, int32_t* page_table, int max_pages,
-                     int32_t* start_pos, void* stream);
+                     int total_q, int max_seq_len, int num_q_heads, void* stream);
 int atf_prefill_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
                             const void* q, int64_t q_st, int64_t q_sh, const void* kv_cache, int num_pages,
                             const int32_t* page_table, int max_pages,
@@ -205,6 +201,24 @@ int atf_prefill_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
                             int max_seq_len, int num_q_heads, int num_kv_heads,
                             const int32_t* zhi, float sm_scale, const float* rope_cs, int rope_max_pos, int layout,
                             const void* plan, size_t plan_bytes, void* stream);
+
+/*
+ * Causal attention of whole prompts packed one after the other, without a cache of
+ * the caller's: q and out as above, k and v bf16 [total_q][num_kv_heads][128] rows
+ * (strides multiples of 8, 16-byte aligned) of the same sequences, at most max_seqlen
+ * rows each (a longer sequence is not computed).  K and V are written to pages of
+ * the workspace (RoPE there, with rope_cs), the tiles are listed, the attention
+ * runs: three kernels.  The workspace needs no initialisation; calls that share one
+ * must be ordered on one stream.
+ */
+size_t atf_flash_packed_workspace_bytes(int batch, int total_q, int max_seqlen, int num_q_heads, int num_kv_heads);
+int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
+                          const void* q, int64_t q_st, int64_t q_sh,
+                          const void* k, int64_t ks_t, int64_t ks_h, const void* v, int64_t vs_t, int64_t vs_h,
+                          const int32_t* cu_seqlens, int batch, int total_q, int max_seqlen,
+                          int num_q_heads, int num_kv_heads, const int32_t* zhi, float sm_scale,
+                          const float* rope_cs, int rope_max_pos, int layout,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Block tables and slot maps of a step from request lengths, on the GPU.  Sequence b

@@ -126,8 +126,10 @@ def test_the_restated_cache_keeps_and_forgets():
     assert int(c.e[1, 0, 1]) == exponent(1000.0) and int(c.e[1, 0, 0]) == exponent(2.0)
 
 
-PLAN = dict(plan=1 << 20, plan_bytes=1 << 20, cu=1 << 20, lens=None, batch=2, total=100, most=60, hq=4, table=None,
-            max_pages=0, start=None, stream=None)
+PLAN = dict(plan=1 << 20, plan_bytes=1 << 20, cu=1 << 20, lens=None, batch=2, total=100, most=60, hq=4, stream=None)
+FLASH = dict(out=1 << 20, o_st=512, o_sh=128, lse=None, q=1 << 20, q_st=512, q_sh=128, k=1 << 20, ks_t=256, ks_h=128,
+             v=1 << 20, vs_t=256, vs_h=128, cu=1 << 20, batch=2, total=100, most=60, hq=4, hkv=2, zhi=None, scale=0.1,
+             rope=None, rope_pos=0, layout=0, ws=1 << 20, ws_bytes=1 << 20, stream=None)
 PREFILL = dict(out=1 << 20, o_st=512, o_sh=128, lse=None, q=1 << 20, q_st=512, q_sh=128, kv=1 << 20, pages=9, table=1 << 20,
                max_pages=4, cu=1 << 20, lens=None, batch=2, total=100, most=60, hq=4, hkv=2, zhi=None, scale=0.1, rope=None,
                rope_pos=0, layout=0, plan=1 << 20, plan_bytes=1 << 20, stream=None)
@@ -139,10 +141,27 @@ RELEASE = dict(table=1 << 20, max_pages=4, lens=1 << 20, free=1 << 20, num_free=
 
 @pytest.mark.parametrize("change,code", [
     (dict(batch=-1), 1), (dict(total=-1), 1), (dict(cu=None), 1), (dict(most=0), 1), (dict(hq=0), 1), (dict(most=1 << 24), 2),
-    (dict(plan=None), 4), (dict(plan_bytes=8), 4), (dict(plan=(1 << 20) + 4), 4), (dict(table=1 << 20), 1),
-    (dict(start=1 << 20), 1), (dict(table=1 << 20, start=1 << 20, max_pages=3), 1), (dict(batch=0), 0), (dict(total=0), 0)])
+    (dict(plan=None), 4), (dict(plan_bytes=8), 4), (dict(plan=(1 << 20) + 4), 4), (dict(batch=0), 0), (dict(total=0), 0)])
 def test_plan_validation(no_gpu, change, code):
     assert call(no_gpu.atf_prefill_plan, PLAN, **change) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(batch=-1), 1), (dict(total=-1), 1), (dict(most=0), 1), (dict(most=1 << 24), 2), (dict(hkv=3), 1), (dict(hq=0), 1),
+    (dict(cu=None), 1), (dict(q=None), 1), (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(ks_t=4), 1),
+    (dict(v=8), 1), (dict(q_st=3), 1), (dict(o_sh=2), 1), (dict(scale=0.0), 1), (dict(rope=1 << 20, rope_pos=59), 1),
+    (dict(layout=2), 1), (dict(ws=None), 4), (dict(ws_bytes=1000), 4), (dict(ws=(1 << 20) + 8), 4), (dict(batch=0), 0),
+    (dict(total=0), 0)])
+def test_flash_packed_validation(no_gpu, change, code):
+    assert call(no_gpu.atf_flash_packed_bf16, FLASH, **change) == code
+
+
+def test_flash_packed_workspace_holds_its_parts(no_gpu):
+    for b, t, most, hq, hkv in ((1, 1, 1, 4, 4), (5, 1000, 517, 24, 8), (300, 20000, 9000, 28, 4), (3, 48, 16, 2, 1)):
+        pages = (t // 16 + b) * hkv * 8192
+        rest = no_gpu.atf_prefill_plan_bytes(b, t, hq) + 4 * b * (-(-most // 16) + 1)
+        assert pages + rest <= no_gpu.atf_flash_packed_workspace_bytes(b, t, most, hq, hkv) <= pages + rest + 48
+    assert no_gpu.atf_flash_packed_workspace_bytes(0, 1, 1, 1, 1) == 0
 
 
 @pytest.mark.parametrize("change,code", [
