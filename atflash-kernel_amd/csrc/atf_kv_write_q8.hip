@@ -86,15 +86,18 @@ __device__ __forceinline__ u32x4 transpose4(const u32x4& w) {
 // row), their codes go to LDS by token, and thread (j, g, r) = tid takes a 4 x 4 square
 // of it (dims 8r + 4j .. + 3, tokens 4g .. + 3), transposes it and writes the 16 bytes at
 // 16 tid.
-// grid: x = page index relative to the call's first page, y = sequence, z = kv head.
+// grid: x = pages (from the call's first) and kv heads, y = sequence.  Workgroups go to the
+// XCDs in turn: a page's heads lie on one XCD, one after the other, so that its (cos,
+// sin) rows, as many bytes as a head's keys and values, come from that XCD's L2.
 __global__ __launch_bounds__(128) void kv_write_q8_kernel(KvWriteArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sv[kPage][kD];
   __shared__ uint32_t s_top[2][2], s_odd[2];
-  const int b = blockIdx.y, h = blockIdx.z, tid = threadIdx.x;
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const int j8 = blockIdx.x / a.page_round, turn = j8 / a.hkv, h = j8 - turn * a.hkv;
   const KvRows rows = kv_rows(a, b);
   const int start = a.start_pos[b];
   const int64_t end64 = static_cast<int64_t>(start) + rows.count;
-  const int pidx = (max(start, 0) >> 4) + static_cast<int>(blockIdx.x);
+  const int pidx = (max(start, 0) >> 4) + turn * a.page_round + (static_cast<int>(blockIdx.x) - j8 * a.page_round);
   const int64_t p0 = static_cast<int64_t>(pidx) * kPage;
   if (pidx >= a.max_pages || p0 >= end64) return;
   const int64_t lo = max(p0, static_cast<int64_t>(max(start, 0)));
@@ -102,26 +105,44 @@ __global__ __launch_bounds__(128) void kv_write_q8_kernel(KvWriteArgs a) {
   if (a.rope_cs != nullptr) hi = min(hi, static_cast<int64_t>(a.rope_max_pos));
   if (lo >= hi) return;
   const int s0 = static_cast<int>(lo - p0), s1 = static_cast<int>(hi - p0);
-  const int pg = a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx];
+  const int pg = a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx];  // waited for behind the rows' loads
+  const int64_t row0 = rows.first + (p0 - start);  // source row of slot 0
+
+  // Every load first (slots outside the call read a row of it, in bounds), then the
+  // arithmetic: one memory round trip for all of them.
+  const int l = tid >> 4, slot = tid & 15;
+  const bool k_on = slot >= s0 && slot < s1;
+  const int c0 = level_chunk0(a.layout, l);
+  const uint16_t* krow = a.k_src + static_cast<int64_t>(b) * a.ks_b + (row0 + min(max(slot, s0), s1 - 1)) * a.ks_t +
+                         static_cast<int64_t>(h) * a.ks_h;
+  const u32x4 xk1 = ldg16(krow + c0), xk2 = ldg16(krow + level_chunk1(a.layout, l));
+  u32x4 xv[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    xv[i] = ldg16(a.v_src + static_cast<int64_t>(b) * a.vs_b + (row0 + min(max(8 * i + l, s0), s1 - 1)) * a.vs_t +
+                  static_cast<int64_t>(h) * a.vs_h + 8 * slot);
+  float cs[16];
+  if (a.rope_cs != nullptr) load_cs8(a.rope_cs, static_cast<int>(p0) + min(max(slot, s0), s1 - 1), c0, cs);
   if (pg < 0 || pg >= a.num_pages) return;
   const size_t blk = static_cast<size_t>(pg) * a.hkv + h;
   uint8_t* codes = reinterpret_cast<uint8_t*>(a.kv_cache) + blk * kQ8BlockBytes;
-  const int64_t row0 = rows.first + (p0 - start);  // source row of slot 0
-
-  const int l = tid >> 4, slot = tid & 15;
-  const bool k_on = slot >= s0 && slot < s1;
+  // what the page keeps: the codes of slots before s0, under their exponents
+  u32x4 old_k = {0u, 0u, 0u, 0u}, old_v = {0u, 0u, 0u, 0u};
+  int ev = kQ8MinExp, ek = kQ8MinExp;
+  if (s0 > 0) {
+    old_v = ldg16(codes + 16 * tid);
+    old_k = ldg16(codes + kQ8HalfBytes + 16 * tid);
+    ev = a.kv_exps[2 * blk];
+    ek = a.kv_exps[2 * blk + 1];
+  }
   float ka[8] = {}, kb[8] = {};  // the level's two slices
   uint32_t k_top = 0, v_top = 0, odd = 0;
   if (k_on) {
-    const uint16_t* krow = a.k_src + static_cast<int64_t>(b) * a.ks_b + (row0 + slot) * a.ks_t + static_cast<int64_t>(h) * a.ks_h;
-    const int c0 = level_chunk0(a.layout, l);
     float x1[8], x2[8];
-    unpack8(ldg16(krow + c0), x1);
-    unpack8(ldg16(krow + level_chunk1(a.layout, l)), x2);
+    unpack8(xk1, x1);
+    unpack8(xk2, x2);
     if (a.rope_cs != nullptr) {
 #pragma clang fp contract(off)
-      float cs[16];
-      load_cs8(a.rope_cs, static_cast<int>(p0) + slot, c0, cs);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float c = cs[2 * i], s = cs[2 * i + 1], u = x1[i], w = x2[i];
@@ -146,22 +167,12 @@ __global__ __launch_bounds__(128) void kv_write_q8_kernel(KvWriteArgs a) {
   float v[2][8] = {};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int tok = 8 * i + (tid >> 4);
+    const int tok = 8 * i + l;
     if (tok >= s0 && tok < s1) {
-      unpack8(ldg16(a.v_src + static_cast<int64_t>(b) * a.vs_b + (row0 + tok) * a.vs_t +
-                    static_cast<int64_t>(h) * a.vs_h + 8 * (tid & 15)), v[i]);
+      unpack8(xv[i], v[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) note(v[i][j], v_top, odd);
     }
-  }
-  // what the page keeps: the codes of slots before s0, under their exponents
-  u32x4 old_k = {0u, 0u, 0u, 0u}, old_v = {0u, 0u, 0u, 0u};
-  int ev = kQ8MinExp, ek = kQ8MinExp;
-  if (s0 > 0) {
-    old_v = ldg16(codes + 16 * tid);
-    old_k = ldg16(codes + kQ8HalfBytes + 16 * tid);
-    ev = a.kv_exps[2 * blk];
-    ek = a.kv_exps[2 * blk + 1];
   }
   const int wave = tid >> 6;
   k_top = wave_max(k_top);
@@ -223,7 +234,11 @@ hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s) {
   if (a.n_tokens <= 0 || a.batch <= 0) return hipSuccess;
   // a call of n tokens touches at most ceil(n / 16) + 1 pages per sequence
   const int pages = (a.n_tokens + kPage - 1) / kPage + 1;
-  hipLaunchKernelGGL(kv_write_q8_kernel, dim3(pages, a.batch, a.hkv), dim3(128), 0, s, a);
+  KvWriteArgs k = a;
+  k.page_round = pages < 8 ? pages : 8;
+  const int64_t blocks = static_cast<int64_t>(pages + k.page_round - 1) / k.page_round * k.page_round * a.hkv;
+  if (blocks > INT32_MAX) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kv_write_q8_kernel, dim3(blocks, a.batch), dim3(128), 0, s, k);
   return hipGetLastError();
 }
 

@@ -44,6 +44,7 @@ struct KvWriteArgs {
   const int32_t* cu_tokens;
   int total_tokens;
   int8_t* kv_exps;  // the 8-bit cache's exponents [num_pages][hkv][2] (kv_cache: its codes)
+  int page_round;   // 8-bit writer: pages that are dealt out to the XCDs together
 };
 
 // The rows of sequence b in a call: the first, relative to k_src's and v_src's row 0
