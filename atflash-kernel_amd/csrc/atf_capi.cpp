@@ -284,7 +284,7 @@ int check_plan(const void* plan, size_t plan_bytes, const int32_t* cu_seqlens, i
     return fail(ATF_ERR_INVALID, "num_q_heads and max_seq_len must be positive");
   if (max_seq_len >= (1 << 24)) return fail(ATF_ERR_UNSUPPORTED, "max_seq_len must be < 2^24");
   const size_t need = atf::prefill_plan_bytes(batch, total_q, num_q_heads);
-  if (!plan || plan_bytes < need || !aligned(plan, 8))
+  if (need > 0 && (!plan || plan_bytes < need || !aligned(plan, 8)))
     return fail(ATF_ERR_WORKSPACE, "plan of %zu bytes (8-byte aligned) required, got %zu", need, plan ? plan_bytes : 0);
   return ATF_OK;
 }
@@ -302,10 +302,10 @@ atf::PrefillArgs plan_args(const int32_t* cu_seqlens, const int32_t* seq_lens, i
 }
 
 // Workspace of a call on packed rows of queries, keys and values: the pages (a page of
-// its own for each 16 rows of each sequence), the tile list, the page table, the starts.
+// its own for each 16 rows of each sequence), the tile list, the page table.
 struct PackedLayout {
   int pages, width;
-  size_t plan, table, start, bytes;
+  size_t plan, table, bytes;
 };
 PackedLayout packed_layout(int batch, int total_q, int max_seqlen, int num_q_heads, int num_kv_heads) {
   PackedLayout w{};
@@ -313,9 +313,7 @@ PackedLayout packed_layout(int batch, int total_q, int max_seqlen, int num_q_hea
   w.width = (max_seqlen + atf::kPage - 1) / atf::kPage;
   w.plan = static_cast<size_t>(w.pages) * num_kv_heads * atf::kKvBlockElems * 2;
   w.table = (w.plan + atf::prefill_plan_bytes(batch, total_q, num_q_heads) + 15) / 16 * 16;
-  w.start = w.table + static_cast<size_t>(batch) * w.width * sizeof(int32_t);
-  w.bytes = w.start + static_cast<size_t>(batch) * sizeof(int32_t);
-  w.bytes = (w.bytes + 15) / 16 * 16;
+  w.bytes = (w.table + static_cast<size_t>(batch) * w.width * sizeof(int32_t) + 15) / 16 * 16;
   return w;
 }
 
@@ -445,7 +443,7 @@ int atf_prefill_plan(void* plan, size_t plan_bytes, const int32_t* cu_seqlens, c
   if (batch == 0 || total_q == 0) return ok();
   if (int r = check_plan(plan, plan_bytes, cu_seqlens, batch, total_q, max_seq_len, num_q_heads)) return r;
   const atf::PrefillArgs a = plan_args(cu_seqlens, seq_lens, batch, total_q, max_seq_len, num_q_heads);
-  hipError_t e = atf::launch_prefill_plan(a, static_cast<int32_t*>(plan), nullptr, nullptr, static_cast<hipStream_t>(stream));
+  hipError_t e = atf::launch_prefill_plan(a, static_cast<int32_t*>(plan), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "prefill plan launch");
   return ok();
 }
@@ -472,7 +470,6 @@ int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse, con
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   int32_t* plan = reinterpret_cast<int32_t*>(ws + w.plan);
   int32_t* table = reinterpret_cast<int32_t*>(ws + w.table);
-  int32_t* start = reinterpret_cast<int32_t*>(ws + w.start);
   // every argument is checked before the first launch
   atf::PrefillArgs a{};
   if (int r = prefill_prepare(out, 0, o_st, o_sh, lse, q, 0, q_st, q_sh, ws, w.pages, table, w.width, batch, max_seqlen,
@@ -481,13 +478,14 @@ int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse, con
   if (int r = check_plan(plan, w.table - w.plan, cu_seqlens, batch, total_q, max_seqlen, num_q_heads)) return r;
   atf::KvWriteArgs k_args{};
   if (int r = kv_write_prepare(ws, w.pages, num_kv_heads, k, 0, ks_t, ks_h, v, 0, vs_t, vs_h, batch,
-                               std::min(max_seqlen, total_q), start, table, w.width, rope_cs, rope_max_pos, layout, &k_args))
+                               std::min(max_seqlen, total_q), table, table, w.width, rope_cs, rope_max_pos, layout, &k_args))
     return r;
   k_args.cu_tokens = cu_seqlens;
   k_args.total_tokens = total_q;
+  k_args.own_table = table;
   a.pk = atf::PackedRows{cu_seqlens, nullptr, total_q, max_seqlen, plan};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (hipError_t e = atf::launch_prefill_plan(a, plan, table, start, s); e != hipSuccess) return hip_fail(e, "prefill plan launch");
+  if (hipError_t e = atf::launch_prefill_plan(a, plan, s); e != hipSuccess) return hip_fail(e, "prefill plan launch");
   if (hipError_t e = atf::launch_kv_write(k_args, s); e != hipSuccess) return hip_fail(e, "packed kv_write launch");
   if (hipError_t e = atf::launch_prefill_packed(a, s); e != hipSuccess) return hip_fail(e, "packed prefill launch");
   return ok();

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
   const int h0 = (kHeadsFirst ? (blockIdx.x + blockIdx.y / 8) % gridDim.x : blockIdx.z) * per;
   const int h_end = min(a.hkv, h0 + per);
   const int tid = threadIdx.x;
-  const int start = a.start_pos[b];
+  const int start = kv_start(a, b);
   const KvRows rows = kv_rows(a, b);
   const int64_t end64 = static_cast<int64_t>(start) + rows.count;  // exclusive
   const int first = max(start, 0) >> 4;
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
   if (a.rope_cs != nullptr) hi = min(hi, static_cast<int64_t>(a.rope_max_pos));
   if (lo >= hi) return;
   const int s0 = static_cast<int>(lo - p0), s1 = static_cast<int>(hi - p0);
-  const int pg = a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx];
+  const int pg = kv_page(a, rows, b, pidx, h0 == 0 && tid == 0);
   if (pg < 0 || pg >= a.num_pages) return;
   const size_t blk0 = static_cast<size_t>(pg) * a.hkv * kKvBlockElems;  // the page's block of head 0
   const int64_t t0 = rows.first + (p0 - start);  // source row of slot 0
@@ -168,12 +168,12 @@ __global__ __launch_bounds__(128) void kv_append_kernel(KvWriteArgs a) {
   const int c0 = level_chunk0(a.layout, l);
   const u32x4 x1 = ldg16(krow + c0), x2 = ldg16(krow + level_chunk1(a.layout, l));
   const uint16_t v = vrow[tid];
-  const int64_t pos = static_cast<int64_t>(a.start_pos[b]) + t;
+  const int64_t pos = static_cast<int64_t>(kv_start(a, b)) + t;
   const int64_t pidx = pos >> 4;
   if (pos < 0 || pidx >= a.max_pages || (a.rope_cs != nullptr && pos >= a.rope_max_pos)) return;
   float cs[16];
   if (a.rope_cs != nullptr) load_cs8(a.rope_cs, static_cast<int>(pos), c0, cs);
-  const int pg = a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx];
+  const int pg = kv_page(a, rows, b, pidx, h == 0 && tid == 0);
   if (pg < 0 || pg >= a.num_pages) return;
   const int slot = static_cast<int>(pos) & (kPage - 1);
   uint16_t* blk = a.kv_cache + (static_cast<size_t>(pg) * a.hkv + h) * kKvBlockElems;

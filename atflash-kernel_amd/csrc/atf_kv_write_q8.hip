@@ -94,8 +94,8 @@ __global__ __launch_bounds__(128) void kv_write_q8_kernel(KvWriteArgs a) {
   __shared__ uint32_t s_top[2][2], s_odd[2];
   const int b = blockIdx.y, tid = threadIdx.x;
   const int j8 = blockIdx.x / a.page_round, turn = j8 / a.hkv, h = j8 - turn * a.hkv;
-  const KvRows rows = kv_rows(a, b);
   const int start = a.start_pos[b];
+  const KvRows rows = kv_rows(a, b);
   const int64_t end64 = static_cast<int64_t>(start) + rows.count;
   const int pidx = (max(start, 0) >> 4) + turn * a.page_round + (static_cast<int>(blockIdx.x) - j8 * a.page_round);
   const int64_t p0 = static_cast<int64_t>(pidx) * kPage;

@@ -43,6 +43,9 @@ struct KvWriteArgs {
   // sequence b lies at b ks_b + t ks_t.
   const int32_t* cu_tokens;
   int total_tokens;
+  // Packed rows into pages of their own (start_pos and page_table are not read): row i of
+  // sequence b goes to page cu_tokens[b] / 16 + b + i / 16, which is entered here.
+  int32_t* own_table;
   int8_t* kv_exps;  // the 8-bit cache's exponents [num_pages][hkv][2] (kv_cache: its codes)
   int page_round;   // 8-bit writer: pages that are dealt out to the XCDs together
 };
@@ -53,6 +56,15 @@ struct KvRows {
   int64_t first;
   int count;
 };
+__device__ __forceinline__ int kv_start(const KvWriteArgs& a, int b) { return a.own_table != nullptr ? 0 : a.start_pos[b]; }
+// The page of entry `pidx` of sequence b, and in a call with pages of its own its entry.
+__device__ __forceinline__ int kv_page(const KvWriteArgs& a, const KvRows& rows, int b, int64_t pidx, bool enter) {
+  const int64_t at = static_cast<int64_t>(b) * a.max_pages + pidx;
+  if (a.own_table == nullptr) return a.page_table[at];
+  const int pg = static_cast<int>(rows.first / kPage + b + pidx);
+  if (enter) a.own_table[at] = pg;
+  return pg;
+}
 __device__ __forceinline__ KvRows kv_rows(const KvWriteArgs& a, int b) {
   if (a.cu_tokens == nullptr) return KvRows{0, a.n_tokens};
   const int lo = max(a.cu_tokens[b], 0), hi = min(a.cu_tokens[b + 1], a.total_tokens);
@@ -65,7 +77,7 @@ struct PackedRows {
   const int32_t* seq_lens;  // [batch] keys, the sequence's queries the last of them; null: as many as queries
   int total_q;              // rows of q, out and lse
   int max_k;                // keys of a sequence at most
-  const int32_t* tiles;     // launch_prefill_plan's list
+  const int32_t* tiles;     // launch_prefill_plan's list (null: not needed)
 };
 
 struct PrefillArgs {
@@ -174,12 +186,10 @@ struct KvExpandArgs {
 };
 hipError_t launch_kv_expand_q8(const KvExpandArgs& a, hipStream_t s);
 hipError_t launch_prefill(const PrefillArgs& a, hipStream_t s);
-// Packed rows: the list of query tiles (prefill_plan_bytes; a.pk, batch, heads and with
-// `table` max_pages are read), then the attention over it.  table, start: a page table
-// [batch][max_pages] with a page of its own for each 16 rows of each sequence and
-// starts of 0, for rows that are to be written into pages; or null.
+// Packed rows: the list of query tiles (prefill_plan_bytes, 0 where none is needed; a.pk,
+// batch and heads are read), then the attention over it.
 size_t prefill_plan_bytes(int batch, int total_q, int hq);
-hipError_t launch_prefill_plan(const PrefillArgs& a, int32_t* tiles, int32_t* table, int32_t* start, hipStream_t s);
+hipError_t launch_prefill_plan(const PrefillArgs& a, int32_t* tiles, hipStream_t s);
 hipError_t launch_prefill_packed(const PrefillArgs& a, hipStream_t s);
 // The MFMA-ceiling probe of the prefill (measurement only): sink holds
 // ceil(ceil(nq / 256) / 8) * 8 * hq * 512 floats.

@@ -1272,22 +1272,58 @@ void prefill_solo_kernel(PrefillArgs a) {
 // prefill_plan_kernel lists the query tiles, the one with the most keys first, and a
 // workgroup takes its tile, and q head, from the list as prefill_block deals out
 // units.  The grid covers as many tiles as total_q rows of `batch` sequences can have
-// (total_q / rows + batch); workgroups past the list end at once.  A sequence's results
+// (total_q / rows + batch); workgroups past the list end at once.  Where all workgroups
+// run at once (the 128-row kernel) their order does not matter: a workgroup finds the
+// tile of its place itself, and there is no list.  A sequence's results
 // are those of a prefill call of its own to the bit (the same tiles of 32 rows, the
 // same order of keys).
 
-// The tile of block `bid`: false past the list.
-__device__ __forceinline__ bool packed_block(const PrefillArgs& a, int bid, int rows, int& b, int& h, int& qt) {
+// Place of block `bid` among the tiles, and its q head.
+__device__ __forceinline__ int packed_rank(const PrefillArgs& a, int bid, int& h) {
   const int xcd = bid & 7;
   const int j = bid >> 3;
   const int rnd = j / a.group;
   const int unit = rnd * 8 + ((rnd & 1) ? 7 - xcd : xcd);
   const int rank = unit / a.hkv;
   h = (unit - rank * a.hkv) * a.group + (j - rnd * a.group);
+  return rank;
+}
+
+// The tile of block `bid` in the list: false past it.
+__device__ __forceinline__ bool packed_block(const PrefillArgs& a, int bid, int rows, int& b, int& h, int& qt) {
+  const int rank = packed_rank(a, bid, h);
   if (rank >= min(a.pk.tiles[0], a.n_qtiles)) return false;
   b = a.pk.tiles[2 + 2 * rank];
   qt = a.pk.tiles[3 + 2 * rank];
   return b >= 0 && b < a.batch && qt >= 0 && qt <= INT32_MAX / rows - 1;  // (a list of another call: in bounds all the same)
+}
+
+// Places of tiles: sequence b's start at cu[b] / rows + b, which leaves room for ceil(n /
+// rows) tiles of each, so that no sums over sequences have to be formed first.  The
+// sequence of a place is found by counting the starts up to it, 64 sequences at a
+// time (-1: none; every lane takes part); total: the tiles of all sequences.
+__device__ __forceinline__ int first_place(const PrefillArgs& a, const PackedSeq& sq, int rows) {
+  return min(sq.row0, a.pk.total_q) / rows + sq.b;
+}
+__device__ __forceinline__ int place_seq(const PrefillArgs& a, int rows, int place, int& total) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    bool reached = false;
+    int n = 0;
+    if (b < a.batch) {
+      const PackedSeq sq = packed_seq(a, b);
+      reached = first_place(a, sq, rows) <= place;
+      n = (sq.n_q + rows - 1) / rows;
+    }
+    before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(reached));
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) n += __shfl_xor(n, m);
+    total += n;
+  }
+  return before - 1;
 }
 
 template <bool kRaw>
@@ -1301,57 +1337,31 @@ __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_packed_kernel(Prefil
 template <bool kRaw>
 __global__ __launch_bounds__(kSoloWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void prefill_packed_solo_kernel(PrefillArgs a) {
-  int b, h, qt;
-  if (!packed_block(a, blockIdx.x, kSoloRowsWg, b, h, qt)) return;
+  int h, total;
+  const int place = packed_rank(a, blockIdx.x, h);
+  const int b = place_seq(a, kSoloRowsWg, place, total);
+  if (b < 0) return;
   const PackedSeq sq = packed_seq(a, b);
-  if (qt * kSoloRowsWg < sq.n_q) prefill_solo_rows<kRaw>(sq, h, qt);
+  const int qt = place - first_place(a, sq, kSoloRowsWg);
+  if (qt >= 0 && qt * kSoloRowsWg < sq.n_q) prefill_solo_rows<kRaw>(sq, h, qt);
 }
 
 // The tile list: [0] the number of tiles, then (sequence, tile) pairs from [2] on, most
-// keys first (ties: by sequence).  A wave per tile place: sequence b's places start at
-// cu[b] / rows + b, which leaves room for ceil(n / rows) tiles of each, so that no sums
-// over sequences have to be formed first; the wave finds its sequence by counting the
-// starts up to its place, 64 sequences at a time, and its rank by counting the tiles of
-// every sequence that have more keys, a closed form each.
-//   Latency bound: the lengths are read twice.  With `table`, workgroups also lay out a
-// page table for rows that are to be written page by page: page p of sequence b is
-// cu[b] / 16 + b + p, start 0.
+// keys first (ties: by sequence).  A wave per place: its rank is the number of tiles
+// of every sequence that have more keys, a closed form each.
+//   Latency bound: the lengths are read twice.
 constexpr int kPlanWaves = 4;
-__global__ __launch_bounds__(kPlanWaves * 64) void prefill_plan_kernel(PrefillArgs a, int rows, int places, int32_t* tiles,
-                                                                       int32_t* table, int32_t* start) {
+__global__ __launch_bounds__(kPlanWaves * 64) void prefill_plan_kernel(PrefillArgs a, int rows, int places,
+                                                                       int32_t* tiles) {
   const int lane = threadIdx.x & 63;
   const int place = blockIdx.x * kPlanWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (table != nullptr) {
-    const int64_t n = static_cast<int64_t>(a.batch) * a.max_pages, step = static_cast<int64_t>(gridDim.x) * kPlanWaves * 64;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kPlanWaves * 64 + threadIdx.x; i < n; i += step) {
-      const int b = static_cast<int>(i / a.max_pages), p = static_cast<int>(i - static_cast<int64_t>(b) * a.max_pages);
-      const int lo = min(max(a.pk.cu[b], 0), a.pk.total_q);
-      table[i] = lo / kPage + b + p;
-      if (p == 0) start[b] = 0;
-    }
-  }
   if (place >= places) return;
-  // the sequence of this place, and the number of tiles of all
-  int before = 0, total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int b = b0 + lane;
-    bool reached = false;
-    int n = 0;
-    if (b < a.batch) {
-      const PackedSeq sq = packed_seq(a, b);
-      reached = min(sq.row0, a.pk.total_q) / rows + b <= place;
-      n = (sq.n_q + rows - 1) / rows;
-    }
-    before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(reached));
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) n += __shfl_xor(n, m);
-    total += n;
-  }
+  int total;
+  const int mine = place_seq(a, rows, place, total);
   if (place == 0 && lane == 0) tiles[0] = total;
-  if (before == 0) return;
-  const int mine = before - 1;
+  if (mine < 0) return;
   const PackedSeq me = packed_seq(a, mine);
-  const int i = place - (min(me.row0, a.pk.total_q) / rows + mine);
+  const int i = place - first_place(a, me, rows);
   if (i < 0 || i * rows >= me.n_q) return;  // (i < 0: first rows that decrease)
   const int keys = me.q_offset() + min(me.n_q, (i + 1) * rows);
   int rank = 0;
@@ -1566,16 +1576,15 @@ static bool packed_solo(int batch, int total_q, int hq) {
 }
 
 size_t prefill_plan_bytes(int batch, int total_q, int hq) {
-  const int rows = packed_solo(batch, total_q, hq) ? kSoloRowsWg : kPfRowsWg;
-  return (2 + 2 * static_cast<size_t>(packed_tiles(batch, total_q, rows))) * sizeof(int32_t);
+  if (packed_solo(batch, total_q, hq)) return 0;
+  return (2 + 2 * static_cast<size_t>(packed_tiles(batch, total_q, kPfRowsWg))) * sizeof(int32_t);
 }
 
-hipError_t launch_prefill_plan(const PrefillArgs& a, int32_t* tiles, int32_t* table, int32_t* start, hipStream_t s) {
-  if (a.batch <= 0 || a.pk.total_q <= 0) return hipSuccess;
-  const int rows = packed_solo(a.batch, a.pk.total_q, a.hq) ? kSoloRowsWg : kPfRowsWg;
-  const int places = packed_tiles(a.batch, a.pk.total_q, rows);
+hipError_t launch_prefill_plan(const PrefillArgs& a, int32_t* tiles, hipStream_t s) {
+  if (a.batch <= 0 || a.pk.total_q <= 0 || packed_solo(a.batch, a.pk.total_q, a.hq)) return hipSuccess;
+  const int places = packed_tiles(a.batch, a.pk.total_q, kPfRowsWg);
   hipLaunchKernelGGL(prefill_plan_kernel, dim3((places + kPlanWaves - 1) / kPlanWaves), dim3(kPlanWaves * 64), 0, s, a,
-                     rows, places, tiles, table, start);
+                     kPfRowsWg, places, tiles);
   return hipGetLastError();
 }
 

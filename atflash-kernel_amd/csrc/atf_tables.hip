@@ -111,10 +111,10 @@ __global__ __launch_bounds__(kTabThreads) void extend_tables_kernel(ExtendTables
 }
 
 hipError_t launch_extend_tables(const ExtendTablesArgs& a, hipStream_t s) {
-  // a workgroup for each 1024 tokens: a step of a few hundred tokens is one workgroup's
-  // work, and the sums that each forms again stay small beside its tokens
-  const int64_t work = static_cast<int64_t>(a.total) + 1;
-  const int blocks = static_cast<int>((work + 4 * kTabThreads - 1) / (4 * kTabThreads));
+  // a token a thread (at most 1024 workgroups): its search and its loads wait for one
+  // another
+  const int64_t blocks64 = (static_cast<int64_t>(a.total) + kTabThreads) / kTabThreads;
+  const int blocks = static_cast<int>(blocks64 < 1024 ? blocks64 : 1024);
   const size_t lds = 2 * (static_cast<size_t>(a.batch) + 1) * sizeof(int32_t);
   hipLaunchKernelGGL(extend_tables_kernel, dim3(blocks), dim3(kTabThreads), lds, s, a);
   return hipGetLastError();

@@ -188,7 +188,7 @@ int atf_prefill_bf16(void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float*
  * queries than keys or more than max_seq_len keys.
  *   atf_prefill_plan first lists the query tiles in `plan` (device memory of
  * atf_prefill_plan_bytes, no initialisation needed), heaviest first; one plan serves
- * every layer of a step.  A plan made for other lengths gives rows that are not
+ * every layer of a step.  Small calls need none (0 bytes; the call then does nothing).  A plan made for other lengths gives rows that are not
  * computed, never an access out of bounds.
  */
 size_t atf_prefill_plan_bytes(int batch, int total_q, int num_q_heads);
@@ -207,8 +207,8 @@ int atf_prefill_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
  * the caller's: q and out as above, k and v bf16 [total_q][num_kv_heads][128] rows
  * (strides multiples of 8, 16-byte aligned) of the same sequences, at most max_seqlen
  * rows each (a longer sequence is not computed).  K and V are written to pages of
- * the workspace (RoPE there, with rope_cs), the tiles are listed, the attention
- * runs: three kernels.  The workspace needs no initialisation; calls that share one
+ * the workspace (RoPE there, with rope_cs), the tiles are listed where a list is
+ * needed, the attention runs: two or three kernels.  The workspace needs no initialisation; calls that share one
  * must be ordered on one stream.
  */
 size_t atf_flash_packed_workspace_bytes(int batch, int total_q, int max_seqlen, int num_q_heads, int num_kv_heads);

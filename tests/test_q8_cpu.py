@@ -126,12 +126,12 @@ def test_the_restated_cache_keeps_and_forgets():
     assert int(c.e[1, 0, 1]) == exponent(1000.0) and int(c.e[1, 0, 0]) == exponent(2.0)
 
 
-PLAN = dict(plan=1 << 20, plan_bytes=1 << 20, cu=1 << 20, lens=None, batch=2, total=100, most=60, hq=4, stream=None)
+PLAN = dict(plan=1 << 20, plan_bytes=1 << 20, cu=1 << 20, lens=None, batch=2, total=90000, most=60, hq=4, stream=None)
 FLASH = dict(out=1 << 20, o_st=512, o_sh=128, lse=None, q=1 << 20, q_st=512, q_sh=128, k=1 << 20, ks_t=256, ks_h=128,
              v=1 << 20, vs_t=256, vs_h=128, cu=1 << 20, batch=2, total=100, most=60, hq=4, hkv=2, zhi=None, scale=0.1,
              rope=None, rope_pos=0, layout=0, ws=1 << 20, ws_bytes=1 << 20, stream=None)
 PREFILL = dict(out=1 << 20, o_st=512, o_sh=128, lse=None, q=1 << 20, q_st=512, q_sh=128, kv=1 << 20, pages=9, table=1 << 20,
-               max_pages=4, cu=1 << 20, lens=None, batch=2, total=100, most=60, hq=4, hkv=2, zhi=None, scale=0.1, rope=None,
+               max_pages=4, cu=1 << 20, lens=None, batch=2, total=90000, most=60, hq=4, hkv=2, zhi=None, scale=0.1, rope=None,
                rope_pos=0, layout=0, plan=1 << 20, plan_bytes=1 << 20, stream=None)
 EXTEND = dict(table=1 << 20, max_pages=4, lens=1 << 20, new=1 << 20, free=1 << 20, num_free=4, count=1 << 20, batch=2,
               total=9, pages=9, lens_out=1 << 20, left=1 << 20, cu=1 << 20, pos=1 << 20, slots=1 << 20, stream=None)
@@ -159,7 +159,7 @@ def test_flash_packed_validation(no_gpu, change, code):
 def test_flash_packed_workspace_holds_its_parts(no_gpu):
     for b, t, most, hq, hkv in ((1, 1, 1, 4, 4), (5, 1000, 517, 24, 8), (300, 20000, 9000, 28, 4), (3, 48, 16, 2, 1)):
         pages = (t // 16 + b) * hkv * 8192
-        rest = no_gpu.atf_prefill_plan_bytes(b, t, hq) + 4 * b * (-(-most // 16) + 1)
+        rest = no_gpu.atf_prefill_plan_bytes(b, t, hq) + 4 * b * -(-most // 16)
         assert pages + rest <= no_gpu.atf_flash_packed_workspace_bytes(b, t, most, hq, hkv) <= pages + rest + 48
     assert no_gpu.atf_flash_packed_workspace_bytes(0, 1, 1, 1, 1) == 0
 
@@ -190,10 +190,10 @@ def test_release_validation(no_gpu, change, code):
 
 
 def test_plan_size_covers_every_split_of_the_rows(no_gpu):
-    # tiles of `batch` sequences with total rows: at most one started tile more for each
-    for batch, total, hq in ((1, 1, 4), (3, 1000, 28), (300, 20000, 8), (2, 100, 64), (8, 60, 2)):
-        places = (no_gpu.atf_prefill_plan_bytes(batch, total, hq) // 4 - 2) // 2
-        assert any(places == total // r + batch for r in (128, 256))
+    # tiles of `batch` sequences with total rows: at most one started tile more for each; no list for small calls
+    for batch, total, hq in ((1, 9000, 28), (3, 1500, 28), (300, 20000, 8), (8, 900, 64)):
+        assert (no_gpu.atf_prefill_plan_bytes(batch, total, hq) // 4 - 2) // 2 == total // 256 + batch
+    assert no_gpu.atf_prefill_plan_bytes(1, 1, 4) == no_gpu.atf_prefill_plan_bytes(5, 900, 24) == 0
     assert no_gpu.atf_prefill_plan_bytes(0, 5, 4) == no_gpu.atf_prefill_plan_bytes(1, 0, 4) == 0
 
 
