@@ -31,7 +31,8 @@ namespace atf {
 // are read from memory once; the heads turn every eight pages, so that no XCD
 // writes the same ones throughout (30000 x 8: 55.6 us a call, 58.4 without).
 // Otherwise x = page, y = sequence, z = heads.
-template <int kHeads, bool kHeadsFirst>
+// kPacked: packed rows (kv_rows), possibly into pages of their own (kv_page).
+template <int kHeads, bool kHeadsFirst, bool kPacked>
 __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t sv[kHeads][kPage][kD];
   const int b = kHeadsFirst ? blockIdx.z : blockIdx.y;
@@ -39,8 +40,8 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
   const int h0 = (kHeadsFirst ? (blockIdx.x + blockIdx.y / 8) % gridDim.x : blockIdx.z) * per;
   const int h_end = min(a.hkv, h0 + per);
   const int tid = threadIdx.x;
-  const int start = kv_start(a, b);
-  const KvRows rows = kv_rows(a, b);
+  const int start = kv_start<kPacked>(a, b);
+  const KvRows rows = kv_rows<kPacked>(a, b);
   const int64_t end64 = static_cast<int64_t>(start) + rows.count;  // exclusive
   const int first = max(start, 0) >> 4;
   const int pidx = first + static_cast<int>(kHeadsFirst ? blockIdx.y : blockIdx.x);
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
   if (a.rope_cs != nullptr) hi = min(hi, static_cast<int64_t>(a.rope_max_pos));
   if (lo >= hi) return;
   const int s0 = static_cast<int>(lo - p0), s1 = static_cast<int>(hi - p0);
-  const int pg = kv_page(a, rows, b, pidx, h0 == 0 && tid == 0);
+  const int pg = kv_page<kPacked>(a, rows, b, pidx, h0 == 0 && tid == 0);
   if (pg < 0 || pg >= a.num_pages) return;
   const size_t blk0 = static_cast<size_t>(pg) * a.hkv * kKvBlockElems;  // the page's block of head 0
   const int64_t t0 = rows.first + (p0 - start);  // source row of slot 0
@@ -155,10 +156,11 @@ __global__ __launch_bounds__(128) void kv_write_kernel(KvWriteArgs a) {
 // skips.
 // grid: x = source token, y = kv head, z = sequence.
 constexpr int kKvAppendTokens = 4;
+template <bool kPacked>
 __global__ __launch_bounds__(128) void kv_append_kernel(KvWriteArgs a) {
   const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x;
-  const KvRows rows = kv_rows(a, b);
+  const KvRows rows = kv_rows<kPacked>(a, b);
   if (t >= rows.count) return;
   const uint16_t* krow = a.k_src + static_cast<int64_t>(b) * a.ks_b + (rows.first + t) * a.ks_t +
                          static_cast<int64_t>(h) * a.ks_h;
@@ -168,12 +170,12 @@ __global__ __launch_bounds__(128) void kv_append_kernel(KvWriteArgs a) {
   const int c0 = level_chunk0(a.layout, l);
   const u32x4 x1 = ldg16(krow + c0), x2 = ldg16(krow + level_chunk1(a.layout, l));
   const uint16_t v = vrow[tid];
-  const int64_t pos = static_cast<int64_t>(kv_start(a, b)) + t;
+  const int64_t pos = static_cast<int64_t>(kv_start<kPacked>(a, b)) + t;
   const int64_t pidx = pos >> 4;
   if (pos < 0 || pidx >= a.max_pages || (a.rope_cs != nullptr && pos >= a.rope_max_pos)) return;
   float cs[16];
   if (a.rope_cs != nullptr) load_cs8(a.rope_cs, static_cast<int>(pos), c0, cs);
-  const int pg = kv_page(a, rows, b, pidx, h == 0 && tid == 0);
+  const int pg = kv_page<kPacked>(a, rows, b, pidx, h == 0 && tid == 0);
   if (pg < 0 || pg >= a.num_pages) return;
   const int slot = static_cast<int>(pos) & (kPage - 1);
   uint16_t* blk = a.kv_cache + (static_cast<size_t>(pg) * a.hkv + h) * kKvBlockElems;
@@ -203,16 +205,19 @@ template <int kHeads>
 static void launch_pages(const KvWriteArgs& a, int pages, int64_t rows, hipStream_t s) {
   const int groups = (a.hkv + kHeads - 1) / kHeads;
   const bool even = groups > 1 && rows > 128 * 1024 && a.hkv % groups == 0 && pages <= 65535 && a.batch <= 65535;
+  const bool packed = a.cu_tokens != nullptr;
   if (groups > 65535 || even)
-    hipLaunchKernelGGL((kv_write_kernel<kHeads, true>), dim3(groups, pages, a.batch), dim3(128), 0, s, a);
+    hipLaunchKernelGGL(packed ? (kv_write_kernel<kHeads, true, true>) : (kv_write_kernel<kHeads, true, false>),
+                       dim3(groups, pages, a.batch), dim3(128), 0, s, a);
   else
-    hipLaunchKernelGGL((kv_write_kernel<kHeads, false>), dim3(pages, a.batch, groups), dim3(128), 0, s, a);
+    hipLaunchKernelGGL(packed ? (kv_write_kernel<kHeads, false, true>) : (kv_write_kernel<kHeads, false, false>),
+                       dim3(pages, a.batch, groups), dim3(128), 0, s, a);
 }
 
 hipError_t launch_kv_write(const KvWriteArgs& a, hipStream_t s) {
   if (a.n_tokens <= 0 || a.batch <= 0) return hipSuccess;
   if (a.n_tokens <= kKvAppendTokens && a.hkv <= 65535 && a.batch <= 65535) {
-    hipLaunchKernelGGL(kv_append_kernel, dim3(a.n_tokens, a.hkv, a.batch), dim3(128), 0, s, a);
+    hipLaunchKernelGGL(a.cu_tokens != nullptr ? kv_append_kernel<true> : kv_append_kernel<false>, dim3(a.n_tokens, a.hkv, a.batch), dim3(128), 0, s, a);
     return hipGetLastError();
   }
   // a call of n tokens touches at most ceil(n / 16) + 1 pages per sequence

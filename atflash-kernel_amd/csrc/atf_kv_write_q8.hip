@@ -95,7 +95,7 @@ __global__ __launch_bounds__(128) void kv_write_q8_kernel(KvWriteArgs a) {
   const int b = blockIdx.y, tid = threadIdx.x;
   const int j8 = blockIdx.x / a.page_round, turn = j8 / a.hkv, h = j8 - turn * a.hkv;
   const int start = a.start_pos[b];
-  const KvRows rows = kv_rows(a, b);
+  const KvRows rows = a.cu_tokens != nullptr ? kv_rows<true>(a, b) : kv_rows<false>(a, b);
   const int64_t end64 = static_cast<int64_t>(start) + rows.count;
   const int pidx = (max(start, 0) >> 4) + turn * a.page_round + (static_cast<int>(blockIdx.x) - j8 * a.page_round);
   const int64_t p0 = static_cast<int64_t>(pidx) * kPage;

@@ -56,17 +56,22 @@ struct KvRows {
   int64_t first;
   int count;
 };
-__device__ __forceinline__ int kv_start(const KvWriteArgs& a, int b) { return a.own_table != nullptr ? 0 : a.start_pos[b]; }
+template <bool kPacked>
+__device__ __forceinline__ int kv_start(const KvWriteArgs& a, int b) {
+  return kPacked && a.own_table != nullptr ? 0 : a.start_pos[b];
+}
 // The page of entry `pidx` of sequence b, and in a call with pages of its own its entry.
+template <bool kPacked>
 __device__ __forceinline__ int kv_page(const KvWriteArgs& a, const KvRows& rows, int b, int64_t pidx, bool enter) {
   const int64_t at = static_cast<int64_t>(b) * a.max_pages + pidx;
-  if (a.own_table == nullptr) return a.page_table[at];
+  if (!kPacked || a.own_table == nullptr) return a.page_table[at];
   const int pg = static_cast<int>(rows.first / kPage + b + pidx);
   if (enter) a.own_table[at] = pg;
   return pg;
 }
+template <bool kPacked>
 __device__ __forceinline__ KvRows kv_rows(const KvWriteArgs& a, int b) {
-  if (a.cu_tokens == nullptr) return KvRows{0, a.n_tokens};
+  if (!kPacked) return KvRows{0, a.n_tokens};
   const int lo = max(a.cu_tokens[b], 0), hi = min(a.cu_tokens[b + 1], a.total_tokens);
   return KvRows{lo, max(0, min(hi - lo, a.n_tokens))};
 }

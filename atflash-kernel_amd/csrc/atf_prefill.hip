@@ -100,15 +100,20 @@ __device__ __forceinline__ bf16x8 lds_frag(const lds_u8* p) {
   return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(p);
 }
 
+__device__ __forceinline__ const int32_t* table_row(const PrefillArgs& a, int b) {
+  return a.page_table + static_cast<int64_t>(b) * a.max_pages;
+}
+
 // What a workgroup works on.  One sequence of a batch of equal lengths: the call's own
 // arguments.
 struct BatchSeq {
   const PrefillArgs& a;
   int b;
+  const int32_t* row;  // of the page table
   __device__ __forceinline__ int nq() const { return a.nq; }
   __device__ __forceinline__ int nk() const { return a.nk; }
   __device__ __forceinline__ int q_offset() const { return a.q_offset; }
-  __device__ __forceinline__ const int32_t* pages() const { return a.page_table + static_cast<int64_t>(b) * a.max_pages; }
+  __device__ __forceinline__ const int32_t* pages() const { return row; }
   __device__ __forceinline__ const uint16_t* q(int h) const {
     return a.q + static_cast<int64_t>(b) * a.q_sb + static_cast<int64_t>(h) * a.q_sh;
   }
@@ -122,10 +127,11 @@ struct BatchSeq {
 struct PackedSeq {
   const PrefillArgs& a;
   int b, row0, n_q, n_k;
+  const int32_t* row;  // of the page table
   __device__ __forceinline__ int nq() const { return n_q; }
   __device__ __forceinline__ int nk() const { return n_k; }
   __device__ __forceinline__ int q_offset() const { return n_k - n_q; }
-  __device__ __forceinline__ const int32_t* pages() const { return a.page_table + static_cast<int64_t>(b) * a.max_pages; }
+  __device__ __forceinline__ const int32_t* pages() const { return row; }
   __device__ __forceinline__ const uint16_t* q(int h) const {
     return a.q + static_cast<int64_t>(row0) * a.q_st + static_cast<int64_t>(h) * a.q_sh;
   }
@@ -142,7 +148,7 @@ __device__ __forceinline__ PackedSeq packed_seq(const PrefillArgs& a, int b) {
   int n = max(hi - lo, 0);
   const int keys = a.pk.seq_lens != nullptr ? a.pk.seq_lens[b] : n;
   if (keys < n || keys > a.pk.max_k) n = 0;
-  return PackedSeq{a, b, lo, n, keys};
+  return PackedSeq{a, b, lo, n, keys, table_row(a, b)};
 }
 
 // Raw page-table entry of page `pidx` of the sequence (-1 past the keys), in a
@@ -1256,14 +1262,14 @@ __device__ __forceinline__ void prefill_solo_rows(const Seq& sq, int h, int qt) 
 template <bool kRaw>
 __global__ __launch_bounds__(kPfWaves * 64, 1) void prefill_kernel(PrefillArgs a) {
   int b, h, qt;
-  if (prefill_block(a, blockIdx.x, b, h, qt)) prefill_rows<kRaw>(BatchSeq{a, b}, h, qt);
+  if (prefill_block(a, blockIdx.x, b, h, qt)) prefill_rows<kRaw>(BatchSeq{a, b, table_row(a, b)}, h, qt);
 }
 
 template <bool kRaw>
 __global__ __launch_bounds__(kSoloWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void prefill_solo_kernel(PrefillArgs a) {
   int b, h, qt;
-  if (prefill_block(a, blockIdx.x, b, h, qt)) prefill_solo_rows<kRaw>(BatchSeq{a, b}, h, qt);
+  if (prefill_block(a, blockIdx.x, b, h, qt)) prefill_solo_rows<kRaw>(BatchSeq{a, b, table_row(a, b)}, h, qt);
 }
 
 // ---- packed rows of sequences of different lengths ----
