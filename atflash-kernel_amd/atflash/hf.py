@@ -58,7 +58,7 @@ except ImportError:  # pragma: no cover - the package works without transformers
 from . import _lib
 from . import interface as I
 from . import ops
-from .cache import k_half, new_kv_cache, v_half
+from .cache import k_half, new_kv_cache, new_kv_cache_q8, v_half
 from .model_tables import ModelWindow, window_from_config
 
 ATTN_NAME = "atf_window"
@@ -84,9 +84,13 @@ class PagedLayer(CacheLayerMixin):
         n_pages = owner.batch * owner.pages_per_seq
         self.owner = owner
         self.layer_idx = layer_idx
-        self.kv = new_kv_cache(n_pages, owner.num_kv_heads, owner.device)
-        self.k = k_half(self.kv)  # views of the two halves
-        self.v = v_half(self.kv)
+        self.exps = None  # exponents of a cache of 8-bit floats
+        if owner.kv_dtype == torch.float8_e4m3fn:
+            self.kv, self.exps = new_kv_cache_q8(n_pages, owner.num_kv_heads, owner.device)
+        else:
+            self.kv = new_kv_cache(n_pages, owner.num_kv_heads, owner.device)
+            self.k = k_half(self.kv)  # views of the two halves
+            self.v = v_half(self.kv)
         self.length = 0       # tokens written (every sequence of the batch has the same length)
         self.prev_length = 0  # length before the last update (the last chunk's first position)
         self.last_key = None  # the key tensor of the last update until the hook reads it (identity check)
@@ -115,8 +119,12 @@ class PagedLayer(CacheLayerMixin):
         if self.length + L > o.capacity:
             raise ValueError(f"PagedCache holds {o.capacity} tokens per sequence; "
                              f"{self.length} + {L} would not fit")
-        ops.kv_write(self.kv, key_states.transpose(1, 2), value_states.transpose(1, 2),
-                     o.start_positions(self.length), o.page_table, o.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+        args = (key_states.transpose(1, 2), value_states.transpose(1, 2), o.start_positions(self.length), o.page_table,
+                o.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+        if self.exps is None:
+            ops.kv_write(self.kv, *args)
+        else:
+            ops.kv_write_q8(self.kv, self.exps, *args)
         self.prev_length = self.length
         self.length += L
         self.last_key = key_states
@@ -167,16 +175,23 @@ class PagedCache(Cache):
     sequence b owns pages [b * pages_per_seq, (b + 1) * pages_per_seq).  Memory
     is allocated up front: batch * ceil(capacity / 16) pages per layer, 8 KB per
     page and kv head (a 1M-token Qwen2.5-7B layer with 4 kv heads: 2 GB).
+    kv_dtype=torch.float8_e4m3fn holds 8-bit floats with a power of two for each page,
+    kv head and half instead: half the memory, and half the bytes a decode step reads.
     """
 
-    def __init__(self, config, batch: int, capacity: int, device="cuda", rope_cs=None):
+    def __init__(self, config, batch: int, capacity: int, device="cuda", rope_cs=None,
+                 kv_dtype: torch.dtype = torch.bfloat16):
         """rope_cs: fp32 [>= capacity, 64, 2] (cos, sin) table when the keys
-        arrive unrotated (RoPE applied at write), None when they arrive rotated."""
+        arrive unrotated (RoPE applied at write), None when they arrive rotated.
+        kv_dtype: torch.bfloat16 or torch.float8_e4m3fn."""
         from .model_tables import head_dim_of
         if head_dim_of(config) != _lib.HEAD_DIM:
             raise ValueError(f"head_dim {head_dim_of(config)} unsupported (this build supports {_lib.HEAD_DIM})")
         if rope_cs is not None and rope_cs.shape[0] < capacity:
             raise ValueError(f"rope table has {rope_cs.shape[0]} positions, the cache holds {capacity}")
+        if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"kv_dtype must be bfloat16 or float8_e4m3fn, got {kv_dtype}")
+        self.kv_dtype = kv_dtype
         self.rope_cs = rope_cs
         self.batch = int(batch)
         self.capacity = int(capacity)
@@ -271,11 +286,12 @@ class WindowAttention:
             self._rope[dev] = t
         return t
 
-    def new_cache(self, config, batch: int, capacity: int, device="cuda") -> PagedCache:
+    def new_cache(self, config, batch: int, capacity: int, device="cuda",
+                  kv_dtype: torch.dtype = torch.bfloat16) -> PagedCache:
         """A PagedCache bound to this hook (pass it as past_key_values)."""
         if capacity - 1 > self.window.n_ctx:
             raise ValueError(f"capacity {capacity} exceeds the window tables' n_ctx {self.window.n_ctx}")
-        cache = PagedCache(config, batch, capacity, device, rope_cs=self.rope_table(capacity, device))
+        cache = PagedCache(config, batch, capacity, device, rope_cs=self.rope_table(capacity, device), kv_dtype=kv_dtype)
         self._caches.add(cache)
         return cache
 
@@ -318,12 +334,14 @@ class WindowAttention:
                 raise ValueError("the cache was made for the other RoPE mode of this hook")
             if L == 1:
                 zhi = self.window.decode_zhi8 if windowed else None
-                o = ops.decode_paged(query.select(2, 0), lyr.kv, owner.page_table, owner.seq_lens(S), S, zhi,
-                                     scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+                args = (owner.page_table, owner.seq_lens(S), S, zhi, scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+                o = (ops.decode_paged(query.select(2, 0), lyr.kv, *args) if lyr.exps is None
+                     else ops.decode_paged_q8(query.select(2, 0), lyr.kv, lyr.exps, *args))
                 return o.view(b, 1, hq, d), None
             zhi = self.window.prefill_zhi if windowed else None
-            o, _ = ops.prefill(query.transpose(1, 2), lyr.kv, owner.page_table, S, lyr.prev_length, zhi, scale,
-                               owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+            args = (owner.page_table, S, lyr.prev_length, zhi, scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+            o, _ = (ops.prefill(query.transpose(1, 2), lyr.kv, *args) if lyr.exps is None
+                    else ops.prefill_q8(query.transpose(1, 2), lyr.kv, lyr.exps, *args))
             return o, None  # [b, L, hq, d]
         # any other cache: key/value hold the whole history [b, hkv, S, d]
         if not self._warned_repack and S > 4096:
