@@ -424,7 +424,8 @@ def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
                       zhi, sm_scale: float, rope_cs: Optional[torch.Tensor],
                       layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """prefill_packed of whole prompts whose keys and values are packed rows too
-    (k, v [T, Hkv, 128]): they are written to temporary pages first."""
+    (k, v [T, Hkv, 128]): they are written to temporary pages first.  The rows of a
+    sequence longer than max_seqlen are not computed."""
     dev = _one_device(q, k, v, cu_seqlens, rope_cs)
     (T, Hq, D), qst = _check_packed_q(q)
     _need(k.dim() == 3 and k.shape[0] == T, "q, k and v must have the same rows [T, heads, 128]")
@@ -527,8 +528,10 @@ _WS_BYTES = {}  # (batch, hq, hkv, max_seq_len, 8-bit cache) -> workspace bytes 
 
 
 def _decode_workspace(device, handle, B, hq, hkv, max_seq_len, L, q8=False):
-    """(address, bytes) of the workspace of (device, stream), grown to what a
-    call of this shape needs."""
+    """(address, bytes, tensor) of the workspace of (device, stream), grown to what a
+    call of this shape needs.  A call under stream capture gets one of its own, from
+    the graph's memory: graphs that shared one would race when they are replayed on
+    different streams, and an eager call must not be left with a graph's memory."""
     shape = (B, hq, hkv, max_seq_len, q8)
     nbytes = _WS_BYTES.get(shape)
     if nbytes is None:
@@ -536,6 +539,9 @@ def _decode_workspace(device, handle, B, hq, hkv, max_seq_len, L, q8=False):
             _WS_BYTES.clear()
         size = L.atf_decode_q8_workspace_bytes if q8 else L.atf_decode_workspace_bytes_even
         nbytes = _WS_BYTES[shape] = int(size(B, hq, hkv, max_seq_len))
+    if torch._C._cuda_isCurrentStreamCapturing():
+        t = torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
+        return t.data_ptr(), t.numel() * 4, t
     key = (device.index, handle)
     ws = _DECODE_WS.get(key)
     if ws is None or ws[1] < nbytes:
@@ -720,6 +726,7 @@ class DecodePlan:
         slices = zhi is not None and len(zhi) == _lib.SLICES
         L = _lib.lib()
         self.device = kv_cache.device
+        self._index = kv_cache.get_device()
         self.shape = (B, Hq, D)
         self.q_strides = (q_sb, q_sh, 1)
         size = L.atf_decode_workspace_bytes_even if kv_exps is None else L.atf_decode_q8_workspace_bytes
@@ -745,8 +752,8 @@ class DecodePlan:
             out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
         elif out.shape != self.shape or not out.is_contiguous() or out.dtype != torch.bfloat16:
             raise ValueError(f"out must be contiguous bf16 {self.shape}")
-        _lib.check(self._entry(out.data_ptr(), self.shape[1] * _lib.HEAD_DIM, _lib.HEAD_DIM, q.data_ptr(),
-                               self.q_strides[0], self.q_strides[1], *self._mid, _lib.stream_of(self.device)))
+        _lib.launch(self._index, self._entry, out.data_ptr(), self.shape[1] * _lib.HEAD_DIM, _lib.HEAD_DIM, q.data_ptr(),
+                    self.q_strides[0], self.q_strides[1], *self._mid)
         return out
 
 

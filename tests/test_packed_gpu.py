@@ -223,6 +223,48 @@ def test_captured_steps_follow_the_lengths(dev):
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
 
 
+def test_registered_operators(dev):
+    from atflash import ops
+    held, new = [100, 40], [60, 40]
+    k, v = rows(18, dev, (140, 2, D), (140, 2, D))
+    (q,) = rows(19, dev, (100, 4, D))
+    cache, table = paged(k, v, held, dev)
+    cu, n = ints([0, 60, 100], dev), ints(held, dev)
+    want = ops.prefill_packed(q, cache.kv, table, cu, n, 100, level_table(), SCALE, None, 0)
+    got = torch.ops.atflash.prefill_packed(q, cache.kv, table, cu, n, 100, level_table(), SCALE, None, 0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_plan_shared_by_layers_and_its_refusals(dev):
+    from atflash import interface
+    hq, hkv, held = 48, 4, [900, 40, 300]
+    T = sum(held)
+    q, k, v = rows(22, dev, (T, hq, D), (T, hkv, D), (T, hkv, D))
+    cache, table = paged(k, v, held, dev)
+    cu, n = ints(cumulate(held), dev), ints(held, dev)
+    plan = interface.packed_plan(cu, n, T, 900, hq)
+    want = interface.prefill_packed(q, cache, table, cu, n, 900)
+    for _ in range(2):
+        got = interface.prefill_packed(q, cache, table, cu, n, 900, plan=plan)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for args in ((q[:-1], cu, n, 900), (q[:, :24], cu, n, 900), (q, cu.clone(), n, 900), (q, cu, None, 900), (q, cu, n, 901)):
+        with pytest.raises(ValueError):
+            interface.prefill_packed(args[0], cache, table, *args[1:], plan=plan)
+    # other lengths in the same tensors: refreshed, right again; a stale list stays in bounds
+    for lens in ([300, 500, 440], [1240, 0, 0]):
+        cu.copy_(ints(cumulate(lens), dev))
+        n.copy_(ints(lens, dev))
+        interface.prefill_packed(q, cache, table, cu, n, 900, plan=plan)
+        plan.refresh()
+        got = interface.prefill_packed(q, cache, table, cu, n, 900, plan=plan)
+        torch.cuda.synchronize()
+        want = interface.prefill_packed(q, cache, table, cu, n, 900)
+        for b, m in enumerate(lens):
+            if 0 < m <= 900:  # (a sequence of 1240 keys is past the call's 900: not computed)
+                r = slice(sum(lens[:b]), sum(lens[:b]) + m)
+                assert torch.equal(got[0][r], want[0][r])
+
+
 def test_two_streams_at_once(dev):
     from atflash import interface
     a = rows(20, dev, (500, 8, D), (500, 2, D), (500, 2, D))

@@ -392,6 +392,52 @@ def test_decode_captured_and_on_another_stream(dev):
         assert torch.equal(out, interface.decode_paged(q, cache, table, n, 5000, zhi=tables()[1]))
 
 
+def test_captured_calls_have_a_workspace_of_their_own(dev):
+    from atflash import interface, ops
+    cache, table, _ = filled([9000, 300], 2, dev, 74)
+    q = torch.randn((2, 8, D), generator=torch.Generator(device=dev).manual_seed(5), device=dev).to(BF)
+    n = row_of([9000, 300], dev)
+    want = interface.decode_paged(q, cache, table, n, 9000)
+    before = dict(ops._DECODE_WS)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(interface.decode_paged(q, cache, table, n, 9000))
+        graphs.append(g)
+    assert ops._DECODE_WS == before
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_registered_operators(dev):
+    from atflash import ops
+    g = torch.Generator(device=dev).manual_seed(76)
+    k, v = (torch.randn((2, 40, 2, D), generator=g, device=dev).to(BF) for _ in range(2))
+    table, start, cs = row_of([[0, 1, 2], [5, 4, 3]], dev), row_of([0, 0], dev), ropes(48).to(dev)
+    a, b, c = (new_cache(6, 2, dev) for _ in range(3))
+    ops.kv_write_q8(a.kv, a.exps, k, v, start, table, cs, 0)
+    torch.ops.atflash.kv_write_q8(b.kv, b.exps, k, v, start, table, cs, 0)
+    torch.ops.atflash.kv_write_packed(c.kv, c.exps, k.flatten(0, 1), v.flatten(0, 1), row_of([0, 40, 80], dev), 40, start,
+                                      table, cs, 0)
+    for x in (b, c):
+        assert torch.equal(a.kv.view(torch.uint8), x.kv.view(torch.uint8)) and torch.equal(a.exps, x.exps)
+    q = torch.randn((2, 6, D), generator=g, device=dev).to(BF)
+    n = row_of([40, 17], dev)
+    assert torch.equal(ops.decode_paged_q8(q, a.kv, a.exps, table, n, 48, None, SCALE, cs, 0),
+                       torch.ops.atflash.decode_paged_q8(q, a.kv, a.exps, table, n, 48, None, SCALE, cs, 0))
+    q = torch.randn((2, 40, 6, D), generator=g, device=dev).to(BF)
+    for x, y in zip(ops.prefill_q8(q, a.kv, a.exps, table, 40, 0, None, SCALE, cs, 0),
+                    torch.ops.atflash.prefill_q8(q, a.kv, a.exps, table, 40, 0, None, SCALE, cs, 0)):
+        assert torch.equal(x, y)
+
+
 def test_pool_past_4_gib(dev):
     # block offsets past 32 bits: pages at the end of a pool of 4.5 GB
     from atflash import interface, ops
