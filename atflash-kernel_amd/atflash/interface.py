@@ -46,13 +46,16 @@ def _layout_id(layout):
     return LAYOUTS[layout]
 
 
+_INTS = frozenset((int,))
+
+
 def _zhi_list(zhi, sizes=(_lib.LEVELS,)):
     """A window table as a list of ints: the level table (LEVELS entries), or for
     decode also the per-slice vec8 table (SLICES entries)."""
     if zhi is None:
         return None
-    if type(zhi) is tuple and len(zhi) in sizes:
-        return zhi  # (cannot change: its array is found by identity, ops._table)
+    if type(zhi) is tuple and len(zhi) in sizes and _INTS.issuperset(map(type, zhi)):
+        return zhi  # as it is
     vals = [int(x) for x in (zhi.tolist() if isinstance(zhi, torch.Tensor) else zhi)]
     if len(vals) not in sizes:
         raise ValueError(f"window table must have {' or '.join(map(str, sizes))} entries, got {len(vals)}")
@@ -158,7 +161,7 @@ def prefill_packed(q, cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi=
         pages = -(-int(max_seq_len) // PAGE)
         if page_table.dim() != 2 or page_table.shape[1] < pages:
             raise ValueError(f"page table too small for max_seq_len={max_seq_len}")
-        kv, page_table = ops.kv_expand_q8(kv, cache.exps, page_table, pages)
+        kv, page_table = ops.kv_expand_q8(kv, cache.exps, page_table, pages, seq_lens)
     return ops.prefill_packed(q, kv, page_table, cu_seqlens, seq_lens, int(max_seq_len), _zhi_list(zhi), scale, rope,
                               _layout_id(layout), plan, out, lse)
 

@@ -255,18 +255,22 @@ def _(kv_cache, kv_exps, k, v, cu_seqlens, max_tokens, start_pos, page_table, ro
     return None
 
 
-def kv_expand_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torch.Tensor, n_pages: int):
+def kv_expand_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torch.Tensor, n_pages: int,
+                 seq_lens: Optional[torch.Tensor] = None):
     """The first n_pages pages of each sequence of an 8-bit cache as bf16 pages,
-    exactly: (bf16 cache [B * n_pages, Hkv, 2, 2048], its page table [B, n_pages])."""
-    dev = _one_device(kv_cache, kv_exps, page_table)
+    exactly: (bf16 cache [B * n_pages, Hkv, 2, 2048], its page table [B, n_pages]).
+    seq_lens int32 [B]: pages past a sequence's tokens are left out (-1)."""
+    dev = _one_device(kv_cache, kv_exps, page_table, seq_lens)
     pool = _check_cache_q8(kv_cache, kv_exps)
     B, width = _check_table(page_table)
+    if seq_lens is not None:
+        _check_ints(seq_lens, B, "seq_lens")
     n = int(n_pages)
     _need(n >= 0, "n_pages must be >= 0")
     out = torch.empty((B * n, pool[1], *_lib.KV_BLOCK_SHAPE), dtype=torch.bfloat16, device=kv_cache.device)
     table = page_table.new_empty((B, n))
     _lib.launch(dev, _lib.lib().atf_kv_expand_q8, out.data_ptr(), table.data_ptr(), kv_cache.data_ptr(),
-                kv_exps.data_ptr(), pool[0], pool[1], page_table.data_ptr(), B, width, n)
+                kv_exps.data_ptr(), pool[0], pool[1], page_table.data_ptr(), B, width, n, _lib.ptr(seq_lens))
     return out, table
 
 
@@ -443,8 +447,7 @@ def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     lse = torch.empty((Hq, T), dtype=torch.float32, device=q.device)
     _lib.launch(dev, L.atf_flash_packed_bf16, out.data_ptr(), Hq * D, D, lse.data_ptr(), q.data_ptr(), qst[0], qst[1],
                 k.data_ptr(), ks_t, ks_h, v.data_ptr(), vs_t, vs_h, cu_seqlens.data_ptr(), B, T, most, Hq, hkv,
-                _lib.zhi_array(zhi) if type(zhi) is not tuple else _table(zhi, _lib.LEVELS), float(sm_scale),
-                _lib.ptr(rope_cs), max_pos, _layout(layout), ws.data_ptr(), nbytes)
+                _lib.zhi_array(zhi), float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout), ws.data_ptr(), nbytes)
     return out, lse
 
 
@@ -631,7 +634,7 @@ def decode_paged_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tens
     n, table = 0, None
     if zhi is not None:
         n = len(zhi)
-        table = _table(zhi, _lib.SLICES if n == _lib.SLICES else _lib.LEVELS)
+        table = _lib.zhi_array(zhi, _lib.SLICES if n == _lib.SLICES else _lib.LEVELS)
     most = int(max_seq_len)
     ws = _decode_workspace(q.device, _lib.raw_stream(dev), B, Hq, hkv, most, L, True)
     out = q.new_empty(qs)

@@ -310,7 +310,7 @@ struct PackedLayout {
 PackedLayout packed_layout(int batch, int total_q, int max_seqlen, int num_q_heads, int num_kv_heads) {
   PackedLayout w{};
   w.pages = total_q / atf::kPage + batch;
-  w.width = (max_seqlen + atf::kPage - 1) / atf::kPage;
+  w.width = (std::min(max_seqlen, total_q) + atf::kPage - 1) / atf::kPage;
   w.plan = static_cast<size_t>(w.pages) * num_kv_heads * atf::kKvBlockElems * 2;
   w.table = (w.plan + atf::prefill_plan_bytes(batch, total_q, num_q_heads) + 15) / 16 * 16;
   w.bytes = (w.table + static_cast<size_t>(batch) * w.width * sizeof(int32_t) + 15) / 16 * 16;
@@ -392,7 +392,8 @@ int atf_kv_write_q8(void* kv_cache, int8_t* kv_exps, int num_pages, int num_kv_h
 }
 
 int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const int8_t* kv_exps, int num_pages,
-                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages, void* stream) {
+                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages,
+                     const int32_t* seq_lens, void* stream) {
   if (batch < 0 || n_pages < 0) return fail(ATF_ERR_INVALID, "batch and n_pages must be >= 0");
   if (batch == 0 || n_pages == 0) return ok();
   if (!out || !out_table || !kv_cache || !kv_exps || !page_table) return fail(ATF_ERR_INVALID, "null pointer argument");
@@ -404,7 +405,7 @@ int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const 
     return fail(ATF_ERR_UNSUPPORTED, "at most 65535 sequences and kv heads and 2^31 - 1 pages, got %d, %d and %lld", batch,
                 num_kv_heads, static_cast<long long>(batch) * n_pages);
   const atf::KvExpandArgs a{static_cast<const uint8_t*>(kv_cache), kv_exps, num_pages, num_kv_heads, page_table, batch,
-                            max_pages, n_pages, static_cast<uint16_t*>(out), out_table};
+                            max_pages, n_pages, seq_lens, static_cast<uint16_t*>(out), out_table};
   hipError_t e = atf::launch_kv_expand_q8(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "8-bit expand launch");
   return ok();
@@ -463,6 +464,7 @@ int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse, con
   if (max_seqlen <= 0 || num_q_heads <= 0 || num_kv_heads <= 0)
     return fail(ATF_ERR_INVALID, "max_seqlen, num_q_heads and num_kv_heads must be positive");
   if (max_seqlen >= (1 << 24)) return fail(ATF_ERR_UNSUPPORTED, "max_seqlen must be < 2^24");
+  max_seqlen = std::min(max_seqlen, total_q);  // (no sequence has more rows than the call)
   const PackedLayout w = packed_layout(batch, total_q, max_seqlen, num_q_heads, num_kv_heads);
   if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 16))
     return fail(ATF_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", w.bytes,
@@ -478,7 +480,7 @@ int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse, con
   if (int r = check_plan(plan, w.table - w.plan, cu_seqlens, batch, total_q, max_seqlen, num_q_heads)) return r;
   atf::KvWriteArgs k_args{};
   if (int r = kv_write_prepare(ws, w.pages, num_kv_heads, k, 0, ks_t, ks_h, v, 0, vs_t, vs_h, batch,
-                               std::min(max_seqlen, total_q), table, table, w.width, rope_cs, rope_max_pos, layout, &k_args))
+                               max_seqlen, table, table, w.width, rope_cs, rope_max_pos, layout, &k_args))
     return r;
   k_args.cu_tokens = cu_seqlens;
   k_args.total_tokens = total_q;
@@ -522,6 +524,8 @@ int atf_extend_tables(int32_t* page_table, int max_pages, const int32_t* seq_len
   if (!aligned(slots, 8)) return fail(ATF_ERR_INVALID, "slots must be 8-byte aligned");
   if (batch > atf::kTabMaxBatch)
     return fail(ATF_ERR_UNSUPPORTED, "at most %d sequences, got %d", atf::kTabMaxBatch, batch);
+  if (static_cast<int64_t>(batch) * max_pages > (int64_t(1) << 30))  // (numbers of the call's pages are 32-bit)
+    return fail(ATF_ERR_UNSUPPORTED, "page table of at most 2^30 entries, got %d x %d", batch, max_pages);
   const atf::ExtendTablesArgs a{page_table, max_pages, seq_lens,  new_lens,  free_pages, num_free,  free_count, batch,
                                 total_tokens, num_pages, seq_lens_out, free_left, cu_seqlens, positions, slots};
   hipError_t e = atf::launch_extend_tables(a, static_cast<hipStream_t>(stream));

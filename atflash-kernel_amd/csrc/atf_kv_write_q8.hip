@@ -248,7 +248,8 @@ hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s) {
 __global__ __launch_bounds__(128) void kv_expand_q8_kernel(KvExpandArgs a) {
   const int p = blockIdx.x, b = blockIdx.y, h = blockIdx.z, tid = threadIdx.x;
   const int64_t entry = static_cast<int64_t>(b) * a.n_pages + p;
-  const int pg = a.page_table[static_cast<int64_t>(b) * a.max_pages + p];
+  const bool held = a.seq_lens == nullptr || static_cast<int64_t>(p) * kPage < a.seq_lens[b];
+  const int pg = held ? a.page_table[static_cast<int64_t>(b) * a.max_pages + p] : -1;
   const bool ok = pg >= 0 && pg < a.num_pages;
   if (h == 0 && tid == 0) a.out_table[entry] = ok ? static_cast<int32_t>(entry) : -1;
   if (!ok) return;

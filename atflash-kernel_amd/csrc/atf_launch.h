@@ -186,6 +186,7 @@ struct KvExpandArgs {
   int num_pages, hkv;
   const int32_t* page_table;
   int batch, max_pages, n_pages;
+  const int32_t* seq_lens;  // tokens of each sequence (null: n_pages pages of each); -1 for entries past them
   uint16_t* out;
   int32_t* out_table;
 };

@@ -44,7 +44,8 @@ __global__ __launch_bounds__(kTabThreads) void extend_tables_kernel(ExtendTables
       const int len = length(b);
       n = fresh(b);
       need = max(min(pages_of(static_cast<int64_t>(len) + n), a.max_pages) - pages_of(len), 0);
-      if (blockIdx.x == 0) a.lens_out[b] = len + n;
+      if (blockIdx.x == 0)
+        a.lens_out[b] = static_cast<int>(min(static_cast<int64_t>(len) + n, static_cast<int64_t>(INT32_MAX)));
     }
     int st = n, sp = need;  // inclusive sums of the wave, then of the workgroup
 #pragma unroll
@@ -98,7 +99,8 @@ __global__ __launch_bounds__(kTabThreads) void extend_tables_kernel(ExtendTables
     if (t < carry_t) {
       const int b = last_at_most(cu, a.batch, t);
       const int len = length(b), had = pages_of(len);
-      pos = len + (t - cu[b]);
+      const int64_t at64 = static_cast<int64_t>(len) + t - cu[b];  // (lengths that make no sense: no page)
+      pos = static_cast<int>(min(at64, static_cast<int64_t>(INT32_MAX)));
       const int col = pos / kPage;
       int page = -1;
       if (col < a.max_pages)

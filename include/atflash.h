@@ -149,11 +149,13 @@ int atf_kv_write_q8(void* kv_cache, int8_t* kv_exps, int num_pages, int num_kv_h
  * a bf16 number): entry (b, p), p < n_pages, of the page table (rows of max_pages) to
  * block b * n_pages + p of out (bf16 [batch * n_pages][num_kv_heads][2][2048]), and
  * that number to out_table (int32 [batch][n_pages]).  An entry outside
- * [0, num_pages) gets -1 there and leaves its block as it is.  With out and
- * out_table atf_prefill_bf16 attends to an 8-bit cache.
+ * [0, num_pages), or past the seq_lens[b] tokens of its sequence (seq_lens null: none
+ * is), gets -1 there and leaves its block as it is.  With out and out_table
+ * atf_prefill_bf16 and atf_prefill_packed_bf16 attend to an 8-bit cache.
  */
 int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const int8_t* kv_exps, int num_pages,
-                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages, void* stream);
+                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages,
+                     const int32_t* seq_lens, void* stream);
 
 /*
  * Windowed causal GQA prefill: out[b, i, h, :] = attention of query row i
@@ -188,8 +190,9 @@ int atf_prefill_bf16(void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float*
  * queries than keys or more than max_seq_len keys.
  *   atf_prefill_plan first lists the query tiles in `plan` (device memory of
  * atf_prefill_plan_bytes, no initialisation needed), heaviest first; one plan serves
- * every layer of a step.  Small calls need none (0 bytes; the call then does nothing).  A plan made for other lengths gives rows that are not
- * computed, never an access out of bounds.
+ * every layer of a step.  Small calls need none (0 bytes; the call then does nothing).
+ * A plan made for other lengths gives rows that are not computed, never an access out
+ * of bounds.
  */
 size_t atf_prefill_plan_bytes(int batch, int total_q, int num_q_heads);
 int atf_prefill_plan(void* plan, size_t plan_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens, int batch,
@@ -208,8 +211,8 @@ int atf_prefill_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
  * (strides multiples of 8, 16-byte aligned) of the same sequences, at most max_seqlen
  * rows each (a longer sequence is not computed).  K and V are written to pages of
  * the workspace (RoPE there, with rope_cs), the tiles are listed where a list is
- * needed, the attention runs: two or three kernels.  The workspace needs no initialisation; calls that share one
- * must be ordered on one stream.
+ * needed, the attention runs: two or three kernels.  The workspace needs no
+ * initialisation; calls that share one must be ordered on one stream.
  */
 size_t atf_flash_packed_workspace_bytes(int batch, int total_q, int max_seqlen, int num_q_heads, int num_kv_heads);
 int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
@@ -237,7 +240,9 @@ int atf_flash_packed_bf16(void* out, int64_t o_st, int64_t o_sh, float* lse,
  *                           the last new token.  New tokens past total_tokens are not
  *                           listed.
  * seq_lens and free_count are read only, so that a call can be repeated.  batch is at
- * most 8191; the new tokens of a call and their positions are below 2^31.
+ * most 8191 and batch * max_pages at most 2^30; the new tokens of a call and their
+ * positions are below 2^31 (other lengths give entries without a meaning, never an
+ * access out of bounds).
  */
 int atf_extend_tables(int32_t* page_table, int max_pages, const int32_t* seq_lens, const int32_t* new_lens,
                       const int32_t* free_pages, int num_free, const int32_t* free_count, int batch, int total_tokens,

@@ -78,6 +78,16 @@ def test_whole_prompts_are_the_bits_of_single_calls(dev, lens, hq, hkv, rope):
             assert torch.equal(out[r], o1[0]) and torch.equal(lse[:, r], l1[0])
 
 
+def test_a_bound_far_past_the_rows(dev):
+    from atflash import interface
+    lens = [40, 1, 300]
+    q, k, v = rows(7, dev, (341, 4, D), (341, 2, D), (341, 2, D))
+    cs, cu = ropes(341).to(dev), ints(cumulate(lens), dev)
+    want = interface.flash_attn_packed(q, k, v, cu, 300, zhi=level_table(), rope=cs)
+    got = interface.flash_attn_packed(q, k, v, cu, 1 << 20, zhi=level_table(), rope=cs)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("kv_dtype", [BF, F8])
 @pytest.mark.parametrize("new,held", [([5, 64, 1, 0, 300], [5, 1000, 700, 90, 333]), ([256, 512], [2000, 512]), ([1], [40])])
 def test_queries_behind_cached_prefixes(dev, new, held, kv_dtype):

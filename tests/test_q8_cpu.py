@@ -25,7 +25,7 @@ DECODE = dict(out=1 << 20, o_sb=512, o_sh=128, q=1 << 20, q_sb=512, q_sh=128, kv
               table=1 << 20, max_pages=4, lens=1 << 20, batch=1, hq=4, hkv=2, most=64, zhi=None, entries=0, scale=0.1,
               rope=None, rope_pos=0, layout=0, ws=None, ws_bytes=0, stream=None)
 EXPAND = dict(out=1 << 20, out_table=1 << 20, kv=1 << 20, exps=1 << 20, pages=4, hkv=2, table=1 << 20, batch=1,
-              max_pages=4, n_pages=4, stream=None)
+              max_pages=4, n_pages=4, lens=None, stream=None)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -230,3 +230,15 @@ def test_decode_workspace_holds_every_split(no_gpu):
         unit = shape[0] * shape[2] * 16 * 130 * 4
         assert size % unit == 0 and size // unit <= max(1, -(-shape[3] // 16)) and size <= 64 << 20
     assert no_gpu.atf_decode_q8_workspace_bytes(1, 4, 4, 16) == 0 == no_gpu.atf_decode_q8_workspace_bytes(0, 4, 4, 16)
+
+
+def test_page_tables_past_30_bits_of_entries_are_refused(no_gpu):
+    assert call(no_gpu.atf_extend_tables, EXTEND, batch=1025, max_pages=1 << 20) == 2
+
+
+def test_flash_packed_bound_past_the_rows_costs_nothing(no_gpu):
+    # no sequence has more rows than the call: a generous bound takes no more workspace, nor a longer RoPE table
+    size = no_gpu.atf_flash_packed_workspace_bytes
+    assert size(300, 500, (1 << 24) - 1, 24, 8) == size(300, 500, 500, 24, 8)
+    assert call(no_gpu.atf_flash_packed_bf16, FLASH, most=5000, rope=1 << 20, rope_pos=99) == 1
+    assert call(no_gpu.atf_flash_packed_bf16, FLASH, most=5000, rope=1 << 20, rope_pos=100, ws_bytes=1000) == 4

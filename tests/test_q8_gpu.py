@@ -241,6 +241,20 @@ def test_expansion_is_exact_for_every_code(dev):
         assert torch.equal(torch.nan_to_num(got, nan=1.5), torch.nan_to_num(want, nan=1.5))
 
 
+def test_expansion_of_the_pages_that_hold_tokens(dev):
+    from atflash import ops
+    cache = new_cache(6, 2, dev)
+    cache.kv.view(torch.uint8).random_(0, 120)
+    cache.exps.random_(-4, 5)
+    table = torch.tensor([[5, 1, 0], [2, 3, 4], [4, 5, 5], [1, -1, 2]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([17, 48, 0, 40], dtype=torch.int32, device=dev)
+    all_kv, all_table = ops.kv_expand_q8(cache.kv, cache.exps, table, 3)
+    kv, out = ops.kv_expand_q8(cache.kv, cache.exps, table, 3, lens)
+    assert out.tolist() == [[0, 1, -1], [3, 4, 5], [-1, -1, -1], [9, -1, 11]]
+    live = out[out >= 0].long()
+    assert torch.equal(kv[live], all_kv[live]) and all_table.tolist()[2] == [6, 7, 8]
+
+
 # ---------------------------------------------------------------- decode
 
 def filled(lens, heads, dev, seed, spare=3):

@@ -87,6 +87,22 @@ def test_tables_that_are_too_narrow_and_lengths_below_zero(dev):
     check(dev, table, lens, new, free, sum(max(n, 0) for n in new), 700)
 
 
+def test_lengths_past_31_bits_stay_in_bounds(dev):
+    from atflash import ops
+    top = 2 ** 31 - 1
+    table = ints([[3, 1, 0, 2], [4, -1, -1, -1]], dev)
+    free = ints([9, 8, 7, 6, 5], dev)
+    lens, left, cu, pos, slot = ops.extend_tables(table, ints([top, 5], dev), ints([5, 20], dev), free, ints([5], dev), 25, 10)
+    assert lens.tolist() == [top, 25] and cu.tolist() == [0, 5, 25] and int(left) == 4
+    assert table.tolist() == [[3, 1, 0, 2], [4, 5, -1, -1]]
+    assert slot[:5].tolist() == [-1] * 5 and pos[5:].tolist() == list(range(5, 25))
+    assert slot[5:].tolist() == [(4 if t < 16 else 5) * 16 + t % 16 for t in range(5, 25)]
+    # sums of new tokens that wrap: whatever is listed is -1 or a slot of the pool
+    lens, left, cu, pos, slot = ops.extend_tables(table, ints([top, 5], dev), ints([top, top], dev), free, ints([5], dev), 60, 10)
+    assert lens.tolist() == [top, top] and int(left) == 2 and table[1].tolist() == [4, 5, 6, 7]
+    assert all(-1 <= x < 160 for x in slot.tolist())
+
+
 def test_release(dev):
     from atflash import ops
     batch, width, pool = 6, 40, 200
