@@ -27,18 +27,43 @@
 // zeroed in registers with the per-key rule's.
 //
 // Work.  A sequence of P pages is cut into ceil(P / C) splits (C: a.pages_per_split, from
-// the call's sizes), page s, s + n, s + 2n, ... to split s of n; a workgroup of 8 waves
-// takes a split of a kv head, each wave two pages at a time.  So the splits of a ragged
-// batch are all about C pages, long sequences have more of them, and a sequence's results
-// do not depend on the lengths of others.  The registers of a wave stay below 128, so
-// that four share a SIMD and hide each other's chain of conversions, MFMAs and
-// exponentials, which is what bounds a wave; one pair of pages a wave in flight is
-// enough for the memory then.
+// the call's sizes), page s, s + n, s + 2n, ... to split s of n; a workgroup of 8 or 12
+// waves takes a split of a kv head, each wave two pages at a time.  So the splits of a
+// ragged batch are all about C pages, long sequences have more of them, and a sequence's
+// results do not depend on the lengths of others.
+//
+// What bounds it.  The bytes of the pages: each is read once.  1 x 131072 tokens (28 / 4
+// heads, window OFF, 134 MB): 29.2 us a call with the merge, 4.6 TB/s; 40 x 8192 under the
+// level rule 60 us, 4.7 TB/s, where a large copy reaches 4.7.  A stream of the same 134 MB
+// in 4 KB blocks without any arithmetic takes 20.8 us: the difference is the start (length,
+// table entry, page: three round trips one behind the other), the combination of the
+// waves at the end, and the merge (4 us).  At 40 x 8192 the vector units are busy for 28%
+// of the time and a wave waits for memory for 63% of its own; more pairs of pages in
+// flight a wave were not better, they take the registers of other waves.
 #include "atf_decode_common.h"
 
 namespace atf {
 
+// Waves of a workgroup: 8, two workgroups to a CU; 12 where every workgroup has a CU of
+// its own and its splits are long.  kQFirst: the rows of Q and their (cos, sin) are
+// requested ahead of the first pages (loads return in order) and made ready while those
+// are on their way.  Measured, us a call with 8 waves, 8 and Q first, 12 and Q first (28 / 4
+// heads, vec8 k = 2, where nothing else is said):
+//   one round, pages a split  16  1 x 8192 (24 / 8)     11.7  11.0  11.4
+//                             24  1 x 24576             14.3  13.5  14.3
+//                             32  1 x 32768             15.3  14.8  14.7
+//                             48  1 x 49152             17.4  17.3  16.4
+//                            128  1 x 131072            28.3  29.6  25.9; OFF 30.1  29.8  29.2
+//                            128  4 x 16384 (24 / 8)    27.7  28.8  24.9
+//                            282  30 of 300 to 9000     38.9  43.7  32.9
+//   more rounds                   12 of 1084 to 32768   36.6  39.0  45.8
+//                                 40 x 8192, level rule 59.8  59.4  63.4
+//                                 64 of 140 to 4096     45.1  46.9  44.9
+//   kWide                         1 x 8192 (32 / 2)     12.9  12.3  13.6
+//                                 4 x 65536 (32 / 2)    28.3  28.3  27.6
 constexpr int kQ8Waves = 8;
+constexpr int kQ8WavesLong = 12;
+constexpr int kQ8LongPages = 32;  // of a split, from which on 12 waves take it
 
 // A page's block as a range-checked buffer: V, then the first ns slices of K (whole levels);
 // empty for a page past the sequence or an entry outside the pool.  What lies past the
@@ -109,14 +134,14 @@ __device__ __forceinline__ int q8_splits(int pages, int pages_per_split, int n_s
   return n_splits == 1 ? 1 : max(1, (pages + pages_per_split - 1) / pages_per_split);
 }
 
-template <bool kPerKey, bool kWide>
-__global__ __launch_bounds__(kQ8Waves * 64) __attribute__((amdgpu_waves_per_eu(kWide ? 2 : 4)))
+template <bool kPerKey, bool kWide, int kWaves, bool kQFirst>
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(kWaves == kQ8WavesLong ? 3 : kWide ? 2 : 4)))
 void decode_q8_kernel(const int32_t* page_table, const int32_t* seq_lens, const uint16_t* kv_cache, int max_pages,
                       int pages_per_split, int max_seq_len, int hkv, int num_pages, int n_splits, DecodeArgs a) {
   const DecHot hot{page_table, seq_lens, kv_cache, max_pages, pages_per_split, max_seq_len, hkv, num_pages, n_splits};
   // wave partials
-  __shared__ __attribute__((aligned(16))) float sh_o[kQ8Waves * kDecMaxGroup * kD];
-  __shared__ float sh_m[kQ8Waves * kDecMaxGroup], sh_l[kQ8Waves * kDecMaxGroup];
+  __shared__ __attribute__((aligned(16))) float sh_o[kWaves * kDecMaxGroup * kD];
+  __shared__ float sh_m[kWaves * kDecMaxGroup], sh_l[kWaves * kDecMaxGroup];
   // The splits are turned by head and sequence: workgroups go to the XCDs in turn, and
   // without this the sequences that have few splits would all lie on the first ones (12
   // sequences of 1084 to 32768 tokens, 24 / 8 heads, vec8 k = 2: 66.5 us a call).
@@ -125,7 +150,7 @@ void decode_q8_kernel(const int32_t* page_table, const int32_t* seq_lens, const 
   const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
   const float NEG_INF = -__builtin_huge_valf();
   const float c = a.scale_log2;
-  // Pair i of this wave is pages p and p + n, p = s + 2 n (wave + 8 i).  The entries of the
+  // Pair i of this wave is pages p and p + n, p = s + 2 n (wave + kWaves i).  The entries of the
   // first two pairs are fetched together with the length, as if the sequence had the
   // call's longest length (a round trip less where it has as many splits).
   const int32_t* row = page_table + static_cast<int64_t>(b) * max_pages;
@@ -133,13 +158,37 @@ void decode_q8_kernel(const int32_t* page_table, const int32_t* seq_lens, const 
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     ent[u] = row[min(s + n_splits * (2 * wave + u), max_pages - 1)];
-    ent_next[u] = row[min(s + n_splits * (2 * (wave + kQ8Waves) + u), max_pages - 1)];
+    ent_next[u] = row[min(s + n_splits * (2 * (wave + kWaves) + u), max_pages - 1)];
   }
+  // Q^T fragments: fragment m is slice 2g + m % 2 + 8 (m / 2) of a head.  Lane t holds head
+  // t % 8, its hi part for t < 8, its lo part above; kWide: head t, both parts.
+  const int head = kWide ? t : t & 7;
+  u32x4 x[4];
+  float cs[4][8];
+  auto request_q = [&] {
+    const uint16_t* qrow = a.q + static_cast<int64_t>(b) * a.q_sb +
+                           static_cast<int64_t>(h * a.group + min(head, a.group - 1)) * a.q_sh;
+    if (a.layout == kLayoutHalfSplit) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) x[m] = load_slice(qrow, kLayoutHalfSplit, 2 * g + (m & 1) + 8 * (m >> 1));
+    } else {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) x[m] = load_slice(qrow, kLayoutSortedPair, 2 * g + (m & 1) + 8 * (m >> 1));
+    }
+  };
+  auto request_cs = [&](int pos) {
+    if (a.rope_cs != nullptr) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) load_cs4(a.rope_cs, pos, slice_pair0(2 * g + (m & 1) + 8 * (m >> 1)), cs[m]);
+    }
+  };
+  if constexpr (kQFirst) request_q();
   const int N = max(0, min(seq_lens[b], max_seq_len));
   const int n_pages = (N + kPage - 1) / kPage;
   const int n = q8_splits(n_pages, pages_per_split, n_splits);
   if (s >= n) return;
-  const int step = 2 * kQ8Waves * n;
+  if constexpr (kQFirst) request_cs(max(N - 1, 0));
+  const int step = 2 * kWaves * n;
   int p = s + 2 * n * wave;
   auto fetch = [&](int page) { return row[max(min(page, n_pages - 1), 0)]; };
   if (n != n_splits) {
@@ -172,34 +221,23 @@ void decode_q8_kernel(const int32_t* page_table, const int32_t* seq_lens, const 
     ent[u] = ent_next[u];
   }
 
-  // Q^T fragments: fragment m is slice 2g + m % 2 + 8 (m / 2) of a head.  Lane t holds head
-  // t % 8, its hi part for t < 8, its lo part above; kWide: head t, both parts.
+  if constexpr (!kQFirst) {
+    request_q();
+    request_cs(max(N - 1, 0));
+  }
   u32x4 Qf[4], Ql[kWide ? 4 : 1];
   {
-    const int head = kWide ? t : t & 7;
-    const int qh = h * a.group + min(head, a.group - 1);
     const bool valid = head < a.group && N > 0;
     const float part = !kWide && t >= 8 ? 1.f : 0.f;
-    const uint16_t* qrow = a.q + static_cast<int64_t>(b) * a.q_sb + static_cast<int64_t>(qh) * a.q_sh;
-    u32x4 x[4];
-    if (a.layout == kLayoutHalfSplit) {
-#pragma unroll
-      for (int m = 0; m < 4; ++m) x[m] = load_slice(qrow, kLayoutHalfSplit, 2 * g + (m & 1) + 8 * (m >> 1));
-    } else {
-#pragma unroll
-      for (int m = 0; m < 4; ++m) x[m] = load_slice(qrow, kLayoutSortedPair, 2 * g + (m & 1) + 8 * (m >> 1));
-    }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       float v[8], y[8];
       unpack8(x[m], v);
       if (a.rope_cs != nullptr) {
-        float cs[8];
-        load_cs4(a.rope_cs, max(N - 1, 0), slice_pair0(2 * g + (m & 1) + 8 * (m >> 1)), cs);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          y[i] = rope_first(v[i], v[4 + i], cs[2 * i], cs[2 * i + 1]);
-          y[4 + i] = rope_second(v[i], v[4 + i], cs[2 * i], cs[2 * i + 1]);
+          y[i] = rope_first(v[i], v[4 + i], cs[m][2 * i], cs[m][2 * i + 1]);
+          y[4 + i] = rope_second(v[i], v[4 + i], cs[m][2 * i], cs[m][2 * i + 1]);
         }
       } else {
 #pragma unroll
@@ -359,7 +397,7 @@ void decode_q8_kernel(const int32_t* page_table, const int32_t* seq_lens, const 
     }
   }
   __syncthreads();
-  store_split<kQ8Waves>(a, (static_cast<int64_t>(b) * hkv + h) * n_splits + s, n == 1, h, b, sh_o, sh_m, sh_l);
+  store_split<kWaves>(a, (static_cast<int64_t>(b) * hkv + h) * n_splits + s, n == 1, h, b, sh_o, sh_m, sh_l);
 }
 
 // The merge of the splits that each sequence has (those with one have written their output).
@@ -375,13 +413,18 @@ __global__ __launch_bounds__(512) void decode_q8_merge_kernel(const int32_t* seq
 hipError_t launch_decode_q8(const DecodeArgs& a, hipStream_t s) {
   if (a.batch <= 0) return hipSuccess;
   const dim3 grid(a.n_splits, a.hkv, a.batch);
-#define ATF_Q8_LAUNCH(PK, WIDE)                                                                                         \
-  hipLaunchKernelGGL((decode_q8_kernel<PK, WIDE>), grid, dim3(kQ8Waves * 64), 0, s, a.page_table, a.seq_lens, a.kv_cache, \
-                     a.max_pages, a.pages_per_split, a.max_seq_len, a.hkv, a.num_pages, a.n_splits, a)
+#define ATF_Q8_LAUNCH(PK, WIDE, W, QF)                                                                                  \
+  hipLaunchKernelGGL((decode_q8_kernel<PK, WIDE, W, QF>), grid, dim3((W) * 64), 0, s, a.page_table, a.seq_lens,          \
+                     a.kv_cache, a.max_pages, a.pages_per_split, a.max_seq_len, a.hkv, a.num_pages, a.n_splits, a)
+  const bool one_round = static_cast<int64_t>(a.n_splits) * a.hkv * a.batch <= 256;
   if (a.group > 8) {
-    if (a.per_key) ATF_Q8_LAUNCH(true, true); else ATF_Q8_LAUNCH(false, true);
+    if (a.per_key) ATF_Q8_LAUNCH(true, true, kQ8Waves, true); else ATF_Q8_LAUNCH(false, true, kQ8Waves, true);
+  } else if (!one_round) {
+    if (a.per_key) ATF_Q8_LAUNCH(true, false, kQ8Waves, false); else ATF_Q8_LAUNCH(false, false, kQ8Waves, false);
+  } else if (a.pages_per_split >= kQ8LongPages) {
+    if (a.per_key) ATF_Q8_LAUNCH(true, false, kQ8WavesLong, true); else ATF_Q8_LAUNCH(false, false, kQ8WavesLong, true);
   } else {
-    if (a.per_key) ATF_Q8_LAUNCH(true, false); else ATF_Q8_LAUNCH(false, false);
+    if (a.per_key) ATF_Q8_LAUNCH(true, false, kQ8Waves, true); else ATF_Q8_LAUNCH(false, false, kQ8Waves, true);
   }
 #undef ATF_Q8_LAUNCH
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;

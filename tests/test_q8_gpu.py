@@ -334,6 +334,14 @@ def test_decode_slice_boundaries(dev, k_ret):
     check_decode(dev, [901, 333, 48, 5], 12, 4, 53, "vec8", rope=True, base=1e7, k_ret=k_ret)
 
 
+@pytest.mark.parametrize("kind,layout,rope", [("vec8", 0, True), ("level", 1, False), ("off", 0, True)])
+@pytest.mark.parametrize("lens", [[600, 1, 0, 577, 32, 384, 385, 511, 16, 600, 200, 33, 590, 592, 593, 600, 15, 17, 100, 400],
+                                  [5003, 4096, 700, 1], [33, 3000, 1, 2999, 1500, 0, 2000, 16, 700, 1024, 2900, 256]])
+def test_decode_every_form_of_a_launch(dev, lens, kind, layout, rope):
+    # 24 / 8 heads: one split a head of up to 38 pages; 8 splits of 40 pages; more workgroups than CUs
+    check_decode(dev, lens, 24, 8, 67, kind, layout, rope)
+
+
 def test_decode_longer_bound_than_the_lengths(dev):
     check_decode(dev, [40, 7, 0], 8, 2, 59, "vec8", max_len=9000)
 
