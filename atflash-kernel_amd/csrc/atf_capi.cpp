@@ -126,22 +126,26 @@ void decode_split(int batch, int hkv, int max_seq_len, int* n_splits, int* pages
 // The 8-bit decode: pages of a split and splits of the longest sequence.  A workgroup
 // streams a page in about 0.16 us when one runs on each of 256 CUs (two thirds of that
 // when few do), and costs as much as 16 pages to start and end; merging costs 25 (4 us).
-// With n splits a (sequence, kv head) pair there are `rounds` workgroups a CU:
+// With n splits a (sequence, kv head) pair there are `rounds` workgroups a CU, two at a
+// time where there are more than one:
 //   us = 0.16 (rounds (pages / n + 16) u + 25), u = 0.65 + 0.35 min(1, workgroups / 256).
-// Measured (us a call) at 1, 2, 3 and 5 rounds: 1 x 131072 OFF (28 / 4 heads) 30.2, 34.2,
-// 37.8, 46.3; 4 x 16384 (24 / 8) 28.1, 26.9, 33.9, 37.5; 40 x 8192 (28 / 4) 66, 60.3, 64.9,
-// 65.7; with fewer than 256 workgroups: 1 x 8192 (24 / 8), 256, 128 and 64 of them, 11.7, 12.8,
-// 15.3; 1 x 1003 with 32 and 8 10.6, 12.2.  The lengths of a batch are not known here, and
-// a ragged one is the better for smaller splits: of the choices within 6% of the best a
-// batch takes the finest (12 sequences of 1084 to 32768 tokens, 24 / 8 heads: 2, 5, 8
-// and 16 splits 109, 67, 45 and 37 us).  Not with more than 8 heads a kv head, whose
-// workgroups have a CU each (4 x 65536 at 32 / 2: 1 round 32.3, 2 rounds 41.1).
+// Measured (us a call) for 1, 2, 3, 4 and 6 x 256 workgroups: 1 x 131072 OFF (28 / 4 heads)
+// 29.4, 34.0, 39.3, 39.2, 48.9; 4 x 16384 (24 / 8) 24.6, 25.8, 32.4, 31.4, 38.6; 40 x 8192
+// (28 / 4) 61.7, 56.5, 63.1, 59.4, 67.0; with fewer than 256 workgroups: 1 x 8192 (24 / 8), 256,
+// 128 and 64 of them, 11.1, 12.5, 14.1.
+//   The lengths of a batch are not known here, and a ragged one is the better for
+// smaller splits: of the choices within 12% of the best a batch takes the finest.  Equal
+// lengths, and lengths from 100 up to it, with the best, within 6%, and within 12%:
+// 4 x 65536 (24 / 8) 76, 76, 81 and 49, 49, 34; 8 x 12288 (24 / 8) 34.3, 34.3, 35.8 and
+// 24.2, 24.2, 20.3; 12 x 16384 (24 / 8) 62, 62, 66 and 36, 36, 23; 40 x 8192 (28 / 4) 55, 55,
+// 58 and 32, 32, 26.5.  Not with more than 8 heads a kv head, whose workgroups have a CU each
+// (4 x 65536 at 32 / 2: 1 round 32.3, 2 rounds 41.1).
 void decode_q8_split(int batch, int hkv, int group, int max_seq_len, int* n_splits, int* pages_per_split) {
   const int64_t pages = max_seq_len > 0 ? (max_seq_len + atf::kPage - 1) / atf::kPage : 1;
   const int64_t pairs = static_cast<int64_t>(batch) * hkv;
   const int64_t most = (pages + 15) / 16;  // a workgroup's waves take 16 pages at a time
   auto cost = [&](int64_t n) {
-    const int64_t wgs = pairs * n, rounds = (wgs + 255) / 256, each = (pages + n - 1) / n;
+    const int64_t wgs = pairs * n, rounds = wgs <= 256 ? 1 : (wgs + 511) / 512 * 2, each = (pages + n - 1) / n;
     const double u = 0.65 + 0.35 * static_cast<double>(std::min<int64_t>(wgs, 256)) / 256.0;
     return static_cast<double>(rounds) * static_cast<double>(each + 16) * u + (n > 1 ? 25.0 : 0.0);
   };
@@ -154,7 +158,7 @@ void decode_q8_split(int batch, int hkv, int group, int max_seq_len, int* n_spli
   }
   for (int r = 1; batch > 1 && group <= 8 && r <= kRounds; ++r) {
     const int64_t n = std::min(256 * r / pairs, most);
-    if (n > best && cost(n) <= 1.06 * low) best = n;
+    if (n > best && cost(n) <= 1.12 * low) best = n;
   }
   const int64_t pps = (pages + best - 1) / best;
   *pages_per_split = static_cast<int>(pps);
