@@ -318,9 +318,9 @@ def prefill_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tensor, p
                nk: int, q_offset: int, zhi: Optional[List[int]], sm_scale: float,
                rope_cs: Optional[torch.Tensor], layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """prefill over the cache of 8-bit floats.  The keys' pages are expanded into
-    temporary bf16 pages first (exact; 12 bytes moved an element pair of K and V
-    against the attention's work on it, which grows with the queries), then read by
-    prefill's kernels: their results on the values that the codes stand for."""
+    temporary bf16 pages first (exact; a copy's traffic, where the attention's work
+    grows with the queries), then read by prefill's kernels: their results on the
+    values that the codes stand for."""
     _need(int(nk) >= 0 and -(-int(nk) // _lib.PAGE_SIZE) <= page_table.shape[-1],
           f"page table too small for nk={nk}")
     kv, table = kv_expand_q8(kv_cache, kv_exps, page_table, -(-int(nk) // _lib.PAGE_SIZE))

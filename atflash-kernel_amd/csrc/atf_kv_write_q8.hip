@@ -11,6 +11,11 @@
 // shifted to it.  A call that writes a page's first slot begins the page anew.  Slots
 // behind the call's last token become zero.  Infinities and NaN become the NaN code
 // and count for no exponent.
+//   Bound by HBM on long calls: K and V read once as bf16 (2 bytes an element), codes
+// written once (1 byte), a (cos, sin) row of 512 bytes a position.  3 sequences of 20000
+// tokens, 8 heads, 380 MB: 83 us, 4.6 TB/s, where a large copy reaches 4.7.  One token of
+// each of 32 sequences: 5.1 us, a chain of four round trips (start, page entry and rows,
+// the old codes, the store).
 #include "atf_launch.h"
 
 namespace atf {
@@ -88,7 +93,9 @@ __device__ __forceinline__ u32x4 transpose4(const u32x4& w) {
 // 16 tid.
 // grid: x = pages (from the call's first) and kv heads, y = sequence.  Workgroups go to the
 // XCDs in turn: a page's heads lie on one XCD, one after the other, so that its (cos,
-// sin) rows, as many bytes as a head's keys and values, come from that XCD's L2.
+// sin) rows, as many bytes as a head's keys and values, come from that XCD's L2 (3 x 20000
+// tokens of 8 heads 83.0 us, 89.9 with the heads last in the grid and the loads where their
+// values are used).
 __global__ __launch_bounds__(128) void kv_write_q8_kernel(KvWriteArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sv[kPage][kD];
   __shared__ uint32_t s_top[2][2], s_odd[2];
@@ -244,7 +251,8 @@ hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s) {
 
 // A page of the 8-bit cache as a bf16 page: every code times its power of two, exact.
 // One workgroup of 128 threads per (page-table entry, kv head); the thread takes the 16
-// bytes of each half at 16 tid.
+// bytes of each half at 16 tid.  12 KB moved a (page, head), a copy's work: the prefill
+// behind it grows with the queries, this does not.
 __global__ __launch_bounds__(128) void kv_expand_q8_kernel(KvExpandArgs a) {
   const int p = blockIdx.x, b = blockIdx.y, h = blockIdx.z, tid = threadIdx.x;
   const int64_t entry = static_cast<int64_t>(b) * a.n_pages + p;

