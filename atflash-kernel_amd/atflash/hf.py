@@ -119,12 +119,12 @@ class PagedLayer(CacheLayerMixin):
         if self.length + L > o.capacity:
             raise ValueError(f"PagedCache holds {o.capacity} tokens per sequence; "
                              f"{self.length} + {L} would not fit")
-        args = (key_states.transpose(1, 2), value_states.transpose(1, 2), o.start_positions(self.length), o.page_table,
-                o.rope_cs, _lib.LAYOUT_HALF_SPLIT)
         if self.exps is None:
-            ops.kv_write(self.kv, *args)
+            ops.kv_write(self.kv, key_states.transpose(1, 2), value_states.transpose(1, 2),
+                         o.start_positions(self.length), o.page_table, o.rope_cs, _lib.LAYOUT_HALF_SPLIT)
         else:
-            ops.kv_write_q8(self.kv, self.exps, *args)
+            ops.kv_write_q8(self.kv, self.exps, key_states.transpose(1, 2), value_states.transpose(1, 2),
+                            o.start_positions(self.length), o.page_table, o.rope_cs, _lib.LAYOUT_HALF_SPLIT)
         self.prev_length = self.length
         self.length += L
         self.last_key = key_states
@@ -334,9 +334,12 @@ class WindowAttention:
                 raise ValueError("the cache was made for the other RoPE mode of this hook")
             if L == 1:
                 zhi = self.window.decode_zhi8 if windowed else None
-                args = (owner.page_table, owner.seq_lens(S), S, zhi, scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
-                o = (ops.decode_paged(query.select(2, 0), lyr.kv, *args) if lyr.exps is None
-                     else ops.decode_paged_q8(query.select(2, 0), lyr.kv, lyr.exps, *args))
+                if lyr.exps is None:
+                    o = ops.decode_paged(query.select(2, 0), lyr.kv, owner.page_table, owner.seq_lens(S), S, zhi,
+                                         scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+                else:
+                    o = ops.decode_paged_q8(query.select(2, 0), lyr.kv, lyr.exps, owner.page_table, owner.seq_lens(S),
+                                            S, zhi, scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
                 return o.view(b, 1, hq, d), None
             zhi = self.window.prefill_zhi if windowed else None
             args = (owner.page_table, S, lyr.prev_length, zhi, scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)

@@ -527,6 +527,8 @@ def _(page_table, seq_lens, free_pages, free_count, rows, num_pages):
 # needs no initialisation (each call writes the split partials it reads), and
 # calls on one stream are ordered, so they can share it.
 _DECODE_WS = {}
+_current_device = torch._C._cuda_getDevice
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 _WS_BYTES = {}  # (batch, hq, hkv, max_seq_len, 8-bit cache) -> workspace bytes the split rule needs
 
 
@@ -542,7 +544,7 @@ def _decode_workspace(device, handle, B, hq, hkv, max_seq_len, L, q8=False):
             _WS_BYTES.clear()
         size = L.atf_decode_q8_workspace_bytes if q8 else L.atf_decode_workspace_bytes_even
         nbytes = _WS_BYTES[shape] = int(size(B, hq, hkv, max_seq_len))
-    if torch._C._cuda_isCurrentStreamCapturing():
+    if _capturing():
         t = torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
         return t.data_ptr(), t.numel() * 4, t
     key = (device.index, handle)
@@ -755,8 +757,14 @@ class DecodePlan:
             out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
         elif out.shape != self.shape or not out.is_contiguous() or out.dtype != torch.bfloat16:
             raise ValueError(f"out must be contiguous bf16 {self.shape}")
-        _lib.launch(self._index, self._entry, out.data_ptr(), self.shape[1] * _lib.HEAD_DIM, _lib.HEAD_DIM, q.data_ptr(),
-                    self.q_strides[0], self.q_strides[1], *self._mid)
+        args = (out.data_ptr(), self.shape[1] * _lib.HEAD_DIM, _lib.HEAD_DIM, q.data_ptr(), self.q_strides[0],
+                self.q_strides[1], *self._mid)
+        if self._index == _current_device():
+            code = self._entry(*args, _lib.raw_stream(self._index))
+            if code:
+                _lib.check(code)
+        else:
+            _lib.launch(self._index, self._entry, *args)
         return out
 
 
