@@ -470,9 +470,9 @@ def extend_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: to
     _check_ints(free_pages, F, "free_pages")
     T = int(total_tokens)
     _need(T >= 0, "total_tokens must be >= 0")
-    # one allocation: slots first (8-byte aligned)
+    # one allocation: slots first (8-byte aligned); its parts do not overlap
     buf = seq_lens.new_empty(3 * T + 2 * B + 2)
-    slots, pos, lens, left, cu = buf.split_with_sizes((2 * T, T, B, 1, B + 1))
+    slots, pos, lens, left, cu = buf.unsafe_split_with_sizes((2 * T, T, B, 1, B + 1))
     at = buf.data_ptr()
     _lib.launch(dev, _lib.lib().atf_extend_tables, page_table.data_ptr(), width, seq_lens.data_ptr(),
                 new_lens.data_ptr(), free_pages.data_ptr(), F, free_count.data_ptr(), B, T, int(num_pages),
