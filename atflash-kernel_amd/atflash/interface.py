@@ -107,7 +107,7 @@ def flash_attn_packed(q, k, v, cu_seqlens, max_seqlen, zhi=None, softmax_scale=N
     [T, Hkv, 128], sequence b's rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 on the
     GPU), at most max_seqlen of each.  Returns (out [T, Hq, 128] bf16, lse [Hq, T] fp32),
     each sequence's the bits of a `_flash_attn_fwd` call of its own."""
-    if q.dim() != 3 or k.dim() != 3 or q.shape[1] % k.shape[1] != 0:
+    if q.dim() != 3 or k.dim() != 3 or k.shape[1] == 0 or q.shape[1] % k.shape[1] != 0:
         raise ValueError("q, k, v must be [T, heads, 128], num q heads a multiple of num kv heads")
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
     return ops.flash_attn_packed(q, k, v, cu_seqlens, int(max_seqlen), _zhi_list(zhi), scale, rope, _layout_id(layout))

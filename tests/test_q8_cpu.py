@@ -242,3 +242,10 @@ def test_flash_packed_bound_past_the_rows_costs_nothing(no_gpu):
     assert size(300, 500, (1 << 24) - 1, 24, 8) == size(300, 500, 500, 24, 8)
     assert call(no_gpu.atf_flash_packed_bf16, FLASH, most=5000, rope=1 << 20, rope_pos=99) == 1
     assert call(no_gpu.atf_flash_packed_bf16, FLASH, most=5000, rope=1 << 20, rope_pos=100, ws_bytes=1000) == 4
+
+
+def test_packed_prompts_without_kv_heads_are_refused():
+    from atflash import interface
+    q, k = torch.zeros((4, 6, 128), dtype=torch.bfloat16), torch.zeros((4, 0, 128), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="multiple"):
+        interface.flash_attn_packed(q, k, k, torch.tensor([0, 4], dtype=torch.int32), 4)
