@@ -742,7 +742,13 @@ int atf_decode_paged_q8(void* out, int64_t o_sb, int64_t o_sh, const void* q, in
   if (static_cast<int64_t>(num_pages) * num_kv_heads >= (int64_t(1) << 30))
     return fail(ATF_ERR_UNSUPPORTED, "at most 2^30 - 1 blocks (pages x kv heads), got %d x %d", num_pages, num_kv_heads);
   a.kv_exps = kv_exps;
-  decode_q8_split(batch, num_kv_heads, a.group, max_seq_len, &a.n_splits, &a.pages_per_split);
+  // A workspace that holds the partials of decode_split's splits only (decode_prepare's) takes those.
+  int ns = 1, pps = 1;
+  decode_q8_split(batch, num_kv_heads, a.group, max_seq_len, &ns, &pps);
+  if (workspace_bytes >= partial_bytes(batch, num_kv_heads, ns)) {
+    a.n_splits = ns;
+    a.pages_per_split = pps;
+  }
   if (int r = set_workspace(workspace, workspace_bytes, &a)) return r;
   hipError_t e = atf::launch_decode_q8(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "8-bit decode launch");

@@ -327,8 +327,9 @@ int atf_decode_paged_slices_bf16(void* out, int64_t o_sb, int64_t o_sh,
  * The decode over the cache of 8-bit floats: arguments and window rules as
  * atf_decode_paged_bf16 (zhi_entries = ATF_LEVELS) or atf_decode_paged_slices_bf16
  * (ATF_SLICES; ignored where zhi is NULL), the workspace of
- * atf_decode_q8_workspace_bytes (atf_decode_workspace_bytes is enough, slower for
- * ragged batches).  Keys and values are the codes times their powers of two,
+ * atf_decode_q8_workspace_bytes.  With less, down to atf_decode_workspace_bytes,
+ * the splits are that decode's, which is slower for ragged batches and gives other
+ * roundings.  Keys and values are the codes times their powers of two,
  * exactly; Q, P and the sums have atf_decode_paged_bf16's precision.
  */
 size_t atf_decode_q8_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_seq_len);
