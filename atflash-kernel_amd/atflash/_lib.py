@@ -53,6 +53,7 @@ SIGNATURES = {
     "atf_kv_write_q8": (_i, [_p, _p, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _p, _i, _p, _p, _i,
                              _p, _i, _i, _p]),
     "atf_kv_expand_q8": (_i, [_p, _p, _p, _p, _i, _i, _p, _i, _i, _i, _p, _p]),
+    "atf_kv_expand_q8_pages": (_i, [_p, _p, _p, _i, _i, _p, _i, _i, _i, _p, _p]),
     "atf_prefill_bf16": (_i, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i, _p, _i,
                               _i, _i, _i, _i, _i, _i, _p, _f, _p, _i, _i, _p]),
     "atf_prefill_plan_bytes": (_sz, [_i, _i, _i]),

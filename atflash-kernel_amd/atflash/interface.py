@@ -154,14 +154,15 @@ def prefill_packed(q, cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi=
                    layout="half_split", plan=None, out=None, lse=None):
     """Windowed causal prefill of packed rows against a PagedKVCache (ops.prefill_packed;
     `plan`: packed_plan of these lengths, shared by the layers of a step).  A cache of
-    8-bit floats is expanded into temporary bf16 pages first, as by prefill_paged."""
+    8-bit floats is expanded into temporary bf16 pages first, as by prefill_paged: as
+    many as the sequences' bound has, and no more than the pool."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
     kv = cache.kv
     if getattr(cache, "exps", None) is not None:
         pages = -(-int(max_seq_len) // PAGE)
         if page_table.dim() != 2 or page_table.shape[1] < pages:
             raise ValueError(f"page table too small for max_seq_len={max_seq_len}")
-        kv, page_table = ops.kv_expand_q8(kv, cache.exps, page_table, pages, seq_lens)
+        kv, page_table = ops.temporary_bf16(kv, cache.exps, page_table, pages, seq_lens)
     return ops.prefill_packed(q, kv, page_table, cu_seqlens, seq_lens, int(max_seq_len), _zhi_list(zhi), scale, rope,
                               _layout_id(layout), plan, out, lse)
 

@@ -274,6 +274,26 @@ def kv_expand_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torc
     return out, table
 
 
+def temporary_bf16(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torch.Tensor, n_pages: int,
+                   seq_lens: Optional[torch.Tensor] = None):
+    """The pages that a prefill over an 8-bit cache reads, in bf16, and their table:
+    kv_expand_q8's blocks by entry of the page table, or where the pool has fewer pages
+    than that (n_pages is a bound and may lie far past the lengths) every page in the
+    block of its own number, under the caller's table."""
+    n = int(n_pages)
+    if page_table.dim() != 2 or page_table.shape[0] * n <= kv_cache.shape[0]:
+        return kv_expand_q8(kv_cache, kv_exps, page_table, n, seq_lens)
+    dev = _one_device(kv_cache, kv_exps, page_table, seq_lens)
+    pool = _check_cache_q8(kv_cache, kv_exps)
+    B, width = _check_table(page_table)
+    if seq_lens is not None:
+        _check_ints(seq_lens, B, "seq_lens")
+    out = torch.empty(pool, dtype=torch.bfloat16, device=kv_cache.device)
+    _lib.launch(dev, _lib.lib().atf_kv_expand_q8_pages, out.data_ptr(), kv_cache.data_ptr(), kv_exps.data_ptr(), pool[0],
+                pool[1], page_table.data_ptr(), B, width, n, _lib.ptr(seq_lens))
+    return out, page_table
+
+
 def prefill(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor,
             nk: int, q_offset: int, zhi: Optional[List[int]], sm_scale: float,
             rope_cs: Optional[torch.Tensor], layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -323,7 +343,7 @@ def prefill_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tensor, p
     values that the codes stand for."""
     _need(int(nk) >= 0 and -(-int(nk) // _lib.PAGE_SIZE) <= page_table.shape[-1],
           f"page table too small for nk={nk}")
-    kv, table = kv_expand_q8(kv_cache, kv_exps, page_table, -(-int(nk) // _lib.PAGE_SIZE))
+    kv, table = temporary_bf16(kv_cache, kv_exps, page_table, -(-int(nk) // _lib.PAGE_SIZE))
     return prefill(q, kv, table, nk, q_offset, zhi, sm_scale, rope_cs, layout)
 
 

@@ -395,12 +395,15 @@ int atf_kv_write_q8(void* kv_cache, int8_t* kv_exps, int num_pages, int num_kv_h
   return ok();
 }
 
-int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const int8_t* kv_exps, int num_pages,
-                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages,
-                     const int32_t* seq_lens, void* stream) {
-  if (batch < 0 || n_pages < 0) return fail(ATF_ERR_INVALID, "batch and n_pages must be >= 0");
-  if (batch == 0 || n_pages == 0) return ok();
-  if (!out || !out_table || !kv_cache || !kv_exps || !page_table) return fail(ATF_ERR_INVALID, "null pointer argument");
+}  // extern "C"
+
+namespace {
+
+// The expansion into blocks by entry, with their table, or by page (out_table null).
+int expand_q8(void* out, int32_t* out_table, const void* kv_cache, const int8_t* kv_exps, int num_pages,
+              int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages,
+              const int32_t* seq_lens, void* stream) {
+  if (!out || !kv_cache || !kv_exps || !page_table) return fail(ATF_ERR_INVALID, "null pointer argument");
   if (num_pages <= 0 || num_kv_heads <= 0 || max_pages < n_pages)
     return fail(ATF_ERR_INVALID, "num_pages and num_kv_heads must be positive, max_pages (%d) at least n_pages (%d)",
                 max_pages, n_pages);
@@ -413,6 +416,29 @@ int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const 
   hipError_t e = atf::launch_kv_expand_q8(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "8-bit expand launch");
   return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const int8_t* kv_exps, int num_pages,
+                     int num_kv_heads, const int32_t* page_table, int batch, int max_pages, int n_pages,
+                     const int32_t* seq_lens, void* stream) {
+  if (batch < 0 || n_pages < 0) return fail(ATF_ERR_INVALID, "batch and n_pages must be >= 0");
+  if (batch == 0 || n_pages == 0) return ok();
+  if (!out_table) return fail(ATF_ERR_INVALID, "null pointer argument");
+  return expand_q8(out, out_table, kv_cache, kv_exps, num_pages, num_kv_heads, page_table, batch, max_pages, n_pages,
+                   seq_lens, stream);
+}
+
+int atf_kv_expand_q8_pages(void* out, const void* kv_cache, const int8_t* kv_exps, int num_pages, int num_kv_heads,
+                           const int32_t* page_table, int batch, int max_pages, int n_pages, const int32_t* seq_lens,
+                           void* stream) {
+  if (batch < 0 || n_pages < 0) return fail(ATF_ERR_INVALID, "batch and n_pages must be >= 0");
+  if (batch == 0 || n_pages == 0) return ok();
+  return expand_q8(out, nullptr, kv_cache, kv_exps, num_pages, num_kv_heads, page_table, batch, max_pages, n_pages,
+                   seq_lens, stream);
 }
 
 int atf_prefill_bf16(void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float* lse, const void* q,

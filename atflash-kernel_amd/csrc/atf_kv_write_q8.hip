@@ -253,19 +253,22 @@ hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s) {
 // One workgroup of 128 threads per (page-table entry, kv head); the thread takes the 16
 // bytes of each half at 16 tid.  12 KB moved a (page, head), a copy's work: the prefill
 // behind it grows with the queries, this does not.
+//   Without an out_table a page goes to the block of its own number, whichever entries
+// name it (several write the same bytes).
 __global__ __launch_bounds__(128) void kv_expand_q8_kernel(KvExpandArgs a) {
   const int p = blockIdx.x, b = blockIdx.y, h = blockIdx.z, tid = threadIdx.x;
   const int64_t entry = static_cast<int64_t>(b) * a.n_pages + p;
   const bool held = a.seq_lens == nullptr || static_cast<int64_t>(p) * kPage < a.seq_lens[b];
   const int pg = held ? a.page_table[static_cast<int64_t>(b) * a.max_pages + p] : -1;
   const bool ok = pg >= 0 && pg < a.num_pages;
-  if (h == 0 && tid == 0) a.out_table[entry] = ok ? static_cast<int32_t>(entry) : -1;
+  const bool own = a.out_table == nullptr;
+  if (!own && h == 0 && tid == 0) a.out_table[entry] = ok ? static_cast<int32_t>(entry) : -1;
   if (!ok) return;
   const size_t blk = static_cast<size_t>(pg) * a.hkv + h;
   const uint8_t* codes = a.codes + blk * kQ8BlockBytes;
   const u32x4 wv = ldg16(codes + 16 * tid), wk = ldg16(codes + kQ8HalfBytes + 16 * tid);
   const float sv = exp2_int(a.exps[2 * blk]), sk = exp2_int(a.exps[2 * blk + 1]);
-  uint16_t* out = a.out + (static_cast<size_t>(entry) * a.hkv + h) * kKvBlockElems;
+  uint16_t* out = a.out + (static_cast<size_t>(own ? pg : entry) * a.hkv + h) * kKvBlockElems;
   auto pair = [](uint32_t w, float s) {
     return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))};

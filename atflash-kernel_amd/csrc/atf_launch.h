@@ -179,7 +179,8 @@ hipError_t launch_kv_write(const KvWriteArgs& a, hipStream_t s);
 hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s);
 // Blocks of the 8-bit cache -> blocks of a bf16 cache: entry (b, p), p < n_pages, of the
 // page table to block b n_pages + p of `out`, that number (or -1 for an entry outside
-// the pool, whose block is left as it is) to out_table[b][p].
+// the pool, whose block is left as it is) to out_table[b][p].  out_table null: page g to
+// block g of `out`, which has num_pages of them.
 struct KvExpandArgs {
   const uint8_t* codes;
   const int8_t* exps;

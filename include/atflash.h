@@ -158,6 +158,16 @@ int atf_kv_expand_q8(void* out, int32_t* out_table, const void* kv_cache, const 
                      const int32_t* seq_lens, void* stream);
 
 /*
+ * The same with every page in the block of its own number: out is bf16
+ * [num_pages][num_kv_heads][2][2048], read with the caller's own page table.  It
+ * takes as much memory as the pool has pages, where atf_kv_expand_q8 takes batch *
+ * n_pages: for n_pages far past the lengths, and for pages that sequences share.
+ */
+int atf_kv_expand_q8_pages(void* out, const void* kv_cache, const int8_t* kv_exps, int num_pages, int num_kv_heads,
+                           const int32_t* page_table, int batch, int max_pages, int n_pages, const int32_t* seq_lens,
+                           void* stream);
+
+/*
  * Windowed causal GQA prefill: out[b, i, h, :] = attention of query row i
  * (absolute position q_offset + i) over keys 0..q_offset+i of sequence b read
  * from the paged cache (nk keys present, q_offset + nq <= nk).  q/out are bf16
