@@ -72,7 +72,7 @@ __device__ __forceinline__ int kv_page(const KvWriteArgs& a, const KvRows& rows,
 template <bool kPacked>
 __device__ __forceinline__ KvRows kv_rows(const KvWriteArgs& a, int b) {
   if (!kPacked) return KvRows{0, a.n_tokens};
-  const int lo = max(a.cu_tokens[b], 0), hi = min(a.cu_tokens[b + 1], a.total_tokens);
+  const int lo = max(a.cu_tokens[b], 0), hi = min(max(a.cu_tokens[b + 1], 0), a.total_tokens);  // (hi - lo: 32 bits)
   return KvRows{lo, max(0, min(hi - lo, a.n_tokens))};
 }
 

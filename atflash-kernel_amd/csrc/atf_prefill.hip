@@ -144,7 +144,7 @@ struct PackedSeq {
 // Rows and keys of sequence b of packed rows; no rows where its lengths do not fit the
 // call (more rows than keys, more keys than the call's bound or the page table).
 __device__ __forceinline__ PackedSeq packed_seq(const PrefillArgs& a, int b) {
-  const int lo = max(a.pk.cu[b], 0), hi = min(a.pk.cu[b + 1], a.pk.total_q);
+  const int lo = max(a.pk.cu[b], 0), hi = min(max(a.pk.cu[b + 1], 0), a.pk.total_q);  // (hi - lo: 32 bits)
   int n = max(hi - lo, 0);
   const int keys = a.pk.seq_lens != nullptr ? a.pk.seq_lens[b] : n;
   if (keys < n || keys > a.pk.max_k) n = 0;
