@@ -160,7 +160,10 @@ def ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+# Private functions of torch that cost a fraction of the public ones, where it has them.
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
 def stream_of(device):
@@ -180,7 +183,7 @@ def raw_stream(index):
 def launch(index, entry, *args):
     """entry(*args, stream): a library call on the current stream of the GPU `index`,
     made with that device current (a kernel is launched on the current device)."""
-    if index == torch._C._cuda_getDevice():
+    if index == current_device():
         code = entry(*args, raw_stream(index))
     else:
         with torch.cuda.device(index):

@@ -547,8 +547,8 @@ def _(page_table, seq_lens, free_pages, free_count, rows, num_pages):
 # needs no initialisation (each call writes the split partials it reads), and
 # calls on one stream are ordered, so they can share it.
 _DECODE_WS = {}
-_current_device = torch._C._cuda_getDevice
-_capturing = torch._C._cuda_isCurrentStreamCapturing
+_current_device = _lib.current_device
+_capturing = _lib.capturing
 _WS_BYTES = {}  # (batch, hq, hkv, max_seq_len, 8-bit cache) -> workspace bytes the split rule needs
 
 
