@@ -771,12 +771,13 @@ class DecodePlan:
     def run(self, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Decode for q [B, Hq, 128] bf16 (the plan's shape and strides);
         returns out (allocated unless given: bf16 [B, Hq, 128], contiguous)."""
-        if q.shape != self.shape or q.stride() != self.q_strides or q.dtype != torch.bfloat16 or not q.is_cuda:
+        if q.shape != self.shape or q.stride() != self.q_strides or q.dtype != torch.bfloat16 or q.get_device() != self._index:
             raise ValueError(f"q must be bf16 {self.shape} with strides {self.q_strides} on the plan's device")
         if out is None:
             out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
-        elif out.shape != self.shape or not out.is_contiguous() or out.dtype != torch.bfloat16:
-            raise ValueError(f"out must be contiguous bf16 {self.shape}")
+        elif (out.shape != self.shape or not out.is_contiguous() or out.dtype != torch.bfloat16
+              or out.get_device() != self._index):
+            raise ValueError(f"out must be contiguous bf16 {self.shape} on the plan's device")
         args = (out.data_ptr(), self.shape[1] * _lib.HEAD_DIM, _lib.HEAD_DIM, q.data_ptr(), self.q_strides[0],
                 self.q_strides[1], *self._mid)
         if self._index == _current_device():
