@@ -409,9 +409,13 @@ def prefill_packed(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Te
     if plan is None:
         plan = PackedPlan(cu_seqlens, seq_lens, T, max_seq_len, Hq)
     else:
+        # (views of the plan's lengths count as those, if the kernels read the same from them)
         _need(plan.cu_seqlens.data_ptr() == cu_seqlens.data_ptr() and plan.max_seq_len == int(max_seq_len)
-              and _lib.ptr(plan.seq_lens) == _lib.ptr(seq_lens) and plan.batch == cu_seqlens.shape[0] - 1
-              and plan.total_q == T and plan.num_q_heads == Hq, "the plan was made for other rows or lengths")
+              and _lib.ptr(plan.seq_lens) == _lib.ptr(seq_lens) and plan.total_q == T and plan.num_q_heads == Hq,
+              "the plan was made for other rows or lengths")
+        _check_ints(cu_seqlens, plan.batch + 1, "cu_seqlens")
+        if seq_lens is not None:
+            _check_ints(seq_lens, plan.batch, "seq_lens")
     width = _check_table(page_table, plan.batch)[1]
     if out is None:
         out = q.new_empty((T, Hq, D))
