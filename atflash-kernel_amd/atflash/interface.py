@@ -187,7 +187,7 @@ def kv_write_packed(cache, k, v, cu_seqlens, max_tokens, start_pos, page_table, 
     """New tokens of several sequences, rows packed one after the other (k, v
     [T, Hkv, 128], sequence b's rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 from
     position start_pos[b] on), into a PagedKVCache (either kv_dtype)."""
-    ops.kv_write_packed(cache.kv, cache.exps, k, v, cu_seqlens, int(max_tokens), start_pos, page_table, rope,
+    ops.kv_write_packed(cache.kv, getattr(cache, "exps", None), k, v, cu_seqlens, int(max_tokens), start_pos, page_table, rope,
                         _layout_id(layout))
 
 
