@@ -58,6 +58,14 @@ def _need(cond, msg):
         raise ValueError(msg)
 
 
+def _i32(x, name):
+    """x as an int that a C entry takes as it is (ctypes cuts wider ones to 32 bits)."""
+    x = int(x)
+    if not -0x80000000 <= x <= 0x7fffffff:
+        raise ValueError(f"{name} must fit 32 bits, got {x}")
+    return x
+
+
 def _check_cache(kv_cache):
     s = kv_cache.shape
     if (kv_cache.dtype == torch.bfloat16 and len(s) == 4 and s[2] == _lib.KV_BLOCK_SHAPE[0]
@@ -233,7 +241,7 @@ def kv_write_packed(kv_cache: torch.Tensor, kv_exps: Optional[torch.Tensor], k: 
     T = k.shape[0]
     _check_ints(cu_seqlens, B + 1, "cu_seqlens")
     _check_ints(start_pos, B, "start_pos")
-    max_tokens = min(int(max_tokens), T)
+    max_tokens = _i32(min(int(max_tokens), T), "max_tokens")
     rope_cs, max_pos = _rope(rope_cs)
     rope = _lib.ptr(rope_cs)
     if kv_exps is None:
@@ -265,7 +273,7 @@ def kv_expand_q8(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: torc
     B, width = _check_table(page_table)
     if seq_lens is not None:
         _check_ints(seq_lens, B, "seq_lens")
-    n = int(n_pages)
+    n = _i32(n_pages, "n_pages")
     _need(n >= 0, "n_pages must be >= 0")
     out = torch.empty((B * n, pool[1], *_lib.KV_BLOCK_SHAPE), dtype=torch.bfloat16, device=kv_cache.device)
     table = page_table.new_empty((B, n))
@@ -280,7 +288,7 @@ def temporary_bf16(kv_cache: torch.Tensor, kv_exps: torch.Tensor, page_table: to
     kv_expand_q8's blocks by entry of the page table, or where the pool has fewer pages
     than that (n_pages is a bound and may lie far past the lengths) every page in the
     block of its own number, under the caller's table."""
-    n = int(n_pages)
+    n = _i32(n_pages, "n_pages")
     if page_table.dim() != 2 or page_table.shape[0] * n <= kv_cache.shape[0]:
         return kv_expand_q8(kv_cache, kv_exps, page_table, n, seq_lens)
     dev = _one_device(kv_cache, kv_exps, page_table, seq_lens)
@@ -313,6 +321,7 @@ def prefill(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor,
     if page_table.dtype != torch.int32 or len(ps) != 2 or ps[0] != B or not page_table.is_contiguous():
         raise ValueError("page_table must be contiguous int32 [B, max_pages]")
     rope_cs, max_pos = _rope(rope_cs)
+    nk, q_offset = _i32(nk, "nk"), _i32(q_offset, "q_offset")
     dev = q.device
     out = torch.empty((B, Nq, Hq, D), dtype=torch.bfloat16, device=dev)
     lse = torch.empty((B, Hq, Nq), dtype=torch.float32, device=dev)
@@ -320,7 +329,7 @@ def prefill(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor,
     _lib.check(_lib.lib().atf_prefill_bf16(
         out.data_ptr(), Nq * Hq * D, Hq * D, D, lse.data_ptr(), q.data_ptr(), q_sb, q_st, q_sh,
         kv_cache.data_ptr(), pool[0], page_table.data_ptr(), ps[1],
-        B, Nq, int(nk), int(q_offset), Hq, pool[1], _lib.zhi_array(zhi), float(sm_scale),
+        B, Nq, nk, q_offset, Hq, pool[1], _lib.zhi_array(zhi), float(sm_scale),
         None if rope_cs is None else rope_cs.data_ptr(), max_pos, _layout(layout), _lib.stream_of(dev)))
     return out, lse
 
@@ -374,7 +383,8 @@ class PackedPlan:
         if seq_lens is not None:
             _check_ints(seq_lens, self.batch, "seq_lens")
         self.cu_seqlens, self.seq_lens = cu_seqlens, seq_lens
-        self.total_q, self.max_seq_len, self.num_q_heads = int(total_q), int(max_seq_len), int(num_q_heads)
+        self.total_q, self.max_seq_len = _i32(total_q, "total_q"), _i32(max_seq_len, "max_seq_len")
+        self.num_q_heads = int(num_q_heads)
         nbytes = int(_lib.lib().atf_prefill_plan_bytes(self.batch, self.total_q, self.num_q_heads))
         self.tiles = torch.empty(max(nbytes, 8) // 4, dtype=torch.int32, device=self.device)
         self.refresh()
@@ -464,7 +474,7 @@ def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     _check_ints(cu_seqlens, B + 1, "cu_seqlens")
     rope_cs, max_pos = _rope(rope_cs)
     L = _lib.lib()
-    most = int(max_seqlen)
+    most = _i32(max_seqlen, "max_seqlen")
     nbytes = int(L.atf_flash_packed_workspace_bytes(B, T, most, Hq, hkv))
     ws = q.new_empty(max(nbytes, 16) // 2)
     out = q.new_empty((T, Hq, D))
@@ -492,14 +502,14 @@ def extend_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: to
     _check_ints(free_count, 1, "free_count")
     F = free_pages.numel()
     _check_ints(free_pages, F, "free_pages")
-    T = int(total_tokens)
+    T, pool = _i32(total_tokens, "total_tokens"), _i32(num_pages, "num_pages")
     _need(T >= 0, "total_tokens must be >= 0")
     # one allocation: slots first (8-byte aligned); its parts do not overlap
     buf = seq_lens.new_empty(3 * T + 2 * B + 2)
     slots, pos, lens, left, cu = buf.unsafe_split_with_sizes((2 * T, T, B, 1, B + 1))
     at = buf.data_ptr()
     _lib.launch(dev, _lib.lib().atf_extend_tables, page_table.data_ptr(), width, seq_lens.data_ptr(),
-                new_lens.data_ptr(), free_pages.data_ptr(), F, free_count.data_ptr(), B, T, int(num_pages),
+                new_lens.data_ptr(), free_pages.data_ptr(), F, free_count.data_ptr(), B, T, pool,
                 at + 12 * T, at + 12 * T + 4 * B, at + 12 * T + 4 * B + 4, at + 8 * T, at)
     return lens, left, cu, pos, slots.view(torch.int64)
 
@@ -535,7 +545,7 @@ def release_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages:
     _check_ints(rows, rows.numel(), "rows")
     _lib.launch(dev, _lib.lib().atf_release_tables, page_table.data_ptr(), width, seq_lens.data_ptr(),
                 free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), rows.data_ptr(), rows.shape[0], B,
-                int(num_pages))
+                _i32(num_pages, "num_pages"))
 
 
 _release_tables_op = torch.library.custom_op("atflash::release_tables", release_tables,
@@ -624,10 +634,11 @@ def decode_paged(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tens
     ks = kv_cache.shape
     num_pages, hkv = ks[0], ks[1]
     rope_cs, max_pos = _rope(rope_cs)
+    most = _i32(max_seq_len, "max_seq_len")
     L = _lib.lib()
     dev = q.device
     stream = _lib.stream_of(dev)
-    ws = _decode_workspace(dev, stream, B, Hq, hkv, int(max_seq_len), L)
+    ws = _decode_workspace(dev, stream, B, Hq, hkv, most, L)
     out = torch.empty((B, Hq, _lib.HEAD_DIM), dtype=torch.bfloat16, device=dev)
     slices = zhi is not None and len(zhi) == _lib.SLICES
     entry = L.atf_decode_paged_slices_bf16 if slices else L.atf_decode_paged_bf16
@@ -637,7 +648,7 @@ def decode_paged(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tens
     _lib.check(entry(
         out.data_ptr(), Hq * _lib.HEAD_DIM, _lib.HEAD_DIM, q.data_ptr(), q_sb, q_sh,
         kv_cache.data_ptr(), num_pages, page_table.data_ptr(), ps[1],
-        seq_lens.data_ptr(), B, Hq, hkv, int(max_seq_len), table, float(sm_scale),
+        seq_lens.data_ptr(), B, Hq, hkv, most, table, float(sm_scale),
         None if rope_cs is None else rope_cs.data_ptr(), max_pos, _layout(layout), ws[0], ws[1], stream))
     return out
 
@@ -661,7 +672,7 @@ def decode_paged_q8(q: torch.Tensor, kv_cache: torch.Tensor, kv_exps: torch.Tens
     if zhi is not None:
         n = len(zhi)
         table = _lib.zhi_array(zhi, _lib.SLICES if n == _lib.SLICES else _lib.LEVELS)
-    most = int(max_seq_len)
+    most = _i32(max_seq_len, "max_seq_len")
     ws = _decode_workspace(q.device, _lib.raw_stream(dev), B, Hq, hkv, most, L, True)
     out = q.new_empty(qs)
     _lib.launch(dev, L.atf_decode_paged_q8, out.data_ptr(), Hq * D, D, q.data_ptr(), qst[0], qst[1], kv_cache.data_ptr(),
@@ -752,6 +763,7 @@ class DecodePlan:
         D = _lib.HEAD_DIM
         q_sb, q_sh = q_strides if q_strides is not None else (Hq * D, D)
         rope_cs, max_pos = _rope(rope_cs)
+        most = _i32(max_seq_len, "max_seq_len")
         slices = zhi is not None and len(zhi) == _lib.SLICES
         L = _lib.lib()
         self.device = kv_cache.device
@@ -759,7 +771,7 @@ class DecodePlan:
         self.shape = (B, Hq, D)
         self.q_strides = (q_sb, q_sh, 1)
         size = L.atf_decode_workspace_bytes_even if kv_exps is None else L.atf_decode_q8_workspace_bytes
-        nbytes = int(size(B, Hq, kv_cache.shape[1], int(max_seq_len)))
+        nbytes = int(size(B, Hq, kv_cache.shape[1], most))
         self._ws = torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=self.device)
         self._keep = (kv_cache, kv_exps, page_table, seq_lens, rope_cs)  # the tensors the addresses point into
         self._table = _lib.zhi_array(None if zhi is None else tuple(zhi), _lib.SLICES if slices else _lib.LEVELS)
@@ -769,7 +781,7 @@ class DecodePlan:
             self._entry = L.atf_decode_paged_q8
             cache, entries = (*cache, kv_exps.data_ptr()), (0 if zhi is None else len(zhi),)
         self._mid = (*cache, kv_cache.shape[0], page_table.data_ptr(), page_table.shape[1],
-                     seq_lens.data_ptr(), B, Hq, kv_cache.shape[1], int(max_seq_len), self._table, *entries,
+                     seq_lens.data_ptr(), B, Hq, kv_cache.shape[1], most, self._table, *entries,
                      float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout), self._ws.data_ptr(), self._ws.numel() * 4)
 
     def run(self, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
