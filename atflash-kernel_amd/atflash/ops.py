@@ -24,6 +24,8 @@ the bf16 cache):
                                       page_table, rope_cs, layout)
     torch.ops.atflash.prefill_packed(q, kv_cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi,
                                      sm_scale, rope_cs, layout) -> (out, lse)
+    torch.ops.atflash.flash_attn_packed(q, k, v, cu_seqlens, max_seqlen, zhi, sm_scale, rope_cs,
+                                        layout) -> (out, lse)
 
 and the tables of such a step, from lengths that the GPU holds:
 
@@ -459,7 +461,7 @@ def _(q, kv_cache, page_table, cu_seqlens, seq_lens, max_seq_len, zhi, sm_scale,
 
 
 def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int,
-                      zhi, sm_scale: float, rope_cs: Optional[torch.Tensor],
+                      zhi: Optional[List[int]], sm_scale: float, rope_cs: Optional[torch.Tensor],
                       layout: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """prefill_packed of whole prompts whose keys and values are packed rows too
     (k, v [T, Hkv, 128]): they are written to temporary pages first.  The rows of a
@@ -483,6 +485,14 @@ def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
                 k.data_ptr(), ks_t, ks_h, v.data_ptr(), vs_t, vs_h, cu_seqlens.data_ptr(), B, T, most, Hq, hkv,
                 _lib.zhi_array(zhi), float(sm_scale), _lib.ptr(rope_cs), max_pos, _layout(layout), ws.data_ptr(), nbytes)
     return out, lse
+
+
+_flash_attn_packed_op = torch.library.custom_op("atflash::flash_attn_packed", flash_attn_packed, mutates_args=())
+
+
+@_flash_attn_packed_op.register_fake
+def _(q, k, v, cu_seqlens, max_seqlen, zhi, sm_scale, rope_cs, layout):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
 
 
 # ---- tables on the GPU ----
