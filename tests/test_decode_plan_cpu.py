@@ -21,11 +21,12 @@ def tensor(device, shape=(2, 4, 128), dtype=torch.bfloat16):
     return torch.empty(shape, dtype=dtype, device=device)
 
 
-@pytest.mark.parametrize("q,out", [("cuda:0", "cpu"), ("cuda:0", "cuda:1"), ("cuda:1", None), ("cuda:1", "cuda:0"), ("cpu", None)])
-def test_tensors_elsewhere_are_refused(q, out):
+@pytest.mark.parametrize("index,q,out", [(0, "cuda:0", "cpu"), (0, "cuda:0", "meta"), (1, "cuda:0", None), (1, "cuda:0", "cuda:0"),
+                                         (0, "cpu", None)])
+def test_tensors_elsewhere_are_refused(index, q, out):
     with FakeTensorMode():
         with pytest.raises(ValueError, match="plan's device"):
-            plan_on(0).run(tensor(q), None if out is None else tensor(out))
+            plan_on(index).run(tensor(q), None if out is None else tensor(out))
 
 
 def test_other_shapes_and_types_are_refused():
