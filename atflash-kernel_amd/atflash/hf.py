@@ -148,7 +148,11 @@ class PagedLayer(CacheLayerMixin):
         """Keep the first max_length tokens (max_length < 0: drop the last
         |max_length|), as HF's DynamicLayer.crop.  The pages keep their
         contents; positions past the new length are rewritten by the next
-        update before anything reads them."""
+        update before anything reads them.  In a cache of 8-bit floats a page
+        that the cut goes through keeps its exponents too: dropped tokens of
+        large magnitude leave its other codes, and those written into it
+        next, as coarse as they made them (a cut at a multiple of 16 leaves
+        no trace)."""
         max_length = int(max_length)
         if max_length < 0:
             max_length = self.length - abs(max_length)

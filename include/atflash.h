@@ -133,7 +133,9 @@ int atf_kv_write_packed_bf16(void* kv_cache, int num_pages, int num_kv_heads,
  * before its first: the exponent is at least the page's, and where it grows the
  * kept codes move to it (exact, save those that become subnormal).  The slots
  * behind the call's last token in its last page become zero: sequences are
- * appended to, and what lay behind is forgotten.  Infinities and NaN become the
+ * appended to, and the codes that lay behind are forgotten.  Not so the exponent of a
+ * page that a call starts inside: tokens that the call overwrites may have raised it,
+ * and the page's codes stay as coarse as they made it.  Infinities and NaN become the
  * NaN code and count for no exponent.  Two sequences of a call must not write the
  * same page.  batch and num_kv_heads are at most 65535.
  */
