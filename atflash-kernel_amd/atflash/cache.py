@@ -91,8 +91,9 @@ class PageTables:
     def extend(self, new_lens: torch.Tensor, total_tokens: int):
         """Room for new_lens[b] (int32 [batch] on the GPU) more tokens of each sequence,
         total_tokens in all.  Returns (start_pos [batch], cu_seqlens [batch + 1], positions
-        [total_tokens], slots [total_tokens]): what the cache writer and the packed
-        prefill take.  Where the pool is short of pages, free_count becomes negative and
+        [total_tokens], slots [total_tokens]).  The packed writer takes start_pos and
+        cu_seqlens, the packed prefill cu_seqlens; positions and slots are for kernels of the
+        caller's own (position embeddings, other per-token caches on these pages).  Where the pool is short of pages, free_count becomes negative and
         the entries, and the slots of the tokens without a page, are -1 (writers skip
         those)."""
         from . import ops

@@ -342,7 +342,8 @@ int atf_decode_paged_slices_bf16(void* out, int64_t o_sb, int64_t o_sh,
  * atf_decode_q8_workspace_bytes.  With less, down to atf_decode_workspace_bytes,
  * the splits are that decode's, which is slower for ragged batches and gives other
  * roundings.  Keys and values are the codes times their powers of two,
- * exactly; Q, P and the sums have atf_decode_paged_bf16's precision.
+ * exactly; Q (rotated in fp32) and P enter the matrix products in two bf16 parts, 2^-17
+ * of a value left, the sums are fp32, and the output is rounded once.
  */
 size_t atf_decode_q8_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int max_seq_len);
 int atf_decode_paged_q8(void* out, int64_t o_sb, int64_t o_sh, const void* q, int64_t q_sb, int64_t q_sh,
