@@ -35,6 +35,9 @@ PREFILL_BLOCK_M = 32
 PREFILL_BLOCK_N = 32
 DECODE_BLOCK_N = 16
 MAX_GQA_GROUP = 16
+MAX_TOP = 64                 # alternatives of token_logprobs
+MAX_SHARED_PAGES = 1 << 19   # pool of select_tables and compact_tables
+LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -65,6 +68,14 @@ SIGNATURES = {
                                      _p, _f, _p, _i, _i, _p, _sz, _p]),
     "atf_extend_tables": (_i, [_p, _i, _p, _p, _p, _i, _p, _i, _i, _i, _p, _p, _p, _p, _p, _p]),
     "atf_release_tables": (_i, [_p, _i, _p, _p, _i, _p, _p, _i, _i, _i, _p]),
+    "atf_qk_norm_rope_bf16": (_i, [_p, _p, _i64, _i64, _i, _p, _p, _i64, _i64, _i, _p, _p, _i, _f, _i, _p, _p, _i, _p]),
+    "atf_qk_norm_write": (_i, [_p, _p, _i64, _i64, _i, _p, _p, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i, _f,
+                               _i, _p, _i, _i, _p, _p, _i, _p, _i, _p]),
+    "atf_logprobs_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "atf_token_logprobs": (_i, [_p, _p, _p, _p, _p, _i, _i64, _i, _i, _p, _i, _i, _p, _sz, _p]),
+    "atf_select_tables": (_i, [_p, _p, _i, _p, _p, _i, _p, _p, _i, _i, _p, _p, _p, _p, _p]),
+    "atf_compact_tables": (_i, [_p, _p, _i, _p, _p, _p, _i, _p, _i, _i, _p, _p, _p, _i, _p, _p]),
+    "atf_copy_pages": (_i, [_p, _p, _i, _i, _p, _p, _i, _p, _p]),
     "atf_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "atf_decode_workspace_bytes_even": (_sz, [_i, _i, _i, _i]),
     "atf_decode_paged_bf16": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i, _p, _i, _p,

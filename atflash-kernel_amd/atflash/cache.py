@@ -77,11 +77,17 @@ class PageTables:
         free_pages int32 [num_pages], free_count int32 [1]
 
     The tensors keep their addresses, so that captured steps and prepared decode plans
-    go on reading them."""
+    go on reading them.
 
-    def __init__(self, num_pages: int, batch: int, max_pages: int, device="cuda"):
+    sharing=True: sequences may begin with the same pages (`select`: forks, drops, a beam's
+    choice).  `release` then gives back only the pages that no other sequence names."""
+
+    def __init__(self, num_pages: int, batch: int, max_pages: int, device="cuda", sharing: bool = False):
         self.num_pages = int(num_pages)
         self.device = torch.device(device)
+        self.sharing = bool(sharing)
+        if self.sharing and self.num_pages > _lib.MAX_SHARED_PAGES:
+            raise ValueError(f"at most {_lib.MAX_SHARED_PAGES} pages with sharing, got {num_pages}")
         i32 = dict(dtype=torch.int32, device=self.device)
         self.page_table = torch.full((int(batch), int(max_pages)), -1, **i32)
         self.seq_lens = torch.zeros(int(batch), **i32)
@@ -107,7 +113,45 @@ class PageTables:
     def release(self, rows: torch.Tensor):
         """Give back the pages of the finished sequences `rows` (int32 on the GPU)."""
         from . import ops
+        if self.sharing:
+            every = torch.arange(self.seq_lens.shape[0], dtype=torch.int32, device=self.device)
+            gone = (rows[:, None] == every[None]).any(0)
+            self.select(torch.where(gone, -1, every))
+            return
         ops.release_tables(self.page_table, self.seq_lens, self.free_pages, self.free_count, rows, self.num_pages)
+
+
+    def select(self, parents: torch.Tensor, caches=()):
+        """Sequence b becomes what sequence parents[b] is now (int32 [batch] on the GPU;
+        outside [0, batch): empty), with sharing=True: `parents` is the identity but
+        for the rows that a fork, a drop or a beam's choice changes.  Whole pages are named by
+        all of a sequence's children, a last page that is not full is copied for all but
+        one of them, in each of `caches`: every layer's page tensors (K/V pages, exponents).
+        Returns (copy_src, copy_dst), the copies, for caches that are not among them."""
+        from . import ops
+        if not self.sharing:
+            raise ValueError("select needs tables made with sharing=True")
+        table, lens, left, src, dst = ops.select_tables(self.page_table, self.seq_lens, self.free_pages,
+                                                        self.free_count, parents, self.num_pages)
+        self.page_table.copy_(table)
+        self.seq_lens.copy_(lens)
+        self.free_count.copy_(left)
+        ops.copy_pages(caches, src, dst)
+        return src, dst
+
+    def compact(self, caches):
+        """The pages of all sequences moved to the front of the pool, in `caches` (every
+        layer's page tensors).  Returns the number of pages moved (int32 [1] on the GPU): the
+        pages in use are then the lowest of those that are in use or free, so that a
+        pool without pages held elsewhere can be cut behind them."""
+        from . import ops
+        table, free, left, src, dst, n = ops.compact_tables(self.page_table, self.seq_lens, self.free_pages,
+                                                            self.free_count, self.num_pages)
+        self.page_table.copy_(table)
+        self.free_pages.copy_(free)
+        self.free_count.copy_(left)
+        ops.copy_pages(caches, src, dst, n)
+        return n
 
 
 class PagedKVCache:

@@ -33,6 +33,22 @@ and the tables of such a step, from lengths that the GPU holds:
                                     num_pages) -> (seq_lens, free_left, cu_seqlens, positions, slots)
     torch.ops.atflash.release_tables(page_table, seq_lens, free_pages, free_count, rows, num_pages)
 
+Norms of queries and keys with the rotation in the same pass, on rows or with the keys
+written to either cache:
+
+    torch.ops.atflash.qk_norm_rope(q, k, q_weight, k_weight, eps, positions, rope_cs) -> (q, k)
+    torch.ops.atflash.qk_norm_write(kv_cache, kv_exps, q, k, v, q_weight, k_weight, eps, cu_seqlens,
+                                    max_tokens, start_pos, page_table, rope_cs) -> q
+
+Sequences that share pages (forks, beams), pages moved, and what a step's logits say:
+
+    torch.ops.atflash.select_tables(page_table, seq_lens, free_pages, free_count, parents, num_pages)
+                                    -> (page_table, seq_lens, free_left, copy_src, copy_dst)
+    torch.ops.atflash.compact_tables(page_table, seq_lens, free_pages, free_count, num_pages)
+                                    -> (page_table, free_pages, free_left, copy_src, copy_dst, n_copies)
+    torch.ops.atflash.copy_pages(caches, src, dst, count)
+    torch.ops.atflash.token_logprobs(logits, tokens, top) -> (logprobs, entropy, top_logprobs, top_ids)
+
 Each op checks shapes and dtypes, then calls the HIP library on the current
 stream of the tensors' device.  There is no CPU or PyTorch fallback: a CPU
 tensor or a missing library is an error.
@@ -42,7 +58,9 @@ same operations called directly from Python, without the dispatcher (whose
 per-call cost, about 20 us, would exceed a short decode's GPU time); the
 package's own entry points use them.
 """
-from typing import List, Optional, Tuple
+import ctypes
+import math
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -565,6 +583,275 @@ _release_tables_op = torch.library.custom_op("atflash::release_tables", release_
 @_release_tables_op.register_fake
 def _(page_table, seq_lens, free_pages, free_count, rows, num_pages):
     return None
+
+
+# ---- sequences that share pages ----
+
+def select_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                  parents: torch.Tensor, num_pages: int
+                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """New row b of the tables from old row parents[b] (int32 [batch]; outside [0, batch):
+    an empty row): forks, drops, a beam's choice.  Whole pages are shared; a last page that
+    the tokens fill in part stays with one child, the others take a free page for it.  Pages
+    that no new row names are appended to free_pages (in place, from free_count on).
+    Returns (page_table, seq_lens, free pages left [1], copy_src [batch], copy_dst
+    [batch]): page copy_src[b] is to be copied to copy_dst[b] in every cache (copy_pages;
+    -1: no copy).  See atf_select_tables in include/atflash.h."""
+    dev = _one_device(page_table, seq_lens, free_pages, free_count, parents)
+    B, width = _check_table(page_table)
+    _check_ints(seq_lens, B, "seq_lens")
+    _check_ints(parents, B, "parents")
+    _check_ints(free_count, 1, "free_count")
+    F = free_pages.numel()
+    _check_ints(free_pages, F, "free_pages")
+    pool = _i32(num_pages, "num_pages")
+    table = torch.empty_like(page_table)
+    lens, src, dst, left = seq_lens.new_empty(3 * B + 1).unsafe_split_with_sizes((B, B, B, 1))
+    _lib.launch(dev, _lib.lib().atf_select_tables, table.data_ptr(), page_table.data_ptr(), width, seq_lens.data_ptr(),
+                free_pages.data_ptr(), F, free_count.data_ptr(), parents.data_ptr(), B, pool, lens.data_ptr(),
+                left.data_ptr(), src.data_ptr(), dst.data_ptr())
+    return table, lens, left, src, dst
+
+
+def _select_tables_schema(page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
+                          free_count: torch.Tensor, parents: torch.Tensor, num_pages: int
+                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    # (an operator's outputs may not share storage)
+    table, *rest = select_tables(page_table, seq_lens, free_pages, free_count, parents, num_pages)
+    return (table, *(x.clone() for x in rest))
+
+
+_select_tables_op = torch.library.custom_op("atflash::select_tables", _select_tables_schema, mutates_args=("free_pages",))
+
+
+@_select_tables_op.register_fake
+def _(page_table, seq_lens, free_pages, free_count, parents, num_pages):
+    B = page_table.shape[0]
+    return (torch.empty_like(page_table), seq_lens.new_empty(B), seq_lens.new_empty(1), seq_lens.new_empty(B),
+            seq_lens.new_empty(B))
+
+
+def compact_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
+                   free_count: torch.Tensor, num_pages: int
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The pages of all rows moved to the lowest of the ids that rows and free pages have.
+    Returns (page_table, free_pages, free pages left [1], copy_src, copy_dst [num_pages //
+    2, at least 1], n_copies [1]): copy_src[i] is to be copied to copy_dst[i], i <
+    n_copies, in every cache (copy_pages).  See atf_compact_tables in include/atflash.h."""
+    dev = _one_device(page_table, seq_lens, free_pages, free_count)
+    B, width = _check_table(page_table)
+    _check_ints(seq_lens, B, "seq_lens")
+    _check_ints(free_count, 1, "free_count")
+    F = free_pages.numel()
+    _check_ints(free_pages, F, "free_pages")
+    pool = _i32(num_pages, "num_pages")
+    half = max(1, pool // 2)
+    table, free = torch.empty_like(page_table), torch.empty_like(free_pages)
+    src, dst, left, n = seq_lens.new_empty(2 * half + 2).unsafe_split_with_sizes((half, half, 1, 1))
+    _lib.launch(dev, _lib.lib().atf_compact_tables, table.data_ptr(), page_table.data_ptr(), width, seq_lens.data_ptr(),
+                free.data_ptr(), free_pages.data_ptr(), F, free_count.data_ptr(), B, pool, left.data_ptr(), src.data_ptr(),
+                dst.data_ptr(), half, n.data_ptr())
+    return table, free, left, src, dst, n
+
+
+def _compact_tables_schema(page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
+                           free_count: torch.Tensor, num_pages: int
+                           ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    table, free, *rest = compact_tables(page_table, seq_lens, free_pages, free_count, num_pages)
+    return (table, free, *(x.clone() for x in rest))
+
+
+_compact_tables_op = torch.library.custom_op("atflash::compact_tables", _compact_tables_schema, mutates_args=())
+
+
+@_compact_tables_op.register_fake
+def _(page_table, seq_lens, free_pages, free_count, num_pages):
+    half = max(1, int(num_pages) // 2)
+    return (torch.empty_like(page_table), torch.empty_like(free_pages), seq_lens.new_empty(1), seq_lens.new_empty(half),
+            seq_lens.new_empty(half), seq_lens.new_empty(1))
+
+
+def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor,
+               count: Optional[torch.Tensor] = None) -> None:
+    """Page dst[i] of every cache becomes a copy of its page src[i] (int32 [n]; pairs with an
+    entry outside the pool are left out), for the first count[0] pairs where count (int32
+    [1]) is given.  caches: contiguous tensors [num_pages, ...] of any type, of one pool: all
+    layers' K/V pages, and their exponents where the cache is of 8-bit floats.  The pages
+    that are written must be different, and none of them a source of the call."""
+    if len(caches) == 0:
+        return
+    n = src.numel()
+    dev = _one_device(caches[0], src, dst, count, *caches)
+    _check_ints(src, n, "src")
+    _check_ints(dst, n, "dst")
+    if count is not None:
+        _check_ints(count, 1, "count")
+    pool = caches[0].shape[0] if caches[0].dim() else 0
+    bases, sizes = [], []
+    for c in caches:
+        if c.dim() < 1 or c.shape[0] != pool or not c.is_contiguous():
+            raise ValueError("caches must be contiguous [num_pages, ...] tensors of one pool")
+        bases.append(c.data_ptr())
+        sizes.append(c.nbytes // pool if pool else 0)
+    if pool == 0:
+        return
+    _lib.launch(dev, _lib.lib().atf_copy_pages, (ctypes.c_void_p * len(bases))(*bases),
+                (ctypes.c_int64 * len(sizes))(*sizes), len(bases), pool, src.data_ptr(), dst.data_ptr(), n, _lib.ptr(count))
+
+
+def _copy_pages_schema(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor,
+                       count: Optional[torch.Tensor]) -> None:
+    copy_pages(caches, src, dst, count)
+
+
+_copy_pages_op = torch.library.custom_op("atflash::copy_pages", _copy_pages_schema, mutates_args=("caches",))
+
+
+@_copy_pages_op.register_fake
+def _(caches, src, dst, count):
+    return None
+
+
+# ---- norms of queries and keys ----
+
+def _norm_weights(q_weight, k_weight):
+    """Whether the weights are fp32."""
+    dt = q_weight.dtype
+    for w in (q_weight, k_weight):
+        if w.shape != (_lib.HEAD_DIM,) or w.dtype != dt or not w.is_contiguous():
+            raise ValueError("q_weight and k_weight must be contiguous [128] of one type")
+    if dt != torch.bfloat16 and dt != torch.float32:
+        raise ValueError(f"q_weight and k_weight must be bf16 or fp32, got {dt}")
+    return dt == torch.float32
+
+
+def _check_eps(eps):
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    return eps
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
+                 positions: Optional[torch.Tensor], rope_cs: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of each head's rows of q [T, Hq, 128] and k [T, Hk, 128] (either may have no
+    heads) and, with rope_cs, their rotation to positions (int32 [T]), in one pass:
+    x (mean(x^2) + eps)^-1/2 w, then rotate-half.  Returns bf16 (q, k), contiguous; rows
+    whose position lies outside the RoPE table are not written."""
+    dev = _one_device(q, k, q_weight, k_weight, positions, rope_cs)
+    (T, Hq, D), qst = _check_packed_q(q)
+    _need(k.dim() == 3 and k.shape[0] == T, "q and k must have the same rows [T, heads, 128]")
+    (_, Hk, _), kst = _check_packed_q(k)
+    fp32 = _norm_weights(q_weight, k_weight)
+    rope_cs, max_pos = _rope(rope_cs)
+    if rope_cs is not None:
+        _need(positions is not None, "positions are needed with rope_cs")
+        _check_ints(positions, T, "positions")
+    out_q, out_k = q.new_empty((T, Hq, D)), k.new_empty((T, Hk, D))
+    _lib.launch(dev, _lib.lib().atf_qk_norm_rope_bf16, out_q.data_ptr(), q.data_ptr(), qst[0], qst[1], Hq,
+                out_k.data_ptr(), k.data_ptr(), kst[0], kst[1], Hk, q_weight.data_ptr(), k_weight.data_ptr(), fp32,
+                _check_eps(eps), T, _lib.ptr(positions), _lib.ptr(rope_cs), max_pos)
+    return out_q, out_k
+
+
+_qk_norm_rope_op = torch.library.custom_op("atflash::qk_norm_rope", qk_norm_rope, mutates_args=())
+
+
+@_qk_norm_rope_op.register_fake
+def _(q, k, q_weight, k_weight, eps, positions, rope_cs):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+def qk_norm_write(kv_cache: torch.Tensor, kv_exps: Optional[torch.Tensor], q: torch.Tensor, k: torch.Tensor,
+                  v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float, cu_seqlens: torch.Tensor,
+                  max_tokens: int, start_pos: torch.Tensor, page_table: torch.Tensor,
+                  rope_cs: Optional[torch.Tensor]) -> torch.Tensor:
+    """kv_write_packed of keys that are normed (and rotated) on the way, and the queries of
+    the same rows normed and rotated beside: q [T, Hq, 128], k, v [T, Hkv, 128], sequence
+    b's rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (at most max_tokens) from position
+    start_pos[b] on.  Returns q as the attention takes it with rope_cs None, bf16 [T, Hq,
+    128]; rows outside every sequence or past the RoPE table are not written."""
+    dev = _one_device(kv_cache, kv_exps, q, k, v, q_weight, k_weight, cu_seqlens, start_pos, page_table, rope_cs)
+    if kv_exps is None:
+        _check_cache(kv_cache)
+        pool = kv_cache.shape
+    else:
+        pool = _check_cache_q8(kv_cache, kv_exps)
+    (T, Hq, D), qst = _check_packed_q(q)
+    (ks_t, ks_h, _), (vs_t, vs_h, _) = _check_rows(k, v, 3, pool[1])
+    _need(k.shape[0] == T, "q, k and v must have the same rows [T, heads, 128]")
+    fp32 = _norm_weights(q_weight, k_weight)
+    B, width = _check_table(page_table)
+    _check_ints(cu_seqlens, B + 1, "cu_seqlens")
+    _check_ints(start_pos, B, "start_pos")
+    most = _i32(min(int(max_tokens), T), "max_tokens")
+    rope_cs, max_pos = _rope(rope_cs)
+    out = q.new_empty((T, Hq, D))
+    _lib.launch(dev, _lib.lib().atf_qk_norm_write, out.data_ptr(), q.data_ptr(), qst[0], qst[1], Hq, kv_cache.data_ptr(),
+                _lib.ptr(kv_exps), pool[0], pool[1], k.data_ptr(), ks_t, ks_h, v.data_ptr(), vs_t, vs_h,
+                q_weight.data_ptr(), k_weight.data_ptr(), fp32, _check_eps(eps), B, cu_seqlens.data_ptr(), T, most,
+                start_pos.data_ptr(), page_table.data_ptr(), width, _lib.ptr(rope_cs), max_pos)
+    return out
+
+
+_qk_norm_write_op = torch.library.custom_op("atflash::qk_norm_write", qk_norm_write,
+                                            mutates_args=("kv_cache", "kv_exps"))
+
+
+@_qk_norm_write_op.register_fake
+def _(kv_cache, kv_exps, q, k, v, q_weight, k_weight, eps, cu_seqlens, max_tokens, start_pos, page_table, rope_cs):
+    return q.new_empty(q.shape)
+
+
+# ---- log probabilities ----
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """What rows of logits [R, V] (bf16, fp16 or fp32, any row stride) say: log probabilities
+    of tokens (int64 [R] or [R, n]; None: none), the entropy, and the `top` (at most 64)
+    likeliest tokens.  Returns fp32 (logprobs, of tokens' shape, entropy [R], top_logprobs
+    [R, top]) and top_ids int64 [R, top], best first, of equal logits the lowest id first.
+    A negative token (padding) gets 0, one past the vocabulary NaN.  See
+    atf_token_logprobs in include/atflash.h for -inf, NaN and rows without a logit left."""
+    dev = _one_device(logits, tokens)
+    kind = _lib.LOGIT_TYPES.get(logits.dtype)
+    if kind is None or logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError("logits must be bf16, fp16 or fp32 [rows, vocab], the last dim contiguous")
+    R, V = (_i32(x, "rows and vocab") for x in logits.shape)
+    top = int(top)
+    if not 0 <= top <= min(_lib.MAX_TOP, V):
+        raise ValueError(f"top must be between 0 and {min(_lib.MAX_TOP, V)}, got {top}")
+    _need(R == 0 or V > 0, "a row needs at least one logit")
+    n = 0
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != R or not tokens.is_contiguous():
+            raise ValueError("tokens must be contiguous int64 [rows] or [rows, n]")
+        n = tokens.numel() // R if R else 0
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    logp = torch.empty((R, 0) if tokens is None else tokens.shape, **f32)
+    entropy, values = torch.empty(R, **f32), torch.empty((R, top), **f32)
+    ids = torch.empty((R, top), dtype=torch.int64, device=logits.device)
+    L = _lib.lib()
+    nbytes = int(L.atf_logprobs_workspace_bytes(R, V, kind, top))
+    ws = torch.empty(nbytes // 4, **f32) if nbytes else None
+    _lib.launch(dev, L.atf_token_logprobs, logp.data_ptr(), entropy.data_ptr(), values.data_ptr(), ids.data_ptr(),
+                logits.data_ptr(), kind, logits.stride(0), R, V, _lib.ptr(tokens), n, top, _lib.ptr(ws), nbytes)
+    return logp, entropy, values, ids
+
+
+def _token_logprobs_schema(logits: torch.Tensor, tokens: Optional[torch.Tensor], top: int
+                           ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return token_logprobs(logits, tokens, top)
+
+
+_token_logprobs_op = torch.library.custom_op("atflash::token_logprobs", _token_logprobs_schema, mutates_args=())
+
+
+@_token_logprobs_op.register_fake
+def _(logits, tokens, top):
+    R, f32 = logits.shape[0], torch.float32
+    return (logits.new_empty((R, 0) if tokens is None else tokens.shape, dtype=f32), logits.new_empty(R, dtype=f32),
+            logits.new_empty((R, top), dtype=f32), logits.new_empty((R, top), dtype=torch.int64))
 
 
 # Decode workspaces, one per (device, stream), grown on demand.  A workspace

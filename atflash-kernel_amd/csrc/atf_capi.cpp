@@ -13,6 +13,10 @@
 
 namespace {
 
+static_assert(ATF_MAX_TOP == atf::kTopMax && ATF_MAX_SHARED_PAGES == atf::kPoolMaxPages, "header and kernels");
+static_assert(ATF_LOGITS_BF16 == atf::kLogitsBf16 && ATF_LOGITS_FP16 == atf::kLogitsFp16 &&
+              ATF_LOGITS_FP32 == atf::kLogitsFp32, "header and kernels");
+
 thread_local std::string g_last_error;
 
 int fail(int code, const char* fmt, ...) {
@@ -574,6 +578,223 @@ int atf_release_tables(int32_t* page_table, int max_pages, int32_t* seq_lens, in
                                  num_pages};
   hipError_t e = atf::launch_release_tables(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "table release launch");
+  return ok();
+}
+
+}  // extern "C"
+
+namespace {
+
+// What atf_qk_norm_rope_bf16 and atf_qk_norm_write check alike: q's rows, weights, eps.
+int norm_prepare(void* q_out, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads, const void* q_weight,
+                 const void* k_weight, int weights_fp32, float eps, atf::QkNormArgs* a) {
+  if (num_q_heads < 0) return fail(ATF_ERR_INVALID, "num_q_heads must be >= 0, got %d", num_q_heads);
+  if (num_q_heads > 0 && (!q_out || !q || !q_weight)) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(ATF_ERR_INVALID, "eps must be finite and not negative");
+  for (const void* p : {static_cast<const void*>(q_out), q, q_weight, k_weight})
+    if (!aligned(p, 16)) return fail(ATF_ERR_INVALID, "rows and weights must be 16-byte aligned");
+  for (int64_t s : {q_st, q_sh})
+    if (s % 8 != 0) return fail(ATF_ERR_INVALID, "source strides must be multiples of 8 elements");
+  a->q = static_cast<const uint16_t*>(q);
+  a->q_st = q_st;
+  a->q_sh = q_sh;
+  a->q_out = static_cast<uint16_t*>(q_out);
+  a->hq = num_q_heads;
+  a->q_weight = q_weight;
+  a->k_weight = k_weight;
+  a->weights_fp32 = weights_fp32 != 0;
+  a->eps = eps;
+  return ATF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int atf_qk_norm_rope_bf16(void* q_out, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads, void* k_out,
+                          const void* k, int64_t k_st, int64_t k_sh, int num_k_heads, const void* q_weight,
+                          const void* k_weight, int weights_fp32, float eps, int rows, const int32_t* positions,
+                          const float* rope_cs, int rope_max_pos, void* stream) {
+  if (rows < 0 || num_k_heads < 0) return fail(ATF_ERR_INVALID, "rows and num_k_heads must be >= 0");
+  if (rows == 0 || (num_q_heads == 0 && num_k_heads == 0)) return ok();
+  atf::QkNormArgs a{};
+  if (int r = norm_prepare(q_out, q, q_st, q_sh, num_q_heads, q_weight, k_weight, weights_fp32, eps, &a)) return r;
+  if (num_k_heads > 0 && (!k_out || !k || !k_weight)) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (!aligned(k_out, 16) || !aligned(k, 16)) return fail(ATF_ERR_INVALID, "rows and weights must be 16-byte aligned");
+  for (int64_t s : {k_st, k_sh})
+    if (s % 8 != 0) return fail(ATF_ERR_INVALID, "source strides must be multiples of 8 elements");
+  if (static_cast<int64_t>(num_q_heads) + num_k_heads > 65535)
+    return fail(ATF_ERR_UNSUPPORTED, "at most 65535 heads, got %d and %d", num_q_heads, num_k_heads);
+  if (int r = check_layout(ATF_LAYOUT_HALF_SPLIT, rope_cs, rope_max_pos)) return r;
+  if (rope_cs && !positions) return fail(ATF_ERR_INVALID, "null pointer argument");
+  a.k = static_cast<const uint16_t*>(k);
+  a.k_st = k_st;
+  a.k_sh = k_sh;
+  a.k_out = static_cast<uint16_t*>(k_out);
+  a.hk = num_k_heads;
+  a.rows = rows;
+  a.positions = positions;
+  a.rope_cs = rope_cs;
+  a.rope_max_pos = rope_max_pos;
+  hipError_t e = atf::launch_qk_norm_rows(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "norm and rotation launch");
+  return ok();
+}
+
+int atf_qk_norm_write(void* q_out, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads, void* kv_cache,
+                      int8_t* kv_exps, int num_pages, int num_kv_heads, const void* k_src, int64_t ks_t, int64_t ks_h,
+                      const void* v_src, int64_t vs_t, int64_t vs_h, const void* q_weight, const void* k_weight,
+                      int weights_fp32, float eps, int batch, const int32_t* cu_tokens, int total_tokens,
+                      int max_tokens, const int32_t* start_pos, const int32_t* page_table, int max_pages,
+                      const float* rope_cs, int rope_max_pos, void* stream) {
+  atf::QkNormArgs a{};
+  if (int r = kv_write_prepare(kv_cache, num_pages, num_kv_heads, k_src, 0, ks_t, ks_h, v_src, 0, vs_t, vs_h, batch,
+                               max_tokens, start_pos, page_table, max_pages, rope_cs, rope_max_pos,
+                               ATF_LAYOUT_HALF_SPLIT, &a.kv))
+    return r;
+  if (int r = check_packed(batch, cu_tokens, total_tokens)) return r;
+  if (batch == 0 || max_tokens == 0 || total_tokens == 0) return ok();
+  if (int r = norm_prepare(q_out, q, q_st, q_sh, num_q_heads, q_weight, k_weight, weights_fp32, eps, &a)) return r;
+  if (!k_weight) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (batch > 65535 || num_kv_heads > 65535 || num_q_heads > 65535)
+    return fail(ATF_ERR_UNSUPPORTED, "at most 65535 sequences and heads, got %d, %d and %d", batch, num_q_heads, num_kv_heads);
+  a.kv.cu_tokens = cu_tokens;
+  a.kv.total_tokens = total_tokens;
+  a.kv.n_tokens = std::min(max_tokens, total_tokens);
+  a.kv.kv_exps = kv_exps;
+  hipError_t e = atf::launch_qk_norm_write(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "norm and kv_write launch");
+  return ok();
+}
+
+size_t atf_logprobs_workspace_bytes(int rows, int vocab, int logits_type, int top) {
+  if (rows <= 0 || vocab <= 0 || top < 0) return 0;
+  const int n = atf::logprob_splits(rows, vocab, logits_type, top);
+  return n <= 1 ? 0 : static_cast<size_t>(rows) * n * (4 * sizeof(float) + top * sizeof(uint64_t));
+}
+
+int atf_token_logprobs(float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, const void* logits,
+                       int logits_type, int64_t stride, int rows, int vocab, const int64_t* tokens, int n_tokens,
+                       int top, void* workspace, size_t workspace_bytes, void* stream) {
+  if (rows < 0 || n_tokens < 0 || top < 0) return fail(ATF_ERR_INVALID, "rows, n_tokens and top must be >= 0");
+  if (logits_type != ATF_LOGITS_BF16 && logits_type != ATF_LOGITS_FP16 && logits_type != ATF_LOGITS_FP32)
+    return fail(ATF_ERR_INVALID, "unknown type of logits %d", logits_type);
+  if (rows == 0) return ok();
+  if (vocab <= 0) return fail(ATF_ERR_INVALID, "a row needs at least one logit");
+  if (vocab > (1 << 30)) return fail(ATF_ERR_UNSUPPORTED, "at most 2^30 logits a row, got %d", vocab);
+  if (top > vocab) return fail(ATF_ERR_INVALID, "top = %d of %d logits", top, vocab);
+  if (top > ATF_MAX_TOP) return fail(ATF_ERR_UNSUPPORTED, "at most %d alternatives, got %d", ATF_MAX_TOP, top);
+  if (!logits || !entropy || (n_tokens > 0 && (!logprobs || !tokens)) || (top > 0 && (!top_logprobs || !top_ids)))
+    return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (!aligned(logits, logits_type == ATF_LOGITS_FP32 ? 4 : 2) || !aligned(tokens, 8) || !aligned(top_ids, 8))
+    return fail(ATF_ERR_INVALID, "logits, tokens and top_ids must be aligned to their elements");
+  const size_t need = atf_logprobs_workspace_bytes(rows, vocab, logits_type, top);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(ATF_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,
+                workspace ? workspace_bytes : 0);
+  atf::LogprobArgs a{};
+  a.logits = logits;
+  a.stride = stride;
+  a.type = logits_type;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.tokens = tokens;
+  a.n_tokens = n_tokens;
+  a.top = top;
+  a.logprobs = logprobs;
+  a.entropy = entropy;
+  a.top_logprobs = top_logprobs;
+  a.top_ids = top_ids;
+  a.splits = atf::logprob_splits(rows, vocab, logits_type, top);
+  a.ws_stats = static_cast<float*>(workspace);
+  a.ws_top = reinterpret_cast<uint64_t*>(a.ws_stats + 4 * static_cast<size_t>(rows) * a.splits);
+  hipError_t e = atf::launch_token_logprobs(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "log probabilities launch");
+  return ok();
+}
+
+}  // extern "C"
+
+namespace {
+
+// Tables and pools that atf_select_tables and atf_compact_tables take.
+int check_tables(int batch, int max_pages, int num_free, int num_pages) {
+  if (batch <= 0 || max_pages <= 0 || num_free < 0 || num_pages <= 0)
+    return fail(ATF_ERR_INVALID, "batch, max_pages and num_pages must be positive, num_free >= 0");
+  if (batch > atf::kTabMaxBatch)
+    return fail(ATF_ERR_UNSUPPORTED, "at most %d sequences, got %d", atf::kTabMaxBatch, batch);
+  if (static_cast<int64_t>(batch) * max_pages > (int64_t(1) << 30))
+    return fail(ATF_ERR_UNSUPPORTED, "page table of at most 2^30 entries, got %d x %d", batch, max_pages);
+  if (num_pages > ATF_MAX_SHARED_PAGES)
+    return fail(ATF_ERR_UNSUPPORTED, "a pool of at most %d pages, got %d", ATF_MAX_SHARED_PAGES, num_pages);
+  return ATF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int atf_select_tables(int32_t* table_out, const int32_t* page_table, int max_pages, const int32_t* seq_lens,
+                      int32_t* free_pages, int num_free, const int32_t* free_count, const int32_t* parents, int batch,
+                      int num_pages, int32_t* seq_lens_out, int32_t* free_left, int32_t* copy_src, int32_t* copy_dst,
+                      void* stream) {
+  if (int r = check_tables(batch, max_pages, num_free, num_pages)) return r;
+  if (!table_out || !page_table || !seq_lens || (num_free > 0 && !free_pages) || !free_count || !parents ||
+      !seq_lens_out || !free_left || !copy_src || !copy_dst)
+    return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (table_out == page_table || seq_lens_out == seq_lens)
+    return fail(ATF_ERR_INVALID, "the new tables must not be the old ones");
+  const atf::SelectTablesArgs a{table_out, page_table, max_pages, seq_lens,     free_pages, num_free, free_count,
+                                parents,   batch,      num_pages, seq_lens_out, free_left,  copy_src, copy_dst};
+  hipError_t e = atf::launch_select_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "table selection launch");
+  return ok();
+}
+
+int atf_compact_tables(int32_t* table_out, const int32_t* page_table, int max_pages, const int32_t* seq_lens,
+                       int32_t* free_out, const int32_t* free_pages, int num_free, const int32_t* free_count,
+                       int batch, int num_pages, int32_t* free_left, int32_t* copy_src, int32_t* copy_dst, int copies,
+                       int32_t* n_copies, void* stream) {
+  if (int r = check_tables(batch, max_pages, num_free, num_pages)) return r;
+  if (!table_out || !page_table || !seq_lens || (num_free > 0 && (!free_pages || !free_out)) || !free_count ||
+      !free_left || !copy_src || !copy_dst || !n_copies)
+    return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (copies < num_pages / 2) return fail(ATF_ERR_INVALID, "room for %d copies needed, got %d", num_pages / 2, copies);
+  if (table_out == page_table || (num_free > 0 && free_out == free_pages))
+    return fail(ATF_ERR_INVALID, "the new tables must not be the old ones");
+  const atf::CompactTablesArgs a{table_out, page_table, max_pages, seq_lens,  free_out, free_pages, num_free, free_count,
+                                 batch,     num_pages,  free_left, copy_src, copy_dst, copies,     n_copies};
+  hipError_t e = atf::launch_compact_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "table compaction launch");
+  return ok();
+}
+
+int atf_copy_pages(void* const* caches, const int64_t* page_bytes, int n_caches, int num_pages, const int32_t* src,
+                   const int32_t* dst, int n, const int32_t* count, void* stream) {
+  if (n_caches < 0 || n < 0) return fail(ATF_ERR_INVALID, "n_caches and n must be >= 0");
+  if (n_caches == 0 || n == 0) return ok();
+  if (!caches || !page_bytes || !src || !dst) return fail(ATF_ERR_INVALID, "null pointer argument");
+  if (num_pages <= 0) return fail(ATF_ERR_INVALID, "num_pages must be positive, got %d", num_pages);
+  for (int i = 0; i < n_caches; ++i) {
+    if (!caches[i]) return fail(ATF_ERR_INVALID, "null pointer argument");
+    if (page_bytes[i] <= 0 || page_bytes[i] > (int64_t(1) << 40) / num_pages)
+      return fail(ATF_ERR_INVALID, "cache %d: a page of %lld bytes", i, static_cast<long long>(page_bytes[i]));
+  }
+  for (int i0 = 0; i0 < n_caches; i0 += atf::kCopyCaches) {
+    atf::CopyPagesArgs a{};
+    a.src = src;
+    a.dst = dst;
+    a.count = count;
+    a.n = n;
+    a.num_pages = num_pages;
+    a.n_caches = std::min(n_caches - i0, atf::kCopyCaches);
+    for (int i = 0; i < a.n_caches; ++i) {
+      a.base[i] = static_cast<uint8_t*>(caches[i0 + i]);
+      a.bytes[i] = page_bytes[i0 + i];
+    }
+    hipError_t e = atf::launch_copy_pages(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "page copy launch");
+  }
   return ok();
 }
 

@@ -174,6 +174,98 @@ struct ReleaseTablesArgs {
 };
 hipError_t launch_release_tables(const ReleaseTablesArgs& a, hipStream_t s);
 
+// Norm and rotation of each head's queries and keys (atf_qk_norm_rope_bf16, atf_qk_norm_write).
+struct QkNormArgs {
+  const uint16_t* q;  // [rows][hq][128] (strided)
+  int64_t q_st, q_sh;
+  uint16_t* q_out;  // [rows][hq][128]
+  int hq;
+  const uint16_t* k;  // [rows][hk][128] (strided)
+  int64_t k_st, k_sh;
+  uint16_t* k_out;  // [rows][hk][128]
+  int hk;
+  const void* q_weight;  // [128] bf16, or fp32
+  const void* k_weight;
+  bool weights_fp32;
+  float eps;
+  int rows;
+  const int32_t* positions;  // [rows]
+  const float* rope_cs;
+  int rope_max_pos;
+  // into a cache: k, v, positions and rope_cs as the writers' (packed rows); hq heads of q beside
+  KvWriteArgs kv;
+};
+hipError_t launch_qk_norm_rows(const QkNormArgs& a, hipStream_t s);
+hipError_t launch_qk_norm_write(const QkNormArgs& a, hipStream_t s);
+
+// Log probabilities, entropy and top alternatives of rows of logits (atf_token_logprobs).
+constexpr int kTopMax = 64;
+enum LogitType { kLogitsBf16 = 0, kLogitsFp16 = 1, kLogitsFp32 = 2 };
+struct LogprobArgs {
+  const void* logits;  // [rows][vocab], element stride between rows
+  int64_t stride;
+  int type;
+  int rows, vocab;
+  const int64_t* tokens;  // [rows][n_tokens]
+  int n_tokens, top;
+  float* logprobs;   // [rows][n_tokens]
+  float* entropy;    // [rows]
+  float* top_logprobs;  // [rows][top]
+  int64_t* top_ids;     // [rows][top]
+  int splits;        // workgroups of a row
+  float* ws_stats;   // [rows][splits][4]: largest logit, sum of exponentials, sum of (distance x exponential)
+  uint64_t* ws_top;  // [rows][splits][top]: the split's best, best first
+};
+int logprob_splits(int rows, int vocab, int type, int top);
+hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t s);
+
+// Page tables of sequences that share pages, and pages moved (atf_select_tables,
+// atf_compact_tables, atf_copy_pages).
+constexpr int kPoolMaxPages = 1 << 19;  // two bit maps of a pool in 128 KB of LDS
+struct SelectTablesArgs {
+  int32_t* table_out;
+  const int32_t* page_table;
+  int max_pages;
+  const int32_t* seq_lens;
+  int32_t* free_pages;
+  int num_free;
+  const int32_t* free_count;
+  const int32_t* parents;
+  int batch, num_pages;
+  int32_t* lens_out;
+  int32_t* free_left;
+  int32_t* copy_src;
+  int32_t* copy_dst;
+};
+hipError_t launch_select_tables(const SelectTablesArgs& a, hipStream_t s);
+struct CompactTablesArgs {
+  int32_t* table_out;
+  const int32_t* page_table;
+  int max_pages;
+  const int32_t* seq_lens;
+  int32_t* free_out;
+  const int32_t* free_pages;
+  int num_free;
+  const int32_t* free_count;
+  int batch, num_pages;
+  int32_t* free_left;
+  int32_t* copy_src;
+  int32_t* copy_dst;
+  int copies;  // entries of copy_src and copy_dst
+  int32_t* n_copies;
+};
+hipError_t launch_compact_tables(const CompactTablesArgs& a, hipStream_t s);
+constexpr int kCopyCaches = 96;  // caches of a launch
+struct CopyPagesArgs {
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* count;  // pairs to copy, of n; null: all
+  int n, num_pages, n_caches;
+  uint8_t* base[kCopyCaches];
+  int64_t bytes[kCopyCaches];  // of a page
+};
+hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s);
+
 hipError_t launch_kv_write(const KvWriteArgs& a, hipStream_t s);
 // The writer of the 8-bit cache.
 hipError_t launch_kv_write_q8(const KvWriteArgs& a, hipStream_t s);

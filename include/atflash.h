@@ -71,6 +71,11 @@ extern "C" {
 #define ATF_MAX_GQA_GROUP 16
 #define ATF_Q8_MIN_EXP (-110)
 #define ATF_Q8_MAX_EXP 119
+#define ATF_LOGITS_BF16 0
+#define ATF_LOGITS_FP16 1
+#define ATF_LOGITS_FP32 2
+#define ATF_MAX_TOP 64                /* alternatives of atf_token_logprobs */
+#define ATF_MAX_SHARED_PAGES (1 << 19) /* pool of atf_select_tables and atf_compact_tables */
 
 enum {
   ATF_OK = 0,
@@ -269,6 +274,111 @@ int atf_extend_tables(int32_t* page_table, int max_pages, const int32_t* seq_len
  */
 int atf_release_tables(int32_t* page_table, int max_pages, int32_t* seq_lens, int32_t* free_pages, int num_free,
                        int32_t* free_count, const int32_t* rows, int n_rows, int batch, int num_pages, void* stream);
+
+/*
+ * RMS norm of each head's query and key rows and the rotation of their positions in one
+ * pass: y = x (mean(x^2) + eps)^-1/2 w over a row's 128 dims, then rotate-half RoPE of y by
+ * rope_cs at the row's position.  q and k are bf16 [rows][heads][128] (strides in
+ * elements, multiples of 8; last dim contiguous; 16-byte aligned), half-split; q_out and
+ * k_out bf16 [rows][heads][128], contiguous.  Weights [128], bf16 or fp32
+ * (weights_fp32), not needed where there are no heads.  positions: device int32 [rows].
+ * With rope_cs NULL rows are normed only.  A row whose position lies outside
+ * [0, rope_max_pos) is left as it is in the outputs.  fp32 throughout, one rounding.
+ */
+int atf_qk_norm_rope_bf16(void* q_out, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads,
+                          void* k_out, const void* k, int64_t k_st, int64_t k_sh, int num_k_heads,
+                          const void* q_weight, const void* k_weight, int weights_fp32, float eps,
+                          int rows, const int32_t* positions, const float* rope_cs, int rope_max_pos, void* stream);
+
+/*
+ * The same with the keys written, beside their values, into the paged cache: packed rows as
+ * atf_kv_write_packed_bf16's (sequence b's rows cu_tokens[b] .. cu_tokens[b + 1] - 1 at
+ * positions from start_pos[b] on), with its skips, into the bf16 cache (kv_exps NULL)
+ * or the cache of 8-bit floats, with atf_kv_write_q8's rules for pages.  q's rows are those
+ * of the same tokens, normed and rotated into q_out [total_tokens][num_q_heads][128]; those
+ * whose position is negative or past the RoPE table, and rows outside every sequence, are left as
+ * they are.  The keys are normed and rotated in fp32 and rounded once; q_out has the bits of
+ * atf_qk_norm_rope_bf16, and so have the bf16 cache's keys.  The attention then takes
+ * q_out with rope_cs NULL.  No counterpart in the reference.
+ */
+int atf_qk_norm_write(void* q_out, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads,
+                      void* kv_cache, int8_t* kv_exps, int num_pages, int num_kv_heads,
+                      const void* k_src, int64_t ks_t, int64_t ks_h, const void* v_src, int64_t vs_t, int64_t vs_h,
+                      const void* q_weight, const void* k_weight, int weights_fp32, float eps,
+                      int batch, const int32_t* cu_tokens, int total_tokens, int max_tokens,
+                      const int32_t* start_pos, const int32_t* page_table, int max_pages,
+                      const float* rope_cs, int rope_max_pos, void* stream);
+
+/*
+ * Log probabilities of given tokens, the entropy and the likeliest tokens of rows of logits
+ * (no counterpart in the reference).  logits: [rows][vocab] of logits_type (ATF_LOGITS_*), rows
+ * `stride` elements apart, any alignment.  With p = softmax of a row in natural logarithms:
+ *   logprobs     fp32 [rows][n_tokens]  log p of tokens[row][i] (device int64); 0 for a
+ *                                       negative token (padding), NaN for one past the vocabulary
+ *   entropy      fp32 [rows]            - sum p log p
+ *   top_ids      int64 [rows][top], top_logprobs fp32 [rows][top]: the `top` likeliest tokens, best
+ *                                       first, of equal logits the lowest id first
+ * top is at most ATF_MAX_TOP and at most vocab.  Logits of -inf have probability 0; a row of
+ * nothing else has log probabilities of -inf and entropy 0.  A NaN or +inf makes the row's log
+ * probabilities and entropy NaN; NaN rank below every number.  Sums are fp32.
+ *   The workspace (atf_logprobs_workspace_bytes; 0 for many rows) needs no initialisation; calls
+ * that share one must be ordered on one stream.
+ */
+size_t atf_logprobs_workspace_bytes(int rows, int vocab, int logits_type, int top);
+int atf_token_logprobs(float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                       const void* logits, int logits_type, int64_t stride, int rows, int vocab,
+                       const int64_t* tokens, int n_tokens, int top,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Forks, drops and a beam's choice on page tables: new row b is old row parents[b] (device
+ * int32 [batch]; outside [0, batch): an empty row).  Sequences then share pages.  Rows
+ * hold the pages of their tokens (entries past them mean nothing and come out as -1).
+ *   The parent's whole pages are named again.  Its last page, where the tokens fill it in part,
+ * stays with the parent if it is its own child, else with its lowest child; each other child
+ * takes a page from the end of the free pages for it, in the order of the rows, and
+ * copy_src[b], copy_dst[b] name the copy that is to be made in every layer's cache
+ * (atf_copy_pages; -1: none).  Before that the pages that no new row names are appended to the
+ * free pages, each once, the lowest id first.  So a page that is not full has one owner.
+ * Written:
+ *   table_out    [batch][max_pages], seq_lens_out [batch] (not the old ones)
+ *   free_pages   [num_free] in place, from *free_count on: the pages that became free
+ *   free_left    [1]  free pages left; negative: so many were missing, their entries are -1
+ *   copy_src, copy_dst [batch]
+ * The old table, its lengths and free_count are read only, so that a call can be repeated.
+ * Entries that are no page of the pool are named again as they are; the child of a last
+ * page that is none gets -1.  atf_release_tables knows nothing of shared pages: sequences
+ * of shared tables end here, with a parent of -1.  batch is at most 8191, batch * max_pages
+ * 2^30, num_pages ATF_MAX_SHARED_PAGES.  No counterpart in the reference.
+ */
+int atf_select_tables(int32_t* table_out, const int32_t* page_table, int max_pages, const int32_t* seq_lens,
+                      int32_t* free_pages, int num_free, const int32_t* free_count, const int32_t* parents, int batch,
+                      int num_pages, int32_t* seq_lens_out, int32_t* free_left, int32_t* copy_src, int32_t* copy_dst,
+                      void* stream);
+
+/*
+ * The pages of all rows moved to the front of the pool: with L pages in rows (shared ones
+ * once), the L lowest of the ids that rows or the free pages have become the rows'.  The i-th
+ * highest page that has to move goes to the i-th lowest free id: copy_src[i] to copy_dst[i],
+ * i < *n_copies, to be made in every layer's cache (atf_copy_pages); entries up to
+ * `copies` (at least num_pages / 2) are -1.  free_out: the free pages afterwards, highest first,
+ * *free_left of them, -1 behind; pages that are neither in a row nor free keep their place.  The
+ * inputs are read only.  Limits as atf_select_tables.  No counterpart in the reference.
+ */
+int atf_compact_tables(int32_t* table_out, const int32_t* page_table, int max_pages, const int32_t* seq_lens,
+                       int32_t* free_out, const int32_t* free_pages, int num_free, const int32_t* free_count,
+                       int batch, int num_pages, int32_t* free_left, int32_t* copy_src, int32_t* copy_dst, int copies,
+                       int32_t* n_copies, void* stream);
+
+/*
+ * Page dst[i] of each cache becomes a copy of its page src[i], i < *count (device; NULL: n), at
+ * most n: caches and page_bytes are HOST arrays of n_caches device pointers and the bytes of
+ * a page in each (of any type: K/V blocks, exponents), num_pages pages in every one.  Pairs with an entry
+ * outside [0, num_pages) are left out.  The pages that are written must be different, and none of
+ * them a source of the call.
+ */
+int atf_copy_pages(void* const* caches, const int64_t* page_bytes, int n_caches, int num_pages, const int32_t* src,
+                   const int32_t* dst, int n, const int32_t* count, void* stream);
 
 /*
  * Bytes of device workspace atf_decode_paged_bf16 needs for these sizes: the
