@@ -213,7 +213,7 @@ struct LogprobArgs {
   float* top_logprobs;  // [rows][top]
   int64_t* top_ids;     // [rows][top]
   int splits;        // workgroups of a row
-  float* ws_stats;   // [rows][splits][4]: largest logit, sum of exponentials, sum of (distance x exponential)
+  float* ws_stats;   // [rows][splits][4]: a split's sums and their reference
   uint64_t* ws_top;  // [rows][splits][top]: the split's best, best first
 };
 int logprob_splits(int rows, int vocab, int type, int top);

@@ -1,27 +1,33 @@
 // Log probabilities of given tokens, the entropy and the likeliest tokens of rows of logits.
 //
-// Mathematics.  One pass over a row x of V logits keeps, for each thread, m = the largest
-// so far, s = sum exp(x - m) and t = sum (x - m) exp(x - m), all fp32; two of them
-// join as s = s1 f1 + s2 f2, t = f1 (t1 + s1 (m1 - m)) + .., f = exp(m_i - m).  Then
-//   log p(i) = (x_i - m) - log s,   entropy = log s - t / s.
-// Logits of -inf count for nothing (0 in s and t); a row of nothing else has log
+// Mathematics.  One pass over a row x of V logits, in fp32 and powers of two: with u_i =
+// (x_i - m) log2 e, m a logit, every thread keeps s = sum 2^u and t = sum u 2^u.  m is a wave's:
+// its largest so far, give or take kSlack; when it is raised by d powers of two, s and t become
+// s f and f (t - s d), f = 2^-d.  Then
+//   log p(i) = x_i - m - log s,   entropy = (log2 s - t / s) / log2 e.
+//   Logits of -inf count for nothing (0 in s and t); a row of nothing else has log
 // probabilities of -inf and entropy 0.  NaN and +inf make the row's numbers NaN.
 //   The likeliest tokens in the same pass.  A logit and its place make one number of 64
-// bits, ordered as (value, lowest place first).  A chunk of the row stays in registers;
-// a wave takes the top-th largest of its lanes' best as a bound (so many are at least that
-// good), the workgroup the best bound of its waves and of the list so far, and only
-// what passes it, about `top` a row, goes through LDS to be ranked by counting.
+// bits, ordered as (value, lowest place first).  A wave keeps the best of what it has seen in
+// LDS and gives the others its q-th best, q = ceil(top / 8): each of the 8 waves has q that
+// reach the least of these, so that it is a bound, and 16 bytes of logits are looked at
+// closer only if their largest reaches it.  For the first chunk the q-th best of a
+// wave's lanes (each lane's largest) serve.
 //   Bound by HBM: every logit is read once.
+#include <type_traits>
+
 #include "atf_launch.h"
 
 namespace atf {
 
 constexpr int kLpThreads = 512;
 constexpr int kLpWaves = kLpThreads / 64;
-constexpr int kLpRoom = 2048;  // candidates ranked at a time
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kLpRoom = 256;    // candidates of a wave
+constexpr int kLpMerge = 2048;  // of a row's splits
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLowest = -3.402823466e+38f;
+constexpr float kSlack = 0.7f;  // a wave's m is raised for logits so far above it (2^u: 2 at most)
 
 template <int kType>
 struct LogitVec {  // 16 bytes of logits
@@ -43,40 +49,81 @@ struct LogitVec {  // 16 bytes of logits
 };
 
 // A value as 32 bits that are ordered as the values are; equal values (0 and -0) the same
-// bits, NaN below everything.
+// bits, NaN as -inf.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return x == x ? k : 0u;
+  return x == x ? k : 0x007fffffu;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);  // (0: a NaN)
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 __device__ __forceinline__ uint64_t entry_of(float x, uint32_t at) {
   return (static_cast<uint64_t>(order_key(x)) << 32) | (0xffffffffu - at);
 }
-__device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) {
-  const uint32_t lo = __shfl(static_cast<int>(x), lane), hi = __shfl(static_cast<int>(x >> 32), lane);
+__device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {  // of a lane that is the same for the wave
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), lane);
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
+__device__ __forceinline__ uint64_t max64(uint64_t x, uint64_t y) { return x > y ? x : y; }
+__device__ __forceinline__ uint64_t min64(uint64_t x, uint64_t y) { return x < y ? x : y; }
+
+// The largest of the wave's lanes, in every lane (unsigned 32 bits): maxima over rows of 16
+// lanes, then over the rows.
+__device__ __forceinline__ uint32_t wave_max32(uint32_t x) {
+  auto with = [](uint32_t v, int moved) { return max(v, static_cast<uint32_t>(moved)); };
+  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0xb1, 0xf, 0xf, true));   // lane ^ 1
+  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x4e, 0xf, 0xf, true));   // lane ^ 2
+  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x141, 0xf, 0xf, true));  // mirrored in 8
+  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x140, 0xf, 0xf, true));  // mirrored in 16
+  const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+  return max(max(a, b), max(c, d));
+}
 __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const uint32_t lo = __shfl_xor(static_cast<int>(x), m), hi = __shfl_xor(static_cast<int>(x >> 32), m);
-    const uint64_t y = (static_cast<uint64_t>(hi) << 32) | lo;
-    x = y > x ? y : x;
+  const uint32_t hi = wave_max32(static_cast<uint32_t>(x >> 32));
+  const uint32_t lo = wave_max32(static_cast<uint32_t>(x >> 32) == hi ? static_cast<uint32_t>(x) : 0u);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+// The n-th largest of the lanes' numbers (different ones but for zeros), 0 if there are fewer.
+__device__ __forceinline__ uint64_t wave_nth64(uint64_t x, int n) {
+  if (n <= 8) {
+    uint64_t y = 0;
+    for (int i = 0; i < n; ++i) {
+      y = wave_max64(x);
+      x = x == y ? 0 : x;
+    }
+    return y;
   }
-  return x;
+  int above = 0;
+#pragma unroll 8
+  for (int l = 0; l < 64; ++l) above += lane64(x, l) > x ? 1 : 0;
+  const uint64_t at = __builtin_amdgcn_ballot_w64(above == n - 1 && x != 0);
+  return at != 0 ? lane64(x, __builtin_ctzll(at)) : 0;
+}
+// The largest of three, not NaN if one is not.  (Of fmaxf the compiler makes one more instruction
+// an operand, which would quiet a signalling NaN.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// LDS that only one wave uses: its accesses before and after keep their order.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
+// s and t relative to m (-inf: nothing yet).
 struct LpStats {
   float m, s, t;
 };
-// The same sums relative to a maximum that is no smaller.
+// The same sums relative to a larger m.
 __device__ __forceinline__ void lp_raise(LpStats& a, float m) {
+  const float d = (m - a.m) * kLog2e, f = __builtin_amdgcn_exp2f(-d);
   if (a.s != 0.f) {
-    const float d = a.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
-    a.t = f == 0.f ? 0.f : f * __builtin_fmaf(a.s, d, a.t);  // (s d may pass fp32 where nothing is left of it)
+    a.t = f == 0.f ? 0.f : f * __builtin_fmaf(a.s, -d, a.t);  // (s d may pass fp32 where nothing is left of it)
     a.s *= f;
   }
   a.m = m;
@@ -88,16 +135,16 @@ __device__ __forceinline__ void lp_join(LpStats& a, LpStats b) {
   a.s += b.s;
   a.t += b.t;
 }
-__device__ __forceinline__ LpStats lp_wave(LpStats a) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) lp_join(a, LpStats{__shfl_xor(a.m, m), __shfl_xor(a.s, m), __shfl_xor(a.t, m)});
-  return a;
-}
 // log p of a logit x
-__device__ __forceinline__ float lp_of(const LpStats& a, float log_s, float x) {
-  const float d = x - a.m;
-  return x == kNegInf && a.s == a.s ? kNegInf : d - log_s;
+__device__ __forceinline__ float lp_of(const LpStats& a, float log2_s, float x) {
+  return x == kNegInf && a.s == a.s ? kNegInf : __builtin_fmaf(-log2_s, kLn2, x - a.m);
 }
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
 // The `top` best of n entries of `buf`, best first, to `out`; every thread of the workgroup.
 __device__ __forceinline__ void rank_entries(const uint64_t* buf, int n, int top, uint64_t* out, int threads) {
   for (int i = threadIdx.x; i < n; i += threads) {
@@ -108,84 +155,129 @@ __device__ __forceinline__ void rank_entries(const uint64_t* buf, int n, int top
   }
 }
 
+// What a wave has found: `len` entries in LDS, its `top` best among them.  Nothing below
+// `floor` is among the row's best.
+struct LpList {
+  uint64_t* buf;    // [kLpRoom]
+  uint64_t* given;  // the wave's q-th best, read by the others (q = 0: it gives none)
+  int len, top, q;
+  uint64_t floor;
+};
+__device__ __forceinline__ void lp_give(uint64_t* given, uint64_t x) {
+  __hip_atomic_store(given, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+// The least of what the waves have given by now (it only grows).
+__device__ __forceinline__ uint64_t lp_least(uint64_t* given) {
+  uint64_t x = ~0ull;
+#pragma unroll
+  for (int w = 0; w < kLpWaves; ++w)
+    x = min64(x, __hip_atomic_load(given + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+  return lane64(x, 0);
+}
+// Only the `top` best are kept, best first.
+__device__ __forceinline__ void lp_prune(LpList& a) {
+  const int lane = threadIdx.x & 63;
+  wave_fence();
+  if (a.len <= 64) {
+    const uint64_t x = lane < a.len ? a.buf[lane] : 0;
+    int above = 0;
+    for (int j = 0; j < a.len; ++j) above += lane64(x, j) > x ? 1 : 0;
+    if (lane < a.len && above < a.top) a.buf[above] = x;
+  } else {
+    uint64_t x[kLpRoom / 64];
+    int above[kLpRoom / 64];
+#pragma unroll
+    for (int i = 0; i < kLpRoom / 64; ++i) {
+      x[i] = 64 * i + lane < a.len ? a.buf[64 * i + lane] : 0;
+      above[i] = 0;
+    }
+    for (int j = 0; j < a.len; ++j) {
+      const uint64_t y = a.buf[j];
+#pragma unroll
+      for (int i = 0; i < kLpRoom / 64; ++i) above[i] += y > x[i] ? 1 : 0;
+    }
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < kLpRoom / 64; ++i)
+      if (64 * i + lane < a.len && above[i] < a.top) a.buf[above[i]] = x[i];
+  }
+  wave_fence();
+  a.len = min(a.len, a.top);
+  if (a.len == a.top) a.floor = max64(a.floor, lane64(a.buf[a.top - 1], 0));
+  if (a.q > 0 && a.len >= a.q && lane == 0) lp_give(a.given, a.buf[a.q - 1]);
+}
+// The lanes' entries that reach the floor (0: none) into the list.
+__device__ __forceinline__ void lp_push(LpList& a, uint64_t y) {
+  uint64_t mask = __builtin_amdgcn_ballot_w64(y != 0 && y >= a.floor);
+  if (a.len + __builtin_popcountll(mask) > kLpRoom) {
+    lp_prune(a);
+    mask = __builtin_amdgcn_ballot_w64(y != 0 && y >= a.floor);
+  }
+  const int at = a.len + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0u));
+  if (y != 0 && y >= a.floor) a.buf[at] = y;
+  a.len += __builtin_popcountll(mask);
+}
+
 // The outputs of a row from its sums and its list.
 template <int kType>
 __device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, const void* x, const LpStats& st,
                                          const uint64_t* list, int len, int threads) {
-  const float log_s = logf(st.s);
+  const float log2_s = log2f(st.s);
   for (int i = threadIdx.x; i < a.n_tokens; i += threads) {
     const int64_t at = static_cast<int64_t>(row) * a.n_tokens + i;
     const int64_t tok = a.tokens[at];
     a.logprobs[at] = tok < 0 ? 0.f
                      : tok >= a.vocab ? __uint_as_float(0x7fc00000u)
-                                      : lp_of(st, log_s, LogitVec<kType>::one(x, tok));
+                                      : lp_of(st, log2_s, LogitVec<kType>::one(x, tok));
   }
-  if (threadIdx.x == 0) a.entropy[row] = st.s == 0.f ? 0.f : log_s - st.t / st.s;
+  if (threadIdx.x == 0) a.entropy[row] = st.s == 0.f ? 0.f : (log2_s - st.t / st.s) * kLn2;
   for (int i = threadIdx.x; i < a.top; i += threads) {
     const uint64_t e = i < len ? list[i] : 0;
     const int64_t at = static_cast<int64_t>(row) * a.top + i;
     a.top_ids[at] = 0xffffffffu - static_cast<uint32_t>(e);
-    a.top_logprobs[at] = lp_of(st, log_s, key_value(static_cast<uint32_t>(e >> 32)));
+    a.top_logprobs[at] = lp_of(st, log2_s, key_value(static_cast<uint32_t>(e >> 32)));
   }
 }
 
 // One workgroup of 512 threads per (row, split): chunks of kVecs vectors of 16 bytes a
-// thread, split y takes chunks y, y + gridDim.y, ..  The few logits before the row's first
-// 16-byte boundary and behind its last are two more vectors, read one by one.
+// thread, split y takes chunks y, y + gridDim.y, ..  The waves go through them by
+// themselves; they meet at the end.  The few logits before the row's first 16-byte
+// boundary and behind its last are lanes of split 0's first wave.
 template <int kType, int kVecs, bool kTop>
-__global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobArgs a) {
   using V = LogitVec<kType>;
   constexpr int kE = V::kE;
-  __shared__ uint64_t buf[kTop ? kLpRoom : 1], list[kTopMax];
-  __shared__ uint64_t s_bound, s_wave[kLpWaves];
+  __shared__ uint64_t s_buf[kTop ? kLpWaves : 1][kTop ? kLpRoom : 1], s_all[kTop ? kLpWaves * kTopMax : 1], s_list[kTopMax];
+  __shared__ uint64_t s_given[kLpWaves];
   __shared__ int s_count;
   __shared__ LpStats s_stats[kLpWaves];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const char* x = static_cast<const char*>(a.logits) + static_cast<int64_t>(row) * a.stride * V::kBytes;
   const int head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / V::kBytes, a.vocab);
-  const int n_vec = (a.vocab - head) / kE;            // whole vectors
-  const int rest = a.vocab - head - n_vec * kE;       // logits behind them
-  const int n_all = n_vec + (rest > 0 ? 1 : 0) + (head > 0 ? 1 : 0);
+  const int n_vec = (a.vocab - head) / kE;       // whole vectors
+  const int rest = a.vocab - head - n_vec * kE;  // logits behind them
   const char* x0 = x + head * V::kBytes;
-  // the place of element 0 of vector j: the vectors, the rest, the head (its last elements)
-  auto place = [&](int j) {
-    return j < n_vec ? head + j * kE : (j == n_vec && rest > 0) ? head + n_vec * kE : head - kE;
-  };
-  auto edge = [&](int j) {
-    u32x4 v = {V::kFill, V::kFill, V::kFill, V::kFill};
-    if (j < n_all) {
-      const int at = place(j);
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const int i = at + e;
-        if (i >= 0 && i < a.vocab && (j == n_vec && rest > 0 ? true : i < head)) {
-          if constexpr (kType == kLogitsFp32) {
-            v[e] = reinterpret_cast<const uint32_t*>(x)[i];
-          } else {
-            const uint32_t h = reinterpret_cast<const uint16_t*>(x)[i];
-            v[e >> 1] = (e & 1) ? ((v[e >> 1] & 0x0000ffffu) | (h << 16)) : ((v[e >> 1] & 0xffff0000u) | h);
-          }
-        }
-      }
-    }
-    return v;
-  };
-  // whether element e of vector j is a logit of the row
-  auto real = [&](int j, int e) {
-    const int i = place(j) + e;
-    return j < n_vec || (j < n_all && i >= 0 && i < a.vocab && (j != n_vec || rest > 0 || i < head));
-  };
-
-  LpStats st{kNegInf, 0.f, 0.f};
-  uint64_t bound = 0;  // of the list: nothing below it is among the best
-  int len = 0;
-  if (kTop && tid == 0) {
-    s_count = 0;
-    s_bound = 0;
+  if (kTop) {
+    if (tid == 0) s_count = 0;
+    if (tid < kLpWaves) s_given[tid] = 0;
+    __syncthreads();
   }
-  if (kTop) __syncthreads();
+  LpStats st{kNegInf, 0.f, 0.f};  // (m is the wave's)
+  bool careful = false;           // the wave has seen logits of which (x - m) log2 e is -inf
+  LpList list{s_buf[kTop ? wave : 0], s_given + wave, 0, a.top, 0, 0};
+  if (blockIdx.y == 0 && wave == 0 && head + rest > 0) {
+    const int i = lane < 32 ? lane : a.vocab - rest + lane - 32;
+    const bool on = lane < 32 ? lane < head : lane - 32 < rest;
+    const float y = on ? V::one(x, i) : kNegInf;
+    st.m = key_value(wave_max32(order_key(y)));
+    const float u = (y - st.m) * kLog2e;
+    st.s = y == kNegInf ? 0.f : __builtin_amdgcn_exp2f(u);
+    st.t = st.s == 0.f ? 0.f : st.s * u;
+    if (kTop) lp_push(list, on ? entry_of(y, i) : 0);
+  }
   constexpr int kChunk = kLpThreads * kVecs;
-  for (int c0 = blockIdx.y * kChunk; c0 < n_all; c0 += gridDim.y * kChunk) {
+  for (int c0 = blockIdx.y * kChunk; c0 < n_vec; c0 += gridDim.y * kChunk) {
     u32x4 v[kVecs];
     if (c0 + kChunk <= n_vec) {
 #pragma unroll
@@ -194,131 +286,132 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
         const int j = c0 + k * kLpThreads + tid;
-        v[k] = j < n_vec ? ldg16(x0 + static_cast<int64_t>(j) * 16) : edge(j);
+        v[k] = ldg16(x0 + static_cast<int64_t>(min(j, n_vec - 1)) * 16);
+        if (j >= n_vec) v[k] = u32x4{V::kFill, V::kFill, V::kFill, V::kFill};
       }
     }
-    float cm = kNegInf;
+    float vm[kVecs];  // the vectors' largest
+    // The chunk's sums, a vector at a time.  The short way has a NaN in t where 2^u is 0 and u
+    // -inf (masked logits): the chunk is then done again with u held above -inf, and so are
+    // those after it.
+    auto sums = [&](auto hold) {
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k)
+      for (int k = 0; k < kVecs; ++k) {
+        float y[kE];
 #pragma unroll
-      for (int e = 0; e < kE; ++e) cm = fmaxf(cm, V::get(v[k], e));
-    if (cm > st.m) lp_raise(st, cm);
-    const float m = st.m == kNegInf ? 0.f : st.m;
+        for (int e = 0; e < kE; ++e) y[e] = V::get(v[k], e);
+        vm[k] = max3(y[0], y[1], y[kE - 1]);
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
+        for (int e = 2; e < kE - 1; e += 2) vm[k] = max3(vm[k], y[e], y[e + 1]);
+        if (__builtin_amdgcn_ballot_w64(vm[k] > st.m + kSlack) != 0) lp_raise(st, key_value(wave_max32(order_key(vm[k]))));
+        const float m = st.m == kNegInf ? 0.f : st.m;
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const float d = V::get(v[k], e) - m, p = __builtin_amdgcn_exp2f(d * kLog2e);
-        st.s += p;
-        st.t = __builtin_fmaf(p, fmaxf(d, kLowest), st.t);
+        for (int e = 0; e < kE; ++e) {
+          const float u = (y[e] - m) * kLog2e, p = __builtin_amdgcn_exp2f(u);
+          st.s += p;
+          st.t = __builtin_fmaf(p, decltype(hold)::value ? fmaxf(u, kLowest) : u, st.t);
+        }
+      }
+    };
+    if (!careful) {
+      const LpStats before = st;
+      sums(std::false_type{});
+      if (__builtin_amdgcn_ballot_w64(st.t != st.t) != 0) {
+        careful = true;
+        st = before;
+      }
+    }
+    if (careful) sums(std::true_type{});
+    float cm = vm[0];
+#pragma unroll
+    for (int k = 1; k < kVecs; ++k) cm = fmaxf(cm, vm[k]);
+    // The first chunk's bounds, from the waves whose lanes all have logits.
+    const int full = kTop && c0 == static_cast<int>(blockIdx.y) * kChunk ? min(kLpWaves, (n_vec - c0) / 64) : 0;
+    if constexpr (kTop) {
+      if (full > wave) {
+        list.q = (a.top + full - 1) / full;
+        int at = 0;  // the first place of the lane's largest (a NaN at the front counts as -inf)
+        u32x4 w = v[0];
+#pragma unroll
+        for (int k = kVecs - 1; k >= 0; --k) {
+          if (vm[k] == cm) {
+            at = k;
+            w = v[k];
+          }
+        }
+        int el = 0;
+#pragma unroll
+        for (int e = kE - 1; e >= 0; --e) el = V::get(w, e) == cm ? e : el;
+        const uint64_t nth = wave_nth64(entry_of(cm, head + (c0 + at * kLpThreads + tid) * kE + el), list.q);
+        if (lane == 0) lp_give(list.given, nth);
+      } else if (full > 0 && lane == 0) {
+        lp_give(list.given, ~0ull);
       }
     }
     if constexpr (kTop) {
-      const bool maybe = order_key(cm) >= static_cast<uint32_t>(bound >> 32);
-      uint64_t best = 0, limit = bound;
-      if (__builtin_amdgcn_ballot_w64(maybe) != 0) {
-        if (maybe) {
+      if (full > 0) __syncthreads();  // (uniform: a workgroup's first chunk)
+      list.floor = max64(list.floor, lp_least(s_given));
+      const float bar = list.floor == 0 ? kNegInf : key_value(static_cast<uint32_t>(list.floor >> 32));
+      if (__builtin_amdgcn_ballot_w64(!(cm < bar)) != 0) {
+        uint32_t todo = 0;  // vectors in which some lane has a candidate
 #pragma unroll
-          for (int k = 0; k < kVecs; ++k) {
-            const int j = c0 + k * kLpThreads + tid;
+        for (int k = 0; k < kVecs; ++k) todo |= __builtin_amdgcn_ballot_w64(!(vm[k] < bar)) != 0 ? 1u << k : 0u;
+        const int had = list.len;
+        while (todo != 0) {
+          const int k = __builtin_ctz(todo);
+          todo &= todo - 1;
+          u32x4 w = v[0];
 #pragma unroll
-            for (int e = 0; e < kE; ++e) {
-              const uint64_t y = real(j, e) ? entry_of(V::get(v[k], e), place(j) + e) : 0;
-              best = y > best ? y : best;
-            }
-          }
-        }
-        const uint64_t over = __builtin_amdgcn_ballot_w64(best > bound);
-        if (__builtin_popcountll(over) >= a.top) {  // the top-th best lane: a bound
-          int above = 0;
-          for (int l = 0; l < 64; ++l) above += shfl64(best, l) > best ? 1 : 0;
-          const uint64_t at = __builtin_amdgcn_ballot_w64(above == a.top - 1 && best > bound);
-          if (at != 0) {
-            limit = shfl64(best, __builtin_ctzll(at));
-            if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&s_bound), limit);
-          }
-        }
-      }
-      __syncthreads();
-      limit = s_bound > bound ? s_bound : bound;
-      if (best >= limit && best > bound) {
+          for (int i = 1; i < kVecs; ++i)
+            if (i == k) w = v[i];
+          uint32_t some = 0;  // elements
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k) {
+          for (int e = 0; e < kE; ++e) some |= __builtin_amdgcn_ballot_w64(!(V::get(w, e) < bar)) != 0 ? 1u << e : 0u;
           const int j = c0 + k * kLpThreads + tid;
+          while (some != 0) {
+            const int e = __builtin_ctz(some);
+            some &= some - 1;
+            float y = V::get(w, 0);
 #pragma unroll
-          for (int e = 0; e < kE; ++e) {
-            const uint64_t y = real(j, e) ? entry_of(V::get(v[k], e), place(j) + e) : 0;
-            if (y >= limit && y > bound) {
-              const int at = len + atomicAdd(&s_count, 1);
-              if (at < kLpRoom) buf[at] = y;
-            }
+            for (int i = 1; i < kE; ++i)
+              if (i == e) y = V::get(w, i);
+            lp_push(list, j < n_vec ? entry_of(y, head + j * kE + e) : 0);
           }
         }
-      }
-      __syncthreads();
-      const int fresh = s_count;
-      if (fresh > 0) {  // (uniform)
-        int n = len + fresh;
-        if (n <= kLpRoom) {
-          rank_entries(buf, n, a.top, list, kLpThreads);
-          n = min(n, a.top);
-        } else {
-          // More candidates than room (a thread's chunk holds many of the best): one by one.
-          uint64_t last = ~0ull;
-          for (n = 0; n < a.top; ++n) {
-            uint64_t y = tid < len && buf[tid] < last ? buf[tid] : 0;
-#pragma unroll
-            for (int k = 0; k < kVecs; ++k) {
-              const int j = c0 + k * kLpThreads + tid;
-#pragma unroll
-              for (int e = 0; e < kE; ++e) {
-                const uint64_t z = real(j, e) ? entry_of(V::get(v[k], e), place(j) + e) : 0;
-                y = z < last && z > y ? z : y;
-              }
-            }
-            y = wave_max64(y);
-            if (lane == 0) s_wave[wave] = y;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kLpWaves; ++w) y = s_wave[w] > y ? s_wave[w] : y;
-            __syncthreads();
-            if (y == 0) break;
-            if (tid == 0) list[n] = y;
-            last = y;
-          }
-        }
-        __syncthreads();
-        for (int i = tid; i < n; i += kLpThreads) buf[i] = list[i];
-        len = n;
-        bound = n == a.top ? list[n - 1] : 0;
-        if (tid == 0) {
-          s_count = 0;
-          s_bound = bound;
-        }
-        __syncthreads();
+        if (list.len > had) lp_prune(list);
       }
     }
   }
-  st = lp_wave(st);
+  st.s = wave_sum(st.s);
+  st.t = wave_sum(st.t);
   if (lane == 0) s_stats[wave] = st;
+  if constexpr (kTop) lp_prune(list);
   __syncthreads();
+  if constexpr (kTop) {
+    const uint64_t y = lane < list.len ? list.buf[lane] : 0;
+    if (y != 0 && y >= lp_least(s_given)) s_all[atomicAdd(&s_count, 1)] = y;
+    __syncthreads();
+    rank_entries(s_all, s_count, a.top, s_list, kLpThreads);
+    __syncthreads();
+  }
+  const int len = kTop ? min(s_count, a.top) : 0;
   st = s_stats[0];
 #pragma unroll
   for (int w = 1; w < kLpWaves; ++w) lp_join(st, s_stats[w]);
   if (gridDim.y == 1) {
-    lp_write<kType>(a, row, x, st, buf, len, kLpThreads);
+    lp_write<kType>(a, row, x, st, s_list, len, kLpThreads);
     return;
   }
   const int64_t part = static_cast<int64_t>(row) * gridDim.y + blockIdx.y;
   if (tid == 0) *reinterpret_cast<f32x4*>(a.ws_stats + 4 * part) = f32x4{st.m, st.s, st.t, 0.f};
-  if (tid < a.top) a.ws_top[part * a.top + tid] = tid < len ? buf[tid] : 0;
+  if (tid < a.top) a.ws_top[part * a.top + tid] = tid < len ? s_list[tid] : 0;
 }
 
 // The splits of a row joined: one workgroup a row.
 constexpr int kLpMergeThreads = 256;
 template <int kType>
 __global__ __launch_bounds__(kLpMergeThreads) void logprobs_merge_kernel(LogprobArgs a) {
-  __shared__ uint64_t buf[kLpRoom], list[kTopMax];
+  __shared__ uint64_t buf[kLpMerge], list[kTopMax];
   __shared__ int s_count;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int64_t part = static_cast<int64_t>(row) * a.splits;
@@ -333,7 +426,8 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprobs_merge_kernel(Logprob
       bound = y > bound ? y : bound;
     }
   }
-  st = lp_wave(st);
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) lp_join(st, LpStats{__shfl_xor(st.m, m), __shfl_xor(st.s, m), __shfl_xor(st.t, m)});
   bound = wave_max64(bound);
   __syncthreads();
   for (int i = tid; i < a.splits * a.top; i += kLpMergeThreads) {
@@ -356,7 +450,7 @@ int logprob_splits(int rows, int vocab, int type, int top) {
   const int64_t bytes = static_cast<int64_t>(vocab) * (type == kLogitsFp32 ? 4 : 2);
   int64_t n = (bytes + 16 * kLpThreads * kLpVecsSplit - 1) / (16 * kLpThreads * kLpVecsSplit);
   if (rows > 0 && n > 512 / rows) n = 512 / rows;
-  if (top > 0 && n > kLpRoom / top) n = kLpRoom / top;
+  if (top > 0 && n > kLpMerge / top) n = kLpMerge / top;
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
