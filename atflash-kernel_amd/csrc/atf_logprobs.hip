@@ -159,19 +159,20 @@ __device__ __forceinline__ void rank_entries(const uint64_t* buf, int n, int top
 // `floor` is among the row's best.
 struct LpList {
   uint64_t* buf;    // [kLpRoom]
-  uint64_t* given;  // the wave's q-th best, read by the others (q = 0: it gives none)
+  uint64_t* given;  // [kLpWaves] each wave's q-th best (a wave with q = 0 gives none)
+  unsigned long long* shared;  // the largest floor that a wave has found
   int len, top, q;
   uint64_t floor;
 };
-__device__ __forceinline__ void lp_give(uint64_t* given, uint64_t x) {
-  __hip_atomic_store(given, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-}
-// The least of what the waves have given by now (it only grows).
-__device__ __forceinline__ uint64_t lp_least(uint64_t* given) {
-  uint64_t x = ~0ull;
+// The least of what the waves have given (it only grows): lane w looks at wave w's.
+__device__ __forceinline__ uint64_t lp_least(const uint64_t* given) {
+  static_assert(kLpWaves == 8, "three exchanges below");
+  uint64_t x = __hip_atomic_load(given + (threadIdx.x & 7), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 #pragma unroll
-  for (int w = 0; w < kLpWaves; ++w)
-    x = min64(x, __hip_atomic_load(given + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+  for (int m = 1; m < 8; m <<= 1) {
+    const uint32_t lo = __shfl_xor(static_cast<int>(x), m), hi = __shfl_xor(static_cast<int>(x >> 32), m);
+    x = min64(x, (static_cast<uint64_t>(hi) << 32) | lo);
+  }
   return lane64(x, 0);
 }
 // Only the `top` best are kept, best first.
@@ -203,8 +204,13 @@ __device__ __forceinline__ void lp_prune(LpList& a) {
   }
   wave_fence();
   a.len = min(a.len, a.top);
-  if (a.len == a.top) a.floor = max64(a.floor, lane64(a.buf[a.top - 1], 0));
-  if (a.q > 0 && a.len >= a.q && lane == 0) lp_give(a.given, a.buf[a.q - 1]);
+  if (a.q > 0 && a.len >= a.q) {
+    if (lane == 0) __hip_atomic_store(a.given + (threadIdx.x >> 6), a.buf[a.q - 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    wave_fence();
+    a.floor = max64(a.floor, lp_least(a.given));
+  }
+  if (a.len == a.top) a.floor = max64(a.floor, lane64(a.buf[a.top - 1], 0));  // one wave's `top` best are as good a bound
+  if (lane == 0) atomicMax(a.shared, a.floor);
 }
 // The lanes' entries that reach the floor (0: none) into the list.
 __device__ __forceinline__ void lp_push(LpList& a, uint64_t y) {
@@ -250,6 +256,7 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
   constexpr int kE = V::kE;
   __shared__ uint64_t s_buf[kTop ? kLpWaves : 1][kTop ? kLpRoom : 1], s_all[kTop ? kLpWaves * kTopMax : 1], s_list[kTopMax];
   __shared__ uint64_t s_given[kLpWaves];
+  __shared__ unsigned long long s_floor;
   __shared__ int s_count;
   __shared__ LpStats s_stats[kLpWaves];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -259,13 +266,16 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
   const int rest = a.vocab - head - n_vec * kE;  // logits behind them
   const char* x0 = x + head * V::kBytes;
   if (kTop) {
-    if (tid == 0) s_count = 0;
+    if (tid == 0) {
+      s_count = 0;
+      s_floor = 0;
+    }
     if (tid < kLpWaves) s_given[tid] = 0;
     __syncthreads();
   }
   LpStats st{kNegInf, 0.f, 0.f};  // (m is the wave's)
   bool careful = false;           // the wave has seen logits of which (x - m) log2 e is -inf
-  LpList list{s_buf[kTop ? wave : 0], s_given + wave, 0, a.top, 0, 0};
+  LpList list{s_buf[kTop ? wave : 0], s_given, &s_floor, 0, a.top, 0, 0};
   if (blockIdx.y == 0 && wave == 0 && head + rest > 0) {
     const int i = lane < 32 ? lane : a.vocab - rest + lane - 32;
     const bool on = lane < 32 ? lane < head : lane - 32 < rest;
@@ -277,19 +287,22 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
     if (kTop) lp_push(list, on ? entry_of(y, i) : 0);
   }
   constexpr int kChunk = kLpThreads * kVecs;
-  for (int c0 = blockIdx.y * kChunk; c0 < n_vec; c0 += gridDim.y * kChunk) {
-    u32x4 v[kVecs];
+  auto load = [&](int c0, u32x4 (&to)[kVecs]) {
     if (c0 + kChunk <= n_vec) {
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) v[k] = ldg16(x0 + static_cast<int64_t>(c0 + k * kLpThreads + tid) * 16);
+      for (int k = 0; k < kVecs; ++k) to[k] = ldg16(x0 + 16 * static_cast<uint32_t>(c0 + k * kLpThreads + tid));
     } else {
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
         const int j = c0 + k * kLpThreads + tid;
-        v[k] = ldg16(x0 + static_cast<int64_t>(min(j, n_vec - 1)) * 16);
-        if (j >= n_vec) v[k] = u32x4{V::kFill, V::kFill, V::kFill, V::kFill};
+        to[k] = ldg16(x0 + 16 * static_cast<uint32_t>(min(j, n_vec - 1)));
+        if (j >= n_vec) to[k] = u32x4{V::kFill, V::kFill, V::kFill, V::kFill};
       }
     }
+  };
+  for (int c0 = blockIdx.y * kChunk; c0 < n_vec; c0 += gridDim.y * kChunk) {
+    u32x4 v[kVecs];
+    load(c0, v);
     float vm[kVecs];  // the vectors' largest
     // The chunk's sums, a vector at a time.  The short way has a NaN in t where 2^u is 0 and u
     // -inf (masked logits): the chunk is then done again with u held above -inf, and so are
@@ -305,11 +318,13 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
         for (int e = 2; e < kE - 1; e += 2) vm[k] = max3(vm[k], y[e], y[e + 1]);
         if (__builtin_amdgcn_ballot_w64(vm[k] > st.m + kSlack) != 0) lp_raise(st, key_value(wave_max32(order_key(vm[k]))));
         const float m = st.m == kNegInf ? 0.f : st.m;
+        if (c0 + k * kLpThreads + tid < n_vec) {
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const float u = (y[e] - m) * kLog2e, p = __builtin_amdgcn_exp2f(u);
-          st.s += p;
-          st.t = __builtin_fmaf(p, decltype(hold)::value ? fmaxf(u, kLowest) : u, st.t);
+          for (int e = 0; e < kE; ++e) {
+            const float u = (y[e] - m) * kLog2e, p = __builtin_amdgcn_exp2f(u);
+            st.s += p;
+            st.t = __builtin_fmaf(p, decltype(hold)::value ? fmaxf(u, kLowest) : u, st.t);
+          }
         }
       }
     };
@@ -343,14 +358,18 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
 #pragma unroll
         for (int e = kE - 1; e >= 0; --e) el = V::get(w, e) == cm ? e : el;
         const uint64_t nth = wave_nth64(entry_of(cm, head + (c0 + at * kLpThreads + tid) * kE + el), list.q);
-        if (lane == 0) lp_give(list.given, nth);
+        if (lane == 0) s_given[wave] = nth;
+        if (a.top == 1 && lane == 0) atomicMax(&s_floor, nth);
       } else if (full > 0 && lane == 0) {
-        lp_give(list.given, ~0ull);
+        s_given[wave] = ~0ull;
       }
     }
     if constexpr (kTop) {
-      if (full > 0) __syncthreads();  // (uniform: a workgroup's first chunk)
-      list.floor = max64(list.floor, lp_least(s_given));
+      if (full > 0) {  // (uniform: a workgroup's first chunk)
+        __syncthreads();
+        list.floor = max64(list.floor, lp_least(s_given));
+      }
+      list.floor = max64(list.floor, lane64(__hip_atomic_load(&s_floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP), 0));
       const float bar = list.floor == 0 ? kNegInf : key_value(static_cast<uint32_t>(list.floor >> 32));
       if (__builtin_amdgcn_ballot_w64(!(cm < bar)) != 0) {
         uint32_t todo = 0;  // vectors in which some lane has a candidate
@@ -385,21 +404,37 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
   st.s = wave_sum(st.s);
   st.t = wave_sum(st.t);
   if (lane == 0) s_stats[wave] = st;
-  if constexpr (kTop) lp_prune(list);
-  __syncthreads();
   if constexpr (kTop) {
-    const uint64_t y = lane < list.len ? list.buf[lane] : 0;
-    if (y != 0 && y >= lp_least(s_given)) s_all[atomicAdd(&s_count, 1)] = y;
-    __syncthreads();
+    const uint64_t floor = max64(list.floor, lane64(__hip_atomic_load(&s_floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP), 0));
+    for (int i = lane; i < list.len; i += 64) {
+      const uint64_t y = list.buf[i];
+      if (y >= floor) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kLpRoom) s_all[at] = y;
+      }
+    }
+  }
+  __syncthreads();
+  int len = 0;
+  if constexpr (kTop) {
+    if (s_count > kLpRoom) {  // (uniform) more than there is room for: each wave's best first
+      lp_prune(list);
+      __syncthreads();
+      if (tid == 0) s_count = 0;
+      __syncthreads();
+      if (lane < list.len) s_all[atomicAdd(&s_count, 1)] = list.buf[lane];
+      __syncthreads();
+    }
+    len = min(s_count, a.top);
     rank_entries(s_all, s_count, a.top, s_list, kLpThreads);
     __syncthreads();
   }
-  const int len = kTop ? min(s_count, a.top) : 0;
-  st = s_stats[0];
+  if (wave > 0) return;
+  st = s_stats[lane & 7];
 #pragma unroll
-  for (int w = 1; w < kLpWaves; ++w) lp_join(st, s_stats[w]);
+  for (int m = 1; m < kLpWaves; m <<= 1) lp_join(st, LpStats{__shfl_xor(st.m, m), __shfl_xor(st.s, m), __shfl_xor(st.t, m)});
   if (gridDim.y == 1) {
-    lp_write<kType>(a, row, x, st, s_list, len, kLpThreads);
+    lp_write<kType>(a, row, x, st, s_list, len, 64);
     return;
   }
   const int64_t part = static_cast<int64_t>(row) * gridDim.y + blockIdx.y;
