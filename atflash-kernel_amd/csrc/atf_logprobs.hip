@@ -372,59 +372,45 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
       list.floor = max64(list.floor, lane64(__hip_atomic_load(&s_floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP), 0));
       const float bar = list.floor == 0 ? kNegInf : key_value(static_cast<uint32_t>(list.floor >> 32));
       if (__builtin_amdgcn_ballot_w64(!(cm < bar)) != 0) {
-        uint32_t todo = 0;  // vectors in which some lane has a candidate
+        // every lane takes its first vector with a candidate, of that the first candidate, then the
+        // next, until no lane has one left
+        uint32_t vectors = 0;
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k) todo |= __builtin_amdgcn_ballot_w64(!(vm[k] < bar)) != 0 ? 1u << k : 0u;
-        const int had = list.len;
-        while (todo != 0) {
-          const int k = __builtin_ctz(todo);
-          todo &= todo - 1;
+        for (int k = 0; k < kVecs; ++k)
+          vectors |= !(vm[k] < bar) && c0 + k * kLpThreads + tid < n_vec ? 1u << k : 0u;
+        while (__builtin_amdgcn_ballot_w64(vectors != 0) != 0) {
+          const int k = vectors != 0 ? __builtin_ctz(vectors) : 0;
           u32x4 w = v[0];
 #pragma unroll
-          for (int i = 1; i < kVecs; ++i)
-            if (i == k) w = v[i];
-          uint32_t some = 0;  // elements
+          for (int i = 1; i < kVecs; ++i) w = k == i ? v[i] : w;
+          uint32_t some = 0;
 #pragma unroll
-          for (int e = 0; e < kE; ++e) some |= __builtin_amdgcn_ballot_w64(!(V::get(w, e) < bar)) != 0 ? 1u << e : 0u;
-          const int j = c0 + k * kLpThreads + tid;
-          while (some != 0) {
-            const int e = __builtin_ctz(some);
-            some &= some - 1;
+          for (int e = 0; e < kE; ++e) some |= V::get(w, e) < bar ? 0u : 1u << e;
+          if (vectors == 0) some = 0;
+          vectors &= vectors - 1;
+          const int at = head + (c0 + k * kLpThreads + tid) * kE;
+          while (__builtin_amdgcn_ballot_w64(some != 0) != 0) {
+            const int e = some != 0 ? __builtin_ctz(some) : 0;
             float y = V::get(w, 0);
 #pragma unroll
-            for (int i = 1; i < kE; ++i)
-              if (i == e) y = V::get(w, i);
-            lp_push(list, j < n_vec ? entry_of(y, head + j * kE + e) : 0);
+            for (int i = 1; i < kE; ++i) y = e == i ? V::get(w, i) : y;
+            lp_push(list, some != 0 ? entry_of(y, at + e) : 0);
+            some &= some - 1;
           }
         }
-        if (list.len > had) lp_prune(list);
+        if (full > 0) lp_prune(list);  // (later chunks add little: what they do is put in order when the room ends)
       }
     }
   }
+  if constexpr (kTop) lp_prune(list);
   st.s = wave_sum(st.s);
   st.t = wave_sum(st.t);
   if (lane == 0) s_stats[wave] = st;
-  if constexpr (kTop) {
-    const uint64_t floor = max64(list.floor, lane64(__hip_atomic_load(&s_floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP), 0));
-    for (int i = lane; i < list.len; i += 64) {
-      const uint64_t y = list.buf[i];
-      if (y >= floor) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < kLpRoom) s_all[at] = y;
-      }
-    }
-  }
   __syncthreads();
   int len = 0;
   if constexpr (kTop) {
-    if (s_count > kLpRoom) {  // (uniform) more than there is room for: each wave's best first
-      lp_prune(list);
-      __syncthreads();
-      if (tid == 0) s_count = 0;
-      __syncthreads();
-      if (lane < list.len) s_all[atomicAdd(&s_count, 1)] = list.buf[lane];
-      __syncthreads();
-    }
+    if (lane < list.len && list.buf[lane] >= s_floor) s_all[atomicAdd(&s_count, 1)] = list.buf[lane];
+    __syncthreads();
     len = min(s_count, a.top);
     rank_entries(s_all, s_count, a.top, s_list, kLpThreads);
     __syncthreads();
