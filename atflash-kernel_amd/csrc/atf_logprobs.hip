@@ -20,7 +20,7 @@
 
 namespace atf {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / 64;
 constexpr int kLpRoom = 256;    // candidates of a wave
 constexpr int kLpMerge = 2048;  // of a row's splits
@@ -166,10 +166,9 @@ struct LpList {
 };
 // The least of what the waves have given (it only grows): lane w looks at wave w's.
 __device__ __forceinline__ uint64_t lp_least(const uint64_t* given) {
-  static_assert(kLpWaves == 8, "three exchanges below");
-  uint64_t x = __hip_atomic_load(given + (threadIdx.x & 7), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  uint64_t x = __hip_atomic_load(given + (threadIdx.x & (kLpWaves - 1)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 #pragma unroll
-  for (int m = 1; m < 8; m <<= 1) {
+  for (int m = 1; m < kLpWaves; m <<= 1) {
     const uint32_t lo = __shfl_xor(static_cast<int>(x), m), hi = __shfl_xor(static_cast<int>(x >> 32), m);
     x = min64(x, (static_cast<uint64_t>(hi) << 32) | lo);
   }
@@ -246,7 +245,7 @@ __device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, const vo
   }
 }
 
-// One workgroup of 512 threads per (row, split): chunks of kVecs vectors of 16 bytes a
+// One workgroup of 256 threads per (row, split): chunks of kVecs vectors of 16 bytes a
 // thread, split y takes chunks y, y + gridDim.y, ..  The waves go through them by
 // themselves; they meet at the end.  The few logits before the row's first 16-byte
 // boundary and behind its last are lanes of split 0's first wave.
@@ -416,7 +415,7 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
     __syncthreads();
   }
   if (wave > 0) return;
-  st = s_stats[lane & 7];
+  st = s_stats[lane & (kLpWaves - 1)];
 #pragma unroll
   for (int m = 1; m < kLpWaves; m <<= 1) lp_join(st, LpStats{__shfl_xor(st.m, m), __shfl_xor(st.s, m), __shfl_xor(st.t, m)});
   if (gridDim.y == 1) {
@@ -463,30 +462,25 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprobs_merge_kernel(Logprob
   lp_write<kType>(a, row, x, st, list, min(n, a.top), kLpMergeThreads);
 }
 
-constexpr int kLpVecs = 8, kLpVecsSplit = 2;  // vectors of a thread's chunk: rows whole, rows split
+// Vectors of a thread's chunk, with alternatives and without.
+constexpr int kLpVecsTop = 8, kLpVecsSums = 4;
 
-// Workgroups of a row: two a CU for all rows together, a chunk of 16 KB each at least, and no
-// more than the merge has room for.
+// Workgroups of a row: four a CU for all rows together, a chunk each at least, and no more than
+// the merge has room for.
 int logprob_splits(int rows, int vocab, int type, int top) {
   const int64_t bytes = static_cast<int64_t>(vocab) * (type == kLogitsFp32 ? 4 : 2);
-  int64_t n = (bytes + 16 * kLpThreads * kLpVecsSplit - 1) / (16 * kLpThreads * kLpVecsSplit);
-  if (rows > 0 && n > 512 / rows) n = 512 / rows;
+  const int64_t chunk = 16 * kLpThreads * (top > 0 ? kLpVecsTop : kLpVecsSums);
+  int64_t n = (bytes + chunk - 1) / chunk;
+  if (rows > 0 && n > 1024 / rows) n = 1024 / rows;
   if (top > 0 && n > kLpMerge / top) n = kLpMerge / top;
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
 template <int kType>
 static void launch_logprobs(const LogprobArgs& a, hipStream_t s) {
-  const dim3 grid(a.rows, a.splits), block(kLpThreads);
-  if (a.splits == 1) {
-    hipLaunchKernelGGL(a.top > 0 ? (token_logprobs_kernel<kType, kLpVecs, true>) : (token_logprobs_kernel<kType, kLpVecs, false>),
-                       grid, block, 0, s, a);
-  } else {
-    hipLaunchKernelGGL(a.top > 0 ? (token_logprobs_kernel<kType, kLpVecsSplit, true>)
-                                 : (token_logprobs_kernel<kType, kLpVecsSplit, false>),
-                       grid, block, 0, s, a);
-    hipLaunchKernelGGL(logprobs_merge_kernel<kType>, dim3(a.rows), dim3(kLpMergeThreads), 0, s, a);
-  }
+  hipLaunchKernelGGL(a.top > 0 ? (token_logprobs_kernel<kType, kLpVecsTop, true>) : (token_logprobs_kernel<kType, kLpVecsSums, false>),
+                     dim3(a.rows, a.splits), dim3(kLpThreads), 0, s, a);
+  if (a.splits > 1) hipLaunchKernelGGL(logprobs_merge_kernel<kType>, dim3(a.rows), dim3(kLpMergeThreads), 0, s, a);
 }
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t s) {
