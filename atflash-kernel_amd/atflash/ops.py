@@ -60,6 +60,7 @@ package's own entry points use them.
 """
 import ctypes
 import math
+import operator
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -671,6 +672,10 @@ def _(page_table, seq_lens, free_pages, free_count, num_pages):
             seq_lens.new_empty(half), seq_lens.new_empty(1))
 
 
+_shape, _nbytes = operator.attrgetter("shape"), operator.attrgetter("nbytes")
+_data_ptr, _is_contiguous, _get_device = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
+
+
 def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor,
                count: Optional[torch.Tensor] = None) -> None:
     """Page dst[i] of every cache becomes a copy of its page src[i] (int32 [n]; pairs with an
@@ -680,23 +685,24 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
     that are written must be different, and none of them a source of the call."""
     if len(caches) == 0:
         return
-    n = src.numel()
-    dev = _one_device(caches[0], src, dst, count, *caches)
+    dev = _one_device(src, dst, count)
+    n = src.shape[0] if src.dim() == 1 else -1
     _check_ints(src, n, "src")
     _check_ints(dst, n, "dst")
     if count is not None:
         _check_ints(count, 1, "count")
-    pool = caches[0].shape[0] if caches[0].dim() else 0
-    bases, sizes = [], []
-    for c in caches:
-        if c.dim() < 1 or c.shape[0] != pool or not c.is_contiguous():
-            raise ValueError("caches must be contiguous [num_pages, ...] tensors of one pool")
-        bases.append(c.data_ptr())
-        sizes.append(c.nbytes // pool if pool else 0)
+    # (a model's caches are many: each check over all of them at once)
+    shapes = list(map(_shape, caches))
+    pool = shapes[0][0] if shapes[0] else -1
+    if not (all(s and s[0] == pool for s in shapes) and all(map(_is_contiguous, caches))
+            and set(map(_get_device, caches)) == {dev}):
+        raise ValueError("caches must be contiguous [num_pages, ...] tensors of one pool, on the device of the pairs")
     if pool == 0:
         return
-    _lib.launch(dev, _lib.lib().atf_copy_pages, (ctypes.c_void_p * len(bases))(*bases),
-                (ctypes.c_int64 * len(sizes))(*sizes), len(bases), pool, src.data_ptr(), dst.data_ptr(), n, _lib.ptr(count))
+    bases, sizes = list(map(_data_ptr, caches)), [x // pool for x in map(_nbytes, caches)]
+    m = len(bases)
+    _lib.launch(dev, _lib.lib().atf_copy_pages, (ctypes.c_void_p * m)(*bases), (ctypes.c_int64 * m)(*sizes), m, pool,
+                src.data_ptr(), dst.data_ptr(), n, _lib.ptr(count))
 
 
 def _copy_pages_schema(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor,
@@ -805,6 +811,9 @@ def _(kv_cache, kv_exps, q, k, v, q_weight, k_weight, eps, cu_seqlens, max_token
 
 # ---- log probabilities ----
 
+_LOGPROB_BYTES = {}  # (rows, vocab, type, top) -> workspace bytes of atf_token_logprobs
+
+
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0
                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """What rows of logits [R, V] (bf16, fp16 or fp32, any row stride) say: log probabilities
@@ -817,23 +826,32 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     kind = _lib.LOGIT_TYPES.get(logits.dtype)
     if kind is None or logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits must be bf16, fp16 or fp32 [rows, vocab], the last dim contiguous")
-    R, V = (_i32(x, "rows and vocab") for x in logits.shape)
+    R, V = logits.shape
     top = int(top)
     if not 0 <= top <= min(_lib.MAX_TOP, V):
         raise ValueError(f"top must be between 0 and {min(_lib.MAX_TOP, V)}, got {top}")
     _need(R == 0 or V > 0, "a row needs at least one logit")
+    _need(R < 2 ** 31 and V < 2 ** 31, "rows and vocab must fit 32 bits")
+    entropy = logits.new_empty(R, dtype=torch.float32)
     n = 0
-    if tokens is not None:
-        if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != R or not tokens.is_contiguous():
+    if tokens is None:
+        logp, ids = entropy.new_empty((R, 0)), logits.new_empty((R, top), dtype=torch.int64)
+    else:
+        s = tokens.shape
+        if tokens.dtype != torch.int64 or len(s) not in (1, 2) or s[0] != R or not tokens.is_contiguous():
             raise ValueError("tokens must be contiguous int64 [rows] or [rows, n]")
-        n = tokens.numel() // R if R else 0
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    logp = torch.empty((R, 0) if tokens is None else tokens.shape, **f32)
-    entropy, values = torch.empty(R, **f32), torch.empty((R, top), **f32)
-    ids = torch.empty((R, top), dtype=torch.int64, device=logits.device)
+        n = s[1] if len(s) == 2 else 1
+        _need(n < 2 ** 31, "tokens of a row must fit 32 bits")
+        logp, ids = entropy.new_empty(s), tokens.new_empty((R, top))
+    values = entropy.new_empty((R, top))
     L = _lib.lib()
-    nbytes = int(L.atf_logprobs_workspace_bytes(R, V, kind, top))
-    ws = torch.empty(nbytes // 4, **f32) if nbytes else None
+    shape = (R, V, kind, top)
+    nbytes = _LOGPROB_BYTES.get(shape)
+    if nbytes is None:
+        if len(_LOGPROB_BYTES) >= 4096:
+            _LOGPROB_BYTES.clear()
+        nbytes = _LOGPROB_BYTES[shape] = int(L.atf_logprobs_workspace_bytes(*shape))
+    ws = entropy.new_empty(nbytes // 4) if nbytes else None
     _lib.launch(dev, L.atf_token_logprobs, logp.data_ptr(), entropy.data_ptr(), values.data_ptr(), ids.data_ptr(),
                 logits.data_ptr(), kind, logits.stride(0), R, V, _lib.ptr(tokens), n, top, _lib.ptr(ws), nbytes)
     return logp, entropy, values, ids

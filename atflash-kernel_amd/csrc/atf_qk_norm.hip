@@ -156,12 +156,24 @@ __global__ __launch_bounds__(128) void qk_norm_write_kernel(QkNormArgs n) {
   if (unit >= a.hkv) {  // ---- Q ----
     load_weights(n.q_weight, n.weights_fp32, i, w1, w2);
     const int h0 = (unit - a.hkv) * kNormQHeads;
-    for (int h = h0; h < min(h0 + kNormQHeads, n.hq); ++h) {
-      const uint16_t* x = n.q + row * n.q_st + h * n.q_sh;
-      const u32x4 x1 = ldg16(x + 8 * i), x2 = ldg16(x + kP + 8 * i);
-      float z1[8], z2[8];
-      norm_rotate(x1, x2, w1, w2, n.eps, rope, cs, z1, z2);
-      if (on) store_row(n.q_out + (row * n.hq + h) * kD, i, z1, z2);
+    const uint16_t* x = n.q + row * n.q_st;
+    constexpr int kBatch = 4;  // heads whose loads are in flight together
+#pragma unroll
+    for (int j0 = 0; j0 < kNormQHeads; j0 += kBatch) {
+      u32x4 x1[kBatch], x2[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int64_t at = min(h0 + j0 + j, n.hq - 1) * n.q_sh;
+        x1[j] = ldg16(x + at + 8 * i);
+        x2[j] = ldg16(x + at + kP + 8 * i);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int h = h0 + j0 + j;
+        float z1[8], z2[8];
+        norm_rotate(x1[j], x2[j], w1, w2, n.eps, rope, cs, z1, z2);
+        if (on && h < n.hq) store_row(n.q_out + (row * n.hq + h) * kD, i, z1, z2);
+      }
     }
     return;
   }
@@ -296,8 +308,66 @@ __global__ __launch_bounds__(128) void qk_norm_write_kernel(QkNormArgs n) {
   }
 }
 
+// A few tokens into the bf16 cache (a decode step's append): one wave per (eight heads, token,
+// sequence), the heads q's, then k's, then v's.  V's elements go to their slots one by one, so
+// nothing is read back or staged.  Same results, same skips.
+// grid: x = heads in eights, y = token of the sequence, z = sequence.
+constexpr int kNormAppendTokens = 4;
+__global__ __launch_bounds__(64) void qk_norm_append_kernel(QkNormArgs n) {
+  const KvWriteArgs& a = n.kv;
+  const int lane = threadIdx.x, i = lane & 7, b = blockIdx.z, t = blockIdx.y;
+  const int u = 8 * blockIdx.x + (lane >> 3);
+  const KvRows rows = kv_rows<true>(a, b);
+  if (t >= rows.count) return;
+  const int64_t row = rows.first + t;
+  const int kind = u < n.hq ? 0 : u < n.hq + a.hkv ? 1 : 2;  // q, k, v
+  const int h = u - (kind == 0 ? 0 : kind == 1 ? n.hq : n.hq + a.hkv);
+  const bool on = kind < 2 || h < a.hkv;
+  const uint16_t* x = kind == 0 ? n.q + row * n.q_st + h * n.q_sh
+                      : kind == 1 ? a.k_src + row * a.ks_t + h * a.ks_h
+                                  : a.v_src + row * a.vs_t + min(h, a.hkv - 1) * a.vs_h;
+  const u32x4 x1 = ldg16(x + 8 * i), x2 = ldg16(x + kP + 8 * i);
+  float w1[8], w2[8];
+  load_weights(kind == 0 ? n.q_weight : n.k_weight, n.weights_fp32, i, w1, w2);
+  const bool rope = a.rope_cs != nullptr;
+  const int64_t pos = static_cast<int64_t>(a.start_pos[b]) + t, pidx = pos >> 4;
+  if (pos < 0 || (rope && pos >= a.rope_max_pos)) return;
+  float cs[16] = {};
+  if (rope) load_cs8(a.rope_cs, static_cast<int>(pos), 8 * i, cs);
+  const int pg = pidx < a.max_pages ? a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx] : -1;
+  float z1[8], z2[8];
+  norm_rotate(x1, x2, w1, w2, n.eps, rope, cs, z1, z2);
+  if (kind == 0) {
+    store_row(n.q_out + (row * n.hq + h) * kD, i, z1, z2);
+    return;
+  }
+  if (!on || pg < 0 || pg >= a.num_pages) return;
+  uint16_t* page = a.kv_cache + (static_cast<size_t>(pg) * a.hkv + h) * kKvBlockElems;
+  const int slot = static_cast<int>(pos) & (kPage - 1);
+  if (kind == 1) {
+    const float ka[8] = {z1[4], z1[5], z1[6], z1[7], z2[4], z2[5], z2[6], z2[7]};
+    const float kb[8] = {z1[0], z1[1], z1[2], z1[3], z2[0], z2[1], z2[2], z2[3]};
+    uint16_t* kdst = page + kKHalfElems + 2 * (kLevels - 1 - i) * (kPage * kSliceDims) + slot * kSliceDims;
+    *reinterpret_cast<u32x4*>(kdst) = pack8(ka);
+    *reinterpret_cast<u32x4*>(kdst + kPage * kSliceDims) = pack8(kb);
+  } else {
+    uint16_t* vdst = page + v_slot(slot);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      vdst[(8 * i + 2 * e) * kPage] = static_cast<uint16_t>(x1[e]);
+      vdst[(8 * i + 2 * e + 1) * kPage] = static_cast<uint16_t>(x1[e] >> 16);
+      vdst[(kP + 8 * i + 2 * e) * kPage] = static_cast<uint16_t>(x2[e]);
+      vdst[(kP + 8 * i + 2 * e + 1) * kPage] = static_cast<uint16_t>(x2[e] >> 16);
+    }
+  }
+}
+
 hipError_t launch_qk_norm_write(const QkNormArgs& a, hipStream_t s) {
   if (a.kv.n_tokens <= 0 || a.kv.batch <= 0) return hipSuccess;
+  if (a.kv.n_tokens <= kNormAppendTokens && a.kv.kv_exps == nullptr) {
+    hipLaunchKernelGGL(qk_norm_append_kernel, dim3((a.hq + 2 * a.kv.hkv + 7) / 8, a.kv.n_tokens, a.kv.batch), dim3(64), 0, s, a);
+    return hipGetLastError();
+  }
   // a call of n tokens touches at most ceil(n / 16) + 1 pages per sequence
   const int pages = (a.kv.n_tokens + kPage - 1) / kPage + 1;
   QkNormArgs n = a;
