@@ -3,6 +3,7 @@ hook and the paged cache, window OFF vs ON; and gate C0 at model level.
 
     python -m atflash.e2e --tokens 262144 [--chunk 65536] [--steps 64] [--modes off,k2,k64]
     python -m atflash.e2e --c0 262144 [--chunk 65536]
+    (--logprobs N records what each greedy token was chosen from)
 
 Follows the reference's timing arm (e2e_pipeline/atflash_e2e_fafi.py:199-265,
 571-612): per mode, a chunked prefill of the prompt against the growing cache
@@ -29,7 +30,7 @@ import time
 
 import torch
 
-from . import hf
+from . import hf, ops
 from .model_tables import WIN_ZHI_CAP
 
 MODES = {"off": None, "k2": 2.0, "k64": 64.0}
@@ -65,9 +66,11 @@ def use_mode(model, mode: str, n_ctx: int):
 
 
 @torch.inference_mode()
-def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None):
+def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None, logprobs: int = None):
     """One request: chunked prefill then `steps` greedy tokens (the first from
-    the prefill's logits).  Returns timings and the generated tokens.  With
+    the prefill's logits).  Returns timings and the generated tokens, and with
+    `logprobs` (a number of alternatives, 0 or more) each token's log probability, the
+    entropy it was chosen from and the likeliest tokens, computed outside the timed steps.  With
     `progress`, a line is printed after every 4th chunk has run (the host waits
     for it first, so long prefills report as they go; the wait costs one
     kernel-launch latency per 4 chunks)."""
@@ -89,6 +92,14 @@ def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None):
     e1.record()
     cur = int(out.logits[:, -1].argmax(-1))
     tokens = [cur]
+    said = []
+
+    def say(logits):
+        if logprobs is not None:
+            tok = torch.tensor([tokens[-1]], device=dev)
+            said.append([x.tolist() for x in ops.token_logprobs(logits, tok, logprobs)])
+
+    say(out.logits[:, -1])
     pend = []
     for _ in range(1, steps):
         s0, s1 = ev(), ev()
@@ -97,14 +108,19 @@ def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None):
         s1.record()
         cur = int(out.logits[:, -1].argmax(-1))
         tokens.append(cur)
+        say(out.logits[:, -1])
         pend.append((s0, s1))
     torch.cuda.synchronize()
     wall = time.perf_counter() - wall0
     step_ms = [a.elapsed_time(b) for a, b in pend]
     del cache
-    return {"prefill_ms": e0.elapsed_time(e1), "decode_ms_total": sum(step_ms),
-            "decode_ms_per_step_median": sorted(step_ms)[len(step_ms) // 2] if step_ms else 0.0,
-            "step_ms": step_ms, "wall_s": wall, "tokens": tokens}
+    got = {"prefill_ms": e0.elapsed_time(e1), "decode_ms_total": sum(step_ms),
+           "decode_ms_per_step_median": sorted(step_ms)[len(step_ms) // 2] if step_ms else 0.0,
+           "step_ms": step_ms, "wall_s": wall, "tokens": tokens}
+    if logprobs is not None:
+        got["logprobs"] = [{"logprob": a[0], "entropy": h[0], "top": [[i, x] for i, x in zip(ids_[0], v[0])]}
+                           for a, h, v, ids_ in said]
+    return got
 
 
 @torch.inference_mode()
@@ -129,6 +145,8 @@ def main(argv=None):
     ap.add_argument("--modes", default="off,k2,k64")
     ap.add_argument("--repeat", type=int, default=1, help="timed requests per mode")
     ap.add_argument("--c0", type=int, default=0, help="run gate C0 at this prompt length instead")
+    ap.add_argument("--logprobs", type=int, default=None, metavar="N",
+                    help="also record each token's log probability, the entropy and N alternatives (0 to 64)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--out", default=None, help="also append the JSON record to this file")
     args = ap.parse_args(argv)
@@ -169,7 +187,8 @@ def main(argv=None):
         for rep in range(args.repeat):
             for mode in args.modes.split(","):
                 hook = use_mode(model, mode, n_ctx)
-                r = run_request(model, hook, ids, args.chunk, args.steps, progress=f"{mode} rep {rep}")
+                r = run_request(model, hook, ids, args.chunk, args.steps, progress=f"{mode} rep {rep}",
+                                logprobs=args.logprobs)
                 print(f"[e2e] {mode} rep {rep}: prefill {r['prefill_ms']:.1f} ms, decode {r['decode_ms_total']:.1f} ms "
                       f"({r['decode_ms_per_step_median']:.2f} ms/step), request {r['wall_s']:.2f} s", flush=True)
                 rec["runs"].setdefault(mode, []).append(r)

@@ -37,7 +37,17 @@ chunk, a PagedCache must be read by this hook alone: an update that no hook
 call consumed (another attention implementation read the layer, or the key
 reached the hook as a copy) makes the next call on that layer raise instead of
 attending to the chunk only, and unregister() closes the caches of the hook it
-removes.  With any other cache (HF's DynamicCache passes the whole history as
+removes.  With sharing=True the rows of a batch may hold the same pages: a beam
+search (reorder_cache) then copies at most one page a row and layer instead of
+the whole history.
+
+Norms of the heads.  Models that norm each head's queries and keys (q_norm and
+k_norm modules) can leave that to the kernels too (register(norm_at_load=True)): the
+norms become the identity, and one call norms and rotates the queries and writes
+the normed, rotated keys beside the values into the pages, in fp32 with one
+rounding, instead of HF's three elementwise passes and their roundings.
+
+With any other cache (HF's DynamicCache passes the whole history as
 key/value) a prefill packs that history into a temporary paged cache per call and
 a decode reads it in place -- correct, but every call goes over the whole context
 again, rotating its keys, and a decode's window saves less than on pages (a
@@ -58,7 +68,7 @@ except ImportError:  # pragma: no cover - the package works without transformers
 from . import _lib
 from . import interface as I
 from . import ops
-from .cache import k_half, new_kv_cache, new_kv_cache_q8, v_half
+from .cache import PageTables, k_half, new_kv_cache, new_kv_cache_q8, v_half
 from .model_tables import ModelWindow, window_from_config
 
 ATTN_NAME = "atf_window"
@@ -91,6 +101,7 @@ class PagedLayer(CacheLayerMixin):
             self.kv = new_kv_cache(n_pages, owner.num_kv_heads, owner.device)
             self.k = k_half(self.kv)  # views of the two halves
             self.v = v_half(self.kv)
+        self.deferred = owner.norm_at_load  # the hook writes, with the norms (update only counts)
         self.length = 0       # tokens written (every sequence of the batch has the same length)
         self.prev_length = 0  # length before the last update (the last chunk's first position)
         self.last_key = None  # the key tensor of the last update until the hook reads it (identity check)
@@ -119,7 +130,11 @@ class PagedLayer(CacheLayerMixin):
         if self.length + L > o.capacity:
             raise ValueError(f"PagedCache holds {o.capacity} tokens per sequence; "
                              f"{self.length} + {L} would not fit")
-        if self.exps is None:
+        if o.tables is not None:
+            o.reserve(self.length, L)
+        if self.deferred:
+            pass
+        elif self.exps is None:
             ops.kv_write(self.kv, key_states.transpose(1, 2), value_states.transpose(1, 2),
                          o.start_positions(self.length), o.page_table, o.rope_cs, _lib.LAYOUT_HALF_SPLIT)
         else:
@@ -141,6 +156,7 @@ class PagedLayer(CacheLayerMixin):
 
     def reset(self) -> None:
         # pages past `length` are never read, so they need not be cleared
+        self.owner.give_back()
         self.length = self.prev_length = 0
         self.last_key = None
 
@@ -158,12 +174,14 @@ class PagedLayer(CacheLayerMixin):
             max_length = self.length - abs(max_length)
         if self.length <= max_length:
             return
+        if self.owner.tables is not None:
+            raise NotImplementedError("a PagedCache with sharing cannot be cropped: other rows may hold the page of the cut")
         self.length = max(0, max_length)
         self.prev_length = min(self.prev_length, self.length)
         self.last_key = None
 
     def reorder_cache(self, beam_idx):
-        raise NotImplementedError("PagedCache does not support beam search")
+        raise NotImplementedError("PagedCache does not support beam search without sharing=True")
 
     def batch_repeat_interleave(self, repeats: int):
         raise NotImplementedError("PagedCache does not support batch expansion")
@@ -181,13 +199,17 @@ class PagedCache(Cache):
     page and kv head (a 1M-token Qwen2.5-7B layer with 4 kv heads: 2 GB).
     kv_dtype=torch.float8_e4m3fn holds 8-bit floats with a power of two for each page,
     kv head and half instead: half the memory, and half the bytes a decode step reads.
+    sharing=True: rows take their pages from one pool as they grow (atflash.cache.PageTables)
+    and may hold the same ones, so that reorder_cache (beam search) works; such a cache
+    cannot be cropped.
     """
 
     def __init__(self, config, batch: int, capacity: int, device="cuda", rope_cs=None,
-                 kv_dtype: torch.dtype = torch.bfloat16):
+                 kv_dtype: torch.dtype = torch.bfloat16, sharing: bool = False, norm_at_load: bool = False):
         """rope_cs: fp32 [>= capacity, 64, 2] (cos, sin) table when the keys
         arrive unrotated (RoPE applied at write), None when they arrive rotated.
-        kv_dtype: torch.bfloat16 or torch.float8_e4m3fn."""
+        kv_dtype: torch.bfloat16 or torch.float8_e4m3fn.  norm_at_load: the keys
+        arrive without their norm, and the hook writes them."""
         from .model_tables import head_dim_of
         if head_dim_of(config) != _lib.HEAD_DIM:
             raise ValueError(f"head_dim {head_dim_of(config)} unsupported (this build supports {_lib.HEAD_DIM})")
@@ -196,14 +218,24 @@ class PagedCache(Cache):
         if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError(f"kv_dtype must be bfloat16 or float8_e4m3fn, got {kv_dtype}")
         self.kv_dtype = kv_dtype
+        self.norm_at_load = bool(norm_at_load)
         self.rope_cs = rope_cs
         self.batch = int(batch)
         self.capacity = int(capacity)
         self.num_kv_heads = int(getattr(config, "num_key_value_heads", None) or config.num_attention_heads)
         self.device = torch.device(device)
         self.pages_per_seq = -(-self.capacity // PAGE)
-        self.page_table = torch.arange(self.batch * self.pages_per_seq, dtype=torch.int32,
-                                       device=self.device).view(self.batch, self.pages_per_seq)
+        self.tables = None
+        if sharing:
+            self.tables = PageTables(self.batch * self.pages_per_seq, self.batch, self.pages_per_seq, self.device,
+                                     sharing=True)
+            self.page_table = self.tables.page_table
+        else:
+            self.page_table = torch.arange(self.batch * self.pages_per_seq, dtype=torch.int32,
+                                           device=self.device).view(self.batch, self.pages_per_seq)
+        self._held = 0             # sharing: tokens of a row that its pages are for
+        self._new = (None, None)   # sharing: (tokens, device int32 [batch])
+        self._cu = (None, None)    # (tokens of a row, first row of each sequence in packed order [batch + 1])
         self._pos = (None, None)   # (value, device int32 [batch] tensor), reused by every layer of a step
         self._lens = (None, None)
         self.closed = False
@@ -222,6 +254,46 @@ class PagedCache(Cache):
         if self._lens[0] != n:
             self._lens = (n, torch.full((self.batch,), n, dtype=torch.int32, device=self.device))
         return self._lens[1]
+
+    def packed_rows(self, n: int) -> torch.Tensor:
+        """First rows of the sequences where each has n, packed one after the other."""
+        if self._cu[0] != n:
+            self._cu = (n, torch.arange(0, (self.batch + 1) * n, n, dtype=torch.int32, device=self.device))
+        return self._cu[1]
+
+    def reserve(self, length: int, n: int):
+        """Pages for tokens length .. length + n - 1 of every row (with sharing; the first
+        layer of a step takes them for all)."""
+        if length > self._held:
+            raise RuntimeError("a layer of this PagedCache holds tokens whose pages were given back (reset all layers)")
+        if length + n > self._held:
+            more = length + n - self._held
+            if self._new[0] != more:
+                self._new = (more, torch.full((self.batch,), more, dtype=torch.int32, device=self.device))
+            self.tables.extend(self._new[1], 0)
+            self._held = length + n
+
+    def give_back(self):
+        """All pages back to the pool (with sharing)."""
+        if self.tables is not None and self._held:
+            self.tables.release(torch.arange(self.batch, dtype=torch.int32, device=self.device))
+            self._held = 0
+
+    def page_tensors(self):
+        """Every layer's page tensors (K/V pages, exponents)."""
+        return [t for lyr in self.layers for t in (lyr.kv, lyr.exps) if t is not None]
+
+    def reorder_cache(self, beam_idx: torch.Tensor):
+        """Row b becomes what row beam_idx[b] is (with sharing): whole pages are shared, a page
+        that is filled in part is copied for all but one of its rows."""
+        if self.tables is None:
+            return super().reorder_cache(beam_idx)
+        if beam_idx.shape != (self.batch,):
+            raise ValueError(f"beam_idx must be [{self.batch}], got {tuple(beam_idx.shape)}")
+        for lyr in self.layers:
+            if lyr.length != self._held or lyr.last_key is not None:
+                raise RuntimeError("reorder_cache inside a step: the layers hold different numbers of tokens")
+        self.tables.select(beam_idx.to(device=self.device, dtype=torch.int32).contiguous(), self.page_tensors())
 
     def layer_of(self, layer_idx, key):
         """The layer whose last (unread) update returned `key`, or None."""
@@ -261,13 +333,56 @@ class IdentityRotary(nn.Module):
         return one.expand(shape), torch.zeros_like(one).expand(shape)
 
 
+class IdentityNorm(nn.Module):
+    """Stands in for the norm of a head's queries or keys when the kernels apply it."""
+
+    def __init__(self, original: nn.Module):
+        super().__init__()
+        self.original = original
+
+    def forward(self, x):
+        return x
+
+
+def _original(norm):
+    return norm.original if isinstance(norm, IdentityNorm) else norm
+
+
+def _norm_eps(norm) -> float:
+    """The eps of an RMS norm module over a head's dims, x (mean(x^2) + eps)^-1/2 weight; ValueError for any other
+    module.  What the module computes is tried out: norms are alike by name and differ in their weights."""
+    w = getattr(norm, "weight", None)
+    eps = getattr(norm, "variance_epsilon", getattr(norm, "eps", None))
+    if not isinstance(w, torch.Tensor) or tuple(w.shape) != (_lib.HEAD_DIM,) or eps is None:
+        raise ValueError(f"{type(norm).__name__} is not an RMS norm over {_lib.HEAD_DIM} dims with a weight")
+    x = torch.randn((4, _lib.HEAD_DIM), generator=torch.Generator().manual_seed(0)).to(w.device, w.dtype) * 3
+    with torch.no_grad():
+        got, x = norm(x).double(), x.double()
+        want = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + float(eps)) * w.double()
+    # the module rounds twice to the weight's type
+    if not ((got - want).abs() <= 2.1 * (torch.finfo(w.dtype).eps / 2) * want.abs() + 1e-5 * want.abs()).all():
+        raise ValueError(f"{type(norm).__name__} computes something else than x (mean(x^2) + eps)^-1/2 weight")
+    return float(eps)
+
+
 class WindowAttention:
     """The registered attention function; `mode` is "win" (window on) or "off".
-    With rope_at_load, q and k reach it unrotated (see IdentityRotary)."""
+    With rope_at_load, q and k reach it unrotated (see IdentityRotary).  norms: per layer
+    the (q_norm, k_norm) modules that the kernels apply, q and k arriving without them."""
 
-    def __init__(self, window: ModelWindow, mode: str = "win", rope_at_load: bool = True):
+    def __init__(self, window: ModelWindow, mode: str = "win", rope_at_load: bool = True, norms=None):
         if mode not in ("win", "off"):
             raise ValueError("mode must be 'win' or 'off'")
+        if norms is not None and not rope_at_load:
+            raise ValueError("norm_at_load needs rope_at_load (the norm comes before the rotation)")
+        self.norms = None
+        if norms is not None:
+            self.norms = []
+            for q, k in norms:
+                eps = _norm_eps(q)
+                if _norm_eps(k) != eps:
+                    raise ValueError("q_norm and k_norm must have the same eps")
+                self.norms.append((q, k, eps))
         self.window = window
         self.mode = mode
         self.rope_at_load = bool(rope_at_load)
@@ -291,11 +406,13 @@ class WindowAttention:
         return t
 
     def new_cache(self, config, batch: int, capacity: int, device="cuda",
-                  kv_dtype: torch.dtype = torch.bfloat16) -> PagedCache:
-        """A PagedCache bound to this hook (pass it as past_key_values)."""
+                  kv_dtype: torch.dtype = torch.bfloat16, sharing: bool = False) -> PagedCache:
+        """A PagedCache bound to this hook (pass it as past_key_values).  sharing=True: for
+        beam search (batch: the beams of all prompts)."""
         if capacity - 1 > self.window.n_ctx:
             raise ValueError(f"capacity {capacity} exceeds the window tables' n_ctx {self.window.n_ctx}")
-        cache = PagedCache(config, batch, capacity, device, rope_cs=self.rope_table(capacity, device), kv_dtype=kv_dtype)
+        cache = PagedCache(config, batch, capacity, device, rope_cs=self.rope_table(capacity, device), kv_dtype=kv_dtype,
+                           sharing=sharing, norm_at_load=self.norms is not None)
         self._caches.add(cache)
         return cache
 
@@ -317,6 +434,19 @@ class WindowAttention:
                     "key tensor (a copy of the one update() returned); the hook cannot find the cached history")
         return None
 
+    def _normed(self, layer_idx, query, key, rt):
+        """Queries [b, hq, L, d] and a plain cache's whole keys [b, hkv, S, d], normed and rotated."""
+        qn, kn, eps = self.norms[layer_idx]
+        S, out = key.shape[-2], []
+        for x, heads_of in ((query, 0), (key, 1)):
+            b, h, n, d = x.shape
+            pos = torch.arange(S - n, S, dtype=torch.int32, device=x.device).repeat(b)
+            rows = x.transpose(1, 2).reshape(b * n, h, d)
+            pair = (rows, rows[:, :0]) if heads_of == 0 else (rows[:, :0], rows)
+            y = ops.qk_norm_rope(*pair, qn.weight, kn.weight, eps, pos, rt)[heads_of]
+            out.append(y.view(b, n, h, d).transpose(1, 2))
+        return out
+
     def __call__(self, module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
         b, hq, L, d = query.shape
         if d != self.window.head_dim:
@@ -336,17 +466,26 @@ class WindowAttention:
             owner = lyr.owner
             if (owner.rope_cs is not None) != self.rope_at_load:
                 raise ValueError("the cache was made for the other RoPE mode of this hook")
+            if lyr.deferred != (self.norms is not None):
+                raise ValueError("the cache was made for the other norm mode of this hook")
+            rope_cs = owner.rope_cs
+            if lyr.deferred:
+                qn, kn, eps = self.norms[module.layer_idx]
+                rows = [x.transpose(1, 2).reshape(b * L, x.shape[1], d) for x in (query, key, value)]
+                query = ops.qk_norm_write(lyr.kv, lyr.exps, *rows, qn.weight, kn.weight, eps, owner.packed_rows(L), L,
+                                          owner.start_positions(lyr.prev_length), owner.page_table, rope_cs)
+                query, rope_cs = query.view(b, L, hq, d).transpose(1, 2), None
             if L == 1:
                 zhi = self.window.decode_zhi8 if windowed else None
                 if lyr.exps is None:
                     o = ops.decode_paged(query.select(2, 0), lyr.kv, owner.page_table, owner.seq_lens(S), S, zhi,
-                                         scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+                                         scale, rope_cs, _lib.LAYOUT_HALF_SPLIT)
                 else:
                     o = ops.decode_paged_q8(query.select(2, 0), lyr.kv, lyr.exps, owner.page_table, owner.seq_lens(S),
-                                            S, zhi, scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+                                            S, zhi, scale, rope_cs, _lib.LAYOUT_HALF_SPLIT)
                 return o.view(b, 1, hq, d), None
             zhi = self.window.prefill_zhi if windowed else None
-            args = (owner.page_table, S, lyr.prev_length, zhi, scale, owner.rope_cs, _lib.LAYOUT_HALF_SPLIT)
+            args = (owner.page_table, S, lyr.prev_length, zhi, scale, rope_cs, _lib.LAYOUT_HALF_SPLIT)
             o, _ = (ops.prefill(query.transpose(1, 2), lyr.kv, *args) if lyr.exps is None
                     else ops.prefill_q8(query.transpose(1, 2), lyr.kv, lyr.exps, *args))
             return o, None  # [b, L, hq, d]
@@ -358,6 +497,9 @@ class WindowAttention:
                           "hook.new_cache(...) as past_key_values to attend on persistent pages", RuntimeWarning,
                           stacklevel=2)
         rt = self.rope_table(S, query.device)
+        if self.norms is not None:
+            query, key = self._normed(module.layer_idx, query, key, rt)
+            rt = None
         if L == 1:
             zhi = self.window.decode_zhi8 if windowed else None
             o = I.decode_contiguous(query[:, :, 0, :], key.transpose(1, 2), value.transpose(1, 2), zhi, scale, rt,
@@ -370,18 +512,27 @@ class WindowAttention:
 
 
 def register(model, k_prefill: float = 2.0, k_decode: float = 2.0, n_ctx: int = None,
-             mode: str = "win", rope_at_load: bool = True) -> WindowAttention:
+             mode: str = "win", rope_at_load: bool = True, norm_at_load: bool = False) -> WindowAttention:
     """Build the tables from model.config, register the hook and switch the
     model's attention implementation to it.  Returns the hook (its .mode can be
     changed between calls; hook.new_cache(...) makes a bound PagedCache).
     rope_at_load=True (default) replaces model.model.rotary_emb by
-    IdentityRotary, so the kernels apply RoPE; unregister() undoes that."""
+    IdentityRotary, so the kernels apply RoPE; norm_at_load=True replaces every
+    layer's q_norm and k_norm (RMS norms over a head's dims) by IdentityNorm, so they
+    apply those too; unregister() undoes both."""
     from transformers import AttentionInterface
     window = window_from_config(model.config, k_prefill, k_decode, n_ctx)
     scaling = getattr(getattr(model.model.layers[0], "self_attn", None), "scaling", None)
     if scaling is not None and abs(float(scaling) - window.sm_scale) > 1e-9:
         raise ValueError(f"attention scaling {scaling} != head_dim ** -0.5")
-    hook = WindowAttention(window, mode, rope_at_load)
+    norms = None
+    if norm_at_load:
+        norms = [tuple(_original(getattr(layer.self_attn, name, None)) for name in ("q_norm", "k_norm"))
+                 for layer in model.model.layers]
+        if any(n is None for pair in norms for n in pair):
+            raise ValueError("norm_at_load needs q_norm and k_norm modules in every layer")
+    hook = WindowAttention(window, mode, rope_at_load, norms)
+    _set_norms(model, norm_at_load)
     rot = model.model.rotary_emb
     if rope_at_load and not isinstance(rot, IdentityRotary):
         model.model.rotary_emb = IdentityRotary(rot)
@@ -396,8 +547,18 @@ def register(model, k_prefill: float = 2.0, k_decode: float = 2.0, n_ctx: int = 
     return hook
 
 
+def _set_norms(model, identity: bool) -> None:
+    """Every layer's q_norm and k_norm behind an IdentityNorm, or themselves."""
+    for layer in model.model.layers:
+        attn = getattr(layer, "self_attn", None)
+        for name in ("q_norm", "k_norm"):
+            norm = getattr(attn, name, None)
+            if norm is not None and isinstance(norm, IdentityNorm) != identity:
+                setattr(attn, name, IdentityNorm(norm) if identity else norm.original)
+
+
 def unregister(model, attn_implementation: str = "eager") -> None:
-    """Give the model back its own rotary embedding and the given attention.
+    """Give the model back its own rotary embedding, norms and the given attention.
     Closes the PagedCaches that register()'s hook on this model made: another
     attention implementation cannot read them, and their update() refuses
     further tokens."""
@@ -405,6 +566,7 @@ def unregister(model, attn_implementation: str = "eager") -> None:
     if hook is not None:
         for c in list(hook._caches):
             c.closed = True
+    _set_norms(model, False)
     rot = model.model.rotary_emb
     if isinstance(rot, IdentityRotary):
         model.model.rotary_emb = rot.original

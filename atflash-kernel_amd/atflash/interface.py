@@ -191,6 +191,14 @@ def kv_write_packed(cache, k, v, cu_seqlens, max_tokens, start_pos, page_table, 
                         _layout_id(layout))
 
 
+def qk_norm_write(cache, q, k, v, q_weight, k_weight, cu_seqlens, max_tokens, start_pos, page_table, eps=1e-6, rope=None):
+    """kv_write_packed into a PagedKVCache (either kv_dtype) of keys that are normed per head
+    (and rotated) on the way; returns the queries of the same rows, normed and rotated, for
+    the attention calls with rope=None (ops.qk_norm_write)."""
+    return ops.qk_norm_write(cache.kv, getattr(cache, "exps", None), q, k, v, q_weight, k_weight, eps, cu_seqlens,
+                             int(max_tokens), start_pos, page_table, rope)
+
+
 def decode_plan(cache, page_table, seq_lens, max_seq_len, num_q_heads, zhi=None, sm_scale=None, rope=None,
                 layout="half_split", q_strides=None):
     """ops.DecodePlan for a PagedKVCache: the decode step of a serving loop

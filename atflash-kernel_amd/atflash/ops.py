@@ -692,10 +692,9 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
     if count is not None:
         _check_ints(count, 1, "count")
     # (a model's caches are many: each check over all of them at once)
-    shapes = list(map(_shape, caches))
-    pool = shapes[0][0] if shapes[0] else -1
-    if not (all(s and s[0] == pool for s in shapes) and all(map(_is_contiguous, caches))
-            and set(map(_get_device, caches)) == {dev}):
+    firsts = {s[0] if s else -1 for s in set(map(_shape, caches))}
+    pool = firsts.pop()
+    if firsts or pool < 0 or not all(map(_is_contiguous, caches)) or set(map(_get_device, caches)) != {dev}:
         raise ValueError("caches must be contiguous [num_pages, ...] tensors of one pool, on the device of the pairs")
     if pool == 0:
         return
