@@ -339,12 +339,10 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
     float cm = vm[0];
 #pragma unroll
     for (int k = 1; k < kVecs; ++k) cm = fmaxf(cm, vm[k]);
-    // The first chunk's bounds, from the waves whose lanes all have logits.
-    const int full = kTop && c0 == static_cast<int>(blockIdx.y) * kChunk ? min(kLpWaves, (n_vec - c0) / 64) : 0;
     if constexpr (kTop) {
-      if (full > wave) {
-        list.q = (a.top + full - 1) / full;
-        int at = 0;  // the first place of the lane's largest (a NaN at the front counts as -inf)
+      // a lane's best: the first place of its largest (a NaN at the front counts as -inf), 0 without one
+      auto lane_best = [&] {
+        int at = 0;
         u32x4 w = v[0];
 #pragma unroll
         for (int k = kVecs - 1; k >= 0; --k) {
@@ -356,21 +354,37 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
         int el = 0;
 #pragma unroll
         for (int e = kE - 1; e >= 0; --e) el = V::get(w, e) == cm ? e : el;
-        const uint64_t nth = wave_nth64(entry_of(cm, head + (c0 + at * kLpThreads + tid) * kE + el), list.q);
-        if (lane == 0) s_given[wave] = nth;
-        if (a.top == 1 && lane == 0) atomicMax(&s_floor, nth);
-      } else if (full > 0 && lane == 0) {
-        s_given[wave] = ~0ull;
-      }
-    }
-    if constexpr (kTop) {
-      if (full > 0) {  // (uniform: a workgroup's first chunk)
+        const int j = c0 + at * kLpThreads + tid;
+        return j < n_vec ? entry_of(cm, head + j * kE + el) : 0;
+      };
+      // The first chunk's bounds, from the waves whose lanes all have logits.
+      const int full = c0 == static_cast<int>(blockIdx.y) * kChunk ? min(kLpWaves, (n_vec - c0) / 64) : 0;
+      if (full > 0) {  // (uniform)
+        if (wave < full) {
+          list.q = (a.top + full - 1) / full;
+          const uint64_t nth = wave_nth64(lane_best(), list.q);
+          if (lane == 0) s_given[wave] = nth;
+          if (a.top == 1 && lane == 0) atomicMax(&s_floor, nth);
+        } else if (lane == 0) {
+          s_given[wave] = ~0ull;
+        }
         __syncthreads();
         list.floor = max64(list.floor, lp_least(s_given));
       }
       list.floor = max64(list.floor, lane64(__hip_atomic_load(&s_floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP), 0));
-      const float bar = list.floor == 0 ? kNegInf : key_value(static_cast<uint32_t>(list.floor >> 32));
-      if (__builtin_amdgcn_ballot_w64(!(cm < bar)) != 0) {
+      // what a logit has to reach: the floor's value, or the next one where all that is equal lies behind its place
+      auto bar_of = [&] {
+        const uint32_t key = static_cast<uint32_t>(list.floor >> 32), place = 0xffffffffu - static_cast<uint32_t>(list.floor);
+        return list.floor == 0 ? kNegInf : key_value(key + (place < static_cast<uint32_t>(head + c0 * kE) ? 1u : 0u));
+      };
+      float bar = bar_of();
+      const int over = __builtin_popcountll(__builtin_amdgcn_ballot_w64(!(cm < bar)));
+      if (over != 0) {
+        if (over >= 2 * a.top || over > 32) {  // many: the top-th best of the lanes is a better floor
+          const uint64_t nth = wave_nth64(lane_best(), a.top);
+          list.floor = max64(list.floor, nth);
+          bar = bar_of();
+        }
         // every lane takes its first vector with a candidate, of that the first candidate, then the
         // next, until no lane has one left
         uint32_t vectors = 0;
