@@ -150,6 +150,7 @@ __device__ __forceinline__ void rank_entries(const uint64_t* buf, int n, int top
   for (int i = threadIdx.x; i < n; i += threads) {
     const uint64_t x = buf[i];
     int above = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) above += buf[j] > x ? 1 : 0;
     if (above < top) out[above] = x;
   }
@@ -163,6 +164,7 @@ struct LpList {
   unsigned long long* shared;  // the largest floor that a wave has found
   int len, top, q;
   uint64_t floor;
+  int ordered;  // of the entries: as many as were there when they were last put in order
 };
 // The least of what the waves have given (it only grows): lane w looks at wave w's.
 __device__ __forceinline__ uint64_t lp_least(const uint64_t* given) {
@@ -177,6 +179,7 @@ __device__ __forceinline__ uint64_t lp_least(const uint64_t* given) {
 // Only the `top` best are kept, best first.
 __device__ __forceinline__ void lp_prune(LpList& a) {
   const int lane = threadIdx.x & 63;
+  if (a.len == a.ordered) return;
   wave_fence();
   if (a.len <= 64) {
     const uint64_t x = lane < a.len ? a.buf[lane] : 0;
@@ -202,7 +205,7 @@ __device__ __forceinline__ void lp_prune(LpList& a) {
       if (64 * i + lane < a.len && above[i] < a.top) a.buf[above[i]] = x[i];
   }
   wave_fence();
-  a.len = min(a.len, a.top);
+  a.ordered = a.len = min(a.len, a.top);
   if (a.q > 0 && a.len >= a.q) {
     if (lane == 0) __hip_atomic_store(a.given + (threadIdx.x >> 6), a.buf[a.q - 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     wave_fence();
@@ -224,17 +227,29 @@ __device__ __forceinline__ void lp_push(LpList& a, uint64_t y) {
   a.len += __builtin_popcountll(mask);
 }
 
-// The outputs of a row from its sums and its list.
+// A given token and its logit.
+struct LpToken {
+  int64_t id;
+  float x;
+};
+template <int kType>
+__device__ __forceinline__ LpToken lp_token(const LogprobArgs& a, int row, const void* x, int i) {
+  LpToken t{-1, 0.f};
+  if (i < a.n_tokens) {
+    t.id = a.tokens[static_cast<int64_t>(row) * a.n_tokens + i];
+    if (t.id >= 0 && t.id < a.vocab) t.x = LogitVec<kType>::one(x, t.id);
+  }
+  return t;
+}
+// The outputs of a row from its sums and its list.  token: the thread's first, requested before.
 template <int kType>
 __device__ __forceinline__ void lp_write(const LogprobArgs& a, int row, const void* x, const LpStats& st,
-                                         const uint64_t* list, int len, int threads) {
+                                         const uint64_t* list, int len, LpToken token, int threads) {
   const float log2_s = log2f(st.s);
   for (int i = threadIdx.x; i < a.n_tokens; i += threads) {
-    const int64_t at = static_cast<int64_t>(row) * a.n_tokens + i;
-    const int64_t tok = a.tokens[at];
-    a.logprobs[at] = tok < 0 ? 0.f
-                     : tok >= a.vocab ? __uint_as_float(0x7fc00000u)
-                                      : lp_of(st, log2_s, LogitVec<kType>::one(x, tok));
+    if (i >= threads) token = lp_token<kType>(a, row, x, i);
+    a.logprobs[static_cast<int64_t>(row) * a.n_tokens + i] =
+        token.id < 0 ? 0.f : token.id >= a.vocab ? __uint_as_float(0x7fc00000u) : lp_of(st, log2_s, token.x);
   }
   if (threadIdx.x == 0) a.entropy[row] = st.s == 0.f ? 0.f : (log2_s - st.t / st.s) * kLn2;
   for (int i = threadIdx.x; i < a.top; i += threads) {
@@ -272,9 +287,11 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
     if (tid < kLpWaves) s_given[tid] = 0;
     __syncthreads();
   }
+  LpToken token{-1, 0.f};
+  if (gridDim.y == 1 && wave == 0) token = lp_token<kType>(a, row, x, lane);
   LpStats st{kNegInf, 0.f, 0.f};  // (m is the wave's)
   bool careful = false;           // the wave has seen logits of which (x - m) log2 e is -inf
-  LpList list{s_buf[kTop ? wave : 0], s_given, &s_floor, 0, a.top, 0, 0};
+  LpList list{s_buf[kTop ? wave : 0], s_given, &s_floor, 0, a.top, 0, 0, 0};
   if (blockIdx.y == 0 && wave == 0 && head + rest > 0) {
     const int i = lane < 32 ? lane : a.vocab - rest + lane - 32;
     const bool on = lane < 32 ? lane < head : lane - 32 < rest;
@@ -433,7 +450,7 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
 #pragma unroll
   for (int m = 1; m < kLpWaves; m <<= 1) lp_join(st, LpStats{__shfl_xor(st.m, m), __shfl_xor(st.s, m), __shfl_xor(st.t, m)});
   if (gridDim.y == 1) {
-    lp_write<kType>(a, row, x, st, s_list, len, 64);
+    lp_write<kType>(a, row, x, st, s_list, len, token, 64);
     return;
   }
   const int64_t part = static_cast<int64_t>(row) * gridDim.y + blockIdx.y;
@@ -449,31 +466,44 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprobs_merge_kernel(Logprob
   __shared__ int s_count;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int64_t part = static_cast<int64_t>(row) * a.splits;
+  const char* x = static_cast<const char*>(a.logits) + static_cast<int64_t>(row) * a.stride * LogitVec<kType>::kBytes;
+  const LpToken token = lp_token<kType>(a, row, x, tid);
   if (tid == 0) s_count = 0;
+  const int n = a.splits * a.top;
+  constexpr int kMine = kLpMerge / kLpMergeThreads;
+  uint64_t mine[kMine];
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int i = k * kLpMergeThreads + tid;
+    mine[k] = i < n ? a.ws_top[part * a.top + i] : 0;
+  }
+  // Bounds: a split's last (so many are at least that good), and the least of the splits' q-th best.
+  const int q = (a.top + a.splits - 1) / a.splits;
+  uint64_t last = 0, not_qth = 0;
   LpStats st{kNegInf, 0.f, 0.f};
-  uint64_t bound = 0;  // the best of the splits' last: so many are at least that good
   for (int i = lane; i < a.splits; i += 64) {  // (every wave the same)
     const f32x4 p = *reinterpret_cast<const f32x4*>(a.ws_stats + 4 * (part + i));
     lp_join(st, LpStats{p[0], p[1], p[2]});
     if (a.top > 0) {
-      const uint64_t y = a.ws_top[(part + i) * a.top + a.top - 1];
-      bound = y > bound ? y : bound;
+      last = max64(last, a.ws_top[(part + i) * a.top + a.top - 1]);
+      not_qth = max64(not_qth, ~a.ws_top[(part + i) * a.top + q - 1]);
     }
   }
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) lp_join(st, LpStats{__shfl_xor(st.m, m), __shfl_xor(st.s, m), __shfl_xor(st.t, m)});
-  bound = wave_max64(bound);
-  __syncthreads();
-  for (int i = tid; i < a.splits * a.top; i += kLpMergeThreads) {
-    const uint64_t y = a.ws_top[part * a.top + i];
-    if (y >= bound && y != 0) buf[atomicAdd(&s_count, 1)] = y;
+  int len = 0;
+  if (a.top > 0) {
+    const uint64_t bound = max64(wave_max64(last), ~wave_max64(not_qth));
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kMine; ++k)
+      if (mine[k] != 0 && mine[k] >= bound) buf[atomicAdd(&s_count, 1)] = mine[k];
+    __syncthreads();
+    len = min(s_count, a.top);
+    rank_entries(buf, s_count, a.top, list, kLpMergeThreads);
+    __syncthreads();
   }
-  __syncthreads();
-  const int n = s_count;
-  rank_entries(buf, n, a.top, list, kLpMergeThreads);
-  __syncthreads();
-  const char* x = static_cast<const char*>(a.logits) + static_cast<int64_t>(row) * a.stride * LogitVec<kType>::kBytes;
-  lp_write<kType>(a, row, x, st, list, min(n, a.top), kLpMergeThreads);
+  lp_write<kType>(a, row, x, st, list, len, token, kLpMergeThreads);
 }
 
 // Vectors of a thread's chunk, with alternatives and without.
