@@ -121,6 +121,10 @@ class PageTables:
         ops.release_tables(self.page_table, self.seq_lens, self.free_pages, self.free_count, rows, self.num_pages)
 
 
+    def _check_caches(self, caches):
+        if any(c.dim() == 0 or c.shape[0] != self.num_pages for c in caches):
+            raise ValueError(f"caches must have the tables' {self.num_pages} pages")
+
     def select(self, parents: torch.Tensor, caches=()):
         """Sequence b becomes what sequence parents[b] is now (int32 [batch] on the GPU;
         outside [0, batch): empty), with sharing=True: `parents` is the identity but
@@ -131,6 +135,7 @@ class PageTables:
         from . import ops
         if not self.sharing:
             raise ValueError("select needs tables made with sharing=True")
+        self._check_caches(caches)
         table, lens, left, src, dst = ops.select_tables(self.page_table, self.seq_lens, self.free_pages,
                                                         self.free_count, parents, self.num_pages)
         self.page_table.copy_(table)
@@ -145,6 +150,7 @@ class PageTables:
         pages in use are then the lowest of those that are in use or free, so that a
         pool without pages held elsewhere can be cut behind them."""
         from . import ops
+        self._check_caches(caches)
         table, free, left, src, dst, n = ops.compact_tables(self.page_table, self.seq_lens, self.free_pages,
                                                             self.free_count, self.num_pages)
         self.page_table.copy_(table)

@@ -9,11 +9,21 @@
 // probabilities of -inf and entropy 0.  NaN and +inf make the row's numbers NaN.
 //   The likeliest tokens in the same pass.  A logit and its place make one number of 64
 // bits, ordered as (value, lowest place first).  A wave keeps the best of what it has seen in
-// LDS and gives the others its q-th best, q = ceil(top / 8): each of the 8 waves has q that
+// LDS and gives the others its q-th best, q = ceil(top / 4): each of the 4 waves has q that
 // reach the least of these, so that it is a bound, and 16 bytes of logits are looked at
 // closer only if their largest reaches it.  For the first chunk the q-th best of a
 // wave's lanes (each lane's largest) serve.
-//   Bound by HBM: every logit is read once.
+//   Bound by HBM on many rows (every logit is read once), with alternatives by the vector
+// units as well: 2048 rows of 152064 bf16 logits 116 us without alternatives (5.4 TB/s), 130
+// with one, 139 with 20, 176 with 64; of fp32 logits 228 and, with 20, 258.  What it came from, us
+// for bf16 with none, 1 and 20: a workgroup of 512 that put its candidates in order together after
+// every chunk, every element pushed by itself, one alternative 490; waves by themselves, the
+// bound of all of them 136, 164, 195; joined by one wave, the row's filler left out 117, 137, 187;
+// lanes' candidates side by side, ordered once 118, 135, 147; workgroups of 256 (four a CU, so that
+// one's end runs beside the others' loads) 116, 130, 139.  One row takes 3.8 + 2.7 us of the two
+// kernels, with five alternatives 8.3 + 4.2: a chain of loads, sums and LDS.
+//   Requesting a chunk while the one before is summed changed nothing (130 without alternatives,
+// 164 with one, before and after) and took 32 registers.
 #include <type_traits>
 
 #include "atf_launch.h"
@@ -22,7 +32,7 @@ namespace atf {
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / 64;
-constexpr int kLpRoom = 256;    // candidates of a wave
+constexpr int kLpRoom = 256;    // candidates of a wave (kTopMax and a push of 64 fit twice)
 constexpr int kLpMerge = 2048;  // of a row's splits
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
@@ -506,11 +516,14 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprobs_merge_kernel(Logprob
   lp_write<kType>(a, row, x, st, list, len, token, kLpMergeThreads);
 }
 
-// Vectors of a thread's chunk, with alternatives and without.
+// Vectors of a thread's chunk, with alternatives and without: with them the chunks are few (each
+// begins with a look at the others' bounds), without them more waves fit (2048 x 152064 bf16 with
+// 20 alternatives 147 us at 8 and 161 at 4 in workgroups of 512; without 118 and 115).
 constexpr int kLpVecsTop = 8, kLpVecsSums = 4;
 
 // Workgroups of a row: four a CU for all rows together, a chunk each at least, and no more than
-// the merge has room for.
+// the merge has room for.  Chunks of 8 KB instead of 32 KB for the splits were slower with
+// alternatives, whose first chunk costs the most (300 x 152064 bf16 with 20: 53 us, 37 with 32 KB).
 int logprob_splits(int rows, int vocab, int type, int top) {
   const int64_t bytes = static_cast<int64_t>(vocab) * (type == kLogitsFp32 ? 4 : 2);
   const int64_t chunk = 16 * kLpThreads * (top > 0 ? kLpVecsTop : kLpVecsSums);

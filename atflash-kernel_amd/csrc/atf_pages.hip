@@ -74,7 +74,9 @@ static hipError_t allow_lds(const void* kernel, size_t bytes) {
 // without a child named go to the end of the free pages before that, the lowest id first.
 //   Latency bound.  Workgroup 0 finds the pages that become free (bits of the dropped rows'
 // pages, less the surviving rows'), and hands out the new ones; the others write the new
-// rows, all but the entries of new pages.
+// rows, all but the entries of new pages.  8 beams of 375 pages 6.4 us, one prompt of 1876 pages
+// forked into 48 rows 5.6; 64 rows of 500 pages 15, of 2000 53, half a million entries 190: one
+// workgroup reads every entry of the old rows, where it is one launch for all others.
 constexpr int kSelChunk = 4096;  // entries of a row that a workgroup writes
 __global__ __launch_bounds__(kPgThreads) void select_tables_kernel(SelectTablesArgs a) {
   extern __shared__ uint32_t sh[];
@@ -205,7 +207,8 @@ hipError_t launch_select_tables(const SelectTablesArgs& a, hipStream_t s) {
 // rows' pages from T on move, free ones below T take them, the i-th highest of the former to
 // the i-th lowest of the latter (as many of each).  The free pages come out highest first,
 // so that the lowest is taken first.  Latency bound (the pages' copies are not its part);
-// one workgroup: a page's place depends on all before it.
+// one workgroup: a page's place depends on all before it.  Pools of 300 pages 9.7 us, 6000 19,
+// 160000 183, 2^19 820; the copies of the 6000 move 2.7 GB in 541 us.
 __global__ __launch_bounds__(kPgThreads) void compact_tables_kernel(CompactTablesArgs a) {
   extern __shared__ uint32_t sh[];
   __shared__ int32_t part[kPgWaves], before_live[kPgThreads];
@@ -308,7 +311,7 @@ hipError_t launch_compact_tables(const CompactTablesArgs& a, hipStream_t s) {
 }
 
 // Page dst[i] of every cache becomes a copy of its page src[i].  Bound by HBM: a page's
-// bytes read and written.  grid: x = pieces of 16 KB of the pairs' pages, y = cache.
+// bytes read and written; 1500 pages of 28 layers, 2.75 GB, 541 us, 5.1 TB/s.  grid: x = pieces of 16 KB of the pairs' pages, y = cache.
 constexpr int kCopyThreads = 256, kCopyUnroll = 4;
 constexpr int kCopyPiece = kCopyThreads * kCopyUnroll * 16;
 

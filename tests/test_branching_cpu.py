@@ -220,7 +220,10 @@ def test_tables_share_only_where_asked():
         t.select(torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError, match="524288"):
         PageTables(2 ** 19 + 1, 2, 4, "cpu", sharing=True)
-    assert PageTables(8, 2, 4, "cpu", sharing=True).sharing
+    shared = PageTables(8, 2, 4, "cpu", sharing=True)
+    for call in (lambda c: shared.select(torch.zeros(2, dtype=torch.int32), [c]), lambda c: t.compact([c])):
+        with pytest.raises(ValueError, match="8 pages"):
+            call(torch.zeros(7, 4))
 
 
 transformers = pytest.importorskip("transformers")

@@ -331,6 +331,25 @@ def test_captured_steps(dev):
                 t.release(ints([0, 1, 2, 3], dev))
 
 
+def test_captured_calls_on_a_large_pool(dev):
+    from atflash import ops
+    pool = 2 ** 19
+    table, lens, free = state(11, 5, 300, 4700, 5000)
+    far = {x: pool - 1 - 100 * x for x in range(5000)}
+    t, n = ints([[far.get(x, -1) for x in r] for r in table], dev), ints(lens, dev)
+    f, c, parents = ints([far[x] for x in free] + [0] * 5000, dev), ints([len(free)], dev), ints([0, 0, 2, 1, -1], dev)
+    args = (t, n, f, c)
+    want = (ops.select_tables(*args, parents, pool), ops.compact_tables(*args, pool))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = (ops.select_tables(*args, parents, pool), ops.compact_tables(*args, pool))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*want[0], *want[1]), (*got[0], *got[1])):
+            assert torch.equal(a, b)
+
+
 def test_registered_operators(dev):
     from atflash import ops
     table, lens, free = state(9, 6, 9, 140, 100)

@@ -247,6 +247,40 @@ def test_max_tokens_cuts_and_rows_outside_stay(dev):
     assert kv[int(table[0, 0]), 0, 1].view(16, 16, 8)[:, 12:].eq(0).all()
 
 
+@pytest.mark.parametrize("n", [1, 9])
+@pytest.mark.parametrize("eight", [False, True])
+def test_keys_alone(dev, n, eight):
+    """No query heads: the cache as with them."""
+    from atflash import cache, ops
+    q, k, v, qw, kw, cu, start, table, pool, _ = packed([n, n], [15, 0], 4, 3, dev, 21, room=0)
+    cs = table_of(64, dev)
+    made = [cache.new_kv_cache_q8(pool, 3, dev) if eight else (cache.new_kv_cache(pool, 3, dev), None) for _ in range(2)]
+    for (kv, exps), qq in zip(made, (q, q[:, :0])):
+        out = ops.qk_norm_write(kv, exps, qq, k, v, qw, kw, 1e-6, cu, n, start, table, cs)
+        assert out.shape == qq.shape
+    assert torch.equal(made[0][0].view(torch.uint8), made[1][0].view(torch.uint8)) and (not eight or torch.equal(made[0][1], made[1][1]))
+
+
+def test_offsets_past_31_bits(dev):
+    from atflash import cache, ops
+    hq, hkv, T = 2, 1, 40
+    wide = torch.zeros((T, 2 ** 26 + 8), dtype=BF, device=dev)  # 5.4 GB: row 32 on lies past 2^31 elements
+    x = wide[:, 8:8 + (hq + 2 * hkv) * D].unflatten(1, (-1, D))
+    q, k, v, qw, kw = rows(T, hq, hkv, dev, 2)
+    x.copy_(torch.cat([q, k, v], 1))
+    pool = 600000  # 4.9 GB of blocks
+    kv, small = cache.new_kv_cache(pool, hkv, dev), cache.new_kv_cache(3, hkv, dev)
+    cs, pos = table_of(T, dev), torch.arange(T, device=dev, dtype=torch.int32)
+    cu, zero = ints([0, T], dev), ints([0], dev)
+    want = ops.qk_norm_rope(q, k, qw, kw, 1e-6, pos, cs)
+    for a, b in zip(ops.qk_norm_rope(x[:, :hq], x[:, hq:hq + 1], qw, kw, 1e-6, pos, cs), want):
+        assert torch.equal(a, b)
+    far = ints([[pool - 1, pool - 2, 7]], dev)
+    out = ops.qk_norm_write(kv, None, x[:, :hq], x[:, hq:hq + 1], x[:, hq + 1:], qw, kw, 1e-6, cu, T, zero, far, cs)
+    ops.qk_norm_write(small, None, q, k, v, qw, kw, 1e-6, cu, T, zero, ints([[0, 1, 2]], dev), cs)
+    assert torch.equal(out, want[0]) and torch.equal(kv[far[0].long()], small)
+
+
 def test_captured_and_on_another_stream(dev):
     from atflash import cache, ops
     q, k, v, qw, kw, cu, start, table, pool, pos = packed([1, 1, 1], [15, 16, 200], 28, 4, dev, 8, room=0)
