@@ -58,9 +58,9 @@ same operations called directly from Python, without the dispatcher (whose
 per-call cost, about 20 us, would exceed a short decode's GPU time); the
 package's own entry points use them.
 """
-import ctypes
 import math
 import operator
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -700,7 +700,7 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
         return
     bases, sizes = list(map(_data_ptr, caches)), [x // pool for x in map(_nbytes, caches)]
     m = len(bases)
-    _lib.launch(dev, _lib.lib().atf_copy_pages, (ctypes.c_void_p * m)(*bases), (ctypes.c_int64 * m)(*sizes), m, pool,
+    _lib.launch(dev, _lib.lib().atf_copy_pages, struct.pack(f"{m}Q", *bases), struct.pack(f"{m}q", *sizes), m, pool,
                 src.data_ptr(), dst.data_ptr(), n, _lib.ptr(count))
 
 
