@@ -80,7 +80,8 @@ class PageTables:
     go on reading them.
 
     sharing=True: sequences may begin with the same pages (`select`: forks, drops, a beam's
-    choice).  `release` then gives back only the pages that no other sequence names."""
+    choice).  `release` then gives back only the pages that no other sequence names.  Lengths
+    of such tables only grow: a page that was full may be named by others and is never written again."""
 
     def __init__(self, num_pages: int, batch: int, max_pages: int, device="cuda", sharing: bool = False):
         self.num_pages = int(num_pages)
@@ -119,7 +120,6 @@ class PageTables:
             self.select(torch.where(gone, -1, every))
             return
         ops.release_tables(self.page_table, self.seq_lens, self.free_pages, self.free_count, rows, self.num_pages)
-
 
     def _check_caches(self, caches):
         if any(c.dim() == 0 or c.shape[0] != self.num_pages for c in caches):

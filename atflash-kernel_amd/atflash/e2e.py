@@ -30,7 +30,7 @@ import time
 
 import torch
 
-from . import hf, ops
+from . import _lib, hf, ops
 from .model_tables import WIN_ZHI_CAP
 
 MODES = {"off": None, "k2": 2.0, "k64": 64.0}
@@ -150,6 +150,8 @@ def main(argv=None):
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--out", default=None, help="also append the JSON record to this file")
     args = ap.parse_args(argv)
+    if args.logprobs is not None and not 0 <= args.logprobs <= _lib.MAX_TOP:
+        raise SystemExit(f"--logprobs must be between 0 and {_lib.MAX_TOP}")
     if args.chunk % 32:
         raise SystemExit("--chunk must be a multiple of 32 (the prefill's 32-row tiles)")
     dev = torch.device("cuda:0")

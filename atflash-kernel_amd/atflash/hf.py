@@ -334,11 +334,13 @@ class IdentityRotary(nn.Module):
 
 
 class IdentityNorm(nn.Module):
-    """Stands in for the norm of a head's queries or keys when the kernels apply it."""
+    """Stands in for the norm of a head's queries or keys when the kernels apply it.  It has the
+    norm's own parameters and buffers, under the norm's own names in the model's state dict."""
 
     def __init__(self, original: nn.Module):
         super().__init__()
-        self.original = original
+        object.__setattr__(self, "original", original)  # (not a submodule)
+        self._parameters, self._buffers = original._parameters, original._buffers
 
     def forward(self, x):
         return x
@@ -434,6 +436,12 @@ class WindowAttention:
                     "key tensor (a copy of the one update() returned); the hook cannot find the cached history")
         return None
 
+    def _check_norms(self, module):
+        """A model whose norms another hook's kernels apply would be computed without them, or with this one's."""
+        qn = getattr(module, "q_norm", None)
+        if isinstance(qn, IdentityNorm) and (self.norms is None or self.norms[module.layer_idx][0] is not qn.original):
+            raise ValueError("the model's norms were left to another hook: register() this model (again)")
+
     def _normed(self, layer_idx, query, key, rt):
         """Queries [b, hq, L, d] and a plain cache's whole keys [b, hkv, S, d], normed and rotated."""
         qn, kn, eps = self.norms[layer_idx]
@@ -453,6 +461,7 @@ class WindowAttention:
             raise ValueError(f"head_dim {d} != the tables' {self.window.head_dim}")
         scale = float(scaling) if scaling is not None else self.window.sm_scale
         windowed = self.mode == "win"
+        self._check_norms(module)
         lyr = self._paged_layer(module, key)
         if lyr is not None:
             lyr.last_key = None  # read: the layer's next update may proceed

@@ -623,6 +623,7 @@ int atf_qk_norm_rope_bf16(void* q_out, const void* q, int64_t q_st, int64_t q_sh
   if (!aligned(k_out, 16) || !aligned(k, 16)) return fail(ATF_ERR_INVALID, "rows and weights must be 16-byte aligned");
   for (int64_t s : {k_st, k_sh})
     if (s % 8 != 0) return fail(ATF_ERR_INVALID, "source strides must be multiples of 8 elements");
+  if (rows > (1 << 25)) return fail(ATF_ERR_UNSUPPORTED, "at most 2^25 rows, got %d", rows);  // (a wave each, 2^32 threads a launch)
   if (static_cast<int64_t>(num_q_heads) + num_k_heads > 65535)
     return fail(ATF_ERR_UNSUPPORTED, "at most 65535 heads, got %d and %d", num_q_heads, num_k_heads);
   if (int r = check_layout(ATF_LAYOUT_HALF_SPLIT, rope_cs, rope_max_pos)) return r;
@@ -682,6 +683,7 @@ int atf_token_logprobs(float* logprobs, float* entropy, float* top_logprobs, int
   if (rows == 0) return ok();
   if (vocab <= 0) return fail(ATF_ERR_INVALID, "a row needs at least one logit");
   if (vocab > (1 << 30)) return fail(ATF_ERR_UNSUPPORTED, "at most 2^30 logits a row, got %d", vocab);
+  if (rows > (1 << 23)) return fail(ATF_ERR_UNSUPPORTED, "at most 2^23 rows, got %d", rows);  // (2^32 threads a launch)
   if (top > vocab) return fail(ATF_ERR_INVALID, "top = %d of %d logits", top, vocab);
   if (top > ATF_MAX_TOP) return fail(ATF_ERR_UNSUPPORTED, "at most %d alternatives, got %d", ATF_MAX_TOP, top);
   if (!logits || !entropy || (n_tokens > 0 && (!logprobs || !tokens)) || (top > 0 && (!top_logprobs || !top_ids)))

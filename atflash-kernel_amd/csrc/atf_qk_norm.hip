@@ -378,7 +378,7 @@ hipError_t launch_qk_norm_write(const QkNormArgs& a, hipStream_t s) {
   n.kv.page_round = pages < 8 ? pages : 8;
   const int64_t units = a.kv.hkv + (a.hq + kNormQHeads - 1) / kNormQHeads;
   const int64_t blocks = static_cast<int64_t>(pages + n.kv.page_round - 1) / n.kv.page_round * n.kv.page_round * units;
-  if (blocks > INT32_MAX) return hipErrorInvalidConfiguration;
+  if (blocks >= (int64_t(1) << 32) / 128) return hipErrorInvalidConfiguration;  // (2^32 threads)
   hipLaunchKernelGGL(a.kv.kv_exps != nullptr ? qk_norm_write_kernel<true> : qk_norm_write_kernel<false>,
                      dim3(blocks, a.kv.batch), dim3(128), 0, s, n);
   return hipGetLastError();

@@ -283,7 +283,8 @@ int atf_release_tables(int32_t* page_table, int max_pages, int32_t* seq_lens, in
  * k_out bf16 [rows][heads][128], contiguous.  Weights [128], bf16 or fp32
  * (weights_fp32), not needed where there are no heads.  positions: device int32 [rows].
  * With rope_cs NULL rows are normed only.  A row whose position lies outside
- * [0, rope_max_pos) is left as it is in the outputs.  fp32 throughout, one rounding.
+ * [0, rope_max_pos) is left as it is in the outputs.  At most 2^25 rows.  fp32 throughout, one
+ * rounding.
  */
 int atf_qk_norm_rope_bf16(void* q_out, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads,
                           void* k_out, const void* k, int64_t k_st, int64_t k_sh, int num_k_heads,
@@ -320,7 +321,8 @@ int atf_qk_norm_write(void* q_out, const void* q, int64_t q_st, int64_t q_sh, in
  *                                       first, of equal logits the lowest id first
  * top is at most ATF_MAX_TOP and at most vocab.  Logits of -inf have probability 0; a row of
  * nothing else has log probabilities of -inf and entropy 0.  A NaN or +inf makes the row's log
- * probabilities and entropy NaN; NaN rank below every number.  Sums are fp32.
+ * probabilities and entropy NaN; NaN rank below every number.  At most 2^23 rows of 2^30 logits.
+ * Sums are fp32.
  *   The workspace (atf_logprobs_workspace_bytes; 0 for many rows) needs no initialisation; calls
  * that share one must be ordered on one stream.
  */

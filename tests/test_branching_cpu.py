@@ -303,3 +303,49 @@ def test_other_norms_are_refused():
     without = transformers.Qwen2ForCausalLM(config("Qwen2Config")).eval()
     with pytest.raises(ValueError, match="q_norm"):
         hf.register(without, n_ctx=4096, norm_at_load=True)
+
+
+def test_row_limits(lib):
+    """A launch has 2^32 threads at most."""
+    assert call(lib.atf_qk_norm_rope_bf16, NORM, rows=(1 << 25) + 1) == 2
+    assert call(lib.atf_token_logprobs, LOGP, rows=(1 << 23) + 1, vocab=8) == 2
+
+
+def test_models_with_kernel_norms_keep_their_state_dict():
+    """Weights are saved and loaded under the norms' own names, replaced ones included; nothing of a model without its norms runs
+    by another model's hook."""
+    import copy
+    from atflash import hf
+    model = transformers.Qwen3ForCausalLM(config()).to(BF).eval()
+    before = {n: p.clone() for n, p in model.state_dict().items()}
+    names = [n for n, _ in model.named_parameters()]
+    hook = hf.register(model, n_ctx=4096, norm_at_load=True)
+    assert list(model.state_dict()) == list(before) and [n for n, _ in model.named_parameters()] == names
+    new = {n: torch.randn(128).to(BF) if "q_norm" in n else p.clone() for n, p in before.items()}
+    for assign in (False, True):
+        model.load_state_dict(new, assign=assign)
+        for i, layer in enumerate(model.model.layers):
+            want = new[f"model.layers.{i}.self_attn.q_norm.weight"]
+            assert torch.equal(hook.norms[i][0].weight, want) and torch.equal(layer.self_attn.q_norm.weight, want)
+    model.float()
+    assert all(q.weight.dtype == torch.float32 for q, _, _ in hook.norms)
+    model.to(BF)
+    x = [torch.zeros((1, h, 3, 128), dtype=BF) for h in (2, 1, 1)]
+    other = transformers.Qwen3ForCausalLM(config()).to(BF).eval()
+    plain = hf.register(other, n_ctx=4096)
+    twin = hf.register(other, n_ctx=4096, norm_at_load=True)
+    for wrong in (plain, twin):
+        with pytest.raises(ValueError, match="another hook"):
+            wrong(model.model.layers[0].self_attn, *x, None)
+    with pytest.raises(ValueError, match="another hook"):
+        hook(copy.deepcopy(model).model.layers[1].self_attn, *x, None)
+    hf.unregister(model)
+    assert isinstance(model.model.layers[0].self_attn.q_norm, type(other.model.layers[0].self_attn.q_norm.original))
+    assert torch.equal(model.model.layers[1].self_attn.q_norm.weight, new["model.layers.1.self_attn.q_norm.weight"])
+
+
+def test_e2e_refuses_too_many_alternatives():
+    from atflash import e2e
+    for n in ("65", "-1"):
+        with pytest.raises(SystemExit, match="logprobs"):
+            e2e.main(["--logprobs", n])
