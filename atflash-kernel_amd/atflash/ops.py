@@ -672,7 +672,9 @@ def _(page_table, seq_lens, free_pages, free_count, num_pages):
             seq_lens.new_empty(half), seq_lens.new_empty(1))
 
 
-_shape, _nbytes = operator.attrgetter("shape"), operator.attrgetter("nbytes")
+# (the base class's, where torch has it: half of the time of a shape; 0 for a tensor without dims)
+_first_dim = getattr(getattr(torch._C, "TensorBase", None), "__len__", lambda t: t.shape[0] if t.dim() else 0)
+_nbytes = operator.attrgetter("nbytes")
 _data_ptr, _is_contiguous, _get_device = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
 
 
@@ -692,9 +694,9 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
     if count is not None:
         _check_ints(count, 1, "count")
     # (a model's caches are many: each check over all of them at once)
-    firsts = {s[0] if s else -1 for s in set(map(_shape, caches))}
+    firsts = set(map(_first_dim, caches))
     pool = firsts.pop()
-    if firsts or pool < 0 or not all(map(_is_contiguous, caches)) or set(map(_get_device, caches)) != {dev}:
+    if firsts or pool == 0 and any(c.dim() == 0 for c in caches) or not all(map(_is_contiguous, caches)) or set(map(_get_device, caches)) != {dev}:
         raise ValueError("caches must be contiguous [num_pages, ...] tensors of one pool, on the device of the pairs")
     if pool == 0:
         return
