@@ -20,8 +20,8 @@
 // every chunk, every element pushed by itself, one alternative 490; waves by themselves, the
 // bound of all of them 136, 164, 195; joined by one wave, the row's filler left out 117, 137, 187;
 // lanes' candidates side by side, ordered once 118, 135, 147; workgroups of 256 (four a CU, so that
-// one's end runs beside the others' loads) 116, 130, 139.  One row takes 3.8 + 2.7 us of the two
-// kernels, with five alternatives 8.3 + 4.2: a chain of loads, sums and LDS.
+// one's end runs beside the others' loads) 116, 130, 139.  One row takes 3.6 + 2.8 us of the two
+// kernels, with five alternatives 7.6 + 4.3: a chain of loads, sums and LDS.
 //   Requesting a chunk while the one before is summed changed nothing (130 without alternatives,
 // 164 with one, before and after) and took 32 registers.
 #include <type_traits>
@@ -79,14 +79,26 @@ __device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {  // of a lane
 __device__ __forceinline__ uint64_t max64(uint64_t x, uint64_t y) { return x > y ? x : y; }
 __device__ __forceinline__ uint64_t min64(uint64_t x, uint64_t y) { return x < y ? x : y; }
 
+// Exchanges within rows of 16 lanes: with each in turn, lanes 0, 16, 32 and 48 get all of their rows.
+constexpr int kLane1 = 0xb1, kLane2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;  // lane ^ 1, ^ 2, mirrored in 8, in 16
+template <int kHow>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), kHow, 0xf, 0xf, true));
+}
+template <int kHow>
+__device__ __forceinline__ float moved(float x) {
+  return __uint_as_float(moved<kHow>(__float_as_uint(x)));
+}
+__device__ __forceinline__ float lane_of(float x, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
+}
 // The largest of the wave's lanes, in every lane (unsigned 32 bits): maxima over rows of 16
 // lanes, then over the rows.
 __device__ __forceinline__ uint32_t wave_max32(uint32_t x) {
-  auto with = [](uint32_t v, int moved) { return max(v, static_cast<uint32_t>(moved)); };
-  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0xb1, 0xf, 0xf, true));   // lane ^ 1
-  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x4e, 0xf, 0xf, true));   // lane ^ 2
-  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x141, 0xf, 0xf, true));  // mirrored in 8
-  x = with(x, __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x140, 0xf, 0xf, true));  // mirrored in 16
+  x = max(x, moved<kLane1>(x));
+  x = max(x, moved<kLane2>(x));
+  x = max(x, moved<kMirror8>(x));
+  x = max(x, moved<kMirror16>(x));
   const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
   const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
   return max(max(a, b), max(c, d));
@@ -149,10 +161,16 @@ __device__ __forceinline__ void lp_join(LpStats& a, LpStats b) {
 __device__ __forceinline__ float lp_of(const LpStats& a, float log2_s, float x) {
   return x == kNegInf && a.s == a.s ? kNegInf : __builtin_fmaf(-log2_s, kLn2, x - a.m);
 }
+template <int kHow>
+__device__ __forceinline__ void lp_join_moved(LpStats& a) {
+  lp_join(a, LpStats{moved<kHow>(a.m), moved<kHow>(a.s), moved<kHow>(a.t)});
+}
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-  return x;
+  x += moved<kLane1>(x);
+  x += moved<kLane2>(x);
+  x += moved<kMirror8>(x);
+  x += moved<kMirror16>(x);
+  return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
 }
 
 // The `top` best of n entries of `buf`, best first, to `out`; every thread of the workgroup.
@@ -178,12 +196,11 @@ struct LpList {
 };
 // The least of what the waves have given (it only grows): lane w looks at wave w's.
 __device__ __forceinline__ uint64_t lp_least(const uint64_t* given) {
+  static_assert(kLpWaves == 4, "two exchanges");
   uint64_t x = __hip_atomic_load(given + (threadIdx.x & (kLpWaves - 1)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-#pragma unroll
-  for (int m = 1; m < kLpWaves; m <<= 1) {
-    const uint32_t lo = __shfl_xor(static_cast<int>(x), m), hi = __shfl_xor(static_cast<int>(x >> 32), m);
-    x = min64(x, (static_cast<uint64_t>(hi) << 32) | lo);
-  }
+  auto other = [&](uint32_t hi, uint32_t lo) { x = min64(x, (static_cast<uint64_t>(hi) << 32) | lo); };
+  other(moved<kLane1>(static_cast<uint32_t>(x >> 32)), moved<kLane1>(static_cast<uint32_t>(x)));
+  other(moved<kLane2>(static_cast<uint32_t>(x >> 32)), moved<kLane2>(static_cast<uint32_t>(x)));
   return lane64(x, 0);
 }
 // Only the `top` best are kept, best first.
@@ -438,18 +455,21 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
             some &= some - 1;
           }
         }
-        if (full > 0) lp_prune(list);  // (later chunks add little: what they do is put in order when the room ends)
+        if (full > 0 && c0 + static_cast<int>(gridDim.y) * kChunk < n_vec) lp_prune(list);  // (later chunks add little: what they do is put in order when the room ends)
       }
     }
   }
-  if constexpr (kTop) lp_prune(list);
+  // (the list of one chunk is short, and what the waves' lists hold is put in order below)
+  if constexpr (kTop) {
+    if (list.len > 64 || static_cast<int>(blockIdx.y + gridDim.y) * kChunk < n_vec) lp_prune(list);
+  }
   st.s = wave_sum(st.s);
   st.t = wave_sum(st.t);
   if (lane == 0) s_stats[wave] = st;
   __syncthreads();
   int len = 0;
   if constexpr (kTop) {
-    if (lane < list.len && list.buf[lane] >= s_floor) s_all[atomicAdd(&s_count, 1)] = list.buf[lane];
+    if (lane < list.len && list.buf[lane] >= max64(list.floor, s_floor)) s_all[atomicAdd(&s_count, 1)] = list.buf[lane];
     __syncthreads();
     len = min(s_count, a.top);
     rank_entries(s_all, s_count, a.top, s_list, kLpThreads);
@@ -457,8 +477,8 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
   }
   if (wave > 0) return;
   st = s_stats[lane & (kLpWaves - 1)];
-#pragma unroll
-  for (int m = 1; m < kLpWaves; m <<= 1) lp_join(st, LpStats{__shfl_xor(st.m, m), __shfl_xor(st.s, m), __shfl_xor(st.t, m)});
+  lp_join_moved<kLane1>(st);
+  lp_join_moved<kLane2>(st);
   if (gridDim.y == 1) {
     lp_write<kType>(a, row, x, st, s_list, len, token, 64);
     return;
@@ -487,23 +507,38 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprobs_merge_kernel(Logprob
     const int i = k * kLpMergeThreads + tid;
     mine[k] = i < n ? a.ws_top[part * a.top + i] : 0;
   }
-  // Bounds: a split's last (so many are at least that good), and the least of the splits' q-th best.
-  const int q = (a.top + a.splits - 1) / a.splits;
-  uint64_t last = 0, not_qth = 0;
-  LpStats st{kNegInf, 0.f, 0.f};
-  for (int i = lane; i < a.splits; i += 64) {  // (every wave the same)
-    const f32x4 p = *reinterpret_cast<const f32x4*>(a.ws_stats + 4 * (part + i));
-    lp_join(st, LpStats{p[0], p[1], p[2]});
-    if (a.top > 0) {
-      last = max64(last, a.ws_top[(part + i) * a.top + a.top - 1]);
-      not_qth = max64(not_qth, ~a.ws_top[(part + i) * a.top + q - 1]);
+  // A bound: of every list each step-th entry, a lane each (every wave the same), the n-th largest of them
+  // with n step >= top.  So many entries reach it, and besides them fewer than `step` of each list
+  // (n is 4 at most: finding it takes as long as a few more entries).  The least of the lists'
+  // q-th best, q = ceil(top / lists), is a bound too, but one that a short last list spoils: 48 rows
+  // with 64 alternatives 34 us for both kernels, 20 with this.  With more lists than lanes a lane takes the largest of several lists' first, and the largest of the lists' last serves too.
+  const int step = a.splits > 64 ? 1 : max((a.top * a.splits + 63) / 64, (a.top + 3) / 4);
+  const int each = a.splits > 64 ? 1 : a.top / max(step, 1);
+  uint64_t some = 0, last = 0;
+  if (a.top > 0) {
+    for (int i = lane; i < a.splits * each; i += 64) {
+      some = max64(some, a.ws_top[(part + i / each) * a.top + (i % each + 1) * step - 1]);
+      if (a.splits > 64) last = max64(last, a.ws_top[(part + i) * a.top + a.top - 1]);
     }
   }
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) lp_join(st, LpStats{__shfl_xor(st.m, m), __shfl_xor(st.s, m), __shfl_xor(st.t, m)});
+  LpStats st{kNegInf, 0.f, 0.f};
+  for (int i = lane; i < a.splits; i += 64) {
+    const f32x4 p = *reinterpret_cast<const f32x4*>(a.ws_stats + 4 * (part + i));
+    lp_join(st, LpStats{p[0], p[1], p[2]});
+  }
+  lp_join_moved<kLane1>(st);
+  lp_join_moved<kLane2>(st);
+  lp_join_moved<kMirror8>(st);
+  lp_join_moved<kMirror16>(st);
+  auto row16 = [&](int l) { return LpStats{lane_of(st.m, l), lane_of(st.s, l), lane_of(st.t, l)}; };
+  LpStats joined = row16(0), far = row16(32);
+  lp_join(joined, row16(16));
+  lp_join(far, row16(48));
+  lp_join(joined, far);
   int len = 0;
   if (a.top > 0) {
-    const uint64_t bound = max64(wave_max64(last), ~wave_max64(not_qth));
+    uint64_t bound = wave_nth64(some, (a.top + step - 1) / step);
+    if (a.splits > 64) bound = max64(bound, wave_max64(last));
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kMine; ++k)
@@ -513,7 +548,7 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprobs_merge_kernel(Logprob
     rank_entries(buf, s_count, a.top, list, kLpMergeThreads);
     __syncthreads();
   }
-  lp_write<kType>(a, row, x, st, list, len, token, kLpMergeThreads);
+  lp_write<kType>(a, row, x, joined, list, len, token, kLpMergeThreads);
 }
 
 // Vectors of a thread's chunk, with alternatives and without: with them the chunks are few (each
