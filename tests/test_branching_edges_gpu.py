@@ -139,3 +139,19 @@ def test_a_captured_step(dev, eight):
         # every page is in use or free
         used = {p for r in a[0].page_table.tolist() for p in r if p >= 0}
         assert len(used) + n == pool and not used & set(a[0].free_pages[:n].tolist())
+
+
+@pytest.mark.parametrize("order", ["random", "rising", "falling", "equal", "last few"])
+@pytest.mark.parametrize("V,top", [(2_500_001, 0), (2_500_001, 1), (2_500_001, 9), (2_500_001, 30), (2_500_001, 64), (1_000_003, 17)])
+def test_a_row_of_many_splits(dev, V, top, order):
+    """More workgroups a row than a wave has lanes, and lists that are all alike, or of which one holds everything."""
+    x = torch.randn((1, V), generator=torch.Generator(device=dev).manual_seed(V + top), device=dev) * 3
+    if order == "rising":
+        x = x.sort(-1).values
+    elif order == "falling":
+        x = x.sort(-1, descending=True).values
+    elif order == "equal":
+        x = torch.full_like(x, 0.25)
+    elif order == "last few":
+        x[:, -100:] += 20
+    check(x.to(BF), torch.tensor([V // 2], device=dev), top)
