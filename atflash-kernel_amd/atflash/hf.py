@@ -437,10 +437,19 @@ class WindowAttention:
         return None
 
     def _check_norms(self, module):
-        """A model whose norms another hook's kernels apply would be computed without them, or with this one's."""
-        qn = getattr(module, "q_norm", None)
-        if isinstance(qn, IdentityNorm) and (self.norms is None or self.norms[module.layer_idx][0] is not qn.original):
-            raise ValueError("the model's norms were left to another hook: register() this model (again)")
+        """The module's norms must be those that this hook's kernels apply, or none that kernels apply: another
+        model's calls (the attention function is registered by name, the last hook gets them all) would be
+        computed without its norms, or with its own and then this one's."""
+        left = [getattr(module, name, None) for name in ("q_norm", "k_norm")]
+        if self.norms is None:
+            wrong = any(isinstance(n, IdentityNorm) for n in left)
+        else:
+            idx = getattr(module, "layer_idx", None)
+            mine = self.norms[idx][:2] if idx is not None and 0 <= idx < len(self.norms) else (None, None)
+            wrong = any(not isinstance(n, IdentityNorm) or n.original is not m for n, m in zip(left, mine))
+        if wrong:
+            raise ValueError("the model's norms were left to another hook, or this hook applies another model's: "
+                             "register() this model (again)")
 
     def _normed(self, layer_idx, query, key, rt):
         """Queries [b, hq, L, d] and a plain cache's whole keys [b, hkv, S, d], normed and rotated."""
