@@ -357,14 +357,19 @@ def _norm_eps(norm) -> float:
     eps = getattr(norm, "variance_epsilon", getattr(norm, "eps", None))
     if not isinstance(w, torch.Tensor) or tuple(w.shape) != (_lib.HEAD_DIM,) or eps is None:
         raise ValueError(f"{type(norm).__name__} is not an RMS norm over {_lib.HEAD_DIM} dims with a weight")
-    x = torch.randn((4, _lib.HEAD_DIM), generator=torch.Generator().manual_seed(0)).to(w.device, w.dtype) * 3
+    eps, t = float(eps), torch.finfo(w.dtype)
+    # rows far above the root of eps show the weight, rows at it and below it what eps does; a row of zeros stays one
+    sizes = [3.0, eps ** 0.5, eps ** 0.5 / 30, 0.0] if eps > 0 else [3.0, 1e-6]
+    x = torch.randn((4, len(sizes), _lib.HEAD_DIM), generator=torch.Generator().manual_seed(0)) * torch.tensor(sizes)[:, None]
+    x = x.to(w.device, w.dtype)
     with torch.no_grad():
         got, x = norm(x).double(), x.double()
-        want = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + float(eps)) * w.double()
+        want = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w.double()
     # the module rounds twice to the weight's type
-    if not ((got - want).abs() <= 2.1 * (torch.finfo(w.dtype).eps / 2) * want.abs() + 1e-5 * want.abs()).all():
+    off = (2.1 * (t.eps / 2) + 1e-5) * want.abs() + t.tiny * t.eps * (1 + w.double().abs())
+    if not ((got - want).abs() <= off).all():
         raise ValueError(f"{type(norm).__name__} computes something else than x (mean(x^2) + eps)^-1/2 weight")
-    return float(eps)
+    return eps
 
 
 class WindowAttention:

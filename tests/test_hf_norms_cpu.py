@@ -68,3 +68,53 @@ def test_both_norms_are_looked_at(name):
         ha(attn, *states(), None)
     hf.unregister(a)
     hf.unregister(b)
+
+
+class Norm(torch.nn.Module):
+    """x f(x, eps) w of 128 dims, computed in fp32 and rounded as the models' norms are."""
+
+    def __init__(self, f, eps=1e-6):
+        super().__init__()
+        self.weight, self.eps, self.f = torch.nn.Parameter((1 + 0.3 * torch.randn(128)).to(BF)), eps, f
+
+    def forward(self, x):
+        y = x.float() * self.f(x.float(), self.eps)
+        return self.weight * y.to(x.dtype)
+
+
+def mean(x):
+    return x.square().mean(-1, keepdim=True)
+
+
+EPS_ELSEWHERE = {
+    "beside the root": lambda x, e: 1 / (mean(x).sqrt() + e),
+    "a bound": lambda x, e: torch.rsqrt(mean(x).clamp(min=e)),
+    "a bound of the root": lambda x, e: 1 / mean(x).sqrt().clamp(min=e),
+    "of the sum": lambda x, e: torch.rsqrt((x.square().sum(-1, keepdim=True) + e) / 128),
+    "squared": lambda x, e: torch.rsqrt(mean(x) + e * e),
+    "not used": lambda x, e: torch.rsqrt(mean(x).clamp(min=1e-30)),
+    "another": lambda x, e: torch.rsqrt(mean(x) + 1e-5),
+}
+
+
+@pytest.mark.parametrize("name", list(EPS_ELSEWHERE))
+@pytest.mark.parametrize("side", ["q_norm", "k_norm"])
+def test_norms_with_eps_elsewhere_are_refused(name, side):
+    from atflash import hf
+    model = model_of()
+    setattr(model.model.layers[1].self_attn, side, Norm(EPS_ELSEWHERE[name]))
+    with pytest.raises(ValueError, match="something else"):
+        hf.register(model, n_ctx=4096, norm_at_load=True)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-12, 1e-6, 1e-5, 1e-3, 0.5])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_the_norm_itself_is_taken(eps, dtype):
+    from atflash import hf
+    g = torch.Generator().manual_seed(2)
+    for norm in (Norm(lambda x, e: torch.rsqrt(mean(x) + e), eps), torch.nn.RMSNorm(128, eps=eps),
+                 transformers.models.qwen3.modeling_qwen3.Qwen3RMSNorm(128, eps=eps)):
+        norm = norm.to(dtype)
+        with torch.no_grad():
+            norm.weight.copy_(torch.randn(128, generator=g) * 2)
+        assert hf._norm_eps(norm) == eps
