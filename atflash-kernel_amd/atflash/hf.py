@@ -372,6 +372,43 @@ def _norm_eps(norm) -> float:
     return eps
 
 
+class _Seen(Exception):
+    """Ends a trial of an attention module once both of its norms were called."""
+
+
+def _check_order(attn, rotary, hidden: int) -> None:
+    """ValueError unless an attention module applies q_norm and k_norm before the rotation, as the kernels do: what
+    reaches them is looked at, at two pairs of positions, and must be the same."""
+    w = next(p for p in attn.parameters() if p.is_floating_point())
+    x = torch.randn((1, 2, hidden), generator=torch.Generator().manual_seed(0)).to(w.device, w.dtype)
+    calls = []
+
+    def note(module, args):
+        calls.append(args[0].detach())
+        if len(calls) % 2 == 0:
+            raise _Seen
+    hooks = [n.register_forward_pre_hook(note) for n in {attn.q_norm, attn.k_norm}]
+    why = None
+    try:
+        for first in (0, 5):
+            pos = torch.tensor([[first, first + 2]], device=w.device)
+            try:
+                with torch.no_grad():
+                    attn(hidden_states=x, position_embeddings=rotary(x, pos), attention_mask=None)
+            except _Seen:
+                pass
+    except Exception as e:  # noqa: BLE001  (whatever such a module raises)
+        why = e
+    finally:
+        for h in hooks:
+            h.remove()
+    # (a rotation by 5 turns the fast pairs by most of a circle: far more than a product's own rounding)
+    if why is not None or len(calls) != 4 or any((a - b).double().norm() > 1e-2 * a.double().norm()
+                                                 for a, b in zip(calls[:2], calls[2:])):
+        raise ValueError(f"norm_at_load needs q_norm and k_norm before the rotation: {type(attn).__name__} does not apply both "
+                         "there") from why
+
+
 class WindowAttention:
     """The registered attention function; `mode` is "win" (window on) or "off".
     With rope_at_load, q and k reach it unrotated (see IdentityRotary).  norms: per layer
@@ -541,8 +578,8 @@ def register(model, k_prefill: float = 2.0, k_decode: float = 2.0, n_ctx: int = 
     changed between calls; hook.new_cache(...) makes a bound PagedCache).
     rope_at_load=True (default) replaces model.model.rotary_emb by
     IdentityRotary, so the kernels apply RoPE; norm_at_load=True replaces every
-    layer's q_norm and k_norm (RMS norms over a head's dims) by IdentityNorm, so they
-    apply those too; unregister() undoes both."""
+    layer's q_norm and k_norm (RMS norms over a head's dims, before the rotation: both
+    are tried out) by IdentityNorm, so they apply those too; unregister() undoes both."""
     from transformers import AttentionInterface
     window = window_from_config(model.config, k_prefill, k_decode, n_ctx)
     scaling = getattr(getattr(model.model.layers[0], "self_attn", None), "scaling", None)
@@ -555,8 +592,11 @@ def register(model, k_prefill: float = 2.0, k_decode: float = 2.0, n_ctx: int = 
         if any(n is None for pair in norms for n in pair):
             raise ValueError("norm_at_load needs q_norm and k_norm modules in every layer")
     hook = WindowAttention(window, mode, rope_at_load, norms)
-    _set_norms(model, norm_at_load)
     rot = model.model.rotary_emb
+    if norm_at_load:
+        for layer in model.model.layers:
+            _check_order(layer.self_attn, rot.original if isinstance(rot, IdentityRotary) else rot, model.config.hidden_size)
+    _set_norms(model, norm_at_load)
     if rope_at_load and not isinstance(rot, IdentityRotary):
         model.model.rotary_emb = IdentityRotary(rot)
     elif not rope_at_load and isinstance(rot, IdentityRotary):

@@ -118,3 +118,59 @@ def test_the_norm_itself_is_taken(eps, dtype):
         with torch.no_grad():
             norm.weight.copy_(torch.randn(128, generator=g) * 2)
         assert hf._norm_eps(norm) == eps
+
+
+def attention(model, how):
+    """Layer 1's attention with its norms elsewhere."""
+    Q = transformers.models.qwen3.modeling_qwen3
+    base = type(model.model.layers[1].self_attn)
+
+    class Changed(base):
+        def forward(self, hidden_states, position_embeddings, attention_mask, past_key_values=None, **kwargs):
+            if how == "raises":
+                raise RuntimeError("not this way")
+            shape = (*hidden_states.shape[:-1], -1, self.head_dim)
+            q, k, v = (p(hidden_states).view(shape).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
+            cos, sin = position_embeddings
+            if how == "one before, one behind":
+                k = self.k_norm(k)
+            q, k = Q.apply_rotary_pos_emb(q, k, cos, sin)
+            if how != "one left out":
+                q = self.q_norm(q)
+            if how != "one before, one behind":
+                k = self.k_norm(k)
+            return q, k
+    model.model.layers[1].self_attn.__class__ = Changed
+
+
+@pytest.mark.parametrize("how", ["both behind", "one before, one behind", "one left out", "raises"])
+@pytest.mark.parametrize("before", [False, True])
+def test_norms_behind_the_rotation_are_refused(how, before):
+    """The kernels norm before they rotate; the weight makes that another result than the other order."""
+    from atflash import hf
+    model = model_of()
+    if before:
+        hf.register(model, n_ctx=4096)  # (the rotation left to the kernels already)
+    rot = model.model.rotary_emb
+    attention(model, how)
+    norms = [getattr(layer.self_attn, n) for layer in model.model.layers for n in ("q_norm", "k_norm")]
+    with pytest.raises(ValueError, match="before the rotation"):
+        hf.register(model, n_ctx=4096, norm_at_load=True)
+    assert [getattr(layer.self_attn, n) for layer in model.model.layers for n in ("q_norm", "k_norm")] == norms
+    assert all(not n._forward_pre_hooks for n in norms) and model.model.rotary_emb is rot
+    assert hf.register(model, n_ctx=4096).norms is None  # without them as ever
+    hf.unregister(model)
+
+
+def test_the_trial_leaves_nothing():
+    """Neither hooks, gradients, random numbers nor a cache's state; a model in training as well, twice, and behind another hook."""
+    from atflash import hf
+    model = model_of(3).train()
+    state = torch.random.get_rng_state()
+    for _ in range(2):
+        hook = hf.register(model, n_ctx=4096, norm_at_load=True)
+    assert len(hook.norms) == 3 and torch.equal(torch.random.get_rng_state(), state)
+    for layer in model.model.layers:
+        for n in (layer.self_attn.q_norm, layer.self_attn.k_norm):
+            assert not n._forward_pre_hooks and not n.original._forward_pre_hooks and n.original.weight.grad is None
+    hf.unregister(model)
