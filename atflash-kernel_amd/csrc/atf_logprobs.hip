@@ -59,7 +59,7 @@ struct LogitVec {  // 16 bytes of logits
 };
 
 // A value as 32 bits that are ordered as the values are; equal values (0 and -0) the same
-// bits, NaN as -inf.
+// bits, NaN of any kind as -inf.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
@@ -124,11 +124,18 @@ __device__ __forceinline__ uint64_t wave_nth64(uint64_t x, int n) {
   const uint64_t at = __builtin_amdgcn_ballot_w64(above == n - 1 && x != 0);
   return at != 0 ? lane64(x, __builtin_ctzll(at)) : 0;
 }
-// The largest of three, not NaN if one is not.  (Of fmaxf the compiler makes one more instruction
-// an operand, which would quiet a signalling NaN.)
+// The largest of three, not NaN if one is not, unless there is a signalling NaN among them: that
+// makes it NaN.  (For fmaxf the compiler quiets the first pair of a chain and takes the others as they are.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// A signalling NaN as a quiet one, all else as it is.  (Logits of bf16 and fp32 are taken bit by bit; those
+// of fp16 come quiet from their conversion.)
+__device__ __forceinline__ float quiet(float a) {
+  float r;
+  asm("v_max_f32 %0, %1, %1" : "=v"(r) : "v"(a));
   return r;
 }
 // LDS that only one wave uses: its accesses before and after keep their order.
@@ -348,8 +355,8 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
     load(c0, v);
     float vm[kVecs];  // the vectors' largest
     // The chunk's sums, a vector at a time.  The short way has a NaN in t where 2^u is 0 and u
-    // -inf (masked logits): the chunk is then done again with u held above -inf, and so are
-    // those after it.
+    // -inf (masked logits), and where a logit is NaN: the chunk is then done again with u held above
+    // -inf, and the largest taken past signalling NaN, and so are those after it.
     auto sums = [&](auto hold) {
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
@@ -367,6 +374,13 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_kernel(LogprobAr
             const float u = (y[e] - m) * kLog2e, p = __builtin_amdgcn_exp2f(u);
             st.s += p;
             st.t = __builtin_fmaf(p, decltype(hold)::value ? fmaxf(u, kLowest) : u, st.t);
+          }
+        }
+        if constexpr (decltype(hold)::value && kTop && kType != kLogitsFp16) {
+          if (__builtin_amdgcn_ballot_w64(st.s != st.s) != 0) {  // a NaN, here or before: past a signalling one
+            vm[k] = max3(quiet(y[0]), quiet(y[1]), quiet(y[kE - 1]));
+#pragma unroll
+            for (int e = 2; e < kE - 1; e += 2) vm[k] = max3(vm[k], quiet(y[e]), quiet(y[e + 1]));
           }
         }
       }

@@ -321,7 +321,7 @@ int atf_qk_norm_write(void* q_out, const void* q, int64_t q_st, int64_t q_sh, in
  *                                       first, of equal logits the lowest id first
  * top is at most ATF_MAX_TOP and at most vocab.  Logits of -inf have probability 0; a row of
  * nothing else has log probabilities of -inf and entropy 0.  A NaN or +inf makes the row's log
- * probabilities and entropy NaN; NaN rank below every number.  At most 2^23 rows of 2^30 logits.
+ * probabilities and entropy NaN; a NaN of any kind ranks as -inf does.  At most 2^23 rows of 2^30 logits.
  * Sums are fp32.
  *   The workspace (atf_logprobs_workspace_bytes; 0 for many rows) needs no initialisation; calls
  * that share one must be ordered on one stream.
