@@ -481,14 +481,16 @@ class WindowAttention:
     def _check_norms(self, module):
         """The module's norms must be those that this hook's kernels apply, or none that kernels apply: another
         model's calls (the attention function is registered by name, the last hook gets them all) would be
-        computed without its norms, or with its own and then this one's."""
+        computed without its norms, or with its own and then this one's.  A caller of the hook that has no
+        attention module names a layer alone."""
         left = [getattr(module, name, None) for name in ("q_norm", "k_norm")]
         if self.norms is None:
             wrong = any(isinstance(n, IdentityNorm) for n in left)
         else:
             idx = getattr(module, "layer_idx", None)
-            mine = self.norms[idx][:2] if idx is not None and 0 <= idx < len(self.norms) else (None, None)
-            wrong = any(not isinstance(n, IdentityNorm) or n.original is not m for n, m in zip(left, mine))
+            wrong = idx is None or not 0 <= idx < len(self.norms)
+            if not wrong and (isinstance(module, nn.Module) or any(n is not None for n in left)):
+                wrong = any(not isinstance(n, IdentityNorm) or n.original is not m for n, m in zip(left, self.norms[idx]))
         if wrong:
             raise ValueError("the model's norms were left to another hook, or this hook applies another model's: "
                              "register() this model (again)")

@@ -174,3 +174,17 @@ def test_the_trial_leaves_nothing():
         for n in (layer.self_attn.q_norm, layer.self_attn.k_norm):
             assert not n._forward_pre_hooks and not n.original._forward_pre_hooks and n.original.weight.grad is None
     hf.unregister(model)
+
+
+def test_a_caller_without_an_attention_module_names_a_layer():
+    import types
+    from atflash import hf
+    model = model_of(2)
+    hook = hf.register(model, n_ctx=4096, norm_at_load=True)
+    for i in range(2):
+        hook._check_norms(types.SimpleNamespace(layer_idx=i))
+    for wrong in (dict(layer_idx=2), dict(layer_idx=-1), dict(), dict(layer_idx=0, q_norm=model.model.layers[1].self_attn.q_norm),
+                  dict(layer_idx=0, k_norm=model.model.layers[0].self_attn.k_norm.original)):
+        with pytest.raises(ValueError, match="another hook"):
+            hook(types.SimpleNamespace(**wrong), *states(), None)
+    hf.unregister(model)
