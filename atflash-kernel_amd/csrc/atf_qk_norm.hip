@@ -10,8 +10,7 @@
 // 16 dims are a level of the cache's K half (level 7 - i).  Bound by HBM on long calls: a
 // row read and written, a (cos, sin) row of 512 bytes a position.  37000 packed rows of 24 + 8
 // heads, 613 MB: 117 us, 5.2 TB/s, as a large copy; into the bf16 cache 2 x 16000 tokens of 28 + 4
-// heads with their values, 597 MB: 118 us, 5.1 TB/s (123 with q's heads requested one after the
-// other); turns of 11 sequences into the 8-bit cache, 105 MB: 22 to 24 us.  A step's append of 32
+// heads with their values, 597 MB: 113 us, 5.3 TB/s; turns of 11 sequences into the 8-bit cache, 105 MB: 22 to 24 us.  A step's append of 32
 // tokens 3.6 us, two round trips before the stores.
 #include "atf_launch.h"
 #include "atf_q8.h"
@@ -47,26 +46,52 @@ __device__ __forceinline__ void load_weights(const void* w, bool fp32, int i, fl
   }
 }
 
+// Whether mean(x^2) + eps is a normal fp32 number.  A row of which it is not is scaled by a power of two and squared
+// again (kAny): squares of large rows pass fp32, those of small ones are subnormal, which the root takes for 0.
+// Scaling rounds nothing that a result shows, and a normal mean has lost less than 2^-26 of itself with the squares
+// that are not normal.
+__device__ __forceinline__ bool plain_mean(float m) {
+  constexpr int kPositiveNormal = 0x100;
+  return __builtin_amdgcn_classf(m, kPositiveNormal);
+}
+
 // A lane's 16 dims of a row (a: the first halves of its pairs, b: the second) normed and,
-// with `rope`, rotated by its pairs' (cos, sin).
-__device__ __forceinline__ void norm_rotate(const u32x4& a, const u32x4& b, const float (&w1)[8], const float (&w2)[8],
+// with `rope`, rotated by its pairs' (cos, sin).  Returns plain_mean: without kAny the results of a
+// row that is not are not its own.
+template <bool kAny>
+__device__ __forceinline__ bool norm_rotate(const u32x4& a, const u32x4& b, const float (&w1)[8], const float (&w2)[8],
                                             float eps, bool rope, const float (&cs)[16], float (&z1)[8],
                                             float (&z2)[8]) {
   float x1[8], x2[8];
   unpack8(a, x1);
   unpack8(b, x2);
-  float s = 0.f;
+  auto mean_of = [&](float e) {
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s = __builtin_fmaf(x1[i], x1[i], s);
+    for (int i = 0; i < 8; ++i) s = __builtin_fmaf(x1[i], x1[i], s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s = __builtin_fmaf(x2[i], x2[i], s);
-  const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(sum8(s), 1.f / kD, eps));
+    for (int i = 0; i < 8; ++i) s = __builtin_fmaf(x2[i], x2[i], s);
+    return __builtin_fmaf(sum8(s), 1.f / kD, e);
+  };
+  float m = mean_of(eps);
+  const bool plain = plain_mean(m);
+  if (kAny && __builtin_expect(__builtin_amdgcn_ballot_w64(!plain) != 0, 0)) {
+    const float scale = plain ? 1.f : m < 1.f ? 0x1p100f : 0x1p-70f;  // (a row's eight lanes alike)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x1[i] *= scale;
+      x2[i] *= scale;
+    }
+    m = mean_of(eps * scale * scale);
+  }
+  const float inv = __builtin_amdgcn_rsqf(m);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float y1 = x1[i] * inv * w1[i], y2 = x2[i] * inv * w2[i];
     z1[i] = rope ? rope_first(y1, y2, cs[2 * i], cs[2 * i + 1]) : y1;
     z2[i] = rope ? rope_second(y1, y2, cs[2 * i], cs[2 * i + 1]) : y2;
   }
+  return plain;
 }
 
 __device__ __forceinline__ void store_row(uint16_t* row, int i, const float (&z1)[8], const float (&z2)[8]) {
@@ -97,7 +122,7 @@ __global__ __launch_bounds__(64 * kNormWaves) void qk_norm_rows_kernel(QkNormArg
     const u32x4 x1 = ldg16(x + 8 * i), x2 = ldg16(x + kP + 8 * i);
     float w1[8], w2[8], z1[8], z2[8];
     load_weights(is_q ? a.q_weight : a.k_weight, a.weights_fp32, i, w1, w2);
-    norm_rotate(x1, x2, w1, w2, a.eps, rope, cs, z1, z2);
+    norm_rotate<true>(x1, x2, w1, w2, a.eps, rope, cs, z1, z2);
     uint16_t* out = is_q ? a.q_out + (static_cast<int64_t>(t) * a.hq + hh) * kD
                          : a.k_out + (static_cast<int64_t>(t) * a.hk + hh) * kD;
     store_row(out, i, z1, z2);
@@ -171,12 +196,24 @@ __global__ __launch_bounds__(128) void qk_norm_write_kernel(QkNormArgs n) {
         x1[j] = ldg16(x + at + 8 * i);
         x2[j] = ldg16(x + at + kP + 8 * i);
       }
+      // (rows that are not plain are done again behind the four: a branch after each head made 32 single
+      // tokens into the 8-bit cache 0.2 us slower, this one 0)
+      bool plain = true;
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int h = h0 + j0 + j;
         float z1[8], z2[8];
-        norm_rotate(x1[j], x2[j], w1, w2, n.eps, rope, cs, z1, z2);
+        plain &= norm_rotate<false>(x1[j], x2[j], w1, w2, n.eps, rope, cs, z1, z2);
         if (on && h < n.hq) store_row(n.q_out + (row * n.hq + h) * kD, i, z1, z2);
+      }
+      if (__builtin_amdgcn_ballot_w64(!plain) != 0) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int h = h0 + j0 + j;
+          float z1[8], z2[8];
+          norm_rotate<true>(x1[j], x2[j], w1, w2, n.eps, rope, cs, z1, z2);
+          if (on && h < n.hq) store_row(n.q_out + (row * n.hq + h) * kD, i, z1, z2);
+        }
       }
     }
     return;
@@ -196,7 +233,7 @@ __global__ __launch_bounds__(128) void qk_norm_write_kernel(QkNormArgs n) {
   if (pg < 0 || pg >= a.num_pages) return;
   const size_t blk = static_cast<size_t>(pg) * a.hkv + unit;
   float z1[8], z2[8];
-  norm_rotate(xk1, xk2, w1, w2, n.eps, rope, cs, z1, z2);
+  norm_rotate<true>(xk1, xk2, w1, w2, n.eps, rope, cs, z1, z2);
   // the level's two slices: the upper four of its pairs (first halves, then second), the lower four
   const float ka[8] = {z1[4], z1[5], z1[6], z1[7], z2[4], z2[5], z2[6], z2[7]};
   const float kb[8] = {z1[0], z1[1], z1[2], z1[3], z2[0], z2[1], z2[2], z2[3]};
@@ -340,7 +377,7 @@ __global__ __launch_bounds__(64) void qk_norm_append_kernel(QkNormArgs n) {
   if (rope) load_cs8(a.rope_cs, static_cast<int>(pos), 8 * i, cs);
   const int pg = pidx < a.max_pages ? a.page_table[static_cast<int64_t>(b) * a.max_pages + pidx] : -1;
   float z1[8], z2[8];
-  norm_rotate(x1, x2, w1, w2, n.eps, rope, cs, z1, z2);
+  norm_rotate<true>(x1, x2, w1, w2, n.eps, rope, cs, z1, z2);
   if (kind == 0) {
     store_row(n.q_out + (row * n.hq + h) * kD, i, z1, z2);
     return;

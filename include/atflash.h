@@ -284,7 +284,8 @@ int atf_release_tables(int32_t* page_table, int max_pages, int32_t* seq_lens, in
  * (weights_fp32), not needed where there are no heads.  positions: device int32 [rows].
  * With rope_cs NULL rows are normed only.  A row whose position lies outside
  * [0, rope_max_pos) is left as it is in the outputs.  At most 2^25 rows.  fp32 throughout, one
- * rounding.
+ * rounding; rows of any size, also where their squares leave fp32's range (eps may be 0; a row of
+ * zeros is then NaN).
  */
 int atf_qk_norm_rope_bf16(void* q_out, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads,
                           void* k_out, const void* k, int64_t k_st, int64_t k_sh, int num_k_heads,
