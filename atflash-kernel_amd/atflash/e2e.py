@@ -70,7 +70,8 @@ def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None, 
     """One request: chunked prefill then `steps` greedy tokens (the first from
     the prefill's logits).  Returns timings and the generated tokens, and with
     `logprobs` (a number of alternatives, 0 or more) each token's log probability, the
-    entropy it was chosen from and the likeliest tokens, computed outside the timed steps.  With
+    entropy it was chosen from and the likeliest tokens, computed behind all that is timed
+    (the tokens' logits are kept until then).  With
     `progress`, a line is printed after every 4th chunk has run (the host waits
     for it first, so long prefills report as they go; the wait costs one
     kernel-launch latency per 4 chunks)."""
@@ -92,14 +93,7 @@ def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None, 
     e1.record()
     cur = int(out.logits[:, -1].argmax(-1))
     tokens = [cur]
-    said = []
-
-    def say(logits):
-        if logprobs is not None:
-            tok = torch.tensor([tokens[-1]], device=dev)
-            said.append([x.tolist() for x in ops.token_logprobs(logits, tok, logprobs)])
-
-    say(out.logits[:, -1])
+    rows = [out.logits[:, -1]]  # what each token was chosen from (kept for `logprobs`)
     pend = []
     for _ in range(1, steps):
         s0, s1 = ev(), ev()
@@ -108,7 +102,8 @@ def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None, 
         s1.record()
         cur = int(out.logits[:, -1].argmax(-1))
         tokens.append(cur)
-        say(out.logits[:, -1])
+        if logprobs is not None:
+            rows.append(out.logits[:, -1])
         pend.append((s0, s1))
     torch.cuda.synchronize()
     wall = time.perf_counter() - wall0
@@ -118,8 +113,9 @@ def run_request(model, hook, ids, chunk: int, steps: int, progress: str = None, 
            "decode_ms_per_step_median": sorted(step_ms)[len(step_ms) // 2] if step_ms else 0.0,
            "step_ms": step_ms, "wall_s": wall, "tokens": tokens}
     if logprobs is not None:
-        got["logprobs"] = [{"logprob": a[0], "entropy": h[0], "top": [[i, x] for i, x in zip(ids_[0], v[0])]}
-                           for a, h, v, ids_ in said]
+        said = ops.token_logprobs(torch.cat(rows), torch.tensor(tokens, device=dev), logprobs)
+        got["logprobs"] = [{"logprob": a, "entropy": h, "top": [[i, x] for i, x in zip(best, v)]}
+                           for a, h, v, best in zip(*(t.tolist() for t in said))]
     return got
 
 
