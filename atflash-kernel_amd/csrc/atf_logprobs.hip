@@ -13,15 +13,16 @@
 // reach the least of these, so that it is a bound, and 16 bytes of logits are looked at
 // closer only if their largest reaches it.  For the first chunk the q-th best of a
 // wave's lanes (each lane's largest) serve.
-//   Bound by HBM on many rows (every logit is read once), with alternatives by the vector
-// units as well: 2048 rows of 152064 bf16 logits 116 us without alternatives (5.4 TB/s), 130
-// with one, 139 with 20, 176 with 64; of fp32 logits 228 and, with 20, 258.  What it came from, us
+//   Bound by HBM on many rows (every logit is read once), with many alternatives by the vector
+// units: 2048 rows of 152064 bf16 logits (normal, deviation 2) 118 us without alternatives (5.3 TB/s), 119
+// with one, 135 with 20, 177 with 64; of fp32 logits 228 and, with 20, 248.  Some hundred rows are
+// further from it (300 with 20 38 us, floor 17): whole chunks divide them unevenly.  What it came from, us
 // for bf16 with none, 1 and 20: a workgroup of 512 that put its candidates in order together after
 // every chunk, every element pushed by itself, one alternative 490; waves by themselves, the
 // bound of all of them 136, 164, 195; joined by one wave, the row's filler left out 117, 137, 187;
 // lanes' candidates side by side, ordered once 118, 135, 147; workgroups of 256 (four a CU, so that
 // one's end runs beside the others' loads) 116, 130, 139.  One row takes 3.6 + 2.8 us of the two
-// kernels, with five alternatives 7.6 + 4.3: a chain of loads, sums and LDS.
+// kernels, with five alternatives 8 + 4.3: a chain of loads, sums and LDS.
 //   Requesting a chunk while the one before is summed changed nothing (130 without alternatives,
 // 164 with one, before and after) and took 32 registers.
 #include <type_traits>

@@ -77,7 +77,8 @@ static hipError_t allow_lds(const void* kernel, size_t bytes) {
 // pages, less the surviving rows'), and hands out the new ones; the others write the new
 // rows, all but the entries of new pages.  8 beams of 375 pages 6.4 us, one prompt of 1876 pages
 // forked into 48 rows 5.6; 64 rows of 500 pages 15, of 2000 53, half a million entries 190: one
-// workgroup reads every entry of the old rows, where it is one launch for all others.
+// workgroup reads every entry of the old rows.  Several could, with the bits in memory and another
+// launch, which the small tables would pay for.
 constexpr int kSelChunk = 4096;  // entries of a row that a workgroup writes
 __global__ __launch_bounds__(kPgThreads) void select_tables_kernel(SelectTablesArgs a) {
   extern __shared__ uint32_t sh[];
@@ -207,8 +208,9 @@ hipError_t launch_select_tables(const SelectTablesArgs& a, hipStream_t s) {
 //   With L pages in rows, T = the id of the (L + 1)-th lowest page that is in a row or free:
 // rows' pages from T on move, free ones below T take them, the i-th highest of the former to
 // the i-th lowest of the latter (as many of each).  The free pages come out highest first,
-// so that the lowest is taken first.  Latency bound (the pages' copies are not its part);
-// one workgroup: a page's place depends on all before it.  Pools of 300 pages 9.7 us, 6000 19,
+// so that the lowest is taken first.  Latency bound (the pages' copies are not its part).  One
+// workgroup: a page's place depends on all before it.  Marking and rewriting the entries do not, and
+// large tables would be faster with several workgroups and two launches more.  Pools of 300 pages 9.7 us, 6000 19,
 // 160000 183, 2^19 820; the copies of the 6000 move 2.7 GB in 541 us.
 __global__ __launch_bounds__(kPgThreads) void compact_tables_kernel(CompactTablesArgs a) {
   extern __shared__ uint32_t sh[];

@@ -10,8 +10,9 @@
 // 16 dims are a level of the cache's K half (level 7 - i).  Bound by HBM on long calls: a
 // row read and written, a (cos, sin) row of 512 bytes a position.  37000 packed rows of 24 + 8
 // heads, 613 MB: 117 us, 5.2 TB/s, as a large copy; into the bf16 cache 2 x 16000 tokens of 28 + 4
-// heads with their values, 597 MB: 113 us, 5.3 TB/s; turns of 11 sequences into the 8-bit cache, 105 MB: 22 to 24 us.  A step's append of 32
-// tokens 3.6 us, two round trips before the stores.
+// heads with their values, 597 MB: 113 us, 5.3 TB/s; turns of 11 sequences into the 8-bit cache,
+// 105 MB: 23 to 25 us.  A step's append of 32 tokens 3.7 us, two round trips before the stores, into the
+// 8-bit cache 5.3 (in a graph, the bf16 cache's 3.0): a page's kernel for a token.
 #include "atf_launch.h"
 #include "atf_q8.h"
 
